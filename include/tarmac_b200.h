@@ -66,6 +66,8 @@ extern "C" {
 #define TARMAC_ERR_BITS 9       /* Morton bits outside [1, 16]                */
 #define TARMAC_ERR_SCRATCH 10   /* problem larger than the library's fixed
                                    scratch (no-allocation entry point)      */
+#define TARMAC_ERR_HEADS 11     /* head counts or rotated columns outside the
+                                   supported range (multi-head operators)   */
 
 /* ---- element types ------------------------------------------------------- */
 #define TARMAC_F32 0
@@ -288,6 +290,101 @@ int tarmac_dense_attention_backward_noalloc(
     const void *q, const void *k, const void *v, const void *out,
     const void *dout, const int64_t *strides, int B, int N, int d, int dtype,
     float scale, float *dq, float *dk, float *dv, void *stream);
+
+/* ---- multi-head operators -------------------------------------------------- */
+/* For agents with several heads, limited sight or a history. The reference's
+ * module has one head and no mask beyond the diagonal
+ * (src/agents/mappo.py:138-420); these entry points have no counterpart
+ * there. Tensors are [B, N, heads, d] of `dtype` with unit innermost stride
+ * and 1 <= d <= 128; outputs are contiguous. `strides` holds { batch, row,
+ * head } int64 element strides for each input tensor in argument order, or is
+ * NULL for contiguous tensors. Rows on a 16-byte grid (pointer, strides and
+ * width) move as vectors, others element by element. Element offsets are 64
+ * bits. Inputs that a row sees must be finite. */
+
+/* Norm of every query and key head and the position rotation, in one pass:
+ *   z = x / sqrt(mean_c x_c^2 + eps) * w,
+ *   (y_a, y_b) = (z_a cos - z_b sin, z_a sin + z_b cos)
+ * for the r / 2 column pairs of the first r columns (r even, 0 <= r <= d):
+ * (i, i + r/2), or (2i, 2i + 1) when `interleaved`; other columns keep z.
+ * q, q_out: [B, N, H, d]; k, k_out: [B, N, Hk, d]; strides: q, k. wq, wk:
+ * fp32 [d] or NULL (ones). cos, sin: fp32 [., N, r / 2], the episodes table_b
+ * elements apart (0: one table for all). All arithmetic is fp32, rounded
+ * once. */
+int tarmac_qk_norm_rotate(const void *q, const void *k, void *q_out,
+                          void *k_out, const int64_t *strides, const float *wq,
+                          const float *wk, const float *cos, const float *sin,
+                          int64_t table_b, int B, int N, int H, int Hk, int d,
+                          int r, int dtype, float eps, int interleaved,
+                          void *stream);
+
+/* Its gradients. dq_out, dk_out: gradients of the outputs; strides: q, k,
+ * dq_out, dk_out. dq, dk: of the inputs, their type, contiguous. dwq, dwk:
+ * fp32 [d] or NULL, summed over all rows in a fixed order (two calls give the
+ * same bits). The tables get no gradient. work: 16-byte aligned scratch of
+ * tarmac_qk_norm_rotate_workspace(d) bytes. */
+int64_t tarmac_qk_norm_rotate_workspace(int d);
+int tarmac_qk_norm_rotate_backward(const void *q, const void *k,
+                                   const void *dq_out, const void *dk_out,
+                                   const int64_t *strides, const float *wq,
+                                   const float *wk, const float *cos,
+                                   const float *sin, int64_t table_b, int B,
+                                   int N, int H, int Hk, int d, int r,
+                                   int dtype, float eps, int interleaved,
+                                   void *dq, void *dk, float *dwq, float *dwk,
+                                   void *work, void *stream);
+
+/* Truth values (bytes, 0: false) [B, Nq, Nk], rows of unit stride, to words
+ * [B, Nq, ceil(Nk / 32)] of 32 keys each, lowest key in the lowest bit. */
+int tarmac_pack_visibility(const void *visible, int64_t stride_b,
+                           int64_t stride_n, int B, int Nq, int Nk, void *bits,
+                           void *stream);
+
+/* peers of the multi-head attention */
+#define TARMAC_PEERS_ALL 0
+#define TARMAC_PEERS_OTHERS 1 /* a row leaves its own position out */
+#define TARMAC_PEERS_PAST 2   /* a row sees positions up to its own */
+
+/* Masked attention with heads. q, out: [B, Nq, H, d]; k, v: [B, Nk, Hk, d],
+ * H a multiple of Hk: query head h reads key head h / (H / Hk). strides: q,
+ * k, v. Row i of episode b stands at position q_start[b] + i (Nk - Nq + i
+ * when q_start is NULL) and sees key j when j < key_len[b] (key_len: int32
+ * [B], clamped to [0, Nk], or NULL), `peers` allows it and its bit in `bits`
+ * (tarmac_pack_visibility words, episodes bits_b words apart, 0 for one mask;
+ * or NULL) is set. out = softmax(scale q k^T over the keys seen) v; lse
+ * (fp32 [B, H, Nq], optional) the natural log of the softmax's sum of
+ * exponentials. A row that sees nothing gets out = 0, lse = -inf. Rows of k
+ * and v from key_len on are not read. fp32: products as good as fp32 FMAs;
+ * bf16: bf16 products with fp32 sums, the softmax weights rounded to bf16.
+ * work: 16-byte aligned scratch of tarmac_head_attention_workspace bytes (0
+ * for most shapes; then NULL is fine). */
+int64_t tarmac_head_attention_workspace(int B, int Nq, int Nk, int H, int Hk,
+                                        int d);
+int tarmac_head_attention(const void *q, const void *k, const void *v,
+                          void *out, float *lse, const int64_t *strides,
+                          const int32_t *key_len, const int32_t *q_start,
+                          const void *bits, int64_t bits_b, int B, int Nq,
+                          int Nk, int H, int Hk, int d, int dtype, int peers,
+                          float scale, void *work, void *stream);
+
+/* Its gradients, with P recomputed from lse:
+ *   D_i = dout_i . out_i, dS = P (dout v^T - D),
+ *   dq = scale dS k, dk = scale dS^T q, dv = P^T dout,
+ * shared key heads summed over their query heads. out, lse: the forward's.
+ * strides: q, k, v, out, dout. dq, dk, dv: contiguous, the inputs' type; rows
+ * that see nothing and keys that nothing sees get zeros. No atomics: two
+ * calls give the same bits. work: 16-byte aligned scratch of
+ * tarmac_head_attention_backward_workspace bytes. */
+int64_t tarmac_head_attention_backward_workspace(int B, int Nq, int H);
+int tarmac_head_attention_backward(const void *q, const void *k, const void *v,
+                                   const void *out, const float *lse,
+                                   const void *dout, const int64_t *strides,
+                                   const int32_t *key_len,
+                                   const int32_t *q_start, const void *bits,
+                                   int64_t bits_b, int B, int Nq, int Nk,
+                                   int H, int Hk, int d, int dtype, int peers,
+                                   float scale, void *dq, void *dk, void *dv,
+                                   void *work, void *stream);
 
 /* Which kernel, and with which tiling, a call with these arguments would
  * take — host-only: no launch, no device access, callable without a GPU.

@@ -327,6 +327,9 @@ const char* tarmac_strerror(int status) {
     case TARMAC_ERR_BITS: return "Morton bits must lie in [1, 16]";
     case TARMAC_ERR_SCRATCH:
       return "problem larger than the library's fixed scratch (B * N <= 524288)";
+    case TARMAC_ERR_HEADS:
+      return "heads must be positive, query heads a multiple of key heads, "
+             "rotated columns even and at most d";
     default: return "unknown status";
   }
 }

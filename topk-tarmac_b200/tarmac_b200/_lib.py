@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import c_char_p, c_float, c_int, c_uint64, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int64, c_uint64, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("libtarmac_b200.so")
@@ -28,6 +28,7 @@ ERR_MODE = 7
 ERR_LAUNCH = 8
 ERR_BITS = 9
 ERR_SCRATCH = 10
+ERR_HEADS = 11
 
 F32 = 0
 BF16 = 1
@@ -35,6 +36,10 @@ BF16 = 1
 SELECT_ARGMAX = 0
 SELECT_THRESHOLD = 1
 SELECT_SORT = 2
+
+PEERS_ALL = 0
+PEERS_OTHERS = 1
+PEERS_PAST = 2
 
 # name -> (restype, argtypes); the order follows the header's declarations
 SIGNATURES: dict[str, tuple] = {
@@ -83,6 +88,31 @@ SIGNATURES: dict[str, tuple] = {
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
         c_int, c_int, c_int, c_int, c_float,
         c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tarmac_qk_norm_rotate": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int,
+        c_int, c_float, c_int, c_void_p]),
+    "tarmac_qk_norm_rotate_workspace": (c_int64, [c_int]),
+    "tarmac_qk_norm_rotate_backward": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int,
+        c_int, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p]),
+    "tarmac_pack_visibility": (c_int, [
+        c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "tarmac_head_attention_workspace": (c_int64, [
+        c_int, c_int, c_int, c_int, c_int, c_int]),
+    "tarmac_head_attention": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int,
+        c_int, c_int, c_float, c_void_p, c_void_p]),
+    "tarmac_head_attention_backward_workspace": (c_int64, [
+        c_int, c_int, c_int]),
+    "tarmac_head_attention_backward": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int,
+        c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p]),
     "tarmac_kernel_plan": (c_int, [
         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p,
         c_char_p, c_int]),

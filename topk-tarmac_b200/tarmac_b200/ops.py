@@ -15,6 +15,7 @@ diagonal excluded, softmax over the retained peers, weighted sum of V rows.
 from __future__ import annotations
 
 import contextlib
+import functools
 import struct
 
 import torch
@@ -403,6 +404,278 @@ def comm_forward(x: torch.Tensor, w_qkv: torch.Tensor, b_qkv: torch.Tensor,
                   _ptr(w_proj), _ptr(b_proj), B, N, D, m, int(topk),
                   _ptr(out), _stream(x.device))
     return out
+
+
+# ---------------------------------------------------------------------------
+# multi-head operators
+# ---------------------------------------------------------------------------
+
+_PEERS = {"all": _lib.PEERS_ALL, "others": _lib.PEERS_OTHERS,
+          "past": _lib.PEERS_PAST}
+_PACK6 = struct.Struct("=6q").pack
+_PACK9 = struct.Struct("=9q").pack
+_PACK12 = struct.Struct("=12q").pack
+_PACK15 = struct.Struct("=15q").pack
+
+
+def _check_heads(named: dict, like: torch.Tensor) -> None:
+    """Every tensor 4-D, of one supported dtype, on the CUDA device of ``like``."""
+    if not like.is_cuda:
+        raise RuntimeError("tarmac_b200 kernels need CUDA tensors (there is no "
+                           "CPU implementation)")
+    if like.dtype not in _DTYPES:
+        raise TypeError(f"tensors must be float32 or bfloat16; got {like.dtype}")
+    for name, t in named.items():
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [B, N, heads, d]; got {tuple(t.shape)}")
+        if t.device != like.device:
+            raise ValueError(f"{name} must be on the device of the queries")
+        if t.dtype != like.dtype:
+            raise TypeError(f"{name} must have the queries' dtype {like.dtype}; "
+                            f"got {t.dtype}")
+
+
+def _norm_weight(w, name: str, d: int, dev) -> torch.Tensor | None:
+    if w is None:
+        return None
+    if tuple(w.shape) != (d,):
+        raise ValueError(f"{name} must be [{d}]; got {tuple(w.shape)}")
+    if w.device != dev:
+        raise ValueError(f"{name} must be on the device of the queries")
+    return w if w.dtype == torch.float32 and w.is_contiguous() \
+        else w.float().contiguous()
+
+
+def _check_rotate(q, k, wq, wk, cos, sin):
+    _check_heads({"q": q, "k": k}, q)
+    B, N, H, d = q.shape
+    if k.shape[0] != B or k.shape[1] != N or k.shape[3] != d:
+        raise ValueError(f"k must be [{B}, {N}, heads, {d}]; got {tuple(k.shape)}")
+    wq, wk = _norm_weight(wq, "wq", d, q.device), _norm_weight(wk, "wk", d, q.device)
+    if cos.shape != sin.shape or cos.dim() != 3 or cos.shape[0] not in (1, B) \
+            or cos.shape[1] != N or 2 * cos.shape[2] > d:
+        raise ValueError(f"cos and sin must be [1 or {B}, {N}, r / 2] with "
+                         f"r <= {d}; got {tuple(cos.shape)}, {tuple(sin.shape)}")
+    for t in (cos, sin):
+        if t.device != q.device:
+            raise ValueError("cos and sin must be on the device of the queries")
+        if t.dtype != torch.float32:
+            raise TypeError(f"cos and sin must be float32; got {t.dtype}")
+    return (_unit_inner(q), _unit_inner(k), wq, wk, cos.contiguous(),
+            sin.contiguous())
+
+
+def _table_stride(cos: torch.Tensor, B: int) -> int:
+    """Elements between two episodes' tables (0: one table for all)."""
+    return cos.shape[1] * cos.shape[2] if cos.shape[0] == B and B > 1 else 0
+
+
+def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor,
+                   wq: torch.Tensor | None, wk: torch.Tensor | None,
+                   cos: torch.Tensor, sin: torch.Tensor, eps: float = 1e-6,
+                   interleaved: bool = False):
+    """Norm every head of q ([B, N, H, d]) and k ([B, N, Hk, d]) by its root
+    mean square, scale by ``wq`` / ``wk`` ([d], None for ones) and rotate the
+    first r columns by the rows' angles, in one pass. ``cos``, ``sin``: fp32
+    [1 or B, N, r / 2]; column pairs are (i, i + r / 2), or (2i, 2i + 1) with
+    ``interleaved``. Returns contiguous (q', k') in the inputs' dtype. The
+    single-token form is N = 1 with the token's row of the table."""
+    q, k, wq, wk, cos, sin = _check_rotate(q, k, wq, wk, cos, sin)
+    B, N, H, d = q.shape
+    qo, ko = _empty_as(q), _empty_as(k)
+    with _on(q.device):
+        _lib.call("tarmac_qk_norm_rotate", _ptr(q), _ptr(k), _ptr(qo),
+                  _ptr(ko), _PACK6(*q.stride()[:3], *k.stride()[:3]), _ptr(wq),
+                  _ptr(wk), _ptr(cos), _ptr(sin), _table_stride(cos, B), B, N,
+                  H, k.shape[2], d, 2 * cos.shape[2], _DTYPES[q.dtype], eps,
+                  int(interleaved), _stream(q.device))
+    return qo, ko
+
+
+def qk_norm_rotate_backward(q: torch.Tensor, k: torch.Tensor,
+                            wq: torch.Tensor | None, wk: torch.Tensor | None,
+                            cos: torch.Tensor, sin: torch.Tensor,
+                            dq_out: torch.Tensor, dk_out: torch.Tensor,
+                            eps: float = 1e-6, interleaved: bool = False):
+    """Gradients of :func:`qk_norm_rotate` for its inputs and the gradients of
+    its outputs: (dq, dk) in the inputs' dtype and (dwq, dwk) fp32 [d] (None
+    where there is no weight). Deterministic."""
+    q, k, wq, wk, cos, sin = _check_rotate(q, k, wq, wk, cos, sin)
+    _check_heads({"dq_out": dq_out, "dk_out": dk_out}, q)
+    if dq_out.shape != q.shape or dk_out.shape != k.shape:
+        raise ValueError("dq_out and dk_out must have the shapes of q and k")
+    gq, gk = _unit_inner(dq_out), _unit_inner(dk_out)
+    B, N, H, d = q.shape
+    dq, dk = _empty_as(q), _empty_as(k)
+    new = dict(device=q.device, dtype=torch.float32)
+    dwq = None if wq is None else torch.empty(d, **new)
+    dwk = None if wk is None else torch.empty(d, **new)
+    work = torch.empty(_rotate_work(d) // 4, **new)
+    with _on(q.device):
+        _lib.call("tarmac_qk_norm_rotate_backward", _ptr(q), _ptr(k), _ptr(gq),
+                  _ptr(gk),
+                  _PACK12(*q.stride()[:3], *k.stride()[:3], *gq.stride()[:3],
+                          *gk.stride()[:3]),
+                  _ptr(wq), _ptr(wk), _ptr(cos), _ptr(sin),
+                  _table_stride(cos, B), B, N, H, k.shape[2], d,
+                  2 * cos.shape[2], _DTYPES[q.dtype], eps, int(interleaved),
+                  _ptr(dq), _ptr(dk), _ptr(dwq), _ptr(dwk), _ptr(work),
+                  _stream(q.device))
+    return dq, dk, dwq, dwk
+
+
+@functools.lru_cache(maxsize=None)
+def _rotate_work(d: int) -> int:
+    return _lib.lib().tarmac_qk_norm_rotate_workspace(d)
+
+
+def pack_visibility(visible: torch.Tensor) -> torch.Tensor:
+    """Truth values [1 or B, Nq, Nk] to the words the attention kernels read:
+    int32 [1 or B, Nq, ceil(Nk / 32)], 32 keys each, lowest key in the lowest
+    bit. A program that uses one mask in several calls packs it once."""
+    if visible.dim() != 3:
+        raise ValueError(f"visible must be [B, Nq, Nk]; got {tuple(visible.shape)}")
+    if visible.dtype != torch.bool:
+        raise TypeError(f"visible must be bool; got {visible.dtype}")
+    if not visible.is_cuda:
+        raise RuntimeError("tarmac_b200 kernels need CUDA tensors")
+    visible = _unit_inner(visible)
+    B, Nq, Nk = visible.shape
+    bits = torch.empty((B, Nq, (Nk + 31) // 32), device=visible.device,
+                       dtype=torch.int32)
+    with _on(visible.device):
+        _lib.call("tarmac_pack_visibility", _ptr(visible), visible.stride(0),
+                  visible.stride(1), B, Nq, Nk, _ptr(bits),
+                  _stream(visible.device))
+    return bits
+
+
+def _check_attention(q, k, v, peers, key_len, q_start, visible):
+    """Checked q, k, v, lengths, starts and visibility words."""
+    _check_heads({"q": q, "k": k, "v": v}, q)
+    B, Nq, H, d = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != d:
+        raise ValueError(f"k and v must share one [{B}, Nk, heads, {d}] shape; "
+                         f"got {tuple(k.shape)}, {tuple(v.shape)}")
+    Nk, Hk = k.shape[1], k.shape[2]
+    if Hk < 1 or H % Hk:
+        raise ValueError(f"the query heads ({H}) must be a multiple of the key "
+                         f"heads ({Hk})")
+    if peers not in _PEERS:
+        raise ValueError(f"peers must be 'all', 'others' or 'past'; got {peers!r}")
+    ints = []
+    for name, t in (("key_len", key_len), ("q_start", q_start)):
+        if t is not None:
+            if tuple(t.shape) != (B,):
+                raise ValueError(f"{name} must be [{B}]; got {tuple(t.shape)}")
+            if t.dtype not in (torch.int32, torch.int64):
+                raise TypeError(f"{name} must be int32 or int64; got {t.dtype}")
+            if t.device != q.device:
+                raise ValueError(f"{name} must be on the device of the queries")
+            t = t.to(torch.int32).contiguous()
+        ints.append(t)
+    if visible is not None:
+        if visible.device != q.device:
+            raise ValueError("visible must be on the device of the queries")
+        words = (Nk + 31) // 32
+        wide = Nk if visible.dtype == torch.bool else words
+        if visible.dim() != 3 or visible.shape[0] not in (1, B) \
+                or tuple(visible.shape[1:]) != (Nq, wide):
+            raise ValueError(
+                f"visible must be bool [1 or {B}, {Nq}, {Nk}] or its words "
+                f"int32 [1 or {B}, {Nq}, {words}]; got {tuple(visible.shape)}")
+        if visible.dtype == torch.bool:
+            visible = pack_visibility(visible)
+        elif visible.dtype != torch.int32:
+            raise TypeError(f"visible must be bool or int32; got {visible.dtype}")
+        visible = visible.contiguous()
+    return _unit_inner(q), _unit_inner(k), _unit_inner(v), *ints, visible
+
+
+def _bits_stride(bits: torch.Tensor | None) -> int:
+    """Words between two episodes' masks (0: one mask for all)."""
+    if bits is None or bits.shape[0] == 1:
+        return 0
+    return bits.shape[1] * bits.shape[2]
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_work(B, Nq, Nk, H, Hk, d) -> int:
+    return _lib.lib().tarmac_head_attention_workspace(B, Nq, Nk, H, Hk, d)
+
+
+def head_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                   peers: str = "all", key_len: torch.Tensor | None = None,
+                   q_start: torch.Tensor | None = None,
+                   visible: torch.Tensor | None = None,
+                   scale: float | None = None, return_lse: bool = False):
+    """Masked attention with heads: q [B, Nq, H, d], k and v [B, Nk, Hk, d]
+    with H a multiple of Hk; returns out [B, Nq, H, d] (and lse, fp32
+    [B, H, Nq]).
+
+    Row i stands at position ``q_start[b] + i`` (default ``Nk - Nq + i``) and
+    sees key j when ``j < key_len[b]``, ``peers`` allows it ("all"; "others":
+    not its own position; "past": positions up to its own) and
+    ``visible[b, i, j]`` holds (bool [1 or B, Nq, Nk], or the words of
+    :func:`pack_visibility`). A row that sees nothing gets 0 (lse -inf). Keys
+    and values from ``key_len`` on are not read; what a row sees must be
+    finite. One token over a long history is Nq = 1: the key axis is then
+    split over the GPU."""
+    q, k, v, key_len, q_start, bits = _check_attention(
+        q, k, v, peers, key_len, q_start, visible)
+    B, Nq, H, d = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    out = _empty_as(q)
+    lse = (torch.empty((B, H, Nq), device=q.device, dtype=torch.float32)
+           if return_lse else None)
+    nbytes = _attention_work(B, Nq, Nk, H, Hk, d)
+    work = (torch.empty(nbytes, device=q.device, dtype=torch.uint8)
+            if nbytes else None)
+    with _on(q.device):
+        _lib.call("tarmac_head_attention", _ptr(q), _ptr(k), _ptr(v),
+                  _ptr(out), _ptr(lse),
+                  _PACK9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]),
+                  _ptr(key_len), _ptr(q_start), _ptr(bits), _bits_stride(bits),
+                  B, Nq, Nk, H, Hk, d, _DTYPES[q.dtype], _PEERS[peers],
+                  _scale(d, scale), _ptr(work), _stream(q.device))
+    return (out, lse) if return_lse else out
+
+
+def head_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                            out: torch.Tensor, lse: torch.Tensor,
+                            dout: torch.Tensor, peers: str = "all",
+                            key_len: torch.Tensor | None = None,
+                            q_start: torch.Tensor | None = None,
+                            visible: torch.Tensor | None = None,
+                            scale: float | None = None):
+    """Gradients (dq, dk, dv) of :func:`head_attention` in the inputs' dtype,
+    given its ``out`` and ``lse`` and the gradient of out. The probabilities
+    are recomputed; shared key heads are summed over their query heads;
+    deterministic."""
+    q, k, v, key_len, q_start, bits = _check_attention(
+        q, k, v, peers, key_len, q_start, visible)
+    B, Nq, H, d = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    _check_heads({"out": out, "dout": dout}, q)
+    if out.shape != q.shape or dout.shape != q.shape:
+        raise ValueError("out and dout must have the shape of q")
+    if tuple(lse.shape) != (B, H, Nq) or lse.dtype != torch.float32 \
+            or lse.device != q.device:
+        raise ValueError(f"lse must be float32 [{B}, {H}, {Nq}] on the device "
+                         "of the queries")
+    out, dout, lse = _unit_inner(out), _unit_inner(dout), lse.contiguous()
+    dq, dk, dv = _empty_as(q), _empty_as(k), _empty_as(v)
+    work = torch.empty(2 * B * Nq * H, device=q.device, dtype=torch.float32)
+    with _on(q.device):
+        _lib.call("tarmac_head_attention_backward", _ptr(q), _ptr(k), _ptr(v),
+                  _ptr(out), _ptr(lse), _ptr(dout),
+                  _PACK15(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                          *out.stride()[:3], *dout.stride()[:3]),
+                  _ptr(key_len), _ptr(q_start), _ptr(bits), _bits_stride(bits),
+                  B, Nq, Nk, H, Hk, d, _DTYPES[q.dtype], _PEERS[peers],
+                  _scale(d, scale), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(work),
+                  _stream(q.device))
+    return dq, dk, dv
 
 
 _PLAN_OPS = {"dense": 0, "topk": 1, "streaming": 2}
