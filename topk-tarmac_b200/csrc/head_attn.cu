@@ -812,7 +812,14 @@ static cudaError_t bwd_any(const HeadAttnParams& p, cudaStream_t s) {
   return bwd_go<T, 128>(p, s);
 }
 
+cudaError_t launch_head_fwd_tc(const HeadAttnParams& p, cudaStream_t s, bool* done);
+
 cudaError_t launch_head_fwd(const HeadAttnParams& p, bool bf16, cudaStream_t s) {
+  if (bf16) {
+    bool done;
+    const cudaError_t e = launch_head_fwd_tc(p, s, &done);
+    if (done || e != cudaSuccess) return e;
+  }
   return bf16 ? fwd_any<__nv_bfloat16>(p, s) : fwd_any<float>(p, s);
 }
 cudaError_t launch_head_bwd(const HeadAttnParams& p, bool bf16, cudaStream_t s) {

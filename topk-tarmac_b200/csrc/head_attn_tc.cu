@@ -1,0 +1,469 @@
+// head_attn_tc.cu — forward masked attention with heads on the tensor memory
+// (tcgen05), bf16. The operator is defined in head_attn.cu.
+//
+// A block owns two 128-row query tiles of one key head — two heads of the
+// same rows, or neighbouring tiles — that share every staged K and V tile of
+// 128 keys. Roles of its 10 warps:
+// * warps 0..3 and 4..7: one warpgroup per tile, a thread per row. It reads
+//   its row of S from TMEM, masks, runs the softmax in base 2, and writes P
+//   as bf16 over the columns S had. The reference maximum moves, and O is
+//   rescaled, only when a score exceeds it by 2^8, which few tiles do.
+// * warp 8: one thread issues the TMA loads (Q once, K and V in a ring).
+// * warp 9: one thread issues the products, alternating the groups:
+//   S_g = Q_g K^T, then O_g += P_g V with P from TMEM. While one group runs
+//   its softmax the tensor core serves the other.
+// Bound: the special-function unit's 16 exponentials per clock per SM (1024
+// clocks for a 128 x 128 tile) against 256 d / 64 clocks for each of the two
+// products. Blocks are persistent, one per SM, and walk their items in
+// alternating direction, so that under the past rule each gets long and short
+// tiles.
+// Every wait is bounded; one that runs out raises a flag that ends all roles,
+// and the rows concerned are written as NaN.
+#include "head_tc.cuh"
+
+namespace tarmac {
+
+namespace {
+
+constexpr int HT_THREADS = 320;
+constexpr int HT_TMA_WARP = 8, HT_MMA_WARP = 9;
+constexpr int HT_KEYS = 128;
+constexpr float HT_LOG2E = 1.4426950408889634f;
+constexpr float HT_LN2 = 0.6931471805599453f;
+constexpr float HT_MOVE = 8.0f;  // exponent units
+
+template <int DP>
+struct HtPlan {
+  static constexpr int TILE = 128 * DP * 2;                 // bytes of 128 rows
+  static constexpr int NS = DP == 64 ? 4 : 2;               // ring stages (K and V)
+  static constexpr int SMEM = 2 * TILE + NS * 2 * TILE + 1024;
+};
+
+template <int NS>
+struct HtShared {
+  uint64_t qfull, qempty, kfull[NS], vfull[NS], empty[NS], sfull[2], pfull[2], odone[2];
+  uint32_t tmem;
+  int abort_flag;
+};
+
+struct HtItem {
+  int b, hk, n;       // n: key tiles that either tile needs
+  int tile[2], g[2];  // query tile and head inside the group (tile -1: none)
+  int nt[2];          // key tiles of each
+};
+
+}  // namespace
+
+struct HtGrid {
+  int nqt, pairs, items, pair_major;
+};
+
+// item -> its two tiles. Tiles run from the last to the first, as the last
+// have the most keys under the past rule.
+__device__ __forceinline__ HtItem ht_item(const HeadAttnParams& p, const HtGrid& gr, int item) {
+  HtItem w;
+  const int bh = p.B * p.Hk;
+  const int pair = gr.pair_major ? item / bh : item % gr.pairs;
+  const int x = gr.pair_major ? item % bh : item / gr.pairs;
+  w.hk = x % p.Hk;
+  w.b = x / p.Hk;
+  const int start = p.q_start ? __ldg(p.q_start + w.b) : p.Nk - p.Nq;
+  int len = p.key_len ? __ldg(p.key_len + w.b) : p.Nk;
+  len = max(0, min(len, p.Nk));
+  w.n = 0;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int unit = 2 * pair + u;
+    w.tile[u] = -1;
+    w.g[u] = 0;
+    w.nt[u] = 0;
+    if (unit >= gr.nqt * p.G) continue;
+    w.tile[u] = gr.nqt - 1 - unit / p.G;
+    w.g[u] = unit % p.G;
+    int kend = len;
+    if (p.peers == PEERS_PAST) {
+      const int64_t last = (int64_t)start + min(p.Nq, (w.tile[u] + 1) * 128) - 1;
+      kend = (int)max((int64_t)0, min((int64_t)len, last + 1));
+    }
+    w.nt[u] = cdiv(kend, HT_KEYS);
+    w.n = max(w.n, w.nt[u]);
+  }
+  return w;
+}
+
+// items of this block, in alternating direction
+__device__ __forceinline__ int ht_next(int k) {
+  const int g = (int)gridDim.x, x = (int)blockIdx.x;
+  return k * g + ((k & 1) ? g - 1 - x : x);
+}
+
+template <int DP>
+__global__ void __launch_bounds__(HT_THREADS, 1)
+    head_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                       const __grid_constant__ CUtensorMap mv, HeadAttnParams p, HtGrid gr) {
+  using Plan = HtPlan<DP>;
+  constexpr int NS = Plan::NS, TILE = Plan::TILE;
+  extern __shared__ unsigned char ht_raw[];
+  __shared__ HtShared<NS> sh;
+  // 1024-byte grid of the swizzle
+  const uint32_t base = (tc::smem_addr(ht_raw) + 1023u) & ~1023u;
+  const uint32_t qa = base, kva = base + 2 * TILE;
+  volatile int* abort_flag = &sh.abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    tc::mbar_init(&sh.qfull, 1);
+    tc::mbar_init(&sh.qempty, 1);
+    for (int s = 0; s < NS; ++s) {
+      tc::mbar_init(&sh.kfull[s], 1);
+      tc::mbar_init(&sh.vfull[s], 1);
+      tc::mbar_init(&sh.empty[s], 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      tc::mbar_init(&sh.sfull[w], 1);
+      tc::mbar_init(&sh.pfull[w], 4);
+      tc::mbar_init(&sh.odone[w], 1);
+    }
+    sh.abort_flag = 0;
+    tc::mbar_init_fence();
+  }
+  if (warp == HT_MMA_WARP) tc::tmem_alloc(&sh.tmem, 512);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp == HT_TMA_WARP) {
+    if (lane == 0) {
+      uint32_t kc = 0;
+      int k = 0;
+      for (;; ++k) {
+        const int item = ht_next(k);
+        if (item >= gr.items) break;
+        const HtItem w = ht_item(p, gr, item);
+        if (!ws::wait(&sh.qempty, (k & 1) ^ 1, abort_flag)) goto tma_done;
+        const int both = w.tile[1] >= 0;
+        ht::expect_tx(&sh.qfull, (uint32_t)(TILE * (1 + both)));
+        for (int u = 0; u <= both; ++u)
+          ht::tma_tile<DP, 128>(qa + u * TILE, &mq, &sh.qfull, w.hk * p.G + w.g[u],
+                                w.tile[u] * 128, w.b);
+        for (int t = 0; t < w.n; ++t, ++kc) {
+          const int s = kc % NS;
+          if (!ws::wait(&sh.empty[s], ((kc / NS) & 1) ^ 1, abort_flag)) goto tma_done;
+          const uint32_t slot = kva + s * 2 * TILE;
+          ht::expect_tx(&sh.kfull[s], TILE);
+          ht::tma_tile<DP, 128>(slot, &mk, &sh.kfull[s], w.hk, t * HT_KEYS, w.b);
+          ht::expect_tx(&sh.vfull[s], TILE);
+          ht::tma_tile<DP, 128>(slot + TILE, &mv, &sh.vfull[s], w.hk, t * HT_KEYS, w.b);
+        }
+      }
+    tma_done:
+      // the copies in flight land before the block ends
+      if (*abort_flag) {
+        if (k > 0 || kc > 0) tc::mbar_wait(&sh.qfull, 0, 1u << 16);
+        for (uint32_t c = kc > (uint32_t)NS ? kc - NS : 0; c < kc; ++c) {
+          tc::mbar_wait(&sh.kfull[c % NS], (c / NS) & 1, 1u << 16);
+          tc::mbar_wait(&sh.vfull[c % NS], (c / NS) & 1, 1u << 16);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == HT_MMA_WARP) {
+    if (lane == 0) {
+      const int nks = cdiv(p.d, 16);
+      const uint32_t id_s = tc::idesc_bf16(128, HT_KEYS, false, false);
+      const uint32_t id_o = tc::idesc_bf16(128, nks * 16, false, true);
+      const uint64_t dq0 = ht::desc128(qa, 16), dk0 = ht::desc128(kva, 16);
+      const uint64_t dv0 = ht::desc128(kva + TILE, 128 * 128);
+      uint32_t kc = 0, pc[2] = {0, 0};
+      auto scores = [&](int w, int s) {
+        const uint64_t dq = dq0 + (uint64_t)((w * TILE) >> 4);
+        const uint64_t dk = dk0 + (uint64_t)((s * 2 * TILE) >> 4);
+        for (int ks = 0; ks < nks; ++ks)
+          tc::mma_bf16(tmem + w * 128, dq + ht::kstep(ks, 128), dk + ht::kstep(ks, 128), id_s,
+                       ks > 0);
+        tc::mma_commit(&sh.sfull[w]);
+      };
+      for (int k = 0;; ++k) {
+        const int item = ht_next(k);
+        if (item >= gr.items) break;
+        const HtItem it = ht_item(p, gr, item);
+        if (!ws::wait(&sh.qfull, k & 1, abort_flag)) goto mma_done;
+        if (it.n > 0) {
+          const int s = kc % NS;
+          if (!ws::wait(&sh.kfull[s], (kc / NS) & 1, abort_flag)) goto mma_done;
+          tc::fence_after_sync();
+          for (int w = 0; w < 2; ++w)
+            if (it.nt[w] > 0) scores(w, s);
+        }
+        if (it.n <= 1) tc::mma_commit(&sh.qempty);
+        for (int t = 0; t < it.n; ++t, ++kc) {
+          const int s = kc % NS, s1 = (kc + 1) % NS;
+          if (!ws::wait(&sh.vfull[s], (kc / NS) & 1, abort_flag)) goto mma_done;
+          if (t + 1 < it.n && !ws::wait(&sh.kfull[s1], ((kc + 1) / NS) & 1, abort_flag))
+            goto mma_done;
+          const uint64_t dv = dv0 + (uint64_t)((s * 2 * TILE) >> 4);
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            if (t >= it.nt[w]) continue;
+            if (!ws::wait(&sh.pfull[w], pc[w] & 1, abort_flag)) goto mma_done;
+            ++pc[w];
+            tc::fence_after_sync();
+            for (int ks = 0; ks < HT_KEYS / 16; ++ks)
+              ht::mma_ts(tmem + 256 + w * DP, tmem + w * 128 + ks * 8,
+                         dv + (uint64_t)((ks * 2048) >> 4), id_o, t > 0 || ks > 0);
+            if (t + 1 < it.nt[w])
+              scores(w, s1);
+            else
+              tc::mma_commit(&sh.odone[w]);
+          }
+          tc::mma_commit(&sh.empty[s]);
+          if (t + 2 == it.n) tc::mma_commit(&sh.qempty);
+        }
+      }
+      // the last commits land before the block ends
+      for (uint32_t c = kc > (uint32_t)NS ? kc - NS : 0; c < kc; ++c)
+        if (!ws::wait(&sh.empty[c % NS], (c / NS) & 1, abort_flag)) break;
+    mma_done:;
+    }
+    __syncwarp();
+  } else {
+    // ---------------- softmax groups ----------------
+    const int w = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + w * 128 + lane_off, t_o = tmem + 256 + w * DP + lane_off;
+    const float c2 = p.scale * HT_LOG2E;
+    uint32_t kc = 0, sc = 0, oc = 0;
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      const int item = ht_next(k);
+      if (item >= gr.items) break;
+      const HtItem it = ht_item(p, gr, item);
+      const uint32_t kc0 = kc;
+      kc += (uint32_t)it.n;
+      const int tile = w ? it.tile[1] : it.tile[0], nt = w ? it.nt[1] : it.nt[0];
+      if (tile < 0) continue;
+      const int h = it.hk * p.G + (w ? it.g[1] : it.g[0]);
+      const int i = tile * 128 + row;
+      const int64_t pos = (int64_t)(p.q_start ? __ldg(p.q_start + it.b) : p.Nk - p.Nq) + i;
+      int len = p.key_len ? __ldg(p.key_len + it.b) : p.Nk;
+      len = max(0, min(len, p.Nk));
+      const int jlim = p.peers == PEERS_PAST ? (int)max((int64_t)0, min((int64_t)len, pos + 1)) : len;
+      const int self = p.peers == PEERS_OTHERS && pos >= 0 && pos < p.Nk ? (int)pos : -1;
+      const uint32_t* words =
+          p.bits ? p.bits + it.b * p.bits_b + (int64_t)min(i, p.Nq - 1) * p.bits_w : nullptr;
+      float mref = -INFINITY;  // reference maximum in exponent units
+      float l = 0.f;
+      for (int t = 0; t < nt; ++t) {
+        const int k0 = t * HT_KEYS;
+        if (!ws::wait(&sh.sfull[w], sc & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        ++sc;
+        tc::fence_after_sync();
+        uint32_t s[2][64];
+        ht::tmem_ld(t_s, s[0]);
+        ht::tmem_ld(t_s + 64, s[1]);
+        if (words || k0 + HT_KEYS > jlim || (self >= k0 && self < k0 + HT_KEYS)) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t bits = 0xffffffffu;
+            if (words) bits = (k0 >> 5) + x < p.bits_w ? __ldg(words + (k0 >> 5) + x) : 0u;
+            const uint32_t seen = ht::key_word(k0 + 32 * x, jlim, self, bits);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((seen >> e) & 1u)) s[x >> 1][(x & 1) * 32 + e] = 0xff800000u;  // -inf
+          }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int x = 0; x < 64; x += 4)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            mx[2 * u] = max3f(mx[2 * u], __uint_as_float(s[u][x]), __uint_as_float(s[u][x + 1]));
+            mx[2 * u + 1] =
+                max3f(mx[2 * u + 1], __uint_as_float(s[u][x + 2]), __uint_as_float(s[u][x + 3]));
+          }
+        const float m2 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2;
+        float alpha = 1.f;
+        const bool move = m2 > mref + HT_MOVE || (mref == -INFINITY && m2 != -INFINITY);
+        if (move) {
+          alpha = tc::ex2_approx(mref - m2);
+          l *= alpha;
+          mref = m2;
+        }
+        // rescale O where any lane of the warp moved (PV of the last tile is
+        // complete: it was issued before the S that just arrived)
+        if (t > 0 && __any_sync(0xffffffffu, move)) {
+          for (int c = 0; c < p.d; c += 16) {
+            uint32_t o[16];
+            ht::tmem_ld(t_o + c, o);
+#pragma unroll
+            for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * alpha);
+            ht::tmem_st(t_o + c, o);
+          }
+        }
+        const float mb = mref == -INFINITY ? 0.f : -mref;
+        const uint64_t cc = pack2(c2, c2), mm = pack2(mb, mb);
+        float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float2 y = unpack2(ffma2(
+                pack2(__uint_as_float(s[x][2 * e]), __uint_as_float(s[x][2 * e + 1])), cc, mm));
+            const float a = tc::ex2_approx(y.x), b = tc::ex2_approx(y.y);
+            l4[(e & 1) * 2] += a;
+            l4[(e & 1) * 2 + 1] += b;
+            pk[e] = tc::pack_bf16x2(a, b);
+          }
+          ht::tmem_st(t_s + x * 32, pk);
+        }
+        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        if (len < p.Nk && k0 + HT_KEYS > len) {
+          // keys beyond the length may hold anything: their weights are zero,
+          // their V rows become zero too
+          const uint32_t s_ = (kc0 + t) % NS;
+          if (!ws::wait(&sh.vfull[s_], ((kc0 + t) / NS) & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const int r0 = len - k0;  // > 0: the tile has a visible key
+          const uint32_t v = kva + s_ * 2 * TILE + TILE;
+          for (int e = row; e < (128 - r0) * (DP / 8); e += 128) {
+            const int r = r0 + e / (DP / 8), c = e % (DP / 8);
+            st_shared_zero16(v + (uint32_t)((c >> 3) * 128 * 128 + r * 128 + (c & 7) * 16));
+          }
+          tc::fence_async_smem();
+        }
+        ht::st_wait();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ws::arrive(&sh.pfull[w]);
+      }
+      if (ok && nt > 0) {
+        ok = ws::wait(&sh.odone[w], oc & 1, abort_flag);
+        ++oc;
+        tc::fence_after_sync();
+      }
+      const bool nan = !ok;
+      const float inv = nan ? __int_as_float(0x7fffffff) : (l == 0.f ? 0.f : 1.f / l);
+      __nv_bfloat16* O = static_cast<__nv_bfloat16*>(p.o) +
+                         (((int64_t)it.b * p.Nq + i) * p.H + h) * p.d;
+      for (int c = 0; c < p.d; c += 16) {
+        uint32_t o[16];
+        if (nt > 0) {
+          ht::tmem_ld(t_o + c, o);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 16; ++u) o[u] = 0u;
+        }
+        if (i < p.Nq) {
+#pragma unroll
+          for (int u = 0; u < 16; u += 8) {
+            if (c + u >= p.d) break;
+            uint4 x;
+            x.x = tc::pack_bf16x2(__uint_as_float(o[u]) * inv, __uint_as_float(o[u + 1]) * inv);
+            x.y = tc::pack_bf16x2(__uint_as_float(o[u + 2]) * inv, __uint_as_float(o[u + 3]) * inv);
+            x.z = tc::pack_bf16x2(__uint_as_float(o[u + 4]) * inv, __uint_as_float(o[u + 5]) * inv);
+            x.w = tc::pack_bf16x2(__uint_as_float(o[u + 6]) * inv, __uint_as_float(o[u + 7]) * inv);
+            *reinterpret_cast<uint4*>(O + c + u) = x;
+          }
+        }
+      }
+      tc::fence_before_sync();
+      if (p.lse && i < p.Nq)
+        p.lse[((int64_t)it.b * p.H + h) * p.Nq + i] =
+            nan ? inv : (l == 0.f ? -INFINITY : (mref + log2f(l)) * HT_LN2);
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == HT_MMA_WARP) tc::tmem_dealloc(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------
+// tensor maps and launch
+// ---------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encode_fn() {
+  static const EncodeTiledFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return static_cast<EncodeTiledFn>(nullptr);
+    return reinterpret_cast<EncodeTiledFn>(f);
+  }();
+  return fn;
+}
+
+bool head_tensor_map(CUtensorMap* map, const void* ptr, const HeadStrides& s, int B, int N, int h,
+                     int d) {
+  const EncodeTiledFn fn = encode_fn();
+  if (!fn || (uintptr_t)ptr % 16) return false;
+  const cuuint64_t size[4] = {(cuuint64_t)d, (cuuint64_t)h, (cuuint64_t)N, (cuuint64_t)B};
+  const int64_t st[3] = {s.h, s.n, s.b};
+  cuuint64_t bytes[3];
+  for (int i = 0; i < 3; ++i) {
+    // the stride of a dimension of one is never used
+    const int64_t e = size[i + 1] == 1 ? 8 : st[i];
+    if (e <= 0 || e % 8 || e * 2 >= ((int64_t)1 << 40)) return false;
+    bytes[i] = (cuuint64_t)(e * 2);
+  }
+  const cuuint32_t box[4] = {64, 1, ht::BOX_ROWS, 1}, one[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), size, bytes, box,
+            one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DP>
+static cudaError_t fwd_tc_go(const CUtensorMap* m, const HeadAttnParams& p, const HtGrid& gr,
+                             int grid, cudaStream_t s) {
+  const void* fn = reinterpret_cast<const void*>(&head_fwd_tc_kernel<DP>);
+  const cudaError_t e = raise_smem_limit(fn, HtPlan<DP>::SMEM);
+  if (e != cudaSuccess) return e;
+  head_fwd_tc_kernel<DP><<<grid, HT_THREADS, HtPlan<DP>::SMEM, s>>>(m[0], m[1], m[2], p, gr);
+  return cudaGetLastError();
+}
+
+int head_sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;
+  return n;
+}
+
+// bf16 rows on the 16-byte grid with at least 128 queries; *done says whether
+// the call was taken.
+cudaError_t launch_head_fwd_tc(const HeadAttnParams& p, cudaStream_t s, bool* done) {
+  *done = false;
+  if (!p.vec || p.splits > 1 || p.Nq < 128 || p.Nk < 1) return cudaSuccess;
+  HtGrid gr;
+  gr.nqt = cdiv(p.Nq, 128);
+  const int64_t pairs = ((int64_t)gr.nqt * p.G + 1) / 2;
+  const int64_t items = pairs * p.B * p.Hk;
+  if (items > (1 << 30)) return cudaSuccess;
+  CUtensorMap m[3];
+  if (!head_tensor_map(&m[0], p.q, p.sq, p.B, p.Nq, p.H, p.d) ||
+      !head_tensor_map(&m[1], p.k, p.sk, p.B, p.Nk, p.Hk, p.d) ||
+      !head_tensor_map(&m[2], p.v, p.sv, p.B, p.Nk, p.Hk, p.d))
+    return cudaSuccess;
+  const int sms = head_sm_count();
+  gr.pairs = (int)pairs;
+  gr.items = (int)items;
+  gr.pair_major = p.peers == PEERS_PAST && p.B * p.Hk <= sms;
+  const int grid = items < sms ? (int)items : sms;
+  *done = true;
+  return p.d <= 64 ? fwd_tc_go<64>(m, p, gr, grid, s) : fwd_tc_go<128>(m, p, gr, grid, s);
+}
+
+}  // namespace tarmac
