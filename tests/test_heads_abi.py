@@ -63,7 +63,7 @@ def test_attention_own_checks():
     so = _lib.lib()
     assert so.tarmac_head_attention_workspace(1, 1, 4096, 4, 2, 16) > 0
     assert so.tarmac_head_attention_workspace(512, 512, 512, 4, 2, 16) == 0
-    assert so.tarmac_head_attention_backward_workspace(2, 8, 4) == 2 * 2 * 8 * 4 * 4
+    assert so.tarmac_head_attention_backward_workspace(2, 8, 4) >= 2 * 2 * 8 * 4 * 4
 
 
 def _rotate(**kw):

@@ -392,22 +392,21 @@ __global__ void __launch_bounds__(256) head_join_kernel(HeadAttnParams p) {
 // ---------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------
-// Row statistics: base-2 lse (+inf for a row that saw nothing, which makes
-// its weights exp2(s - inf) = 0) and D = dout . out. A group of 8 lanes per
-// row.
+// Row statistics, [2][B, H, nqp] with nqp = Nq rounded up to 64: base-2 lse
+// (+inf for a row that saw nothing and for the rows of padding, which makes
+// their weights exp2(s - inf) = 0) and D = dout . out (0 for padding). A group
+// of 8 lanes per row.
 template <typename T>
-__global__ void __launch_bounds__(256) head_delta_kernel(HeadAttnParams p) {
-  const int64_t total = (int64_t)p.B * p.Nq * p.H;
+__global__ void __launch_bounds__(256) head_delta_kernel(HeadAttnParams p, int nqp) {
+  const int64_t total = (int64_t)p.B * nqp * p.H;
   const int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
   const int sub = threadIdx.x & 7;
   float s = 0.f;
-  int64_t srow = 0;
-  if (row < total) {
-    const int h = (int)(row % p.H);
-    const int64_t bi = row / p.H;
-    const int i = (int)(bi % p.Nq);
-    const int64_t b = bi / p.Nq;
-    srow = (b * p.H + h) * p.Nq + i;
+  const int h = (int)(row % p.H);
+  const int64_t bi = row / p.H;
+  const int i = (int)(bi % nqp);
+  const int64_t b = bi / nqp;
+  if (row < total && i < p.Nq) {
     const T* o = static_cast<const T*>(p.o) + b * p.so.b + i * p.so.n + h * p.so.h;
     const T* g = static_cast<const T*>(p.g) + b * p.sg.b + i * p.sg.n + h * p.sg.h;
     if (p.vec) {
@@ -427,7 +426,8 @@ __global__ void __launch_bounds__(256) head_delta_kernel(HeadAttnParams p) {
 #pragma unroll
   for (int x = 4; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
   if (row < total && sub == 0) {
-    const float lse = p.lse[srow];
+    const float lse = i < p.Nq ? p.lse[(b * p.H + h) * p.Nq + i] : -INFINITY;
+    const int64_t srow = (b * p.H + h) * nqp + i;
     p.delta[srow] = lse == -INFINITY ? INFINITY : lse * HA_LOG2E;
     p.delta[total + srow] = s;
   }
@@ -489,7 +489,8 @@ __global__ void __launch_bounds__(HA_THREADS) head_dq_kernel(HeadAttnParams p) {
   float lse2[2], delta[2];
   const uint32_t* words[2];
   int64_t orow[2];
-  const int64_t total = (int64_t)p.B * p.Nq * p.H;
+  const int nqp = head_padded_rows(p.Nq);
+  const int64_t total = (int64_t)p.B * nqp * p.H;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int rr = warp * 16 + (lane >> 2) + 8 * u;
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(HA_THREADS) head_dq_kernel(HeadAttnParams p) {
     jlim[u] = p.peers == PEERS_PAST ? (int)max((int64_t)0, min((int64_t)kend, pos + 1)) : kend;
     self[u] = p.peers == PEERS_OTHERS && pos >= 0 && pos < p.Nk ? (int)pos : -1;
     words[u] = p.bits ? p.bits + w.b * p.bits_b + (int64_t)i * p.bits_w : nullptr;
-    const int64_t srow = ((int64_t)w.b * p.H + h) * p.Nq + i;
+    const int64_t srow = ((int64_t)w.b * p.H + h) * nqp + i;
     lse2[u] = p.delta[srow];
     delta[u] = p.delta[total + srow];
     orow[u] = rr < nrows ? ((int64_t)w.b * p.Nq + i) * p.H + h : -1;
@@ -578,7 +579,8 @@ __global__ void __launch_bounds__(HA_THREADS) head_dkv_kernel(HeadAttnParams p) 
   const T* Gr = static_cast<const T*>(p.g) + w.b * p.sg.b + (int64_t)w.hk * p.G * p.sg.h;
   const T* K = static_cast<const T*>(p.k) + w.b * p.sk.b + w.hk * p.sk.h;
   const T* V = static_cast<const T*>(p.v) + w.b * p.sv.b + w.hk * p.sv.h;
-  const int64_t total = (int64_t)p.B * p.Nq * p.H;
+  const int nqp = head_padded_rows(p.Nq);
+  const int64_t total = (int64_t)p.B * nqp * p.H;
   auto load_rows = [&](int t) {
     const int q0 = rbeg + t * QT;
     T* sQ = ring + (t & 1) * 2 * QT * RS;
@@ -598,7 +600,7 @@ __global__ void __launch_bounds__(HA_THREADS) head_dkv_kernel(HeadAttnParams p) 
       s_word[st][0][x] = s_word[st][1][x] = 0xffffffffu;
       if (r < rows) {
         const int i = r / p.G, g = r - i * p.G;
-        const int64_t srow = ((int64_t)w.b * p.H + w.hk * p.G + g) * p.Nq + i;
+        const int64_t srow = ((int64_t)w.b * p.H + w.hk * p.G + g) * nqp + i;
         s_lse[st][x] = p.delta[srow];
         s_delta[st][x] = p.delta[total + srow];
         const int64_t pos = (int64_t)start + i;
@@ -798,13 +800,21 @@ static cudaError_t fwd_any(const HeadAttnParams& p, cudaStream_t s) {
   return go(std::integral_constant<int, 128>());
 }
 
+cudaError_t launch_head_bwd_tc(const HeadAttnParams& p, int64_t nqp, cudaStream_t s, bool* done);
+
 template <typename T>
 static cudaError_t bwd_any(const HeadAttnParams& p, cudaStream_t s) {
-  const int64_t rows = (int64_t)p.B * p.Nq * p.H;
+  const int nqp = head_padded_rows(p.Nq);
+  const int64_t rows = (int64_t)p.B * nqp * p.H;
   if ((rows + 31) / 32 > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  if (rows) head_delta_kernel<T><<<(unsigned)((rows + 31) / 32), 256, 0, s>>>(p);
+  if (rows) head_delta_kernel<T><<<(unsigned)((rows + 31) / 32), 256, 0, s>>>(p, nqp);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
+  if constexpr (sizeof(T) == 2) {
+    bool done;
+    e = launch_head_bwd_tc(p, nqp, s, &done);
+    if (done || e != cudaSuccess) return e;
+  }
   if (p.d <= 16) return bwd_go<T, 16>(p, s);
   if (p.d <= 32) return bwd_go<T, 32>(p, s);
   if (p.d <= 64) return bwd_go<T, 64>(p, s);

@@ -58,7 +58,10 @@ struct HeadAttnParams {
   int split_keys;             // keys of a part
   float* part_o;              // [splits, B, Nq, H, d]
   float* part_lse;            // [splits, B, H, Nq]
-  float* delta;               // backward: [2, B, H, Nq] base-2 lse, dout . out
+  float* delta;               // backward: row statistics (head_attn.cu)
 };
+
+// rows of the backward's statistics per head: whole 64-row tiles
+__host__ __device__ constexpr int head_padded_rows(int Nq) { return cdiv(Nq, 64) * 64; }
 
 }  // namespace tarmac

@@ -233,7 +233,7 @@ int tarmac_head_attention(const void* q, const void* k, const void* v, void* out
 }
 
 int64_t tarmac_head_attention_backward_workspace(int B, int Nq, int H) {
-  return B < 1 || Nq < 1 || H < 1 ? 0 : (int64_t)2 * B * Nq * H * 4;
+  return B < 1 || Nq < 1 || H < 1 ? 0 : (int64_t)2 * B * head_padded_rows(Nq) * H * 4;
 }
 
 int tarmac_head_attention_backward(const void* q, const void* k, const void* v, const void* out,

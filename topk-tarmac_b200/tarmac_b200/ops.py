@@ -604,6 +604,11 @@ def _attention_work(B, Nq, Nk, H, Hk, d) -> int:
     return _lib.lib().tarmac_head_attention_workspace(B, Nq, Nk, H, Hk, d)
 
 
+@functools.lru_cache(maxsize=1024)
+def _attention_backward_work(B, Nq, H) -> int:
+    return _lib.lib().tarmac_head_attention_backward_workspace(B, Nq, H)
+
+
 def head_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                    peers: str = "all", key_len: torch.Tensor | None = None,
                    q_start: torch.Tensor | None = None,
@@ -665,7 +670,8 @@ def head_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                          "of the queries")
     out, dout, lse = _unit_inner(out), _unit_inner(dout), lse.contiguous()
     dq, dk, dv = _empty_as(q), _empty_as(k), _empty_as(v)
-    work = torch.empty(2 * B * Nq * H, device=q.device, dtype=torch.float32)
+    work = torch.empty(_attention_backward_work(B, Nq, H), device=q.device,
+                       dtype=torch.uint8)
     with _on(q.device):
         _lib.call("tarmac_head_attention_backward", _ptr(q), _ptr(k), _ptr(v),
                   _ptr(out), _ptr(lse), _ptr(dout),
