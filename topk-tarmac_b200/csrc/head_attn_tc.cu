@@ -3,14 +3,15 @@
 //
 // A block owns two 128-row query tiles of one key head — two heads of the
 // same rows, or neighbouring tiles — that share every staged K and V tile of
-// 128 keys. Roles of its 10 warps:
-// * warps 0..3 and 4..7: one warpgroup per tile, a thread per row. It reads
-//   its row of S from TMEM, masks, runs the softmax in base 2, and writes P
-//   as bf16 over the columns S had. The reference maximum moves, and O is
+// 128 keys. Roles of its 18 warps:
+// * warps 0..7 and 8..15: two warpgroups per tile, two threads per row with 64
+//   of the 128 columns each. They read S from TMEM, mask, run the softmax in
+//   base 2 (row maxima meet in shared memory) and write P as bf16 over the
+//   columns of S that they own. The reference maximum moves, and O is
 //   rescaled, only when a score exceeds it by 2^8, which few tiles do.
-// * warp 8: one thread issues the TMA loads (Q once, K and V in a ring).
-// * warp 9: one thread issues the products, alternating the groups:
-//   S_g = Q_g K^T, then O_g += P_g V with P from TMEM. While one group runs
+// * warp 16: one thread issues the TMA loads (Q once, K and V in a ring).
+// * warp 17: one thread issues the products, alternating the tiles:
+//   S_g = Q_g K^T, then O_g += P_g V with P from TMEM. While one tile is in
 //   its softmax the tensor core serves the other.
 // Bound: the special-function unit's 16 exponentials per clock per SM (1024
 // clocks for a 128 x 128 tile) against 256 d / 64 clocks for each of the two
@@ -25,8 +26,8 @@ namespace tarmac {
 
 namespace {
 
-constexpr int HT_THREADS = 320;
-constexpr int HT_TMA_WARP = 8, HT_MMA_WARP = 9;
+constexpr int HT_THREADS = 576;
+constexpr int HT_TMA_WARP = 16, HT_MMA_WARP = 17;
 constexpr int HT_KEYS = 128;
 constexpr float HT_LOG2E = 1.4426950408889634f;
 constexpr float HT_LN2 = 0.6931471805599453f;
@@ -44,6 +45,8 @@ struct HtShared {
   uint64_t qfull, qempty, kfull[NS], vfull[NS], empty[NS], sfull[2], pfull[2], odone[2];
   uint32_t tmem;
   int abort_flag;
+  float top[2][2][2][128];  // row maxima: tile, step parity, group, row
+  float sum[2][2][128];     // row sums: tile, group, row
 };
 
 struct HtItem {
@@ -97,10 +100,11 @@ __device__ __forceinline__ int ht_next(int k) {
   return k * g + ((k & 1) ? g - 1 - x : x);
 }
 
-template <int DP>
+template <int NKS>
 __global__ void __launch_bounds__(HT_THREADS, 1)
     head_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                        const __grid_constant__ CUtensorMap mv, HeadAttnParams p, HtGrid gr) {
+  constexpr int DP = ht::width(NKS);
   using Plan = HtPlan<DP>;
   constexpr int NS = Plan::NS, TILE = Plan::TILE;
   extern __shared__ unsigned char ht_raw[];
@@ -120,7 +124,7 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
     }
     for (int w = 0; w < 2; ++w) {
       tc::mbar_init(&sh.sfull[w], 1);
-      tc::mbar_init(&sh.pfull[w], 4);
+      tc::mbar_init(&sh.pfull[w], 8);
       tc::mbar_init(&sh.odone[w], 1);
     }
     sh.abort_flag = 0;
@@ -169,18 +173,15 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
     __syncwarp();
   } else if (warp == HT_MMA_WARP) {
     if (lane == 0) {
-      const int nks = cdiv(p.d, 16);
       const uint32_t id_s = tc::idesc_bf16(128, HT_KEYS, false, false);
-      const uint32_t id_o = tc::idesc_bf16(128, nks * 16, false, true);
+      const uint32_t id_o = tc::idesc_bf16(128, NKS * 16, false, true);
       const uint64_t dq0 = ht::desc128(qa, 16), dk0 = ht::desc128(kva, 16);
       const uint64_t dv0 = ht::desc128(kva + TILE, 128 * 128);
       uint32_t kc = 0, pc[2] = {0, 0};
       auto scores = [&](int w, int s) {
         const uint64_t dq = dq0 + (uint64_t)((w * TILE) >> 4);
         const uint64_t dk = dk0 + (uint64_t)((s * 2 * TILE) >> 4);
-        for (int ks = 0; ks < nks; ++ks)
-          tc::mma_bf16(tmem + w * 128, dq + ht::kstep(ks, 128), dk + ht::kstep(ks, 128), id_s,
-                       ks > 0);
+        ht::issue_scores<NKS, 128>(tmem + w * 128, dq, dk, id_s);
         tc::mma_commit(&sh.sfull[w]);
       };
       for (int k = 0;; ++k) {
@@ -208,9 +209,7 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
             if (!ws::wait(&sh.pfull[w], pc[w] & 1, abort_flag)) goto mma_done;
             ++pc[w];
             tc::fence_after_sync();
-            for (int ks = 0; ks < HT_KEYS / 16; ++ks)
-              ht::mma_ts(tmem + 256 + w * DP, tmem + w * 128 + ks * 8,
-                         dv + (uint64_t)((ks * 2048) >> 4), id_o, t > 0 || ks > 0);
+            ht::issue_aggregate<HT_KEYS, 64>(tmem + 256 + w * DP, tmem + w * 128, dv, id_o, t > 0);
             if (t + 1 < it.nt[w])
               scores(w, s1);
             else
@@ -228,13 +227,19 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
     __syncwarp();
   } else {
     // ---------------- softmax groups ----------------
-    const int w = warp >> 2, row = threadIdx.x & 127;
+    // tile w of the item, columns [64 half, 64 half + 64) of its key tiles
+    const int w = warp >> 3, half = (warp >> 2) & 1, row = threadIdx.x & 127;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + w * 128 + lane_off, t_o = tmem + 256 + w * DP + lane_off;
+    const uint32_t t_s = tmem + w * 128 + half * 64 + lane_off;
+    const uint32_t t_o = tmem + 256 + w * DP + half * (DP / 2) + lane_off;
+    const int c_lo = half * (DP / 2), c_n = max(0, min(DP / 2, p.d - c_lo));  // columns of O
     const float c2 = p.scale * HT_LOG2E;
+    auto pair_sync = [&] { asm volatile("bar.sync %0, 256;" ::"r"(1 + w) : "memory"); };
     uint32_t kc = 0, sc = 0, oc = 0;
     bool ok = true;
-    for (int k = 0; ok; ++k) {
+    // a group that gave up keeps meeting its partner: it skips the bounded
+    // waits, never the barrier
+    for (int k = 0;; ++k) {
       const int item = ht_next(k);
       if (item >= gr.items) break;
       const HtItem it = ht_item(p, gr, item);
@@ -252,39 +257,39 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
       const uint32_t* words =
           p.bits ? p.bits + it.b * p.bits_b + (int64_t)min(i, p.Nq - 1) * p.bits_w : nullptr;
       float mref = -INFINITY;  // reference maximum in exponent units
-      float l = 0.f;
+      float l = 0.f;           // this group's part of the sum
       for (int t = 0; t < nt; ++t) {
-        const int k0 = t * HT_KEYS;
-        if (!ws::wait(&sh.sfull[w], sc & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
-        ++sc;
-        tc::fence_after_sync();
-        uint32_t s[2][64];
-        ht::tmem_ld(t_s, s[0]);
-        ht::tmem_ld(t_s + 64, s[1]);
-        if (words || k0 + HT_KEYS > jlim || (self >= k0 && self < k0 + HT_KEYS)) {
+        const int k0 = t * HT_KEYS + half * 64;
+        const bool edge = words || k0 + 64 > jlim || (self >= k0 && self < k0 + 64);
+        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+        if (edge) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
+          for (int x = 0; x < 2; ++x) {
             uint32_t bits = 0xffffffffu;
             if (words) bits = (k0 >> 5) + x < p.bits_w ? __ldg(words + (k0 >> 5) + x) : 0u;
-            const uint32_t seen = ht::key_word(k0 + 32 * x, jlim, self, bits);
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((seen >> e) & 1u)) s[x >> 1][(x & 1) * 32 + e] = 0xff800000u;  // -inf
+            seen[x] = ht::key_word(k0 + 32 * x, jlim, self, bits);
           }
+        }
+        if (ok) ok = ht::warp_wait(&sh.sfull[w], sc & 1, abort_flag);
+        ++sc;
+        tc::fence_after_sync();
+        uint32_t s[64];
+        ht::tmem_ld(t_s, s);
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (!((seen[e >> 5] >> (e & 31)) & 1u)) s[e] = 0xff800000u;  // -inf
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int x = 0; x < 64; x += 4)
+        for (int x = 0; x < 64; x += 8)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            mx[2 * u] = max3f(mx[2 * u], __uint_as_float(s[u][x]), __uint_as_float(s[u][x + 1]));
-            mx[2 * u + 1] =
-                max3f(mx[2 * u + 1], __uint_as_float(s[u][x + 2]), __uint_as_float(s[u][x + 3]));
-          }
-        const float m2 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2;
+          for (int u = 0; u < 4; ++u)
+            mx[u] = max3f(mx[u], __uint_as_float(s[x + 2 * u]), __uint_as_float(s[x + 2 * u + 1]));
+        const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        sh.top[w][t & 1][half][row] = mine;
+        pair_sync();
+        const float m2 = fmaxf(mine, sh.top[w][t & 1][half ^ 1][row]) * c2;
         float alpha = 1.f;
         const bool move = m2 > mref + HT_MOVE || (mref == -INFINITY && m2 != -INFINITY);
         if (move) {
@@ -295,7 +300,7 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
         // rescale O where any lane of the warp moved (PV of the last tile is
         // complete: it was issued before the S that just arrived)
         if (t > 0 && __any_sync(0xffffffffu, move)) {
-          for (int c = 0; c < p.d; c += 16) {
+          for (int c = 0; c < c_n; c += 16) {
             uint32_t o[16];
             ht::tmem_ld(t_o + c, o);
 #pragma unroll
@@ -306,32 +311,27 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
         const float mb = mref == -INFINITY ? 0.f : -mref;
         const uint64_t cc = pack2(c2, c2), mm = pack2(mb, mb);
         float l4[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t pk[32];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float2 y = unpack2(ffma2(
-                pack2(__uint_as_float(s[x][2 * e]), __uint_as_float(s[x][2 * e + 1])), cc, mm));
-            const float a = tc::ex2_approx(y.x), b = tc::ex2_approx(y.y);
-            l4[(e & 1) * 2] += a;
-            l4[(e & 1) * 2 + 1] += b;
-            pk[e] = tc::pack_bf16x2(a, b);
-          }
-          ht::tmem_st(t_s + x * 32, pk);
+        for (int e = 0; e < 32; ++e) {
+          const float2 y = unpack2(
+              ffma2(pack2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), cc, mm));
+          const float a = tc::ex2_approx(y.x), b = tc::ex2_approx(y.y);
+          l4[(e & 1) * 2] += a;
+          l4[(e & 1) * 2 + 1] += b;
+          pk[e] = tc::pack_bf16x2(a, b);
         }
+        ht::tmem_st(t_s, pk);
         l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-        if (len < p.Nk && k0 + HT_KEYS > len) {
+        const int kt = t * HT_KEYS;
+        if (len < p.Nk && kt + HT_KEYS > len) {
           // keys beyond the length may hold anything: their weights are zero,
           // their V rows become zero too
           const uint32_t s_ = (kc0 + t) % NS;
-          if (!ws::wait(&sh.vfull[s_], ((kc0 + t) / NS) & 1, abort_flag)) {
-            ok = false;
-            break;
-          }
-          const int r0 = len - k0;  // > 0: the tile has a visible key
+          if (ok) ok = ht::warp_wait(&sh.vfull[s_], ((kc0 + t) / NS) & 1, abort_flag);
+          const int r0 = len - kt;  // > 0: the tile has a visible key
           const uint32_t v = kva + s_ * 2 * TILE + TILE;
-          for (int e = row; e < (128 - r0) * (DP / 8); e += 128) {
+          for (int e = half * 128 + row; e < (128 - r0) * (DP / 8); e += 256) {
             const int r = r0 + e / (DP / 8), c = e % (DP / 8);
             st_shared_zero16(v + (uint32_t)((c >> 3) * 128 * 128 + r * 128 + (c & 7) * 16));
           }
@@ -342,16 +342,18 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
         __syncwarp();
         if (lane == 0) ws::arrive(&sh.pfull[w]);
       }
-      if (ok && nt > 0) {
-        ok = ws::wait(&sh.odone[w], oc & 1, abort_flag);
+      if (nt > 0) {
+        if (ok) ok = ht::warp_wait(&sh.odone[w], oc & 1, abort_flag);
         ++oc;
         tc::fence_after_sync();
+        sh.sum[w][half][row] = l;
+        pair_sync();
+        l += sh.sum[w][half ^ 1][row];
       }
-      const bool nan = !ok;
-      const float inv = nan ? __int_as_float(0x7fffffff) : (l == 0.f ? 0.f : 1.f / l);
+      const float inv = !ok ? __int_as_float(0x7fffffff) : (l == 0.f ? 0.f : 1.f / l);
       __nv_bfloat16* O = static_cast<__nv_bfloat16*>(p.o) +
-                         (((int64_t)it.b * p.Nq + i) * p.H + h) * p.d;
-      for (int c = 0; c < p.d; c += 16) {
+                         (((int64_t)it.b * p.Nq + i) * p.H + h) * p.d + c_lo;
+      for (int c = 0; c < c_n; c += 16) {
         uint32_t o[16];
         if (nt > 0) {
           ht::tmem_ld(t_o + c, o);
@@ -362,7 +364,7 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
         if (i < p.Nq) {
 #pragma unroll
           for (int u = 0; u < 16; u += 8) {
-            if (c + u >= p.d) break;
+            if (c + u >= c_n) break;
             uint4 x;
             x.x = tc::pack_bf16x2(__uint_as_float(o[u]) * inv, __uint_as_float(o[u + 1]) * inv);
             x.y = tc::pack_bf16x2(__uint_as_float(o[u + 2]) * inv, __uint_as_float(o[u + 3]) * inv);
@@ -373,9 +375,9 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
         }
       }
       tc::fence_before_sync();
-      if (p.lse && i < p.Nq)
+      if (half == 0 && p.lse && i < p.Nq)
         p.lse[((int64_t)it.b * p.H + h) * p.Nq + i] =
-            nan ? inv : (l == 0.f ? -INFINITY : (mref + log2f(l)) * HT_LN2);
+            !ok ? inv : (l == 0.f ? -INFINITY : (mref + log2f(l)) * HT_LN2);
     }
   }
   tc::fence_before_sync();
@@ -424,13 +426,14 @@ bool head_tensor_map(CUtensorMap* map, const void* ptr, const HeadStrides& s, in
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DP>
+template <int NKS>
 static cudaError_t fwd_tc_go(const CUtensorMap* m, const HeadAttnParams& p, const HtGrid& gr,
                              int grid, cudaStream_t s) {
-  const void* fn = reinterpret_cast<const void*>(&head_fwd_tc_kernel<DP>);
-  const cudaError_t e = raise_smem_limit(fn, HtPlan<DP>::SMEM);
+  constexpr int SMEM = HtPlan<ht::width(NKS)>::SMEM;
+  const void* fn = reinterpret_cast<const void*>(&head_fwd_tc_kernel<NKS>);
+  const cudaError_t e = raise_smem_limit(fn, SMEM);
   if (e != cudaSuccess) return e;
-  head_fwd_tc_kernel<DP><<<grid, HT_THREADS, HtPlan<DP>::SMEM, s>>>(m[0], m[1], m[2], p, gr);
+  head_fwd_tc_kernel<NKS><<<grid, HT_THREADS, SMEM, s>>>(m[0], m[1], m[2], p, gr);
   return cudaGetLastError();
 }
 
@@ -463,7 +466,10 @@ cudaError_t launch_head_fwd_tc(const HeadAttnParams& p, cudaStream_t s, bool* do
   gr.pair_major = p.peers == PEERS_PAST && p.B * p.Hk <= sms;
   const int grid = items < sms ? (int)items : sms;
   *done = true;
-  return p.d <= 64 ? fwd_tc_go<64>(m, p, gr, grid, s) : fwd_tc_go<128>(m, p, gr, grid, s);
+  if (p.d <= 32) return fwd_tc_go<2>(m, p, gr, grid, s);
+  if (p.d <= 64) return fwd_tc_go<4>(m, p, gr, grid, s);
+  if (p.d <= 96) return fwd_tc_go<6>(m, p, gr, grid, s);
+  return fwd_tc_go<8>(m, p, gr, grid, s);
 }
 
 }  // namespace tarmac

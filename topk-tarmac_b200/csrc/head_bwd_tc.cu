@@ -11,15 +11,20 @@
 //   then dV += P^T dout and dK += dS^T Q. Shared heads add up in TMEM.
 // P and dS return to TMEM as bf16, over the columns S and dP had, and are the
 // A operands of the aggregates, so they never pass through shared memory.
-// Roles of the 10 warps: two warpgroups that take tiles in turn (while one
-// computes weights, the tensor core serves the other), one thread for the TMA
-// ring, one thread that issues products. TMEM: accumulators in columns
-// [0, 256), stage w (S, dP: 64 columns each) at 256 + 128 w.
+// Roles of the 18 warps: two pairs of warpgroups that take tiles in turn (while
+// one pair computes weights, the tensor core serves the other; each group of
+// a pair has 32 of the 64 columns), one thread for the TMA ring, one thread
+// that issues products. TMEM: accumulators in columns [0, 256), stage w (S,
+// dP: 64 columns each) at 256 + 128 w. P and dS of columns 32 c .. 32 c + 31
+// sit at column 32 c of their region, so that no group writes over what the
+// other has still to read.
 // Bound: 7 products for the 5 that the gradient needs (P is formed twice
 // rather than added up across blocks with atomics, so two calls give the same
 // bits) and two exponentials per pair.
 // Every wait is bounded; one that runs out ends all roles and the rows
 // concerned are written as NaN.
+#include <type_traits>
+
 #include "head_tc.cuh"
 
 namespace tarmac {
@@ -28,8 +33,8 @@ int head_sm_count();
 
 namespace {
 
-constexpr int HB_THREADS = 320;
-constexpr int HB_TMA_WARP = 8, HB_MMA_WARP = 9;
+constexpr int HB_THREADS = 576;
+constexpr int HB_TMA_WARP = 16, HB_MMA_WARP = 17;
 constexpr int HB_T = 64;  // streamed rows per tile
 constexpr float HB_LOG2E = 1.4426950408889634f;
 
@@ -121,11 +126,12 @@ __device__ __forceinline__ uint32_t warp_transpose(uint32_t x, int lane) {
 
 // DQ: own tiles Q and dout, streamed K and V; else own K and V, streamed Q
 // and dout. m[0..3]: tensor maps of q, k, v, dout.
-template <int DP, bool DQ>
+template <int NKS, bool DQ>
 __global__ void __launch_bounds__(HB_THREADS, 1)
     head_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                        const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mg,
                        HeadAttnParams p, HbGrid gr, int64_t nqp) {
+  constexpr int DP = ht::width(NKS);
   using Plan = HbPlan<DP>;
   constexpr int NS = Plan::NS, OWN = Plan::OWN, RUN = Plan::RUN, SLOT = 2 * RUN;
   extern __shared__ unsigned char hb_raw[];
@@ -145,10 +151,10 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
     }
     for (int w = 0; w < 2; ++w) {
       tc::mbar_init(&sh.sfull[w], 1);
-      tc::mbar_init(&sh.pfull[w], 4);
+      tc::mbar_init(&sh.pfull[w], 8);
     }
     tc::mbar_init(&sh.acc_full, 1);
-    tc::mbar_init(&sh.acc_empty, 8);
+    tc::mbar_init(&sh.acc_empty, 16);
     sh.abort_flag = 0;
     tc::mbar_init_fence();
   }
@@ -203,9 +209,8 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
     __syncwarp();
   } else if (warp == HB_MMA_WARP) {
     if (lane == 0) {
-      const int nks = cdiv(p.d, 16);
       const uint32_t id_s = tc::idesc_bf16(128, HB_T, false, false);
-      const uint32_t id_o = tc::idesc_bf16(128, nks * 16, false, true);
+      const uint32_t id_o = tc::idesc_bf16(128, NKS * 16, false, true);
       const uint64_t da0 = ht::desc128(own, 16), db0 = ht::desc128(ring, 16);
       const uint64_t dn0 = ht::desc128(ring, HB_T * 128);  // streamed tile, MN-major
       uint32_t c = 0, oc = 0, pc[2] = {0, 0};
@@ -216,11 +221,9 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
         tc::fence_after_sync();
         const uint64_t db = db0 + (uint64_t)((s * SLOT) >> 4);
         const uint32_t d0 = tmem + 256 + w * 128;
-        for (int ks = 0; ks < nks; ++ks)
-          tc::mma_bf16(d0, da0 + ht::kstep(ks, 128), db + ht::kstep(ks, HB_T), id_s, ks > 0);
-        const uint64_t da1 = da0 + (uint64_t)(OWN >> 4), db1 = db + (uint64_t)(RUN >> 4);
-        for (int ks = 0; ks < nks; ++ks)
-          tc::mma_bf16(d0 + 64, da1 + ht::kstep(ks, 128), db1 + ht::kstep(ks, HB_T), id_s, ks > 0);
+        ht::issue_scores<NKS, HB_T>(d0, da0, db, id_s);
+        ht::issue_scores<NKS, HB_T>(d0 + 64, da0 + (uint64_t)(OWN >> 4), db + (uint64_t)(RUN >> 4),
+                                    id_s);
         tc::mma_commit(&sh.sfull[w]);
         return true;
       };
@@ -244,14 +247,10 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
           tc::fence_after_sync();
           const uint64_t dn = dn0 + (uint64_t)((s * SLOT) >> 4);
           const uint32_t a0 = tmem + 256 + w * 128;
-          if constexpr (!DQ) {
-            for (int ks = 0; ks < HB_T / 16; ++ks)  // dV += P^T dout
-              ht::mma_ts(tmem, a0 + ks * 8, dn + (uint64_t)((RUN + ks * 2048) >> 4), id_o,
-                         t > 0 || ks > 0);
-          }
-          for (int ks = 0; ks < HB_T / 16; ++ks)  // dK += dS^T Q, or dQ += dS K
-            ht::mma_ts(tmem + (DQ ? 0 : DP), a0 + 64 + ks * 8, dn + (uint64_t)((ks * 2048) >> 4),
-                       id_o, t > 0 || ks > 0);
+          if constexpr (!DQ)  // dV += P^T dout
+            ht::issue_aggregate<HB_T, 32>(tmem, a0, dn + (uint64_t)(RUN >> 4), id_o, t > 0);
+          // dK += dS^T Q, or dQ += dS K
+          ht::issue_aggregate<HB_T, 32>(tmem + (DQ ? 0 : DP), a0 + 64, dn, id_o, t > 0);
           tc::mma_commit(&sh.empty[s]);
           if (t + 2 < it.n) {
             if (!issue(x + 2)) goto mma_done;
@@ -269,10 +268,12 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
     __syncwarp();
   } else {
     // ---------------- weights ----------------
-    const int w = warp >> 2, row = threadIdx.x & 127;
+    // group: stage w, columns [32 half, 32 half + 32) of its tiles
+    const int w = warp >> 3, half = (warp >> 2) & 1, row = threadIdx.x & 127;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + 256 + w * 128 + lane_off, t_dp = t_s + 64;
+    const uint32_t t_s = tmem + 256 + w * 128 + half * 32 + lane_off, t_dp = t_s + 64;
     const float c2 = p.scale * HB_LOG2E;
+    const uint64_t cc2 = pack2(c2, c2);
     uint32_t c = 0, sc = 0, ac = 0;
     bool ok = true;
     for (int k = 0; ok; ++k) {
@@ -297,92 +298,85 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
       }
       // keys: the query (as an index) that stands at this key's position
       const int64_t twin = (int64_t)own_row - it.start;
+      int tt = it.t0;  // streamed tile inside its head
       for (int t = 0; t < it.n; ++t) {
         const uint32_t x = c + t;
+        const int x0 = tt * HB_T + half * 32;  // first column of this group
+        if (++tt == it.t0 + it.nper) tt = it.t0;
         if ((int)(x & 1) != w) continue;
         const int s = x % NS;
-        const int x0 = (it.t0 + (DQ ? t : t % it.nper)) * HB_T;  // first streamed row
-        if (!ws::wait(&sh.sfull[w], sc & 1, abort_flag)) {
+        uint32_t seen = 0xffffffffu;
+        bool edge;
+        if constexpr (DQ) {
+          edge = words || x0 + 32 > jlim || (self >= x0 && self < x0 + 32);
+          if (edge) {
+            uint32_t bits = 0xffffffffu;
+            if (words) bits = (x0 >> 5) < p.bits_w ? __ldg(words + (x0 >> 5)) : 0u;
+            seen = ht::key_word(x0, jlim, self, bits);
+          }
+        } else {
+          const int64_t e = twin - x0;  // column of the twin
+          edge = p.bits || (p.peers == PEERS_PAST ? e > 0
+                                                  : p.peers == PEERS_OTHERS && e >= 0 && e < 32);
+          if (p.bits) {
+            const int kw = (it.x0 >> 5) + (warp & 3), i = x0 + lane;
+            uint32_t bits = 0u;
+            if (i < p.Nq && kw < p.bits_w)
+              bits = __ldg(p.bits + it.b * p.bits_b + (int64_t)i * p.bits_w + kw);
+            seen = warp_transpose(bits, lane);
+          }
+          if (p.peers == PEERS_PAST)
+            seen &= e <= 0 ? 0xffffffffu : (e >= 32 ? 0u : 0xffffffffu << e);
+          else if (p.peers == PEERS_OTHERS && e >= 0 && e < 32)
+            seen &= ~(1u << e);
+          // the statistics came with the tile
+          if (!ht::warp_wait(&sh.full[s], (x / NS) & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+        }
+        if (!ht::warp_wait(&sh.sfull[w], sc & 1, abort_flag)) {
           ok = false;
           break;
         }
         ++sc;
         tc::fence_after_sync();
-        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-        bool edge;
-        if constexpr (DQ) {
-          edge = words || x0 + HB_T > jlim || (self >= x0 && self < x0 + HB_T);
-          if (edge) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              uint32_t bits = 0xffffffffu;
-              if (words) bits = (x0 >> 5) + u < p.bits_w ? __ldg(words + (x0 >> 5) + u) : 0u;
-              seen[u] = ht::key_word(x0 + 32 * u, jlim, self, bits);
-            }
-          }
-        } else {
-          // the statistics came with the tile
-          if (!ws::wait(&sh.full[s], (x / NS) & 1, abort_flag)) {
-            ok = false;
-            break;
-          }
-          const int64_t e = twin - x0;  // column of the twin
-          edge = p.bits || (p.peers == PEERS_PAST ? e > 0
-                                                  : p.peers == PEERS_OTHERS && e >= 0 && e < HB_T);
-          if (p.bits) {
-            const int kw = (it.x0 >> 5) + (warp & 3);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int i = x0 + 32 * u + lane;
-              uint32_t bits = 0u;
-              if (i < p.Nq && kw < p.bits_w)
-                bits = __ldg(p.bits + it.b * p.bits_b + (int64_t)i * p.bits_w + kw);
-              seen[u] = warp_transpose(bits, lane);
-            }
-          }
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int64_t eu = e - 32 * u;
-            if (p.peers == PEERS_PAST)
-              seen[u] &= eu <= 0 ? 0xffffffffu : (eu >= 32 ? 0u : 0xffffffffu << eu);
-            else if (p.peers == PEERS_OTHERS && eu >= 0 && eu < 32)
-              seen[u] &= ~(1u << eu);
-          }
-        }
-        const float* st = stats_ptr + s * (Plan::STATS / 4);
-        uint32_t sv[64];
+        const float* st = stats_ptr + s * (Plan::STATS / 4) + half * 32;
+        uint32_t sv[32];
         ht::tmem_ld(t_s, sv);
 #pragma unroll
-        for (int e = 0; e < 64; e += 4) {
-          float ls[4] = {lse2, lse2, lse2, lse2};
+        for (int e = 0; e < 32; e += 4) {
+          uint64_t l0 = pack2(-lse2, -lse2), l1 = l0;
           if constexpr (!DQ) {
             const float4 q = *reinterpret_cast<const float4*>(st + e);
-            ls[0] = q.x;
-            ls[1] = q.y;
-            ls[2] = q.z;
-            ls[3] = q.w;
+            l0 = pack2(-q.x, -q.y);
+            l1 = pack2(-q.z, -q.w);
           }
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            sv[e + u] = __float_as_uint(
-                tc::ex2_approx(fmaf(__uint_as_float(sv[e + u]), c2, -ls[u])));
+          const float2 y0 = unpack2(
+              ffma2(pack2(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), cc2, l0));
+          const float2 y1 = unpack2(
+              ffma2(pack2(__uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3])), cc2, l1));
+          sv[e] = __float_as_uint(tc::ex2_approx(y0.x));
+          sv[e + 1] = __float_as_uint(tc::ex2_approx(y0.y));
+          sv[e + 2] = __float_as_uint(tc::ex2_approx(y1.x));
+          sv[e + 3] = __float_as_uint(tc::ex2_approx(y1.y));
         }
         if (edge) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (!((seen[e >> 5] >> (e & 31)) & 1u)) sv[e] = 0u;
-        }
-        if constexpr (!DQ) {
-          uint32_t pk[32];
-#pragma unroll
           for (int e = 0; e < 32; ++e)
+            if (!((seen >> e) & 1u)) sv[e] = 0u;
+        }
+        uint32_t pk[16];
+        if constexpr (!DQ) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
             pk[e] = tc::pack_bf16x2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1]));
           ht::tmem_st(t_s, pk);
         }
-        uint32_t dv[64], pk[32];
+        uint32_t dv[32];
         ht::tmem_ld(t_dp, dv);
 #pragma unroll
-        for (int e = 0; e < 64; e += 4) {
+        for (int e = 0; e < 32; e += 4) {
           float de[4] = {delta, delta, delta, delta};
           if constexpr (!DQ) {
             const float4 q = *reinterpret_cast<const float4*>(st + HB_T + e);
@@ -398,23 +392,24 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
           if (edge) {  // a masked pair's dP may be anything
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-              if (!((seen[(e + u) >> 5] >> ((e + u) & 31)) & 1u)) y[u] = 0.f;
+              if (!((seen >> (e + u)) & 1u)) y[u] = 0.f;
           }
           pk[e / 2] = tc::pack_bf16x2(y[0], y[1]);
           pk[e / 2 + 1] = tc::pack_bf16x2(y[2], y[3]);
         }
         ht::tmem_st(t_dp, pk);
         if constexpr (DQ) {
-          if (it.len < p.Nk && x0 + HB_T > it.len) {
+          const int k0 = x0 - half * 32;
+          if (it.len < p.Nk && k0 + HB_T > it.len) {
             // K rows beyond the length may hold anything: dS is zero there,
             // the rows become zero too (S has been formed)
-            if (!ws::wait(&sh.full[s], (x / NS) & 1, abort_flag)) {
+            if (!ht::warp_wait(&sh.full[s], (x / NS) & 1, abort_flag)) {
               ok = false;
               break;
             }
-            const int r0 = it.len - x0;
+            const int r0 = it.len - k0;
             const uint32_t kt = ring + s * SLOT;
-            for (int e = row; e < (HB_T - r0) * (DP / 8); e += 128) {
+            for (int e = half * 128 + row; e < (HB_T - r0) * (DP / 8); e += 256) {
               const int r = r0 + e / (DP / 8), cc = e % (DP / 8);
               st_shared_zero16(kt + (uint32_t)((cc >> 3) * HB_T * 128 + r * 128 + (cc & 7) * 16));
             }
@@ -428,18 +423,20 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
       }
       c += (uint32_t)it.n;
       if (ok && it.n > 0) {
-        ok = ws::wait(&sh.acc_full, ac & 1, abort_flag);
+        ok = ht::warp_wait(&sh.acc_full, ac & 1, abort_flag);
         ++ac;
         tc::fence_after_sync();
       }
-      // dq: each group stores half of the columns; dk, dv: group 0 dv, 1 dk
+      // dq: each group stores a quarter of the columns; dk, dv: groups 0 and
+      // 1 the halves of dv, 2 and 3 those of dk
       const int own_n = DQ ? p.Nq : p.Nk, heads = DQ ? p.H : p.Hk;
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(DQ ? p.dq : (w ? p.dk : p.dv)) +
                            (((int64_t)it.b * own_n + own_row) * heads + it.h) * p.d;
       float f = DQ || w ? p.scale : 1.f;
       if (!ok) f = __int_as_float(0x7fffffff);
       const bool zero = it.n == 0 || (!DQ && own_row >= it.len);
-      const int c0 = DQ ? w * (DP / 2) : 0, c1 = DQ ? c0 + DP / 2 : DP;
+      const int c0 = DQ ? (2 * w + half) * (DP / 4) : half * (DP / 2);
+      const int c1 = c0 + (DQ ? DP / 4 : DP / 2);
       const uint32_t t_acc = tmem + lane_off + (DQ ? 0 : (w ? DP : 0));
       for (int cc = c0; cc < c1 && cc < p.d; cc += 16) {
         uint32_t o[16];
@@ -471,7 +468,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
   if (warp == HB_MMA_WARP) tc::tmem_dealloc(tmem, 512);
 }
 
-template <int DP, bool DQ>
+template <int NKS, bool DQ>
 static cudaError_t bwd_tc_go(const CUtensorMap* m, const HeadAttnParams& p, int64_t nqp,
                              cudaStream_t s) {
   const int sms = head_sm_count();
@@ -481,11 +478,11 @@ static cudaError_t bwd_tc_go(const CUtensorMap* m, const HeadAttnParams& p, int6
   gr.items = (int)(bh * gr.tiles);
   gr.tile_major = p.peers == PEERS_PAST && bh <= sms;
   const int grid = gr.items < sms ? gr.items : sms;
-  const void* fn = reinterpret_cast<const void*>(&head_bwd_tc_kernel<DP, DQ>);
-  const cudaError_t e = raise_smem_limit(fn, HbPlan<DP>::SMEM);
+  constexpr int SMEM = HbPlan<ht::width(NKS)>::SMEM;
+  const void* fn = reinterpret_cast<const void*>(&head_bwd_tc_kernel<NKS, DQ>);
+  const cudaError_t e = raise_smem_limit(fn, SMEM);
   if (e != cudaSuccess) return e;
-  head_bwd_tc_kernel<DP, DQ><<<grid, HB_THREADS, HbPlan<DP>::SMEM, s>>>(m[0], m[1], m[2], m[3], p,
-                                                                       gr, nqp);
+  head_bwd_tc_kernel<NKS, DQ><<<grid, HB_THREADS, SMEM, s>>>(m[0], m[1], m[2], m[3], p, gr, nqp);
   return cudaGetLastError();
 }
 
@@ -504,13 +501,15 @@ cudaError_t launch_head_bwd_tc(const HeadAttnParams& p, int64_t nqp, cudaStream_
       !head_tensor_map(&m[3], p.g, p.sg, p.B, p.Nq, p.H, p.d))
     return cudaSuccess;
   *done = true;
-  cudaError_t e;
-  if (p.d <= 64) {
-    e = bwd_tc_go<64, false>(m, p, nqp, s);
-    return e != cudaSuccess ? e : bwd_tc_go<64, true>(m, p, nqp, s);
-  }
-  e = bwd_tc_go<128, false>(m, p, nqp, s);
-  return e != cudaSuccess ? e : bwd_tc_go<128, true>(m, p, nqp, s);
+  auto both = [&](auto nks) {
+    constexpr int NKS = decltype(nks)::value;
+    const cudaError_t e = bwd_tc_go<NKS, false>(m, p, nqp, s);
+    return e != cudaSuccess ? e : bwd_tc_go<NKS, true>(m, p, nqp, s);
+  };
+  if (p.d <= 32) return both(std::integral_constant<int, 2>());
+  if (p.d <= 64) return both(std::integral_constant<int, 4>());
+  if (p.d <= 96) return both(std::integral_constant<int, 6>());
+  return both(std::integral_constant<int, 8>());
 }
 
 }  // namespace tarmac

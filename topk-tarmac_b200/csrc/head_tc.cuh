@@ -2,6 +2,7 @@
 // (head_attn_tc.cu, head_bwd_tc.cu): TMA tiles of 64 columns in the 128-byte
 // swizzle, their matrix descriptors, TMEM transfers and row masks.
 //
+// Rows of d columns run as NKS = 2, 4, 6 or 8 steps of 16 columns, zero beyond d.
 // A tile is R rows of DP columns (64 or 128), held as DP / 64 halves of R rows
 // of 128 bytes; TMA writes it in boxes of 64 rows x 64 columns (8 KB), zero
 // beyond the tensor's rows and columns. The same bytes serve as an operand
@@ -17,6 +18,8 @@
 
 namespace tarmac {
 namespace ht {
+
+constexpr int width(int nks) { return nks <= 4 ? 64 : 128; }  // DP
 
 constexpr uint32_t BOX_ROWS = 64;
 constexpr uint32_t BOX_BYTES = 64 * 128;
@@ -76,6 +79,13 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
       : "memory");
 }
 
+// Bounded wait by a whole warp: all lanes take the same result, so the warp
+// stays together for its TMEM transfers.
+__device__ __forceinline__ bool warp_wait(uint64_t* mbar, uint32_t parity,
+                                          volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, ws::wait(mbar, parity, abort_flag));
+}
+
 __device__ __forceinline__ void st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -126,6 +136,27 @@ __device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_
       "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
       "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate));
+}
+
+// C[tmem_d] = A . B^T over NKS steps of 16 columns (A: 128 rows, B: RB rows,
+// both K-major). Straight-line: no product is issued under a condition.
+template <int NKS, int RB>
+__device__ __forceinline__ void issue_scores(uint32_t tmem_d, uint64_t da, uint64_t db,
+                                             uint32_t idesc) {
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks)
+    tc::mma_bf16(tmem_d, da + kstep(ks, 128), db + kstep(ks, RB), idesc, ks > 0);
+}
+// C[tmem_d] (+)= P[tmem_a] . B, contracting over the RB rows of B (MN-major).
+// P's columns come from groups of warps that own GC columns each: as bf16 they
+// take GC / 2 TMEM columns, at every GC-th column.
+template <int RB, int GC>
+__device__ __forceinline__ void issue_aggregate(uint32_t tmem_d, uint32_t tmem_a, uint64_t db,
+                                                uint32_t idesc, bool add) {
+#pragma unroll
+  for (int ks = 0; ks < RB / 16; ++ks)
+    mma_ts(tmem_d, tmem_a + (ks * 16 / GC) * GC + (ks * 16 % GC) / 2,
+           db + (uint64_t)((ks * 2048) >> 4), idesc, add || ks > 0);
 }
 
 // Keys of the 32-key word at key j0 that a row may see: below jlim, not self,
