@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(256) head_join_kernel(HeadAttnParams p) {
 // ---------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------
-// Row statistics, [2][B, H, nqp] with nqp = Nq rounded up to 64: base-2 lse
+// Row statistics, [2][B, H, nqp] with nqp = Nq rounded up to 128: base-2 lse
 // (+inf for a row that saw nothing and for the rows of padding, which makes
 // their weights exp2(s - inf) = 0) and D = dout . out (0 for padding). A group
 // of 8 lanes per row.

@@ -3,24 +3,28 @@
 // statistics come from head_delta_kernel.
 //
 // Two kernels of one shape, each forming S and dP again tile by tile:
-// * dq: a block owns 128 query rows (Q, dout staged once) and streams 64-key
+// * dq: a block owns 128 query rows (Q, dout staged once) and streams 128-key
 //   tiles of K and V: S = Q K^T, dP = dout V^T, dS = P (dP - D) in registers
-//   (a thread per query row), dQ += dS K.
-// * dk, dv: a block owns 128 keys of a key head and streams 64-row tiles of Q
+//   (rows are queries), dQ += dS K.
+// * dk, dv: a block owns 128 keys of a key head and streams 128-row tiles of Q
 //   and dout of all query heads that share it: S^T = K Q^T, dP^T = V dout^T,
-//   then dV += P^T dout and dK += dS^T Q. Shared heads add up in TMEM.
+//   dV += P^T dout, dK += dS^T Q. Shared heads add up in TMEM.
 // P and dS return to TMEM as bf16, over the columns S and dP had, and are the
 // A operands of the aggregates, so they never pass through shared memory.
-// Roles of the 18 warps: two pairs of warpgroups that take tiles in turn (while
-// one pair computes weights, the tensor core serves the other; each group of
-// a pair has 32 of the 64 columns), one thread for the TMA ring, one thread
-// that issues products. TMEM: accumulators in columns [0, 256), stage w (S,
-// dP: 64 columns each) at 256 + 128 w. P and dS of columns 32 c .. 32 c + 31
-// sit at column 32 c of their region, so that no group writes over what the
-// other has still to read.
+// Roles of the 18 warps: 16 form the weights of one tile together (a thread
+// has one row and 32 of the 128 columns), one thread feeds the TMA rings, one
+// issues products. The two halves of a tile's work overlap the products of the
+// other half: while P of tile t + 1 is formed the tensor core runs dK (or dQ)
+// of tile t and dP of t + 1; while dS of tile t is formed it runs dV of t and
+// S of t + 1 (dq: S is held twice and runs two tiles ahead).
+// P and dS of columns 32 c .. 32 c + 31 sit at column 32 c of their region, so
+// that no group of warps writes over what another has still to read.
+// TMEM columns: dk, dv: dV, dK in [0, 256), S at 256, dP at 384; dq: dQ in
+// [0, 128), S at 128 and 256, dP at 384.
 // Bound: 7 products for the 5 that the gradient needs (P is formed twice
 // rather than added up across blocks with atomics, so two calls give the same
-// bits) and two exponentials per pair.
+// bits) and two exponentials per pair, 1024 clocks of the special-function
+// unit per 128 x 128 tile against 256 d / 64 for a product.
 // Every wait is bounded; one that runs out ends all roles and the rows
 // concerned are written as NaN.
 #include <type_traits>
@@ -35,21 +39,24 @@ namespace {
 
 constexpr int HB_THREADS = 576;
 constexpr int HB_TMA_WARP = 16, HB_MMA_WARP = 17;
-constexpr int HB_T = 64;  // streamed rows per tile
+constexpr int HB_T = 128;  // streamed rows per tile
 constexpr float HB_LOG2E = 1.4426950408889634f;
 
-template <int DP>
+// Rings: X is what S contracts with and the last aggregate reads again (Q, or
+// K for dq), Y the other tensor (dout, or V for dq).
+template <int DP, bool DQ>
 struct HbPlan {
-  static constexpr int OWN = 128 * DP * 2;   // an owned tile
-  static constexpr int RUN = HB_T * DP * 2;  // a streamed tile
-  static constexpr int NS = DP == 64 ? 6 : 4;
-  static constexpr int STATS = 2 * HB_T * 4;  // lse2 and D of 64 rows
-  static constexpr int SMEM = 2 * OWN + NS * (2 * RUN + STATS) + 1024;
+  static constexpr int TILE = 128 * DP * 2;  // bytes of 128 rows
+  static constexpr int NX = DP == 64 || DQ ? 3 : 2;
+  static constexpr int NY = 2;
+  static constexpr int STATS = DQ ? 0 : 2 * HB_T * 4;  // lse2 and D of an X tile
+  static constexpr int SMEM = (2 + NX + NY) * TILE + NX * STATS + 1024;
 };
 
-template <int NS>
+template <int NX, int NY>
 struct HbShared {
-  uint64_t own_full, own_empty, full[NS], empty[NS], sfull[2], pfull[2], acc_full, acc_empty;
+  uint64_t own_full, own_empty, xfull[NX], xempty[NX], yfull[NY], yempty[NY];
+  uint64_t sfull[2], dpfull, pfull, dsfull, acc_full, acc_empty;
   uint32_t tmem;
   int abort_flag;
 };
@@ -132,12 +139,14 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
                        const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mg,
                        HeadAttnParams p, HbGrid gr, int64_t nqp) {
   constexpr int DP = ht::width(NKS);
-  using Plan = HbPlan<DP>;
-  constexpr int NS = Plan::NS, OWN = Plan::OWN, RUN = Plan::RUN, SLOT = 2 * RUN;
+  using Plan = HbPlan<DP, DQ>;
+  constexpr int NX = Plan::NX, NY = Plan::NY, TILE = Plan::TILE;
+  constexpr int NSB = DQ ? 2 : 1;                      // copies of S
+  constexpr uint32_t COL_S = DQ ? 128 : 256, COL_DP = 384;
   extern __shared__ unsigned char hb_raw[];
-  __shared__ HbShared<NS> sh;
+  __shared__ HbShared<NX, NY> sh;
   const uint32_t base = (tc::smem_addr(hb_raw) + 1023u) & ~1023u;
-  const uint32_t own = base, ring = base + 2 * OWN, stats = ring + NS * SLOT;
+  const uint32_t own = base, xr = base + 2 * TILE, yr = xr + NX * TILE, stats = yr + NY * TILE;
   const float* stats_ptr =
       reinterpret_cast<const float*>(hb_raw + (stats - tc::smem_addr(hb_raw)));
   volatile int* abort_flag = &sh.abort_flag;
@@ -145,14 +154,18 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
   if (threadIdx.x == 0) {
     tc::mbar_init(&sh.own_full, 1);
     tc::mbar_init(&sh.own_empty, 1);
-    for (int s = 0; s < NS; ++s) {
-      tc::mbar_init(&sh.full[s], 1);
-      tc::mbar_init(&sh.empty[s], 1);
+    for (int s = 0; s < NX; ++s) {
+      tc::mbar_init(&sh.xfull[s], 1);
+      tc::mbar_init(&sh.xempty[s], 1);
     }
-    for (int w = 0; w < 2; ++w) {
-      tc::mbar_init(&sh.sfull[w], 1);
-      tc::mbar_init(&sh.pfull[w], 8);
+    for (int s = 0; s < NY; ++s) {
+      tc::mbar_init(&sh.yfull[s], 1);
+      tc::mbar_init(&sh.yempty[s], 1);
     }
+    for (int s = 0; s < 2; ++s) tc::mbar_init(&sh.sfull[s], 1);
+    tc::mbar_init(&sh.dpfull, 1);
+    tc::mbar_init(&sh.pfull, 16);
+    tc::mbar_init(&sh.dsfull, 16);
     tc::mbar_init(&sh.acc_full, 1);
     tc::mbar_init(&sh.acc_empty, 16);
     sh.abort_flag = 0;
@@ -175,24 +188,27 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
         if (w.n == 0) continue;
         if (!ws::wait(&sh.own_empty, (oc & 1) ^ 1, abort_flag)) goto tma_done;
         ++oc;
-        ht::expect_tx(&sh.own_full, 2 * OWN);
+        ht::expect_tx(&sh.own_full, 2 * TILE);
         ht::tma_tile<DP, 128>(own, DQ ? &mq : &mk, &sh.own_full, w.h, w.x0, w.b);
-        ht::tma_tile<DP, 128>(own + OWN, DQ ? &mg : &mv, &sh.own_full, w.h, w.x0, w.b);
+        ht::tma_tile<DP, 128>(own + TILE, DQ ? &mg : &mv, &sh.own_full, w.h, w.x0, w.b);
         int g = 0, t = w.t0;
         for (int x = 0; x < w.n; ++x, ++c) {
-          const int s = c % NS;
-          if (!ws::wait(&sh.empty[s], ((c / NS) & 1) ^ 1, abort_flag)) goto tma_done;
-          const uint32_t slot = ring + s * SLOT;
-          ht::expect_tx(&sh.full[s], SLOT + (DQ ? 0 : Plan::STATS));
+          const int sx = c % NX, sy = c % NY;
           const int head = DQ ? w.hk : w.hk * p.G + g;
-          ht::tma_tile<DP, HB_T>(slot, DQ ? &mk : &mq, &sh.full[s], head, t * HB_T, w.b);
-          ht::tma_tile<DP, HB_T>(slot + RUN, DQ ? &mv : &mg, &sh.full[s], head, t * HB_T, w.b);
+          if (!ws::wait(&sh.xempty[sx], ((c / NX) & 1) ^ 1, abort_flag)) goto tma_done;
+          ht::expect_tx(&sh.xfull[sx], TILE + Plan::STATS);
+          ht::tma_tile<DP, HB_T>(xr + sx * TILE, DQ ? &mk : &mq, &sh.xfull[sx], head, t * HB_T,
+                                 w.b);
           if constexpr (!DQ) {
             const float* st = p.delta + ((int64_t)w.b * p.H + head) * nqp + t * HB_T;
-            ht::bulk_copy(stats + s * Plan::STATS, st, HB_T * 4, &sh.full[s]);
-            ht::bulk_copy(stats + s * Plan::STATS + HB_T * 4, st + stat_plane, HB_T * 4,
-                          &sh.full[s]);
+            ht::bulk_copy(stats + sx * Plan::STATS, st, HB_T * 4, &sh.xfull[sx]);
+            ht::bulk_copy(stats + sx * Plan::STATS + HB_T * 4, st + stat_plane, HB_T * 4,
+                          &sh.xfull[sx]);
           }
+          if (!ws::wait(&sh.yempty[sy], ((c / NY) & 1) ^ 1, abort_flag)) goto tma_done;
+          ht::expect_tx(&sh.yfull[sy], TILE);
+          ht::tma_tile<DP, HB_T>(yr + sy * TILE, DQ ? &mv : &mg, &sh.yfull[sy], head, t * HB_T,
+                                 w.b);
           if (++t == w.t0 + w.nper) {
             t = w.t0;
             ++g;
@@ -202,29 +218,40 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
     tma_done:
       if (*abort_flag) {  // the copies in flight land before the block ends
         if (oc) tc::mbar_wait(&sh.own_full, (oc - 1) & 1, 1u << 16);
-        for (uint32_t x = c > (uint32_t)NS ? c - NS : 0; x < c; ++x)
-          tc::mbar_wait(&sh.full[x % NS], (x / NS) & 1, 1u << 16);
+        for (uint32_t x = c > 3u ? c - 3 : 0; x <= c; ++x) {
+          tc::mbar_wait(&sh.xfull[x % NX], (x / NX) & 1, 1u << 16);
+          tc::mbar_wait(&sh.yfull[x % NY], (x / NY) & 1, 1u << 16);
+        }
       }
     }
     __syncwarp();
   } else if (warp == HB_MMA_WARP) {
     if (lane == 0) {
-      const uint32_t id_s = tc::idesc_bf16(128, HB_T, false, false);
-      const uint32_t id_o = tc::idesc_bf16(128, NKS * 16, false, true);
-      const uint64_t da0 = ht::desc128(own, 16), db0 = ht::desc128(ring, 16);
-      const uint64_t dn0 = ht::desc128(ring, HB_T * 128);  // streamed tile, MN-major
-      uint32_t c = 0, oc = 0, pc[2] = {0, 0};
+      constexpr uint32_t id_s = tc::idesc_bf16(128, HB_T, false, false);
+      constexpr uint32_t id_o = tc::idesc_bf16(128, NKS * 16, false, true);
+      const uint64_t da0 = ht::desc128(own, 16), dx0 = ht::desc128(xr, 16),
+                     dy0 = ht::desc128(yr, 16);
+      const uint64_t nx0 = ht::desc128(xr, HB_T * 128), ny0 = ht::desc128(yr, HB_T * 128);
+      uint32_t c = 0, oc = 0;
       // S and dP of streamed tile number x (counted over all items)
-      auto issue = [&](uint32_t x) {
-        const int s = x % NS, w = x & 1;
-        if (!ws::wait(&sh.full[s], (x / NS) & 1, abort_flag)) return false;
+      auto issue_s = [&](uint32_t x) {
+        const int s = x % NX;
+        if (!ws::wait(&sh.xfull[s], (x / NX) & 1, abort_flag)) return false;
         tc::fence_after_sync();
-        const uint64_t db = db0 + (uint64_t)((s * SLOT) >> 4);
-        const uint32_t d0 = tmem + 256 + w * 128;
-        ht::issue_scores<NKS, HB_T>(d0, da0, db, id_s);
-        ht::issue_scores<NKS, HB_T>(d0 + 64, da0 + (uint64_t)(OWN >> 4), db + (uint64_t)(RUN >> 4),
-                                    id_s);
-        tc::mma_commit(&sh.sfull[w]);
+        const int u = NSB == 2 ? (x & 1) : 0;
+        ht::issue_scores<NKS, HB_T>(tmem + COL_S + u * 128, da0,
+                                    dx0 + (uint64_t)((s * TILE) >> 4), id_s);
+        tc::mma_commit(&sh.sfull[u]);
+        return true;
+      };
+      auto issue_dp = [&](uint32_t x) {
+        const int s = x % NY;
+        if (!ws::wait(&sh.yfull[s], (x / NY) & 1, abort_flag)) return false;
+        tc::fence_after_sync();
+        ht::issue_scores<NKS, HB_T>(tmem + COL_DP, da0 + (uint64_t)(TILE >> 4),
+                                    dy0 + (uint64_t)((s * TILE) >> 4), id_s);
+        tc::mma_commit(&sh.dpfull);
+        if constexpr (DQ) tc::mma_commit(&sh.yempty[s]);  // V is read once
         return true;
       };
       for (int k = 0;; ++k) {
@@ -233,48 +260,54 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
         const HbItem it = hb_item<DQ>(p, gr, item);
         if (it.n == 0) continue;
         if (!ws::wait(&sh.own_full, oc & 1, abort_flag)) goto mma_done;
-        if (!issue(c)) goto mma_done;
-        if (it.n > 1 && !issue(c + 1)) goto mma_done;
-        if (it.n <= 2) tc::mma_commit(&sh.own_empty);
+        if (!issue_s(c) || !issue_dp(c)) goto mma_done;
+        if (DQ && it.n > 1 && !issue_s(c + 1)) goto mma_done;
+        if (it.n == 1) tc::mma_commit(&sh.own_empty);
         // the accumulators of the item before have been read
         if (!ws::wait(&sh.acc_empty, (oc & 1) ^ 1, abort_flag)) goto mma_done;
         ++oc;
         for (int t = 0; t < it.n; ++t) {
           const uint32_t x = c + t;
-          const int s = x % NS, w = x & 1;
-          if (!ws::wait(&sh.pfull[w], pc[w] & 1, abort_flag)) goto mma_done;
-          ++pc[w];
-          tc::fence_after_sync();
-          const uint64_t dn = dn0 + (uint64_t)((s * SLOT) >> 4);
-          const uint32_t a0 = tmem + 256 + w * 128;
-          if constexpr (!DQ)  // dV += P^T dout
-            ht::issue_aggregate<HB_T, 32>(tmem, a0, dn + (uint64_t)(RUN >> 4), id_o, t > 0);
-          // dK += dS^T Q, or dQ += dS K
-          ht::issue_aggregate<HB_T, 32>(tmem + (DQ ? 0 : DP), a0 + 64, dn, id_o, t > 0);
-          tc::mma_commit(&sh.empty[s]);
-          if (t + 2 < it.n) {
-            if (!issue(x + 2)) goto mma_done;
-            if (t + 3 == it.n) tc::mma_commit(&sh.own_empty);
+          const int sx = x % NX, sy = x % NY;
+          if constexpr (!DQ) {
+            if (!ws::wait(&sh.pfull, x & 1, abort_flag)) goto mma_done;
+            tc::fence_after_sync();
+            ht::issue_aggregate<HB_T, 32>(tmem, tmem + COL_S, ny0 + (uint64_t)((sy * TILE) >> 4),
+                                          id_o, t > 0);  // dV += P^T dout
+            tc::mma_commit(&sh.yempty[sy]);
+            if (t + 1 < it.n && !issue_s(x + 1)) goto mma_done;
           }
+          if (!ws::wait(&sh.dsfull, x & 1, abort_flag)) goto mma_done;
+          tc::fence_after_sync();
+          // dK += dS^T Q, or dQ += dS K
+          ht::issue_aggregate<HB_T, 32>(tmem + (DQ ? 0 : DP), tmem + COL_DP,
+                                        nx0 + (uint64_t)((sx * TILE) >> 4), id_o, t > 0);
+          tc::mma_commit(&sh.xempty[sx]);
+          if (t + 1 < it.n && !issue_dp(x + 1)) goto mma_done;
+          // the last S and dP are issued: the next item's own tiles may load
+          if (t + 2 == it.n) tc::mma_commit(&sh.own_empty);
+          if (DQ && t + 2 < it.n && !issue_s(x + 2)) goto mma_done;
         }
         tc::mma_commit(&sh.acc_full);
         c += (uint32_t)it.n;
       }
       // the last commits land before the block ends
-      for (uint32_t x = c > (uint32_t)NS ? c - NS : 0; x < c; ++x)
-        if (!ws::wait(&sh.empty[x % NS], (x / NS) & 1, abort_flag)) break;
+      for (uint32_t x = c > (uint32_t)NX ? c - NX : 0; x < c; ++x)
+        if (!ws::wait(&sh.xempty[x % NX], (x / NX) & 1, abort_flag)) break;
+      if (oc) ws::wait(&sh.own_empty, (oc - 1) & 1, abort_flag);
     mma_done:;
     }
     __syncwarp();
   } else {
     // ---------------- weights ----------------
-    // group: stage w, columns [32 half, 32 half + 32) of its tiles
-    const int w = warp >> 3, half = (warp >> 2) & 1, row = threadIdx.x & 127;
+    // columns [32 part, 32 part + 32) of each tile
+    const int part = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + 256 + w * 128 + half * 32 + lane_off, t_dp = t_s + 64;
+    const uint32_t t_s = tmem + COL_S + part * 32 + lane_off;
+    const uint32_t t_dp = tmem + COL_DP + part * 32 + lane_off;
     const float c2 = p.scale * HB_LOG2E;
     const uint64_t cc2 = pack2(c2, c2);
-    uint32_t c = 0, sc = 0, ac = 0;
+    uint32_t c = 0, ac = 0;
     bool ok = true;
     for (int k = 0; ok; ++k) {
       const int item = hb_next(k);
@@ -301,10 +334,9 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
       int tt = it.t0;  // streamed tile inside its head
       for (int t = 0; t < it.n; ++t) {
         const uint32_t x = c + t;
-        const int x0 = tt * HB_T + half * 32;  // first column of this group
+        const int x0 = tt * HB_T + part * 32;  // first column of this thread
         if (++tt == it.t0 + it.nper) tt = it.t0;
-        if ((int)(x & 1) != w) continue;
-        const int s = x % NS;
+        const int sx = x % NX;
         uint32_t seen = 0xffffffffu;
         bool edge;
         if constexpr (DQ) {
@@ -329,21 +361,19 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
             seen &= e <= 0 ? 0xffffffffu : (e >= 32 ? 0u : 0xffffffffu << e);
           else if (p.peers == PEERS_OTHERS && e >= 0 && e < 32)
             seen &= ~(1u << e);
-          // the statistics came with the tile
-          if (!ht::warp_wait(&sh.full[s], (x / NS) & 1, abort_flag)) {
-            ok = false;
-            break;
-          }
         }
-        if (!ht::warp_wait(&sh.sfull[w], sc & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
-        ++sc;
+        // dk, dv: the statistics came with the Q tile; dq: its K tile may
+        // have rows to clear
+        const bool tail = DQ && it.len < p.Nk && x0 - part * 32 + HB_T > it.len;
+        if (!DQ || tail) ok = ht::warp_wait(&sh.xfull[sx], (x / NX) & 1, abort_flag);
+        if (ok)
+          ok = ht::warp_wait(&sh.sfull[NSB == 2 ? (x & 1) : 0], (NSB == 2 ? x >> 1 : x) & 1,
+                             abort_flag);
+        if (!ok) break;
         tc::fence_after_sync();
-        const float* st = stats_ptr + s * (Plan::STATS / 4) + half * 32;
+        const float* st = stats_ptr + sx * (Plan::STATS / 4) + part * 32;
         uint32_t sv[32];
-        ht::tmem_ld(t_s, sv);
+        ht::tmem_ld(t_s + (NSB == 2 ? (x & 1) * 128 : 0), sv);
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           uint64_t l0 = pack2(-lse2, -lse2), l1 = l0;
@@ -372,7 +402,14 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
           for (int e = 0; e < 16; ++e)
             pk[e] = tc::pack_bf16x2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1]));
           ht::tmem_st(t_s, pk);
+          ht::st_wait();
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) ws::arrive(&sh.pfull);
         }
+        ok = ht::warp_wait(&sh.dpfull, x & 1, abort_flag);
+        if (!ok) break;
+        tc::fence_after_sync();
         uint32_t dv[32];
         ht::tmem_ld(t_dp, dv);
 #pragma unroll
@@ -398,28 +435,21 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
           pk[e / 2 + 1] = tc::pack_bf16x2(y[2], y[3]);
         }
         ht::tmem_st(t_dp, pk);
-        if constexpr (DQ) {
-          const int k0 = x0 - half * 32;
-          if (it.len < p.Nk && k0 + HB_T > it.len) {
-            // K rows beyond the length may hold anything: dS is zero there,
-            // the rows become zero too (S has been formed)
-            if (!ht::warp_wait(&sh.full[s], (x / NS) & 1, abort_flag)) {
-              ok = false;
-              break;
-            }
-            const int r0 = it.len - k0;
-            const uint32_t kt = ring + s * SLOT;
-            for (int e = half * 128 + row; e < (HB_T - r0) * (DP / 8); e += 256) {
-              const int r = r0 + e / (DP / 8), cc = e % (DP / 8);
-              st_shared_zero16(kt + (uint32_t)((cc >> 3) * HB_T * 128 + r * 128 + (cc & 7) * 16));
-            }
-            tc::fence_async_smem();
+        if (tail) {
+          // K rows beyond the length may hold anything: dS is zero there, the
+          // rows become zero too (S has been formed)
+          const int r0 = it.len - (x0 - part * 32);
+          const uint32_t kt = xr + sx * TILE;
+          for (int e = threadIdx.x; e < (HB_T - r0) * (DP / 8); e += 512) {
+            const int r = r0 + e / (DP / 8), cc = e % (DP / 8);
+            st_shared_zero16(kt + (uint32_t)((cc >> 3) * HB_T * 128 + r * 128 + (cc & 7) * 16));
           }
+          tc::fence_async_smem();
         }
         ht::st_wait();
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) ws::arrive(&sh.pfull[w]);
+        if (lane == 0) ws::arrive(&sh.dsfull);
       }
       c += (uint32_t)it.n;
       if (ok && it.n > 0) {
@@ -430,14 +460,15 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
       // dq: each group stores a quarter of the columns; dk, dv: groups 0 and
       // 1 the halves of dv, 2 and 3 those of dk
       const int own_n = DQ ? p.Nq : p.Nk, heads = DQ ? p.H : p.Hk;
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(DQ ? p.dq : (w ? p.dk : p.dv)) +
+      const bool second = !DQ && part >= 2;
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(DQ ? p.dq : (second ? p.dk : p.dv)) +
                            (((int64_t)it.b * own_n + own_row) * heads + it.h) * p.d;
-      float f = DQ || w ? p.scale : 1.f;
+      float f = DQ || second ? p.scale : 1.f;
       if (!ok) f = __int_as_float(0x7fffffff);
       const bool zero = it.n == 0 || (!DQ && own_row >= it.len);
-      const int c0 = DQ ? (2 * w + half) * (DP / 4) : half * (DP / 2);
+      const int c0 = DQ ? part * (DP / 4) : (part & 1) * (DP / 2);
       const int c1 = c0 + (DQ ? DP / 4 : DP / 2);
-      const uint32_t t_acc = tmem + lane_off + (DQ ? 0 : (w ? DP : 0));
+      const uint32_t t_acc = tmem + lane_off + (second ? DP : 0);
       for (int cc = c0; cc < c1 && cc < p.d; cc += 16) {
         uint32_t o[16];
         if (it.n > 0) ht::tmem_ld(t_acc + cc, o);
@@ -478,7 +509,7 @@ static cudaError_t bwd_tc_go(const CUtensorMap* m, const HeadAttnParams& p, int6
   gr.items = (int)(bh * gr.tiles);
   gr.tile_major = p.peers == PEERS_PAST && bh <= sms;
   const int grid = gr.items < sms ? gr.items : sms;
-  constexpr int SMEM = HbPlan<ht::width(NKS)>::SMEM;
+  constexpr int SMEM = HbPlan<ht::width(NKS), DQ>::SMEM;
   const void* fn = reinterpret_cast<const void*>(&head_bwd_tc_kernel<NKS, DQ>);
   const cudaError_t e = raise_smem_limit(fn, SMEM);
   if (e != cudaSuccess) return e;

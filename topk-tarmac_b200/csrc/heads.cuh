@@ -61,7 +61,7 @@ struct HeadAttnParams {
   float* delta;               // backward: row statistics (head_attn.cu)
 };
 
-// rows of the backward's statistics per head: whole 64-row tiles
-__host__ __device__ constexpr int head_padded_rows(int Nq) { return cdiv(Nq, 64) * 64; }
+// rows of the backward's statistics per head: whole 128-row tiles
+__host__ __device__ constexpr int head_padded_rows(int Nq) { return cdiv(Nq, 128) * 128; }
 
 }  // namespace tarmac
