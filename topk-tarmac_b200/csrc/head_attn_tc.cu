@@ -3,14 +3,14 @@
 //
 // A block owns two 128-row query tiles of one key head — two heads of the
 // same rows, or neighbouring tiles — that share every staged K and V tile of
-// 128 keys. Roles of its 18 warps:
-// * warps 0..7 and 8..15: two warpgroups per tile, two threads per row with 64
+// 128 keys. Roles of its 20 warps (two idle):
+// * warps 4..11 and 12..19: two warpgroups per tile, two threads per row with 64
 //   of the 128 columns each. They read S from TMEM, mask, run the softmax in
 //   base 2 (row maxima meet in shared memory) and write P as bf16 over the
 //   columns of S that they own. The reference maximum moves, and O is
 //   rescaled, only when a score exceeds it by 2^8, which few tiles do.
-// * warp 16: one thread issues the TMA loads (Q once, K and V in a ring).
-// * warp 17: one thread issues the products, alternating the tiles:
+// * warp 1: one thread issues the TMA loads (Q once, K and V in a ring).
+// * warp 0: one thread issues the products, alternating the tiles:
 //   S_g = Q_g K^T, then O_g += P_g V with P from TMEM. While one tile is in
 //   its softmax the tensor core serves the other.
 // Bound: the special-function unit's 16 exponentials per clock per SM (1024
@@ -26,8 +26,10 @@ namespace tarmac {
 
 namespace {
 
-constexpr int HT_THREADS = 576;
-constexpr int HT_TMA_WARP = 16, HT_MMA_WARP = 17;
+constexpr int HT_THREADS = 640;
+// the issuing warps come first: older warps win the issue slots, and a late
+// product stalls all others
+constexpr int HT_MMA_WARP = 0, HT_TMA_WARP = 1, HT_W0 = 4;
 constexpr int HT_KEYS = 128;
 constexpr float HT_LOG2E = 1.4426950408889634f;
 constexpr float HT_LN2 = 0.6931471805599453f;
@@ -225,10 +227,10 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
     mma_done:;
     }
     __syncwarp();
-  } else {
+  } else if (warp >= HT_W0) {
     // ---------------- softmax groups ----------------
     // tile w of the item, columns [64 half, 64 half + 64) of its key tiles
-    const int w = warp >> 3, half = (warp >> 2) & 1, row = threadIdx.x & 127;
+    const int w = (warp - HT_W0) >> 3, half = ((warp - HT_W0) >> 2) & 1, row = threadIdx.x & 127;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + w * 128 + half * 64 + lane_off;
     const uint32_t t_o = tmem + 256 + w * DP + half * (DP / 2) + lane_off;

@@ -11,7 +11,7 @@
 //   dV += P^T dout, dK += dS^T Q. Shared heads add up in TMEM.
 // P and dS return to TMEM as bf16, over the columns S and dP had, and are the
 // A operands of the aggregates, so they never pass through shared memory.
-// Roles of the 18 warps: 16 form the weights of one tile together (a thread
+// Roles of the 20 warps (two idle): 16 form the weights of one tile together (a thread
 // has one row and 32 of the 128 columns), one thread feeds the TMA rings, one
 // issues products. The two halves of a tile's work overlap the products of the
 // other half: while P of tile t + 1 is formed the tensor core runs dK (or dQ)
@@ -37,8 +37,10 @@ int head_sm_count();
 
 namespace {
 
-constexpr int HB_THREADS = 576;
-constexpr int HB_TMA_WARP = 16, HB_MMA_WARP = 17;
+constexpr int HB_THREADS = 640;
+// the issuing warps come first: older warps win the issue slots, and a late
+// product stalls all others
+constexpr int HB_MMA_WARP = 0, HB_TMA_WARP = 1, HB_W0 = 4;
 constexpr int HB_T = 128;  // streamed rows per tile
 constexpr float HB_LOG2E = 1.4426950408889634f;
 
@@ -226,82 +228,101 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
     }
     __syncwarp();
   } else if (warp == HB_MMA_WARP) {
-    if (lane == 0) {
-      constexpr uint32_t id_s = tc::idesc_bf16(128, HB_T, false, false);
-      constexpr uint32_t id_o = tc::idesc_bf16(128, NKS * 16, false, true);
-      const uint64_t da0 = ht::desc128(own, 16), dx0 = ht::desc128(xr, 16),
-                     dy0 = ht::desc128(yr, 16);
-      const uint64_t nx0 = ht::desc128(xr, HB_T * 128), ny0 = ht::desc128(yr, HB_T * 128);
-      uint32_t c = 0, oc = 0;
-      // S and dP of streamed tile number x (counted over all items)
-      auto issue_s = [&](uint32_t x) {
-        const int s = x % NX;
-        if (!ws::wait(&sh.xfull[s], (x / NX) & 1, abort_flag)) return false;
-        tc::fence_after_sync();
-        const int u = NSB == 2 ? (x & 1) : 0;
-        ht::issue_scores<NKS, HB_T>(tmem + COL_S + u * 128, da0,
-                                    dx0 + (uint64_t)((s * TILE) >> 4), id_s);
-        tc::mma_commit(&sh.sfull[u]);
-        return true;
-      };
-      auto issue_dp = [&](uint32_t x) {
-        const int s = x % NY;
-        if (!ws::wait(&sh.yfull[s], (x / NY) & 1, abort_flag)) return false;
-        tc::fence_after_sync();
-        ht::issue_scores<NKS, HB_T>(tmem + COL_DP, da0 + (uint64_t)(TILE >> 4),
-                                    dy0 + (uint64_t)((s * TILE) >> 4), id_s);
-        tc::mma_commit(&sh.dpfull);
-        if constexpr (DQ) tc::mma_commit(&sh.yempty[s]);  // V is read once
-        return true;
-      };
-      for (int k = 0;; ++k) {
-        const int item = hb_next(k);
-        if (item >= gr.items) break;
-        const HbItem it = hb_item<DQ>(p, gr, item);
-        if (it.n == 0) continue;
-        if (!ws::wait(&sh.own_full, oc & 1, abort_flag)) goto mma_done;
-        if (!issue_s(c) || !issue_dp(c)) goto mma_done;
-        if (DQ && it.n > 1 && !issue_s(c + 1)) goto mma_done;
-        if (it.n == 1) tc::mma_commit(&sh.own_empty);
-        // the accumulators of the item before have been read
-        if (!ws::wait(&sh.acc_empty, (oc & 1) ^ 1, abort_flag)) goto mma_done;
-        ++oc;
-        for (int t = 0; t < it.n; ++t) {
-          const uint32_t x = c + t;
-          const int sx = x % NX, sy = x % NY;
-          if constexpr (!DQ) {
-            if (!ws::wait(&sh.pfull, x & 1, abort_flag)) goto mma_done;
-            tc::fence_after_sync();
-            ht::issue_aggregate<HB_T, 32>(tmem, tmem + COL_S, ny0 + (uint64_t)((sy * TILE) >> 4),
-                                          id_o, t > 0);  // dV += P^T dout
-            tc::mma_commit(&sh.yempty[sy]);
-            if (t + 1 < it.n && !issue_s(x + 1)) goto mma_done;
-          }
-          if (!ws::wait(&sh.dsfull, x & 1, abort_flag)) goto mma_done;
-          tc::fence_after_sync();
-          // dK += dS^T Q, or dQ += dS K
-          ht::issue_aggregate<HB_T, 32>(tmem + (DQ ? 0 : DP), tmem + COL_DP,
-                                        nx0 + (uint64_t)((sx * TILE) >> 4), id_o, t > 0);
-          tc::mma_commit(&sh.xempty[sx]);
-          if (t + 1 < it.n && !issue_dp(x + 1)) goto mma_done;
-          // the last S and dP are issued: the next item's own tiles may load
-          if (t + 2 == it.n) tc::mma_commit(&sh.own_empty);
-          if (DQ && t + 2 < it.n && !issue_s(x + 2)) goto mma_done;
-        }
-        tc::mma_commit(&sh.acc_full);
-        c += (uint32_t)it.n;
+    constexpr uint32_t id_s = tc::idesc_bf16(128, HB_T, false, false);
+    constexpr uint32_t id_o = tc::idesc_bf16(128, NKS * 16, false, true);
+    const uint64_t da0 = ht::desc128(own, 16), dx0 = ht::desc128(xr, 16),
+                   dy0 = ht::desc128(yr, 16);
+    const uint64_t nx0 = ht::desc128(xr, HB_T * 128), ny0 = ht::desc128(yr, HB_T * 128);
+    const uint32_t b_own_full = tc::smem_addr(&sh.own_full), b_own_empty = tc::smem_addr(&sh.own_empty);
+    const uint32_t b_xfull = tc::smem_addr(&sh.xfull[0]), b_xempty = tc::smem_addr(&sh.xempty[0]);
+    const uint32_t b_yfull = tc::smem_addr(&sh.yfull[0]), b_yempty = tc::smem_addr(&sh.yempty[0]);
+    const uint32_t b_sfull = tc::smem_addr(&sh.sfull[0]), b_dpfull = tc::smem_addr(&sh.dpfull);
+    const uint32_t b_pfull = tc::smem_addr(&sh.pfull), b_dsfull = tc::smem_addr(&sh.dsfull);
+    const uint32_t b_acc_full = tc::smem_addr(&sh.acc_full), b_acc_empty = tc::smem_addr(&sh.acc_empty);
+    const bool leader = ht::elect_one();
+    // next X tile to score, next X tile to aggregate, next Y tile of each
+    ht::RingPos<NX> xs, xa;
+    ht::RingPos<NY> ys, ya;
+    uint32_t c = 0, oc = 0, sbuf = 0;
+    bool ok = true;
+    auto issue_s = [&] {
+      ok = ok && ht::wait_at(b_xfull + 8 * xs.s, xs.ph, abort_flag);
+      tc::fence_after_sync();
+      if (ok && leader) {
+        ht::issue_scores<NKS, HB_T>(tmem + COL_S + sbuf * 128, da0,
+                                    dx0 + (uint64_t)(xs.s * (TILE >> 4)), id_s);
+        ht::commit_at(b_sfull + 8 * sbuf);
       }
-      // the last commits land before the block ends
-      for (uint32_t x = c > (uint32_t)NX ? c - NX : 0; x < c; ++x)
-        if (!ws::wait(&sh.xempty[x % NX], (x / NX) & 1, abort_flag)) break;
-      if (oc) ws::wait(&sh.own_empty, (oc - 1) & 1, abort_flag);
-    mma_done:;
+      __syncwarp();
+      xs.next();
+      if (NSB == 2) sbuf ^= 1;
+    };
+    auto issue_dp = [&] {
+      ok = ok && ht::wait_at(b_yfull + 8 * ys.s, ys.ph, abort_flag);
+      tc::fence_after_sync();
+      if (ok && leader) {
+        ht::issue_scores<NKS, HB_T>(tmem + COL_DP, da0 + (uint64_t)(TILE >> 4),
+                                    dy0 + (uint64_t)(ys.s * (TILE >> 4)), id_s);
+        ht::commit_at(b_dpfull);
+        if (DQ) ht::commit_at(b_yempty + 8 * ys.s);  // V is read once
+      }
+      __syncwarp();
+      ys.next();
+    };
+    for (int k = 0; ok; ++k) {
+      const int item = hb_next(k);
+      if (item >= gr.items) break;
+      const int n = hb_item<DQ>(p, gr, item).n;
+      if (n == 0) continue;
+      ok = ht::wait_at(b_own_full, oc & 1, abort_flag);
+      issue_s();
+      issue_dp();
+      if (DQ && n > 1) issue_s();
+      if (n == 1 && ok && leader) ht::commit_at(b_own_empty);
+      __syncwarp();
+      // the accumulators of the item before have been read
+      ok = ok && ht::wait_at(b_acc_empty, (oc & 1) ^ 1, abort_flag);
+      ++oc;
+      for (int t = 0; t < n && ok; ++t, ++c) {
+        if constexpr (!DQ) {
+          ok = ht::wait_at(b_pfull, c & 1, abort_flag);
+          tc::fence_after_sync();
+          if (ok && leader) {  // dV += P^T dout
+            ht::issue_aggregate<HB_T, 32>(tmem, tmem + COL_S,
+                                          ny0 + (uint64_t)(ya.s * (TILE >> 4)), id_o, t > 0);
+            ht::commit_at(b_yempty + 8 * ya.s);
+          }
+          __syncwarp();
+          ya.next();
+          if (t + 1 < n) issue_s();
+        }
+        ok = ok && ht::wait_at(b_dsfull, c & 1, abort_flag);
+        tc::fence_after_sync();
+        if (ok && leader) {  // dK += dS^T Q, or dQ += dS K
+          ht::issue_aggregate<HB_T, 32>(tmem + (DQ ? 0 : DP), tmem + COL_DP,
+                                        nx0 + (uint64_t)(xa.s * (TILE >> 4)), id_o, t > 0);
+          ht::commit_at(b_xempty + 8 * xa.s);
+        }
+        __syncwarp();
+        xa.next();
+        if (t + 1 < n) issue_dp();
+        // the last S and dP are issued: the next item's own tiles may load
+        if (t + 2 == n && ok && leader) ht::commit_at(b_own_empty);
+        __syncwarp();
+        if (DQ && t + 2 < n) issue_s();
+      }
+      if (ok && leader) ht::commit_at(b_acc_full);
+      __syncwarp();
     }
+    // the last commits land before the block ends
+    for (uint32_t x = c > (uint32_t)NX ? c - NX : 0; x < c && ok; ++x)
+      ok = ht::wait_at(b_xempty + 8 * (x % NX), (x / NX) & 1, abort_flag);
+    if (oc && ok) ht::wait_at(b_own_empty, (oc - 1) & 1, abort_flag);
     __syncwarp();
-  } else {
+  } else if (warp >= HB_W0) {
     // ---------------- weights ----------------
     // columns [32 part, 32 part + 32) of each tile
-    const int part = warp >> 2, row = threadIdx.x & 127;
+    const int part = (warp - HB_W0) >> 2, row = threadIdx.x & 127;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + COL_S + part * 32 + lane_off;
     const uint32_t t_dp = tmem + COL_DP + part * 32 + lane_off;
@@ -440,7 +461,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
           // rows become zero too (S has been formed)
           const int r0 = it.len - (x0 - part * 32);
           const uint32_t kt = xr + sx * TILE;
-          for (int e = threadIdx.x; e < (HB_T - r0) * (DP / 8); e += 512) {
+          for (int e = threadIdx.x - HB_W0 * 32; e < (HB_T - r0) * (DP / 8); e += 512) {
             const int r = r0 + e / (DP / 8), cc = e % (DP / 8);
             st_shared_zero16(kt + (uint32_t)((cc >> 3) * HB_T * 128 + r * 128 + (cc & 7) * 16));
           }

@@ -79,11 +79,64 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
       : "memory");
 }
 
+// Bounded wait on the barrier at shared address `a`: one poll in line (most
+// phases have completed by then), the rest out of line.
+static __device__ __noinline__ bool poll_wait(uint32_t a, uint32_t parity, volatile int* abort_flag) {
+  for (uint32_t it = 0; it < WS_WAIT_LIMIT; ++it) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((it & 63) == 63 && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  return false;
+}
+__device__ __forceinline__ bool wait_at(uint32_t a, uint32_t parity, volatile int* abort_flag) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(a), "r"(parity)
+      : "memory");
+  return done ? true : poll_wait(a, parity, abort_flag);
+}
+__device__ __forceinline__ void commit_at(uint32_t a) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(a)
+      : "memory");
+}
+// One lane of a converged warp. The issuing warps run their loops with all
+// lanes, so that addresses and descriptors stay in uniform registers, and
+// only the products themselves are under this predicate.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(p));
+  return p != 0;
+}
+// position in a ring of N slots: slot and phase parity
+template <int N>
+struct RingPos {
+  uint32_t s = 0, ph = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == N) {
+      s = 0;
+      ph ^= 1;
+    }
+  }
+};
+
 // Bounded wait by a whole warp: all lanes take the same result, so the warp
 // stays together for its TMEM transfers.
 __device__ __forceinline__ bool warp_wait(uint64_t* mbar, uint32_t parity,
                                           volatile int* abort_flag) {
-  return __all_sync(0xffffffffu, ws::wait(mbar, parity, abort_flag));
+  return __all_sync(0xffffffffu, wait_at(tc::smem_addr(mbar), parity, abort_flag));
 }
 
 __device__ __forceinline__ void st_wait() {
