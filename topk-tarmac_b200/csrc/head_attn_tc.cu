@@ -174,58 +174,76 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
     }
     __syncwarp();
   } else if (warp == HT_MMA_WARP) {
-    if (lane == 0) {
-      const uint32_t id_s = tc::idesc_bf16(128, HT_KEYS, false, false);
-      const uint32_t id_o = tc::idesc_bf16(128, NKS * 16, false, true);
-      const uint64_t dq0 = ht::desc128(qa, 16), dk0 = ht::desc128(kva, 16);
-      const uint64_t dv0 = ht::desc128(kva + TILE, 128 * 128);
-      uint32_t kc = 0, pc[2] = {0, 0};
-      auto scores = [&](int w, int s) {
-        const uint64_t dq = dq0 + (uint64_t)((w * TILE) >> 4);
-        const uint64_t dk = dk0 + (uint64_t)((s * 2 * TILE) >> 4);
-        ht::issue_scores<NKS, 128>(tmem + w * 128, dq, dk, id_s);
-        tc::mma_commit(&sh.sfull[w]);
-      };
-      for (int k = 0;; ++k) {
-        const int item = ht_next(k);
-        if (item >= gr.items) break;
-        const HtItem it = ht_item(p, gr, item);
-        if (!ws::wait(&sh.qfull, k & 1, abort_flag)) goto mma_done;
-        if (it.n > 0) {
-          const int s = kc % NS;
-          if (!ws::wait(&sh.kfull[s], (kc / NS) & 1, abort_flag)) goto mma_done;
-          tc::fence_after_sync();
-          for (int w = 0; w < 2; ++w)
-            if (it.nt[w] > 0) scores(w, s);
-        }
-        if (it.n <= 1) tc::mma_commit(&sh.qempty);
-        for (int t = 0; t < it.n; ++t, ++kc) {
-          const int s = kc % NS, s1 = (kc + 1) % NS;
-          if (!ws::wait(&sh.vfull[s], (kc / NS) & 1, abort_flag)) goto mma_done;
-          if (t + 1 < it.n && !ws::wait(&sh.kfull[s1], ((kc + 1) / NS) & 1, abort_flag))
-            goto mma_done;
-          const uint64_t dv = dv0 + (uint64_t)((s * 2 * TILE) >> 4);
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            if (t >= it.nt[w]) continue;
-            if (!ws::wait(&sh.pfull[w], pc[w] & 1, abort_flag)) goto mma_done;
-            ++pc[w];
-            tc::fence_after_sync();
-            ht::issue_aggregate<HT_KEYS, 64>(tmem + 256 + w * DP, tmem + w * 128, dv, id_o, t > 0);
-            if (t + 1 < it.nt[w])
-              scores(w, s1);
-            else
-              tc::mma_commit(&sh.odone[w]);
-          }
-          tc::mma_commit(&sh.empty[s]);
-          if (t + 2 == it.n) tc::mma_commit(&sh.qempty);
-        }
+    constexpr uint32_t id_s = tc::idesc_bf16(128, HT_KEYS, false, false);
+    constexpr uint32_t id_o = tc::idesc_bf16(128, NKS * 16, false, true);
+    const uint64_t dq0 = ht::desc128(qa, 16), dk0 = ht::desc128(kva, 16);
+    const uint64_t dv0 = ht::desc128(kva + TILE, 128 * 128);
+    const uint32_t b_qfull = tc::smem_addr(&sh.qfull), b_qempty = tc::smem_addr(&sh.qempty);
+    const uint32_t b_kfull = tc::smem_addr(&sh.kfull[0]), b_vfull = tc::smem_addr(&sh.vfull[0]);
+    const uint32_t b_empty = tc::smem_addr(&sh.empty[0]), b_sfull = tc::smem_addr(&sh.sfull[0]);
+    const uint32_t b_pfull = tc::smem_addr(&sh.pfull[0]), b_odone = tc::smem_addr(&sh.odone[0]);
+    const bool leader = ht::elect_one();
+    ht::RingPos<NS> kr, vr;  // next K tile to score, next V tile to aggregate
+    uint32_t pc0 = 0, pc1 = 0, kc = 0;
+    bool ok = true;
+    auto scores = [&](int w) {  // S_w from the K tile at kr
+      if (ok && leader) {
+        ht::issue_scores<NKS, 128>(tmem + w * 128, dq0 + (uint64_t)(w * (TILE >> 4)),
+                                   dk0 + (uint64_t)(kr.s * (2 * TILE >> 4)), id_s);
+        ht::commit_at(b_sfull + 8 * w);
       }
-      // the last commits land before the block ends
-      for (uint32_t c = kc > (uint32_t)NS ? kc - NS : 0; c < kc; ++c)
-        if (!ws::wait(&sh.empty[c % NS], (c / NS) & 1, abort_flag)) break;
-    mma_done:;
+      __syncwarp();
+    };
+    auto wait_k = [&] {
+      ok = ok && ht::wait_at(b_kfull + 8 * kr.s, kr.ph, abort_flag);
+      tc::fence_after_sync();
+    };
+    for (int k = 0; ok; ++k) {
+      const int item = ht_next(k);
+      if (item >= gr.items) break;
+      const HtItem it = ht_item(p, gr, item);
+      const int n = it.n, n0 = it.nt[0], n1 = it.nt[1];
+      ok = ht::wait_at(b_qfull, k & 1, abort_flag);
+      if (n > 0) {
+        wait_k();
+        if (n0 > 0) scores(0);
+        if (n1 > 0) scores(1);
+        kr.next();
+      }
+      if (n <= 1 && ok && leader) ht::commit_at(b_qempty);
+      __syncwarp();
+      for (int t = 0; t < n && ok; ++t, ++kc) {
+        ok = ht::wait_at(b_vfull + 8 * vr.s, vr.ph, abort_flag);
+        if (t + 1 < n) wait_k();
+        const uint64_t dv = dv0 + (uint64_t)(vr.s * (2 * TILE >> 4));
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const int nw = w ? n1 : n0;
+          if (t >= nw) continue;
+          ok = ok && ht::wait_at(b_pfull + 8 * w, (w ? pc1 : pc0) & 1, abort_flag);
+          if (w) ++pc1; else ++pc0;
+          tc::fence_after_sync();
+          if (ok && leader)
+            ht::issue_aggregate<HT_KEYS, 64>(tmem + 256 + w * DP, tmem + w * 128, dv, id_o, t > 0);
+          __syncwarp();
+          if (t + 1 < nw)
+            scores(w);
+          else if (ok && leader)
+            ht::commit_at(b_odone + 8 * w);
+          __syncwarp();
+        }
+        if (ok && leader) {
+          ht::commit_at(b_empty + 8 * vr.s);
+          if (t + 2 == n) ht::commit_at(b_qempty);
+        }
+        __syncwarp();
+        vr.next();
+        if (t + 1 < n) kr.next();
+      }
     }
+    // the last commits land before the block ends
+    for (uint32_t c = kc > (uint32_t)NS ? kc - NS : 0; c < kc && ok; ++c)
+      ok = ht::wait_at(b_empty + 8 * (c % NS), (c / NS) & 1, abort_flag);
     __syncwarp();
   } else if (warp >= HT_W0) {
     // ---------------- softmax groups ----------------
