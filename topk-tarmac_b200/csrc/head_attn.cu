@@ -392,10 +392,10 @@ __global__ void __launch_bounds__(256) head_join_kernel(HeadAttnParams p) {
 // ---------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------
-// Row statistics, [2][B, H, nqp] with nqp = Nq rounded up to 128: base-2 lse
-// (+inf for a row that saw nothing and for the rows of padding, which makes
-// their weights exp2(s - inf) = 0) and D = dout . out (0 for padding). A group
-// of 8 lanes per row.
+// Row statistics, [2][B, H, nqp] with nqp = Nq rounded up to 128: the negative
+// of the base-2 lse (-inf for a row that saw nothing and for the rows of
+// padding, which makes their weights exp2(s - inf) = 0) and -D = -dout . out
+// (0 for padding). A group of 8 lanes per row.
 template <typename T>
 __global__ void __launch_bounds__(256) head_delta_kernel(HeadAttnParams p, int nqp) {
   const int64_t total = (int64_t)p.B * nqp * p.H;
@@ -428,8 +428,8 @@ __global__ void __launch_bounds__(256) head_delta_kernel(HeadAttnParams p, int n
   if (row < total && sub == 0) {
     const float lse = i < p.Nq ? p.lse[(b * p.H + h) * p.Nq + i] : -INFINITY;
     const int64_t srow = (b * p.H + h) * nqp + i;
-    p.delta[srow] = lse == -INFINITY ? INFINITY : lse * HA_LOG2E;
-    p.delta[total + srow] = s;
+    p.delta[srow] = lse == -INFINITY ? -INFINITY : lse * -HA_LOG2E;
+    p.delta[total + srow] = -s;
   }
 }
 
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(HA_THREADS) head_dq_kernel(HeadAttnParams p) {
   cp_async_commit();
 
   int jlim[2], self[2];
-  float lse2[2], delta[2];
+  float nlse[2], ndelta[2];
   const uint32_t* words[2];
   int64_t orow[2];
   const int nqp = head_padded_rows(p.Nq);
@@ -502,8 +502,8 @@ __global__ void __launch_bounds__(HA_THREADS) head_dq_kernel(HeadAttnParams p) {
     self[u] = p.peers == PEERS_OTHERS && pos >= 0 && pos < p.Nk ? (int)pos : -1;
     words[u] = p.bits ? p.bits + w.b * p.bits_b + (int64_t)i * p.bits_w : nullptr;
     const int64_t srow = ((int64_t)w.b * p.H + h) * nqp + i;
-    lse2[u] = p.delta[srow];
-    delta[u] = p.delta[total + srow];
+    nlse[u] = p.delta[srow];
+    ndelta[u] = p.delta[total + srow];
     orow[u] = rr < nrows ? ((int64_t)w.b * p.Nq + i) * p.H + h : -1;
   }
   const float c2 = p.scale * HA_LOG2E;
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(HA_THREADS) head_dq_kernel(HeadAttnParams p) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int j = k0 + 8 * n + 2 * (lane & 3) + e;
-          float x = hm::ex2(fmaf(s[n][2 * u + e], c2, -lse2[u])) * (dp[n][2 * u + e] - delta[u]);
+          float x = hm::ex2(fmaf(s[n][2 * u + e], c2, nlse[u])) * (dp[n][2 * u + e] + ndelta[u]);
           if (edge && !sees(j, jlim[u], self[u], word)) x = 0.f;
           s[n][2 * u + e] = x;
         }
@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(HA_THREADS) head_dkv_kernel(HeadAttnParams p) 
                      [&](int r) { return row_of(Gr, p.sg, r); });
     if (threadIdx.x < QT) {
       const int r = q0 + threadIdx.x, x = threadIdx.x, st = t & 1;
-      s_lse[st][x] = INFINITY;
+      s_lse[st][x] = -INFINITY;
       s_delta[st][x] = 0.f;
       s_lim[st][x] = 0;
       s_self[st][x] = -1;
@@ -650,10 +650,10 @@ __global__ void __launch_bounds__(HA_THREADS) head_dkv_kernel(HeadAttnParams p) 
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const float pr = sees(j0 + 8 * u, lim, self, word)
-                               ? hm::ex2(fmaf(s[n][2 * u + e], c2, -ls))
+                               ? hm::ex2(fmaf(s[n][2 * u + e], c2, ls))
                                : 0.f;
           s[n][2 * u + e] = pr;
-          dp[n][2 * u + e] = pr == 0.f ? 0.f : pr * (dp[n][2 * u + e] - de);
+          dp[n][2 * u + e] = pr == 0.f ? 0.f : pr * (dp[n][2 * u + e] + de);
         }
       }
     hm::aggregate<DP, NT>(dv, s, sG, lane);

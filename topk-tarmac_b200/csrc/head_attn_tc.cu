@@ -72,9 +72,7 @@ __device__ __forceinline__ HtItem ht_item(const HeadAttnParams& p, const HtGrid&
   const int x = gr.pair_major ? item % bh : item / gr.pairs;
   w.hk = x % p.Hk;
   w.b = x / p.Hk;
-  const int start = p.q_start ? __ldg(p.q_start + w.b) : p.Nk - p.Nq;
-  int len = p.key_len ? __ldg(p.key_len + w.b) : p.Nk;
-  len = max(0, min(len, p.Nk));
+  const int start = ht::first_pos(p, w.b), len = ht::key_count(p, w.b);
   w.n = 0;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -85,12 +83,7 @@ __device__ __forceinline__ HtItem ht_item(const HeadAttnParams& p, const HtGrid&
     if (unit >= gr.nqt * p.G) continue;
     w.tile[u] = gr.nqt - 1 - unit / p.G;
     w.g[u] = unit % p.G;
-    int kend = len;
-    if (p.peers == PEERS_PAST) {
-      const int64_t last = (int64_t)start + min(p.Nq, (w.tile[u] + 1) * 128) - 1;
-      kend = (int)max((int64_t)0, min((int64_t)len, last + 1));
-    }
-    w.nt[u] = cdiv(kend, HT_KEYS);
+    w.nt[u] = cdiv(ht::key_limit(p, start + min(p.Nq, (w.tile[u] + 1) * 128) - 1, len), HT_KEYS);
     w.n = max(w.n, w.nt[u]);
   }
   return w;
@@ -269,11 +262,9 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
       if (tile < 0) continue;
       const int h = it.hk * p.G + (w ? it.g[1] : it.g[0]);
       const int i = tile * 128 + row;
-      const int64_t pos = (int64_t)(p.q_start ? __ldg(p.q_start + it.b) : p.Nk - p.Nq) + i;
-      int len = p.key_len ? __ldg(p.key_len + it.b) : p.Nk;
-      len = max(0, min(len, p.Nk));
-      const int jlim = p.peers == PEERS_PAST ? (int)max((int64_t)0, min((int64_t)len, pos + 1)) : len;
-      const int self = p.peers == PEERS_OTHERS && pos >= 0 && pos < p.Nk ? (int)pos : -1;
+      const int pos = ht::first_pos(p, it.b) + i, len = ht::key_count(p, it.b);
+      const int jlim = ht::key_limit(p, pos, len);
+      const int self = p.peers == PEERS_OTHERS ? pos : -1;
       const uint32_t* words =
           p.bits ? p.bits + it.b * p.bits_b + (int64_t)min(i, p.Nq - 1) * p.bits_w : nullptr;
       float mref = -INFINITY;  // reference maximum in exponent units
@@ -330,19 +321,17 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
         }
         const float mb = mref == -INFINITY ? 0.f : -mref;
         const uint64_t cc = pack2(c2, c2), mm = pack2(mb, mb);
-        float l4[4] = {0.f, 0.f, 0.f, 0.f};
+        uint64_t l2[2] = {0, 0};
         uint32_t pk[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const float2 y = unpack2(
-              ffma2(pack2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), cc, mm));
+          const float2 y = unpack2(ffma2(ht::pair(s[2 * e], s[2 * e + 1]), cc, mm));
           const float a = tc::ex2_approx(y.x), b = tc::ex2_approx(y.y);
-          l4[(e & 1) * 2] += a;
-          l4[(e & 1) * 2 + 1] += b;
+          l2[e & 1] = ht::fadd2(l2[e & 1], pack2(a, b));
           pk[e] = tc::pack_bf16x2(a, b);
         }
         ht::tmem_st(t_s, pk);
-        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        l += hsum2(ht::fadd2(l2[0], l2[1]));
         const int kt = t * HT_KEYS;
         if (len < p.Nk && kt + HT_KEYS > len) {
           // keys beyond the length may hold anything: their weights are zero,

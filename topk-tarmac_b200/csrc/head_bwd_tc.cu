@@ -87,26 +87,20 @@ __device__ __forceinline__ HbItem hb_item(const HeadAttnParams& p, const HbGrid&
   w.h = x % heads;
   w.hk = DQ ? w.h / p.G : w.h;
   w.b = x / heads;
-  w.start = p.q_start ? __ldg(p.q_start + w.b) : p.Nk - p.Nq;
-  int len = p.key_len ? __ldg(p.key_len + w.b) : p.Nk;
-  w.len = max(0, min(len, p.Nk));
+  w.start = ht::first_pos(p, w.b);
+  w.len = ht::key_count(p, w.b);
   w.t0 = 0;
   if constexpr (DQ) {  // last tiles first: the most keys under the past rule
     w.x0 = (gr.tiles - 1 - t) * 128;
-    int kend = w.len;
-    if (p.peers == PEERS_PAST) {
-      const int64_t last = (int64_t)w.start + min(p.Nq, w.x0 + 128) - 1;
-      kend = (int)max((int64_t)0, min((int64_t)w.len, last + 1));
-    }
-    w.nper = w.n = cdiv(kend, HB_T);
+    w.nper = w.n = cdiv(ht::key_limit(p, w.start + min(p.Nq, w.x0 + 128) - 1, w.len), HB_T);
   } else {  // first tiles first: the most queries
     w.x0 = t * 128;
     w.nper = 0;
     if (w.x0 < w.len) {
-      int64_t i0 = 0;  // first query that sees a key of the tile
-      if (p.peers == PEERS_PAST) i0 = max((int64_t)0, (int64_t)w.x0 - w.start);
+      // first query that sees a key of the tile
+      const int i0 = p.peers == PEERS_PAST ? max(0, w.x0 - w.start) : 0;
       if (i0 < p.Nq) {
-        w.t0 = (int)i0 / HB_T;
+        w.t0 = i0 / HB_T;
         w.nper = cdiv(p.Nq, HB_T) - w.t0;
       }
     }
@@ -335,23 +329,22 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
       if (item >= gr.items) break;
       const HbItem it = hb_item<DQ>(p, gr, item);
       const int own_row = it.x0 + row;
-      float lse2 = INFINITY, delta = 0.f;
+      float nlse = -INFINITY, ndelta = 0.f;  // -lse2 and -D of a query row
       int jlim = 0, self = -1;
       const uint32_t* words = nullptr;
       if constexpr (DQ) {
         if (own_row < p.Nq) {
           const int64_t srow = ((int64_t)it.b * p.H + it.h) * nqp + own_row;
-          lse2 = p.delta[srow];
-          delta = p.delta[stat_plane + srow];
+          nlse = p.delta[srow];
+          ndelta = p.delta[stat_plane + srow];
         }
-        const int64_t pos = (int64_t)it.start + own_row;
-        jlim = p.peers == PEERS_PAST ? (int)max((int64_t)0, min((int64_t)it.len, pos + 1)) : it.len;
-        self = p.peers == PEERS_OTHERS && pos >= 0 && pos < p.Nk ? (int)pos : -1;
+        jlim = ht::key_limit(p, it.start + own_row, it.len);
+        self = p.peers == PEERS_OTHERS ? it.start + own_row : -1;
         if (p.bits)
           words = p.bits + it.b * p.bits_b + (int64_t)min(own_row, p.Nq - 1) * p.bits_w;
       }
       // keys: the query (as an index) that stands at this key's position
-      const int64_t twin = (int64_t)own_row - it.start;
+      const int twin = own_row - it.start;
       int tt = it.t0;  // streamed tile inside its head
       for (int t = 0; t < it.n; ++t) {
         const uint32_t x = c + t;
@@ -368,7 +361,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
             seen = ht::key_word(x0, jlim, self, bits);
           }
         } else {
-          const int64_t e = twin - x0;  // column of the twin
+          const int e = twin - x0;  // column of the twin
           edge = p.bits || (p.peers == PEERS_PAST ? e > 0
                                                   : p.peers == PEERS_OTHERS && e >= 0 && e < 32);
           if (p.bits) {
@@ -397,16 +390,14 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
         ht::tmem_ld(t_s + (NSB == 2 ? (x & 1) * 128 : 0), sv);
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
-          uint64_t l0 = pack2(-lse2, -lse2), l1 = l0;
+          uint64_t l0 = pack2(nlse, nlse), l1 = l0;
           if constexpr (!DQ) {
-            const float4 q = *reinterpret_cast<const float4*>(st + e);
-            l0 = pack2(-q.x, -q.y);
-            l1 = pack2(-q.z, -q.w);
+            const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(st + e);
+            l0 = q.x;
+            l1 = q.y;
           }
-          const float2 y0 = unpack2(
-              ffma2(pack2(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), cc2, l0));
-          const float2 y1 = unpack2(
-              ffma2(pack2(__uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3])), cc2, l1));
+          const float2 y0 = unpack2(ffma2(ht::pair(sv[e], sv[e + 1]), cc2, l0));
+          const float2 y1 = unpack2(ffma2(ht::pair(sv[e + 2], sv[e + 3]), cc2, l1));
           sv[e] = __float_as_uint(tc::ex2_approx(y0.x));
           sv[e + 1] = __float_as_uint(tc::ex2_approx(y0.y));
           sv[e + 2] = __float_as_uint(tc::ex2_approx(y1.x));
@@ -435,25 +426,25 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
         ht::tmem_ld(t_dp, dv);
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
-          float de[4] = {delta, delta, delta, delta};
+          uint64_t d0 = pack2(ndelta, ndelta), d1 = d0;
           if constexpr (!DQ) {
-            const float4 q = *reinterpret_cast<const float4*>(st + HB_T + e);
-            de[0] = q.x;
-            de[1] = q.y;
-            de[2] = q.z;
-            de[3] = q.w;
+            const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(st + HB_T + e);
+            d0 = q.x;
+            d1 = q.y;
           }
-          float y[4];
+          const float2 y0 = unpack2(
+              ht::fmul2(ht::pair(sv[e], sv[e + 1]), ht::fadd2(ht::pair(dv[e], dv[e + 1]), d0)));
+          const float2 y1 = unpack2(ht::fmul2(ht::pair(sv[e + 2], sv[e + 3]),
+                                              ht::fadd2(ht::pair(dv[e + 2], dv[e + 3]), d1)));
+          pk[e / 2] = tc::pack_bf16x2(y0.x, y0.y);
+          pk[e / 2 + 1] = tc::pack_bf16x2(y1.x, y1.y);
+        }
+        if (edge) {  // a masked pair's dP may be anything
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            y[u] = __uint_as_float(sv[e + u]) * (__uint_as_float(dv[e + u]) - de[u]);
-          if (edge) {  // a masked pair's dP may be anything
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (!((seen >> (e + u)) & 1u)) y[u] = 0.f;
+          for (int e = 0; e < 16; ++e) {
+            if (!((seen >> (2 * e)) & 1u)) pk[e] &= 0xffff0000u;
+            if (!((seen >> (2 * e)) & 2u)) pk[e] &= 0x0000ffffu;
           }
-          pk[e / 2] = tc::pack_bf16x2(y[0], y[1]);
-          pk[e / 2 + 1] = tc::pack_bf16x2(y[2], y[3]);
         }
         ht::tmem_st(t_dp, pk);
         if (tail) {

@@ -212,6 +212,38 @@ __device__ __forceinline__ void issue_aggregate(uint32_t tmem_d, uint32_t tmem_a
            db + (uint64_t)((ks * 2048) >> 4), idesc, add || ks > 0);
 }
 
+// packed fp32 pairs (one issue slot for two IEEE operations)
+__device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+
+// First query position of an episode. Positions beyond +-2^30 act like those
+// bounds (lengths stay below 2^29), which keeps position arithmetic in 32 bits.
+__device__ __forceinline__ int first_pos(const HeadAttnParams& p, int b) {
+  const int s = p.q_start ? __ldg(p.q_start + b) : p.Nk - p.Nq;
+  return max(-(1 << 30), min(1 << 30, s));
+}
+__device__ __forceinline__ int key_count(const HeadAttnParams& p, int b) {
+  const int n = p.key_len ? __ldg(p.key_len + b) : p.Nk;
+  return max(0, min(n, p.Nk));
+}
+// first key a row at `pos` does not see, from its length and the past rule
+__device__ __forceinline__ int key_limit(const HeadAttnParams& p, int pos, int len) {
+  return p.peers == PEERS_PAST ? max(0, min(len, pos + 1)) : len;
+}
+
 // Keys of the 32-key word at key j0 that a row may see: below jlim, not self,
 // and set in `bits`.
 __device__ __forceinline__ uint32_t key_word(int j0, int jlim, int self, uint32_t bits) {

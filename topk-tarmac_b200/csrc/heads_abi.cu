@@ -48,8 +48,9 @@ int fill_attn(HeadAttnParams& p, const void* q, const void* k, const void* v,
               float scale) {
   if (dtype != TARMAC_F32 && dtype != TARMAC_BF16) return TARMAC_ERR_DTYPE;
   if (B < 0 || Nq < 0 || Nk < 0 || d < 1 || d > MAX_D) return TARMAC_ERR_SHAPE;
-  // positions and key counts stay below 2^30, rows of a key head below 2^31
-  if (Nk > (1 << 30) || Nq > (1 << 30)) return TARMAC_ERR_N_TOO_LARGE;
+  // row and key counts stay below 2^29 (position arithmetic in 32 bits), packed
+  // rows of a key head below 2^31
+  if (Nk > (1 << 29) || Nq > (1 << 29)) return TARMAC_ERR_N_TOO_LARGE;
   if (H < 1 || Hk < 1 || H % Hk) return TARMAC_ERR_HEADS;
   if ((int64_t)Nq * (H / Hk) > 0x7fffff00) return TARMAC_ERR_N_TOO_LARGE;
   if (peers < PEERS_ALL || peers > PEERS_PAST) return TARMAC_ERR_MODE;
