@@ -322,8 +322,8 @@ int tarmac_qk_norm_rotate(const void *q, const void *k, void *q_out,
  * dq_out, dk_out. dq, dk: of the inputs, their type, contiguous. dwq, dwk:
  * fp32 [d] or NULL, summed over all rows in a fixed order (two calls give the
  * same bits). The tables get no gradient. work: 16-byte aligned scratch of
- * tarmac_qk_norm_rotate_workspace(d) bytes. */
-int64_t tarmac_qk_norm_rotate_workspace(int d);
+ * tarmac_qk_norm_rotate_workspace bytes. */
+int64_t tarmac_qk_norm_rotate_workspace(int B, int N, int H, int Hk, int d);
 int tarmac_qk_norm_rotate_backward(const void *q, const void *k,
                                    const void *dq_out, const void *dk_out,
                                    const int64_t *strides, const float *wq,

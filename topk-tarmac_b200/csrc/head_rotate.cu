@@ -14,15 +14,16 @@
 // E column pairs as two vectors of E elements, so the rotation never leaves
 // the lane and the only exchange is the row's sum. Columns without a rotation
 // take cos = 1, sin = 0, which makes every lane run the same code. A lane
-// group keeps its row's tables and weights in registers and runs over up to
-// four heads of the same (episode, row), with their loads in flight together.
+// group keeps the weights of its columns in registers, walks over rows
+// (episode, position) with a fixed stride, loads a row's table once and runs
+// over its heads, the loads of two to four heads in flight together.
 #include "heads.cuh"
 
 namespace tarmac {
 
 constexpr int ROT_THREADS = 256;
-constexpr int ROT_HC = 4;           // heads per unit
-constexpr int ROT_BWD_BLOCKS = 148 * 4;
+constexpr int ROT_TILES = 4;    // backward: row tiles per block
+constexpr int ROT_SLICES = 64;  // first stage of the sums for dw
 
 // E consecutive elements as one load or store
 template <typename T, int E>
@@ -30,17 +31,6 @@ struct alignas(sizeof(T) * E) Pack {
   T x[E];
 };
 
-template <typename T, int E>
-__device__ __forceinline__ void ld_pack(float (&f)[E], const T* p, bool ok) {
-  if (ok) {
-    const Pack<T, E> v = *reinterpret_cast<const Pack<T, E>*>(p);
-#pragma unroll
-    for (int e = 0; e < E; ++e) f[e] = to_f32<T>(v.x[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) f[e] = 0.f;
-  }
-}
 template <typename T, int E>
 __device__ __forceinline__ void st_pack(T* p, const float (&f)[E], bool ok) {
   if (!ok) return;
@@ -57,8 +47,8 @@ template <int E, bool ADJ>
 struct LaneCols {
   int ca, cb;
   bool ok_a, ok_b, adjacent;
-  __device__ __forceinline__ LaneCols(int slot, int d, int r, bool interleaved)
-      : adjacent(interleaved) {
+  __device__ __forceinline__ void init(int slot, int d, int r, bool interleaved) {
+    adjacent = interleaved;
     const int nrot = r / 2 / E;
     if (ADJ || interleaved) {
       ca = 2 * E * slot;
@@ -66,9 +56,11 @@ struct LaneCols {
     } else if (slot < nrot) {
       ca = E * slot;
       cb = r / 2 + ca;
-    } else {
-      ca = r + 2 * E * (slot - nrot);
-      cb = ca + E;
+    } else {  // neighbouring lanes take neighbouring columns here too
+      const int pairs = cdiv(d - r, 2 * E);
+      ca = r + E * (slot - nrot);
+      cb = ca + E * pairs;
+      if (slot - nrot >= pairs) ca = cb = d;  // no columns
     }
     ok_a = ca < d;
     ok_b = cb < d;
@@ -83,235 +75,383 @@ struct LaneCols {
   }
 };
 
+// Elementwise arithmetic on E values, two per instruction (fma.rn.f32x2 and
+// its kin: the same IEEE results); these kernels are otherwise bound by issue.
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// d = a b + c
+template <int E>
+__device__ __forceinline__ void vfma(float (&d)[E], const float (&a)[E], const float (&b)[E],
+                                     const float (&c)[E]) {
+  if constexpr (E % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 r = unpack2(ffma2(pack2(a[e], a[e + 1]), pack2(b[e], b[e + 1]),
+                                     pack2(c[e], c[e + 1])));
+      d[e] = r.x;
+      d[e + 1] = r.y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) d[e] = fmaf(a[e], b[e], c[e]);
+  }
+}
+template <int E>
+__device__ __forceinline__ void vmul(float (&d)[E], const float (&a)[E], const float (&b)[E]) {
+  if constexpr (E % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 r = unpack2(mul2(pack2(a[e], a[e + 1]), pack2(b[e], b[e + 1])));
+      d[e] = r.x;
+      d[e + 1] = r.y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) d[e] = a[e] * b[e];
+  }
+}
+// d = a f + c, d = a f with one factor for all
+template <int E>
+__device__ __forceinline__ void vfma1(float (&d)[E], const float (&a)[E], float f,
+                                      const float (&c)[E]) {
+  float ff[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) ff[e] = f;
+  vfma<E>(d, a, ff, c);
+}
+template <int E>
+__device__ __forceinline__ void vmul1(float (&d)[E], const float (&a)[E], float f) {
+  float ff[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) ff[e] = f;
+  vmul<E>(d, a, ff);
+}
+template <int E>
+__device__ __forceinline__ float vsum(const float (&a)[E]) {
+  float t = a[0];
+#pragma unroll
+  for (int e = 1; e < E; ++e) t += a[e];
+  return t;
+}
+
+// Rotate the pairs of (a, b) by (c, s); ns = -s. The inverse takes (ns, s).
 template <int E, bool ADJ>
 __device__ __forceinline__ void turn(float (&a)[E], float (&b)[E], const float (&c)[E],
-                                     const float (&s)[E]) {
+                                     const float (&s)[E], const float (&ns)[E]) {
   if constexpr (ADJ) {
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) {
       const float x = a[2 * e], y = a[2 * e + 1];
-      a[2 * e] = x * c[e] - y * s[e];
-      a[2 * e + 1] = x * s[e] + y * c[e];
+      a[2 * e] = fmaf(x, c[e], y * ns[e]);
+      a[2 * e + 1] = fmaf(x, s[e], y * c[e]);
       const float u = b[2 * e], v = b[2 * e + 1];
-      b[2 * e] = u * c[E / 2 + e] - v * s[E / 2 + e];
-      b[2 * e + 1] = u * s[E / 2 + e] + v * c[E / 2 + e];
+      b[2 * e] = fmaf(u, c[E / 2 + e], v * ns[E / 2 + e]);
+      b[2 * e + 1] = fmaf(u, s[E / 2 + e], v * c[E / 2 + e]);
     }
   } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float x = a[e], y = b[e];
-      a[e] = x * c[e] - y * s[e];
-      b[e] = x * s[e] + y * c[e];
-    }
+    float t[E], u[E];
+    vmul<E>(t, b, ns);
+    vmul<E>(u, b, c);
+    vfma<E>(b, a, s, u);
+    vfma<E>(a, a, c, t);
   }
 }
 
-// sum over the LPR lanes of a row (LPR a power of two)
+// sum over the lpr lanes of a row (a power of two)
 __device__ __forceinline__ float row_sum(float v, int lpr) {
-  for (int o = lpr >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < lpr) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// One slot of a lane: its columns, weights and table values.
+// How a launch is laid out; divisions by N are a multiplication with
+// ceil(2^(31 + ceil(log2 N)) / N), exact for dividends below 2^31.
+struct RotGrid {
+  int lpr, lpr_log2;  // lanes per row
+  int parts, parts_q; // units per row, and those of query heads
+  int four_q, four_k; // units of four heads (else two)
+  int table_vec, weight_vec;
+  float inv_d;
+  uint32_t mul, shift;
+  __device__ __forceinline__ uint32_t episode(uint32_t token) const {
+    return mul ? __umulhi(token, mul) >> shift : token;
+  }
+};
+
+// One slot of a lane: its columns and the row's table values.
 template <int E, bool ADJ>
 struct Slot {
   LaneCols<E, ADJ> col;
-  float wa[E], wb[E], c[E], s[E];
-  __device__ __forceinline__ Slot(int slot, int d, int r, bool interleaved)
-      : col(slot, d, r, interleaved) {}
-  __device__ __forceinline__ void weights(const float* w) {
+  float c[E], s[E];
+  __device__ __forceinline__ void weights(const float* w, float (&wa)[E], float (&wb)[E],
+                                          bool vec) const {
+    if (E >= 4 && vec && w && col.ok_b) {
+#pragma unroll
+      for (int e = 0; e + 3 < E; e += 4) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(w + col.ca + e));
+        const float4 y = __ldg(reinterpret_cast<const float4*>(w + col.cb + e));
+        wa[e] = x.x; wa[e + 1] = x.y; wa[e + 2] = x.z; wa[e + 3] = x.w;
+        wb[e] = y.x; wb[e + 1] = y.y; wb[e + 2] = y.z; wb[e + 3] = y.w;
+      }
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       wa[e] = col.ok_a ? (w ? __ldg(w + col.ca + e) : 1.f) : 0.f;
       wb[e] = col.ok_b ? (w ? __ldg(w + col.cb + e) : 1.f) : 0.f;
     }
   }
-  __device__ __forceinline__ void tables(const float* cs, const float* sn, int r) {
+  // a lane's E entries are neighbours; `vec`: on the 16-byte grid
+  __device__ __forceinline__ void tables(const float* cs, const float* sn, int r, bool vec) {
+    const int first = ADJ ? col.ca / 2 : col.ca;
+    if (E >= 4 && vec && first + E <= r / 2) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int t = col.entry(e, r);
-      c[e] = t >= 0 ? __ldg(cs + t) : 1.f;
-      s[e] = t >= 0 ? __ldg(sn + t) : 0.f;
+      for (int e = 0; e + 3 < E; e += 4) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(cs + first + e));
+        const float4 y = __ldg(reinterpret_cast<const float4*>(sn + first + e));
+        c[e] = x.x; c[e + 1] = x.y; c[e + 2] = x.z; c[e + 3] = x.w;
+        s[e] = y.x; s[e + 1] = y.y; s[e + 2] = y.z; s[e + 3] = y.w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int t = col.entry(e, r);
+        c[e] = t >= 0 ? __ldg(cs + t) : 1.f;
+        s[e] = t >= 0 ? __ldg(sn + t) : 0.f;
+      }
     }
   }
 };
 
-// NP slots of E pairs per lane; LPR lanes per row.
-template <typename T, int E, bool ADJ, int NP>
-__global__ void __launch_bounds__(ROT_THREADS) rotate_kernel(RotateParams p, int lpr) {
-  const int per_warp = 32 / lpr;
-  const int lane = threadIdx.x & 31;
-  const int sub = lane % lpr;
-  const int64_t group = (int64_t)(blockIdx.x * (ROT_THREADS / 32) + (threadIdx.x >> 5)) *
-                            per_warp + lane / lpr;
-  const int cq = cdiv(p.H, ROT_HC), chunks = cq + cdiv(p.Hk, ROT_HC);
-  const int64_t tokens = (int64_t)p.B * p.N;
-  const int64_t unit = group;
-  // lanes of a warp leave together only (the row sums are warp shuffles)
-  const bool live = unit < tokens * chunks;
-  const int64_t token = live ? unit / chunks : 0;
-  const int chunk = live ? (int)(unit - token * chunks) : 0;
-  const bool is_q = chunk < cq;
-  const int h0 = (is_q ? chunk : chunk - cq) * ROT_HC;
-  const int heads = is_q ? p.H : p.Hk;
-  const int b = (int)(token / p.N), n = (int)(token - (int64_t)b * p.N);
-  const HeadStrides st = is_q ? p.sq : p.sk;
-  const T* src = static_cast<const T*>(is_q ? p.q : p.k) + b * st.b + n * st.n + h0 * st.h;
-  T* dst = static_cast<T*>(is_q ? p.oq : p.ok) + (token * heads + h0) * p.d;
-
-  float a[ROT_HC][NP][E], bb[ROT_HC][NP][E];
+// A vector of E elements as loaded, widened when it is used.
+template <typename T, int E>
+struct Raw {
+  Pack<T, E> v;
+  __device__ __forceinline__ void load(const T* p, bool ok) {
+    if (ok) {
+      v = *reinterpret_cast<const Pack<T, E>*>(p);
+    } else {
 #pragma unroll
-  for (int h = 0; h < ROT_HC; ++h)
+      for (int e = 0; e < E; ++e) v.x[e] = from_f32<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ void widen(float (&f)[E]) const {
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = to_f32<T>(v.x[e]);
+  }
+};
+
+// Where a block's rows and heads are: it takes one unit — HC heads, all query
+// or all key heads — of consecutive rows; the units of a row are neighbouring
+// blocks, so its table is in L2 after the first. HC is 4 where the head count
+// is a multiple of four (more independent work to hide the row sums), else 2.
+struct RotUnit {
+  uint32_t tblock;
+  int chunk;
+  bool is_q;
+  __device__ __forceinline__ RotUnit(const RotGrid& g) {
+    tblock = blockIdx.x / (uint32_t)g.parts;
+    chunk = (int)(blockIdx.x - tblock * (uint32_t)g.parts);
+    is_q = chunk < g.parts_q;
+    if (!is_q) chunk -= g.parts_q;
+  }
+};
+
+// NP slots of E pairs per lane.
+template <typename T, int E, bool ADJ, int NP, int HC>
+__device__ __forceinline__ void rotate_unit(const RotateParams& p, const RotGrid& g,
+                                            const RotUnit& w) {
+  const int lane = threadIdx.x & 31;
+  const int sub = lane & (g.lpr - 1);
+  const bool is_q = w.is_q;
+  const int h0 = w.chunk * HC;
+  const int heads = is_q ? p.H : p.Hk;
+  // lanes of a warp leave together only (the row sums are warp shuffles)
+  uint32_t token = (w.tblock * ROT_THREADS + threadIdx.x) >> g.lpr_log2;
+  const bool live = token < (uint32_t)p.B * (uint32_t)p.N;
+  if (!live) token = 0;
+  const uint32_t b = g.episode(token), n = token - b * (uint32_t)p.N;
+  const int64_t sh = is_q ? p.sq.h : p.sk.h;
+  const T* src = is_q ? static_cast<const T*>(p.q) + b * p.sq.b + n * p.sq.n
+                      : static_cast<const T*>(p.k) + b * p.sk.b + n * p.sk.n;
+  src += h0 * sh;
+  T* dst = static_cast<T*>(is_q ? p.oq : p.ok) + ((int64_t)token * heads + h0) * p.d;
+  Slot<E, ADJ> sl[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) sl[i].col.init(sub + i * g.lpr, p.d, p.r, p.interleaved);
+  Raw<T, E> a[HC][NP], bb[HC][NP];
+#pragma unroll
+  for (int h = 0; h < HC; ++h)
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const LaneCols<E, ADJ> col(sub + i * lpr, p.d, p.r, p.interleaved);
       const bool ok = live && h0 + h < heads;
-      ld_pack<T, E>(a[h][i], src + h * st.h + col.ca, ok && col.ok_a);
-      ld_pack<T, E>(bb[h][i], src + h * st.h + col.cb, ok && col.ok_b);
+      a[h][i].load(src + h * sh + sl[i].col.ca, ok && sl[i].col.ok_a);
+      bb[h][i].load(src + h * sh + sl[i].col.cb, ok && sl[i].col.ok_b);
     }
-  float rs[ROT_HC];
-#pragma unroll
-  for (int h = 0; h < ROT_HC; ++h) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < NP; ++i)
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        ss = fmaf(a[h][i][e], a[h][i][e], fmaf(bb[h][i][e], bb[h][i][e], ss));
-    rs[h] = rsqrtf(row_sum(ss, lpr) / (float)p.d + p.eps);
-  }
-  if (!live) return;
-  const int64_t tab = b * p.table_b + (int64_t)n * (p.r / 2);
+  const int64_t tab = (int64_t)b * p.table_b + (int64_t)n * (p.r / 2);
+  float wa[NP][E], wb[NP][E];
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    Slot<E, ADJ> sl(sub + i * lpr, p.d, p.r, p.interleaved);
-    sl.weights(is_q ? p.wq : p.wk);
-    sl.tables(p.cos + tab, p.sin + tab, p.r);
+    sl[i].tables(p.cos + tab, p.sin + tab, p.r, g.table_vec != 0);
+    sl[i].weights(is_q ? p.wq : p.wk, wa[i], wb[i], g.weight_vec != 0);
+  }
+  float ns[NP][E];
 #pragma unroll
-    for (int h = 0; h < ROT_HC; ++h) {
-      if (h0 + h >= heads) break;
+  for (int i = 0; i < NP; ++i)
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        a[h][i][e] *= rs[h] * sl.wa[e];
-        bb[h][i][e] *= rs[h] * sl.wb[e];
-      }
-      turn<E, ADJ>(a[h][i], bb[h][i], sl.c, sl.s);
-      st_pack<T, E>(dst + (int64_t)h * p.d + sl.col.ca, a[h][i], sl.col.ok_a);
-      st_pack<T, E>(dst + (int64_t)h * p.d + sl.col.cb, bb[h][i], sl.col.ok_b);
+    for (int e = 0; e < E; ++e) ns[i][e] = -sl[i].s[e];
+#pragma unroll
+  for (int h = 0; h < HC; ++h) {
+    float x[NP][E], y[NP][E], acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      a[h][i].widen(x[i]);
+      bb[h][i].widen(y[i]);
+      vfma<E>(acc, x[i], x[i], acc);
+      vfma<E>(acc, y[i], y[i], acc);
+    }
+    const float rs = rsqrtf(fmaf(row_sum(vsum<E>(acc), g.lpr), g.inv_d, p.eps));
+    const bool ok = live && h0 + h < heads;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      vmul1<E>(x[i], x[i], rs);
+      vmul1<E>(y[i], y[i], rs);
+      vmul<E>(x[i], x[i], wa[i]);
+      vmul<E>(y[i], y[i], wb[i]);
+      turn<E, ADJ>(x[i], y[i], sl[i].c, sl[i].s, ns[i]);
+      st_pack<T, E>(dst + h * p.d + sl[i].col.ca, x[i], ok && sl[i].col.ok_a);
+      st_pack<T, E>(dst + h * p.d + sl[i].col.cb, y[i], ok && sl[i].col.ok_b);
     }
   }
 }
 
-// Blocks [0, nq) take the query heads, the others the key heads, so that a
-// lane's sums for dw belong to one weight; each block leaves one row of d
-// sums in `work` and rotate_dw_kernel adds the rows in order: the result does
-// not depend on which block ran when.
 template <typename T, int E, bool ADJ, int NP>
-__global__ void __launch_bounds__(ROT_THREADS) rotate_bwd_kernel(RotateParams p, int lpr,
-                                                                 int nq_blocks) {
-  constexpr int HC = 2;
-  __shared__ float red[ROT_THREADS / 32][128];
-  const bool is_q = (int)blockIdx.x < nq_blocks;
-  const int blk = is_q ? blockIdx.x : blockIdx.x - nq_blocks;
-  const int nblk = is_q ? nq_blocks : gridDim.x - nq_blocks;
-  const int per_warp = 32 / lpr;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int sub = lane % lpr;
-  const int heads = is_q ? p.H : p.Hk;
-  const int chunks = cdiv(heads, HC);
-  const int64_t units = (int64_t)p.B * p.N * chunks;
-  const HeadStrides st = is_q ? p.sq : p.sk, sg = is_q ? p.sgq : p.sgk;
-  const T* X = static_cast<const T*>(is_q ? p.q : p.k);
-  const T* Gr = static_cast<const T*>(is_q ? p.gq : p.gk);
-  T* D = static_cast<T*>(is_q ? p.oq : p.ok);
-  const float inv_d = 1.f / (float)p.d;
+__global__ void __launch_bounds__(ROT_THREADS, 4) rotate_kernel(RotateParams p, RotGrid g) {
+  const RotUnit w(g);
+  if (w.is_q ? g.four_q : g.four_k)
+    rotate_unit<T, E, ADJ, NP, 4>(p, g, w);
+  else
+    rotate_unit<T, E, ADJ, NP, 2>(p, g, w);
+}
 
-  Slot<E, ADJ> sl0(sub, p.d, p.r, p.interleaved);
-  Slot<E, ADJ> sl1(sub + (NP > 1 ? lpr : 0), p.d, p.r, p.interleaved);
-  sl0.weights(is_q ? p.wq : p.wk);
-  if constexpr (NP > 1) sl1.weights(is_q ? p.wq : p.wk);
-  float dwa[NP][E], dwb[NP][E];
+// Laid out as the forward pass, ROT_TILES tiles of rows per block. A lane sums
+// its columns' dw over its rows and heads, the block its lanes', and each block
+// leaves one row of d sums in `work`; rotate_dw_kernel adds those rows in a
+// fixed order, so the result does not depend on which block ran when.
+template <typename T, int E, bool ADJ, int NP, int HC>
+__device__ __forceinline__ void rotate_bwd_unit(const RotateParams& p, const RotGrid& g,
+                                                const RotUnit& w, float (&red)[ROT_THREADS / 32][128]) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = lane & (g.lpr - 1);
+  const uint32_t tblock = w.tblock;
+  const bool is_q = w.is_q;
+  const int h0 = w.chunk * HC;
+  const int heads = is_q ? p.H : p.Hk;
+  const uint32_t tokens = (uint32_t)p.B * (uint32_t)p.N;
+  const HeadStrides st = is_q ? p.sq : p.sk, sg = is_q ? p.sgq : p.sgk;
+  const T* X = static_cast<const T*>(is_q ? p.q : p.k) + h0 * st.h;
+  const T* Gr = static_cast<const T*>(is_q ? p.gq : p.gk) + h0 * sg.h;
+  T* D = static_cast<T*>(is_q ? p.oq : p.ok) + h0 * p.d;
+
+  Slot<E, ADJ> sl[NP];
+  float wa[NP][E], wb[NP][E], dwa[NP][E], dwb[NP][E];
 #pragma unroll
-  for (int i = 0; i < NP; ++i)
+  for (int i = 0; i < NP; ++i) {
+    sl[i].col.init(sub + i * g.lpr, p.d, p.r, p.interleaved);
+    sl[i].weights(is_q ? p.wq : p.wk, wa[i], wb[i], g.weight_vec != 0);
 #pragma unroll
     for (int e = 0; e < E; ++e) dwa[i][e] = dwb[i][e] = 0.f;
-
-  const int64_t step = (int64_t)nblk * (ROT_THREADS / 32) * per_warp;
-  const int64_t first = ((int64_t)blk * (ROT_THREADS / 32) + warp) * per_warp;
-  for (int64_t u0 = first; u0 < units; u0 += step) {  // warp-uniform bound
-    const int64_t unit = u0 + lane / lpr;
-    const bool live = unit < units;
-    const int64_t token = live ? unit / chunks : 0;
-    const int h0 = live ? (int)(unit - token * chunks) * HC : 0;
-    const int b = (int)(token / p.N), n = (int)(token - (int64_t)b * p.N);
-    const T* src = X + b * st.b + n * st.n + h0 * st.h;
-    const T* gsrc = Gr + b * sg.b + n * sg.n + h0 * sg.h;
-    T* dst = D + (token * heads + h0) * p.d;
-    float a[HC][NP][E], bb[HC][NP][E], ga[HC][NP][E], gb[HC][NP][E];
-#pragma unroll
-    for (int h = 0; h < HC; ++h)
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const Slot<E, ADJ>& sl = i ? sl1 : sl0;
-        const bool ok = live && h0 + h < heads;
-        ld_pack<T, E>(a[h][i], src + h * st.h + sl.col.ca, ok && sl.col.ok_a);
-        ld_pack<T, E>(bb[h][i], src + h * st.h + sl.col.cb, ok && sl.col.ok_b);
-        ld_pack<T, E>(ga[h][i], gsrc + h * sg.h + sl.col.ca, ok && sl.col.ok_a);
-        ld_pack<T, E>(gb[h][i], gsrc + h * sg.h + sl.col.cb, ok && sl.col.ok_b);
-      }
-    const int64_t tab = b * p.table_b + (int64_t)n * (p.r / 2);
-    sl0.tables(p.cos + tab, p.sin + tab, p.r);
-    if constexpr (NP > 1) sl1.tables(p.cos + tab, p.sin + tab, p.r);
+  }
+  for (int it = 0; it < ROT_TILES; ++it) {
+    uint32_t token = ((tblock * ROT_TILES + it) * ROT_THREADS + threadIdx.x) >> g.lpr_log2;
+    const bool live = token < tokens;
+    if (__all_sync(0xffffffffu, !live)) break;
+    if (!live) token = 0;
+    const uint32_t b = g.episode(token), n = token - b * (uint32_t)p.N;
+    const T* src = X + b * st.b + n * st.n;
+    const T* gsrc = Gr + b * sg.b + n * sg.n;
+    T* dst = D + (int64_t)token * heads * p.d;
+    Raw<T, E> a[HC][NP], bb[HC][NP], ra[HC][NP], rb[HC][NP];
 #pragma unroll
     for (int h = 0; h < HC; ++h) {
-      float ss = 0.f, dot = 0.f;
+      const bool ok = live && h0 + h < heads;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        const Slot<E, ADJ>& sl = i ? sl1 : sl0;
+        a[h][i].load(src + h * st.h + sl[i].col.ca, ok && sl[i].col.ok_a);
+        bb[h][i].load(src + h * st.h + sl[i].col.cb, ok && sl[i].col.ok_b);
+        ra[h][i].load(gsrc + h * sg.h + sl[i].col.ca, ok && sl[i].col.ok_a);
+        rb[h][i].load(gsrc + h * sg.h + sl[i].col.cb, ok && sl[i].col.ok_b);
+      }
+    }
+    const int64_t tab = (int64_t)b * p.table_b + (int64_t)n * (p.r / 2);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) sl[i].tables(p.cos + tab, p.sin + tab, p.r, g.table_vec != 0);
+#pragma unroll
+    for (int h = 0; h < HC; ++h) {
+        float x[NP][E], y[NP][E], ga[NP][E], gb[NP][E];  // ga, gb: dz
+      float acc[E], dot[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = dot[e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        a[h][i].widen(x[i]);
+        bb[h][i].widen(y[i]);
+        ra[h][i].widen(ga[i]);
+        rb[h][i].widen(gb[i]);
         float ns[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) ns[e] = -sl.s[e];
-        turn<E, ADJ>(ga[h][i], gb[h][i], sl.c, ns);  // dz
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          ss = fmaf(a[h][i][e], a[h][i][e], fmaf(bb[h][i][e], bb[h][i][e], ss));
-          dot = fmaf(ga[h][i][e] * sl.wa[e], a[h][i][e],
-                     fmaf(gb[h][i][e] * sl.wb[e], bb[h][i][e], dot));
-        }
+        for (int e = 0; e < E; ++e) ns[e] = -sl[i].s[e];
+        turn<E, ADJ>(ga[i], gb[i], sl[i].c, ns, sl[i].s);
+        vfma<E>(acc, x[i], x[i], acc);
+        vfma<E>(acc, y[i], y[i], acc);
+        float t[E];
+        vmul<E>(t, ga[i], wa[i]);
+        vfma<E>(dot, t, x[i], dot);
+        vmul<E>(t, gb[i], wb[i]);
+        vfma<E>(dot, t, y[i], dot);
       }
-      const float rs = rsqrtf(row_sum(ss, lpr) * inv_d + p.eps);
-      const float m = row_sum(dot, lpr) * inv_d * rs * rs;
+      const float rs = rsqrtf(fmaf(row_sum(vsum<E>(acc), g.lpr), g.inv_d, p.eps));
+      const float m = row_sum(vsum<E>(dot), g.lpr) * g.inv_d * rs * rs;
+      const bool ok = live && h0 + h < heads;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        const Slot<E, ADJ>& sl = i ? sl1 : sl0;
-        float xa[E], xb[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          dwa[i][e] = fmaf(ga[h][i][e], a[h][i][e] * rs, dwa[i][e]);
-          dwb[i][e] = fmaf(gb[h][i][e], bb[h][i][e] * rs, dwb[i][e]);
-          xa[e] = rs * fmaf(-a[h][i][e], m, ga[h][i][e] * sl.wa[e]);
-          xb[e] = rs * fmaf(-bb[h][i][e], m, gb[h][i][e] * sl.wb[e]);
-        }
-        const bool ok = live && h0 + h < heads;
-        st_pack<T, E>(dst + (int64_t)h * p.d + sl.col.ca, xa, ok && sl.col.ok_a);
-        st_pack<T, E>(dst + (int64_t)h * p.d + sl.col.cb, xb, ok && sl.col.ok_b);
+        float t[E], u[E];
+        vmul1<E>(t, x[i], rs);
+        vfma<E>(dwa[i], ga[i], t, dwa[i]);
+        vmul1<E>(t, y[i], rs);
+        vfma<E>(dwb[i], gb[i], t, dwb[i]);
+        vmul<E>(t, ga[i], wa[i]);
+        vfma1<E>(u, x[i], -m, t);
+        vmul1<E>(u, u, rs);
+        st_pack<T, E>(dst + h * p.d + sl[i].col.ca, u, ok && sl[i].col.ok_a);
+        vmul<E>(t, gb[i], wb[i]);
+        vfma1<E>(u, y[i], -m, t);
+        vmul1<E>(u, u, rs);
+        st_pack<T, E>(dst + h * p.d + sl[i].col.cb, u, ok && sl[i].col.ok_b);
       }
     }
   }
   // the warp's groups, then the block's warps, in a fixed order
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const Slot<E, ADJ>& sl = i ? sl1 : sl0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       float x = dwa[i][e], y = dwb[i][e];
-      for (int o = lpr; o < 32; o <<= 1) {
-        x += __shfl_xor_sync(0xffffffffu, x, o);
-        y += __shfl_xor_sync(0xffffffffu, y, o);
-      }
-      if (lane < lpr) {
-        if (sl.col.ok_a) red[warp][sl.col.ca + e] = x;
-        if (sl.col.ok_b) red[warp][sl.col.cb + e] = y;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1)
+        if (o >= g.lpr) {
+          x += __shfl_xor_sync(0xffffffffu, x, o);
+          y += __shfl_xor_sync(0xffffffffu, y, o);
+        }
+      if (lane < g.lpr) {
+        if (sl[i].col.ok_a) red[warp][sl[i].col.ca + e] = x;
+        if (sl[i].col.ok_b) red[warp][sl[i].col.cb + e] = y;
       }
     }
   }
@@ -319,32 +459,58 @@ __global__ void __launch_bounds__(ROT_THREADS) rotate_bwd_kernel(RotateParams p,
   if (threadIdx.x < p.d) {
     float t = 0.f;
 #pragma unroll
-    for (int w = 0; w < ROT_THREADS / 32; ++w) t += red[w][threadIdx.x];
+    for (int x = 0; x < ROT_THREADS / 32; ++x) t += red[x][threadIdx.x];
     p.work[(int64_t)blockIdx.x * p.d + threadIdx.x] = t;
   }
 }
 
-// block 0: dwq from the rows [0, nq) of the per-block sums; block 1: dwk from
-// the rows [nq, n). 8 slices of rows per column, joined in order.
-__global__ void __launch_bounds__(1024) rotate_dw_kernel(const float* work, int nq, int n,
-                                                         int d, float* dwq, float* dwk) {
+template <typename T, int E, bool ADJ, int NP>
+__global__ void __launch_bounds__(ROT_THREADS, 2) rotate_bwd_kernel(RotateParams p, RotGrid g) {
+  __shared__ float red[ROT_THREADS / 32][128];
+  const RotUnit w(g);
+  if (w.is_q ? g.four_q : g.four_k)
+    rotate_bwd_unit<T, E, ADJ, NP, 4>(p, g, w, red);
+  else
+    rotate_bwd_unit<T, E, ADJ, NP, 2>(p, g, w, red);
+}
+
+// Sum rows of `src`, [tb, parts] rows of d: block (x, 0) adds the query
+// chunks, (x, 1) the key chunks of its share of tb, into row x of dst_q or
+// dst_k (rows `dst_stride` apart). Eight lines of rows per column, joined in
+// order.
+__global__ void __launch_bounds__(1024) rotate_dw_kernel(const float* src, int tb, int parts,
+                                                         int cq, int d, float* dst_q,
+                                                         float* dst_k, int dst_stride) {
   __shared__ float red[8][128];
-  const int c = threadIdx.x & 127, slice = threadIdx.x >> 7;
-  const int lo = blockIdx.x ? nq : 0, hi = blockIdx.x ? n : nq;
+  const int c = threadIdx.x & 127, line = threadIdx.x >> 7;
+  const int per = cdiv(tb, (int)gridDim.x), lo = (int)blockIdx.x * per, hi = min(tb, lo + per);
+  const int c0 = blockIdx.y ? cq : 0, c1 = blockIdx.y ? parts : cq;
+  float* dst = blockIdx.y ? dst_k : dst_q;
+  if (!dst) return;
   float t = 0.f;
   if (c < d)
-    for (int i = lo + slice; i < hi; i += 8) t += work[(int64_t)i * d + c];
-  red[slice][c] = t;
+    for (int i = lo + line; i < hi; i += 8)
+      for (int x = c0; x < c1; ++x) t += src[((int64_t)i * parts + x) * d + c];
+  red[line][c] = t;
   __syncthreads();
-  float* out = blockIdx.x ? dwk : dwq;
-  if (slice == 0 && c < d && out) {
+  if (line == 0 && c < d) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) t += red[i][c];
-    out[c] = t;
+    dst[(int64_t)blockIdx.x * dst_stride + c] = t;
   }
 }
 
-int64_t rotate_bwd_work(int d) { return (int64_t)ROT_BWD_BLOCKS * d; }
+
+static int64_t rotate_row_blocks(int64_t tokens, int lpr) {
+  const int64_t rows = (int64_t)ROT_TILES * (ROT_THREADS / lpr);
+  return (tokens + rows - 1) / rows;
+}
+
+int64_t rotate_bwd_work(int64_t tokens, int H, int Hk, int d) {
+  // the narrowest rows of blocks: 32 lanes a row
+  return (rotate_row_blocks(tokens, 32) * (cdiv(H, 2) + cdiv(Hk, 2)) +
+          2 * ROT_SLICES) * d;
+}
 
 static int pow2_at_least(int x) {
   int r = 1;
@@ -352,10 +518,12 @@ static int pow2_at_least(int x) {
   return r;
 }
 
-// Widest vector (in elements) that every row start, head start and column
-// group of these tensors allows.
+// Widest vector (in elements, at most 4) that every row start, head start and
+// column group of these tensors allows. bf16 vectors of 8 were slower: their
+// weights, tables and sums take 176 registers a thread, which leaves too few
+// loads in flight (4 x 8192 rows of 20 heads, d = 128: 157 against 70 us).
 static int rotate_width(const RotateParams& p, int es, bool bwd) {
-  int e = 16 / es;
+  int e = 4;
   auto fits = [&](int w) {
     const uintptr_t a = (uintptr_t)(w * es - 1);
     auto ok = [&](const void* ptr, const HeadStrides& s) {
@@ -382,29 +550,46 @@ static int rotate_lanes(const RotateParams& p, int e) {
 template <typename T, int E, bool ADJ>
 static cudaError_t rotate_go(const RotateParams& p, bool bwd, cudaStream_t s) {
   constexpr int NP = E == 1 ? 2 : 1;  // scalar columns: up to 64 pairs a row
-  const int lpr = E == 1 ? 32 : rotate_lanes(p, E);
-  const int groups = ROT_THREADS / lpr;
+  auto grid16 = [](const void* x) { return (uintptr_t)x % 16 == 0; };
+  RotGrid g = {};
+  g.lpr = E == 1 ? 32 : rotate_lanes(p, E);
+  while ((1 << g.lpr_log2) < g.lpr) ++g.lpr_log2;
+  g.inv_d = 1.f / (float)p.d;
+  g.table_vec = p.r / 2 % 4 == 0 && p.table_b % 4 == 0 && grid16(p.cos) && grid16(p.sin);
+  g.weight_vec = p.d % 4 == 0 && grid16(p.wq) && grid16(p.wk);
+  if (p.N > 1) {
+    int l = 0;
+    while (((uint64_t)1 << l) < (uint64_t)p.N) ++l;
+    g.shift = (uint32_t)l - 1;
+    g.mul = (uint32_t)((((uint64_t)1 << (31 + l)) + (uint64_t)p.N - 1) / (uint64_t)p.N);
+  }
+  const int groups = ROT_THREADS / g.lpr;
   const int64_t tokens = (int64_t)p.B * p.N;
+  g.four_q = p.H % 4 == 0;
+  g.four_k = p.Hk % 4 == 0;
+  const int cq = cdiv(p.H, g.four_q ? 4 : 2);
+  g.parts_q = cq;
+  g.parts = cq + cdiv(p.Hk, g.four_k ? 4 : 2);
   if (!bwd) {
-    const int64_t units = tokens * (cdiv(p.H, ROT_HC) + cdiv(p.Hk, ROT_HC));
-    const int64_t blocks = (units + groups - 1) / groups;
+    const int64_t blocks = (tokens + groups - 1) / groups * g.parts;
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    rotate_kernel<T, E, ADJ, NP><<<(unsigned)blocks, ROT_THREADS, 0, s>>>(p, lpr);
+    rotate_kernel<T, E, ADJ, NP><<<(unsigned)blocks, ROT_THREADS, 0, s>>>(p, g);
     return cudaGetLastError();
   }
-  // enough blocks for the work, at most ROT_BWD_BLOCKS, shared out by heads
-  const int64_t uq = tokens * cdiv(p.H, 2), uk = tokens * cdiv(p.Hk, 2);
-  int64_t want = (uq + uk + groups - 1) / groups;
-  if (want > ROT_BWD_BLOCKS) want = ROT_BWD_BLOCKS;
-  if (want < 2) want = 2;
-  int nq = (int)((want * uq + (uq + uk) / 2) / (uq + uk));
-  if (nq < 1) nq = 1;
-  if (nq > want - 1) nq = (int)want - 1;
-  rotate_bwd_kernel<T, E, ADJ, NP><<<(unsigned)want, ROT_THREADS, 0, s>>>(p, lpr, nq);
+  const int64_t tb = rotate_row_blocks(tokens, g.lpr);
+  if (tb * g.parts > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  rotate_bwd_kernel<T, E, ADJ, NP><<<(unsigned)(tb * g.parts), ROT_THREADS, 0, s>>>(p, g);
   cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  if (p.dwq || p.dwk)
-    rotate_dw_kernel<<<2, 1024, 0, s>>>(p.work, nq, (int)want, p.d, p.dwq, p.dwk);
+  if (e != cudaSuccess || (!p.dwq && !p.dwk)) return e;
+  if (tb <= ROT_SLICES) {
+    rotate_dw_kernel<<<dim3(1, 2), 1024, 0, s>>>(p.work, (int)tb, g.parts, cq, p.d, p.dwq, p.dwk,
+                                                 0);
+  } else {
+    float* part = p.work + tb * g.parts * p.d;  // [ROT_SLICES][2][d]
+    rotate_dw_kernel<<<dim3(ROT_SLICES, 2), 1024, 0, s>>>(p.work, (int)tb, g.parts, cq, p.d, part,
+                                                          part + p.d, 2 * p.d);
+    rotate_dw_kernel<<<dim3(1, 2), 1024, 0, s>>>(part, ROT_SLICES, 2, 1, p.d, p.dwq, p.dwk, 0);
+  }
   return cudaGetLastError();
 }
 
@@ -412,9 +597,6 @@ template <typename T>
 static cudaError_t rotate_any(const RotateParams& p, bool bwd, cudaStream_t s) {
   const int e = rotate_width(p, (int)sizeof(T), bwd);
   const bool adj = p.interleaved != 0;
-  if constexpr (sizeof(T) == 2) {
-    if (e == 8) return adj ? rotate_go<T, 8, true>(p, bwd, s) : rotate_go<T, 8, false>(p, bwd, s);
-  }
   if (e == 4) return adj ? rotate_go<T, 4, true>(p, bwd, s) : rotate_go<T, 4, false>(p, bwd, s);
   if (e == 2) return adj ? rotate_go<T, 2, true>(p, bwd, s) : rotate_go<T, 2, false>(p, bwd, s);
   return rotate_go<T, 1, false>(p, bwd, s);

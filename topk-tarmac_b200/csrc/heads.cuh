@@ -24,7 +24,7 @@ struct RotateParams {
   const float *cos, *sin;     // [Bt, N, r / 2]
   int64_t table_b;            // batch stride of the tables (0: one for all)
   float *dwq, *dwk;           // [d] or NULL
-  float* work;                // backward: one row of d sums per block
+  float* work;                // backward: rows of d sums
   int B, N, H, Hk, d, r;
   float eps;
   int interleaved;
@@ -32,8 +32,8 @@ struct RotateParams {
 
 cudaError_t launch_rotate(const RotateParams& p, bool bf16, cudaStream_t s);
 cudaError_t launch_rotate_bwd(const RotateParams& p, bool bf16, cudaStream_t s);
-// floats of `work` that the backward call needs
-int64_t rotate_bwd_work(int d);
+// floats of `work` that the backward call needs at most
+int64_t rotate_bwd_work(int64_t tokens, int H, int Hk, int d);
 
 // who a row may see (beside key_len and the visibility words)
 enum HeadPeers { PEERS_ALL = 0, PEERS_OTHERS = 1, PEERS_PAST = 2 };

@@ -34,6 +34,7 @@ int check_rotate(const void* q, const void* k, const float* cs, const float* sn,
   if (H < 1 || Hk < 1 || r < 0 || r > d || (r & 1)) return TARMAC_ERR_HEADS;
   if (!(eps >= 0.f) || isinf(eps)) return TARMAC_ERR_SHAPE;
   if ((int64_t)B * N == 0) return TARMAC_OK;
+  if ((int64_t)B * N > 0x7fffffff) return TARMAC_ERR_N_TOO_LARGE;  // rows in 31 bits
   if (!q || !k || (r > 0 && (!cs || !sn))) return TARMAC_ERR_NULL;
   const int es = dtype == TARMAC_BF16 ? 2 : 4;
   if (!aligned(q, es) || !aligned(k, es) || !aligned(cs, 4) || !aligned(sn, 4))
@@ -130,8 +131,9 @@ int tarmac_qk_norm_rotate(const void* q, const void* k, void* q_out, void* k_out
   return status(launch_rotate(p, dtype == TARMAC_BF16, (cudaStream_t)stream));
 }
 
-int64_t tarmac_qk_norm_rotate_workspace(int d) {
-  return d < 1 || d > MAX_D ? 0 : rotate_bwd_work(d) * 4;
+int64_t tarmac_qk_norm_rotate_workspace(int B, int N, int H, int Hk, int d) {
+  if (B < 1 || N < 1 || H < 1 || Hk < 1 || d < 1 || d > MAX_D) return 0;
+  return rotate_bwd_work((int64_t)B * N, H, Hk, d) * 4;
 }
 
 int tarmac_qk_norm_rotate_backward(const void* q, const void* k, const void* dq_out,

@@ -92,7 +92,8 @@ SIGNATURES: dict[str, tuple] = {
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
         c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int,
         c_int, c_float, c_int, c_void_p]),
-    "tarmac_qk_norm_rotate_workspace": (c_int64, [c_int]),
+    "tarmac_qk_norm_rotate_workspace": (c_int64, [
+        c_int, c_int, c_int, c_int, c_int]),
     "tarmac_qk_norm_rotate_backward": (c_int, [
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
         c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int,

@@ -510,7 +510,7 @@ def qk_norm_rotate_backward(q: torch.Tensor, k: torch.Tensor,
     new = dict(device=q.device, dtype=torch.float32)
     dwq = None if wq is None else torch.empty(d, **new)
     dwk = None if wk is None else torch.empty(d, **new)
-    work = torch.empty(_rotate_work(d) // 4, **new)
+    work = torch.empty(_rotate_work(B, N, H, k.shape[2], d) // 4, **new)
     with _on(q.device):
         _lib.call("tarmac_qk_norm_rotate_backward", _ptr(q), _ptr(k), _ptr(gq),
                   _ptr(gk),
@@ -524,9 +524,9 @@ def qk_norm_rotate_backward(q: torch.Tensor, k: torch.Tensor,
     return dq, dk, dwq, dwk
 
 
-@functools.lru_cache(maxsize=None)
-def _rotate_work(d: int) -> int:
-    return _lib.lib().tarmac_qk_norm_rotate_workspace(d)
+@functools.lru_cache(maxsize=1024)
+def _rotate_work(B, N, H, Hk, d) -> int:
+    return _lib.lib().tarmac_qk_norm_rotate_workspace(B, N, H, Hk, d)
 
 
 def pack_visibility(visible: torch.Tensor) -> torch.Tensor:
