@@ -739,7 +739,9 @@ constexpr int HA_SMS = 148;
 constexpr int HA_NARROW_ROWS = 16;
 
 // Parts of the key axis: with fewer blocks than the GPU holds at once, split
-// until there are about four per SM, each of at least 256 keys.
+// until there are about sixteen per SM, each of at least 256 keys: ragged
+// lengths leave parts without keys, and short parts even that out (32 episodes
+// of up to 16384 keys: TODO us with 16 per SM, 110 with 4).
 void head_split_plan(int B, int Nq, int Nk, int H, int Hk, int* splits, int* split_keys) {
   const int64_t rows = (int64_t)Nq * (H / Hk);
   const int tile = rows <= HA_NARROW_ROWS ? 16 : 64;
@@ -747,7 +749,7 @@ void head_split_plan(int B, int Nq, int Nk, int H, int Hk, int* splits, int* spl
   *splits = 1;
   *split_keys = Nk;
   if (base >= 2 * HA_SMS || Nk < 512) return;
-  int64_t n = (4 * HA_SMS + base - 1) / base;
+  int64_t n = (16 * HA_SMS + base - 1) / base;
   if (n > Nk / 256) n = Nk / 256;
   if (n < 2) return;
   const int keys = cdiv(cdiv(Nk, (int)n), 64) * 64;

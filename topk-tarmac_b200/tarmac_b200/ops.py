@@ -465,6 +465,47 @@ def _check_rotate(q, k, wq, wk, cos, sin):
             sin.contiguous())
 
 
+def _rotate_ready(q, k, wq, wk, cos, sin) -> bool:
+    """Whether the arguments can be passed on as they are. Cheap: a call on a
+    few rows is bound by its host work, so the checks that name a fault
+    (:func:`_check_rotate`) run only when this one fails."""
+    qs, ks, cs = q.shape, k.shape, cos.shape
+    if len(qs) != 4 or len(ks) != 4 or len(cs) != 3 or sin.shape != cs:
+        return False
+    B, N, _, d = qs
+    t, dev = q.dtype, q.get_device()
+    f32 = torch.float32
+    return (t in _DTYPES and k.dtype is t and cos.dtype is f32 and sin.dtype is f32
+            and dev >= 0 and k.get_device() == dev and cos.get_device() == dev
+            and sin.get_device() == dev and ks[0] == B and ks[1] == N and ks[3] == d
+            and (cs[0] == 1 or cs[0] == B) and cs[1] == N and 2 * cs[2] <= d
+            and q.stride(3) == 1 and k.stride(3) == 1
+            and cos.is_contiguous() and sin.is_contiguous()
+            and (wq is None or (wq.dtype is f32 and wq.shape == (d,)
+                                and wq.get_device() == dev and wq.stride(0) == 1))
+            and (wk is None or (wk.dtype is f32 and wk.shape == (d,)
+                                and wk.get_device() == dev and wk.stride(0) == 1)))
+
+
+def _launch(dev: int, name: str, *args) -> None:
+    """Call an entry point on the current stream of CUDA device ``dev`` (the
+    stream is the last argument of every entry point)."""
+    if dev == _GET_DEVICE():
+        _lib.call(name, *args, _stream_of(dev))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, _stream_of(dev))
+
+
+_GET_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _stream_of(dev: int) -> int:
+    if _RAW_STREAM is not None:
+        return _RAW_STREAM(dev)
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
 def _table_stride(cos: torch.Tensor, B: int) -> int:
     """Elements between two episodes' tables (0: one table for all)."""
     return cos.shape[1] * cos.shape[2] if cos.shape[0] == B and B > 1 else 0
@@ -480,15 +521,16 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor,
     [1 or B, N, r / 2]; column pairs are (i, i + r / 2), or (2i, 2i + 1) with
     ``interleaved``. Returns contiguous (q', k') in the inputs' dtype. The
     single-token form is N = 1 with the token's row of the table."""
-    q, k, wq, wk, cos, sin = _check_rotate(q, k, wq, wk, cos, sin)
+    if not _rotate_ready(q, k, wq, wk, cos, sin):
+        q, k, wq, wk, cos, sin = _check_rotate(q, k, wq, wk, cos, sin)
     B, N, H, d = q.shape
     qo, ko = _empty_as(q), _empty_as(k)
-    with _on(q.device):
-        _lib.call("tarmac_qk_norm_rotate", _ptr(q), _ptr(k), _ptr(qo),
-                  _ptr(ko), _PACK6(*q.stride()[:3], *k.stride()[:3]), _ptr(wq),
-                  _ptr(wk), _ptr(cos), _ptr(sin), _table_stride(cos, B), B, N,
-                  H, k.shape[2], d, 2 * cos.shape[2], _DTYPES[q.dtype], eps,
-                  int(interleaved), _stream(q.device))
+    _launch(q.get_device(), "tarmac_qk_norm_rotate", q.data_ptr(),
+            k.data_ptr(), qo.data_ptr(), ko.data_ptr(),
+            _PACK6(*q.stride()[:3], *k.stride()[:3]), _ptr(wq), _ptr(wk),
+            cos.data_ptr(), sin.data_ptr(), _table_stride(cos, B), B, N, H,
+            k.shape[2], d, 2 * cos.shape[2], _DTYPES[q.dtype], eps,
+            int(interleaved))
     return qo, ko
 
 
@@ -500,28 +542,35 @@ def qk_norm_rotate_backward(q: torch.Tensor, k: torch.Tensor,
     """Gradients of :func:`qk_norm_rotate` for its inputs and the gradients of
     its outputs: (dq, dk) in the inputs' dtype and (dwq, dwk) fp32 [d] (None
     where there is no weight). Deterministic."""
-    q, k, wq, wk, cos, sin = _check_rotate(q, k, wq, wk, cos, sin)
-    _check_heads({"dq_out": dq_out, "dk_out": dk_out}, q)
-    if dq_out.shape != q.shape or dk_out.shape != k.shape:
-        raise ValueError("dq_out and dk_out must have the shapes of q and k")
-    gq, gk = _unit_inner(dq_out), _unit_inner(dk_out)
+    if not _rotate_ready(q, k, wq, wk, cos, sin):
+        q, k, wq, wk, cos, sin = _check_rotate(q, k, wq, wk, cos, sin)
+    gq, gk = _gradient(dq_out, q, "dq_out"), _gradient(dk_out, k, "dk_out")
     B, N, H, d = q.shape
     dq, dk = _empty_as(q), _empty_as(k)
-    new = dict(device=q.device, dtype=torch.float32)
-    dwq = None if wq is None else torch.empty(d, **new)
-    dwk = None if wk is None else torch.empty(d, **new)
-    work = torch.empty(_rotate_work(B, N, H, k.shape[2], d) // 4, **new)
-    with _on(q.device):
-        _lib.call("tarmac_qk_norm_rotate_backward", _ptr(q), _ptr(k), _ptr(gq),
-                  _ptr(gk),
-                  _PACK12(*q.stride()[:3], *k.stride()[:3], *gq.stride()[:3],
-                          *gk.stride()[:3]),
-                  _ptr(wq), _ptr(wk), _ptr(cos), _ptr(sin),
-                  _table_stride(cos, B), B, N, H, k.shape[2], d,
-                  2 * cos.shape[2], _DTYPES[q.dtype], eps, int(interleaved),
-                  _ptr(dq), _ptr(dk), _ptr(dwq), _ptr(dwk), _ptr(work),
-                  _stream(q.device))
+    work = torch.empty(_rotate_work(B, N, H, k.shape[2], d) // 4,
+                       device=q.device, dtype=torch.float32)
+    dwq, dwk = torch.empty((2, d), device=q.device, dtype=torch.float32)
+    dwq = None if wq is None else dwq
+    dwk = None if wk is None else dwk
+    _launch(q.get_device(), "tarmac_qk_norm_rotate_backward", q.data_ptr(),
+            k.data_ptr(), gq.data_ptr(), gk.data_ptr(),
+            _PACK12(*q.stride()[:3], *k.stride()[:3], *gq.stride()[:3],
+                    *gk.stride()[:3]),
+            _ptr(wq), _ptr(wk), cos.data_ptr(), sin.data_ptr(),
+            _table_stride(cos, B), B, N, H, k.shape[2], d, 2 * cos.shape[2],
+            _DTYPES[q.dtype], eps, int(interleaved), dq.data_ptr(),
+            dk.data_ptr(), _ptr(dwq), _ptr(dwk), work.data_ptr())
     return dq, dk, dwq, dwk
+
+
+def _gradient(g: torch.Tensor, like: torch.Tensor, name: str) -> torch.Tensor:
+    """``g`` checked against the tensor it belongs to, with unit inner stride."""
+    if g.shape != like.shape:
+        raise ValueError(f"{name} must have the shape {tuple(like.shape)}; got "
+                         f"{tuple(g.shape)}")
+    if g.dtype is not like.dtype or g.get_device() != like.get_device():
+        _check_heads({name: g}, like)
+    return g if g.stride(3) == 1 else _unit_inner(g)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -592,6 +641,26 @@ def _check_attention(q, k, v, peers, key_len, q_start, visible):
     return _unit_inner(q), _unit_inner(k), _unit_inner(v), *ints, visible
 
 
+def _attention_ready(q, k, v, peers, key_len, q_start) -> bool:
+    """As :func:`_rotate_ready`, for calls without a visibility mask."""
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or v.shape != ks or peers not in _PEERS:
+        return False
+    t, dev = q.dtype, q.get_device()
+    if not (t in _DTYPES and k.dtype is t and v.dtype is t and dev >= 0
+            and k.get_device() == dev and v.get_device() == dev
+            and ks[0] == qs[0] and ks[3] == qs[3] and ks[2] > 0
+            and qs[2] % ks[2] == 0 and q.stride(3) == 1 and k.stride(3) == 1
+            and v.stride(3) == 1):
+        return False
+    for x in (key_len, q_start):
+        if x is not None and not (
+                x.dtype is torch.int32 and x.shape == (qs[0],)
+                and x.get_device() == dev and x.is_contiguous()):
+            return False
+    return True
+
+
 def _bits_stride(bits: torch.Tensor | None) -> int:
     """Words between two episodes' masks (0: one mask for all)."""
     if bits is None or bits.shape[0] == 1:
@@ -626,23 +695,26 @@ def head_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     and values from ``key_len`` on are not read; what a row sees must be
     finite. One token over a long history is Nq = 1: the key axis is then
     split over the GPU."""
-    q, k, v, key_len, q_start, bits = _check_attention(
-        q, k, v, peers, key_len, q_start, visible)
+    if visible is None and _attention_ready(q, k, v, peers, key_len, q_start):
+        bits = None
+    else:
+        q, k, v, key_len, q_start, bits = _check_attention(
+            q, k, v, peers, key_len, q_start, visible)
     B, Nq, H, d = q.shape
-    Nk, Hk = k.shape[1], k.shape[2]
+    _, Nk, Hk, _ = k.shape
+    dev = q.get_device()
     out = _empty_as(q)
     lse = (torch.empty((B, H, Nq), device=q.device, dtype=torch.float32)
            if return_lse else None)
     nbytes = _attention_work(B, Nq, Nk, H, Hk, d)
     work = (torch.empty(nbytes, device=q.device, dtype=torch.uint8)
             if nbytes else None)
-    with _on(q.device):
-        _lib.call("tarmac_head_attention", _ptr(q), _ptr(k), _ptr(v),
-                  _ptr(out), _ptr(lse),
-                  _PACK9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]),
-                  _ptr(key_len), _ptr(q_start), _ptr(bits), _bits_stride(bits),
-                  B, Nq, Nk, H, Hk, d, _DTYPES[q.dtype], _PEERS[peers],
-                  _scale(d, scale), _ptr(work), _stream(q.device))
+    _launch(dev, "tarmac_head_attention", q.data_ptr(), k.data_ptr(),
+            v.data_ptr(), out.data_ptr(), _ptr(lse),
+            _PACK9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]),
+            _ptr(key_len), _ptr(q_start), _ptr(bits), _bits_stride(bits), B,
+            Nq, Nk, H, Hk, d, _DTYPES[q.dtype], _PEERS[peers],
+            _scale(d, scale), _ptr(work))
     return (out, lse) if return_lse else out
 
 
@@ -657,30 +729,31 @@ def head_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     given its ``out`` and ``lse`` and the gradient of out. The probabilities
     are recomputed; shared key heads are summed over their query heads;
     deterministic."""
-    q, k, v, key_len, q_start, bits = _check_attention(
-        q, k, v, peers, key_len, q_start, visible)
+    if visible is None and _attention_ready(q, k, v, peers, key_len, q_start):
+        bits = None
+    else:
+        q, k, v, key_len, q_start, bits = _check_attention(
+            q, k, v, peers, key_len, q_start, visible)
     B, Nq, H, d = q.shape
-    Nk, Hk = k.shape[1], k.shape[2]
-    _check_heads({"out": out, "dout": dout}, q)
-    if out.shape != q.shape or dout.shape != q.shape:
-        raise ValueError("out and dout must have the shape of q")
-    if tuple(lse.shape) != (B, H, Nq) or lse.dtype != torch.float32 \
-            or lse.device != q.device:
+    _, Nk, Hk, _ = k.shape
+    out, dout = _gradient(out, q, "out"), _gradient(dout, q, "dout")
+    if lse.shape != (B, H, Nq) or lse.dtype is not torch.float32 \
+            or lse.get_device() != q.get_device():
         raise ValueError(f"lse must be float32 [{B}, {H}, {Nq}] on the device "
                          "of the queries")
-    out, dout, lse = _unit_inner(out), _unit_inner(dout), lse.contiguous()
+    lse = lse.contiguous()
     dq, dk, dv = _empty_as(q), _empty_as(k), _empty_as(v)
     work = torch.empty(_attention_backward_work(B, Nq, H), device=q.device,
                        dtype=torch.uint8)
-    with _on(q.device):
-        _lib.call("tarmac_head_attention_backward", _ptr(q), _ptr(k), _ptr(v),
-                  _ptr(out), _ptr(lse), _ptr(dout),
-                  _PACK15(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
-                          *out.stride()[:3], *dout.stride()[:3]),
-                  _ptr(key_len), _ptr(q_start), _ptr(bits), _bits_stride(bits),
-                  B, Nq, Nk, H, Hk, d, _DTYPES[q.dtype], _PEERS[peers],
-                  _scale(d, scale), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(work),
-                  _stream(q.device))
+    _launch(q.get_device(), "tarmac_head_attention_backward", q.data_ptr(),
+            k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+            dout.data_ptr(),
+            _PACK15(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                    *out.stride()[:3], *dout.stride()[:3]),
+            _ptr(key_len), _ptr(q_start), _ptr(bits), _bits_stride(bits), B,
+            Nq, Nk, H, Hk, d, _DTYPES[q.dtype], _PEERS[peers],
+            _scale(d, scale), dq.data_ptr(),
+            dk.data_ptr(), dv.data_ptr(), work.data_ptr())
     return dq, dk, dv
 
 
