@@ -59,6 +59,38 @@ __device__ __forceinline__ void load_tile(T* dst, int n, int limit, int d, int v
   }
 }
 
+// The same for rows a constant stride apart (neighbouring keys). Where a row's
+// pieces divide the block evenly, a thread keeps its column and walks down the
+// rows, which leaves an add and a compare per 16 bytes: a tile's copies are a
+// third of the instructions of a call on few rows otherwise.
+template <typename T, int DP>
+__device__ __forceinline__ void load_keys_tile(T* dst, int n, int limit, int d, int vec,
+                                               const T* first, int64_t stride) {
+  constexpr int E = 16 / (int)sizeof(T);
+  constexpr int CH = DP / E;
+  constexpr int RS = hm::row_stride<T, DP>();
+  if constexpr (HA_THREADS % CH == 0) {
+    if (vec) {
+      constexpr int STEP = HA_THREADS / CH;
+      const int c = (threadIdx.x % CH) * E;
+      int r = threadIdx.x / CH;
+      uint32_t s = tc_smem_base(dst + r * RS + c);
+      const T* g = first + r * stride + c;
+      const int lim = c < d ? limit : 0;
+#pragma unroll
+      for (int i = 0; i < 64 / STEP; ++i, r += STEP, s += STEP * RS * sizeof(T), g += STEP * stride) {
+        if (r >= n) break;
+        // no bytes are read where the row does not exist
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s),
+                     "l"(r < lim ? g : first), "r"(r < lim ? 16 : 0)
+                     : "memory");
+      }
+      return;
+    }
+  }
+  load_tile<T, DP>(dst, n, limit, d, vec, [&](int r) { return first + r * stride; });
+}
+
 // visible: does the row see key j? jlim: first key beyond key_len and, for
 // past, beyond the row's position; self: the key left out, or -1.
 __device__ __forceinline__ bool sees(int j, int jlim, int self, uint32_t word) {
@@ -162,10 +194,9 @@ __global__ void __launch_bounds__(HA_THREADS) head_fwd_kernel(HeadAttnParams p) 
   auto load_keys = [&](int t) {
     T* sK = ring + (t % C::STAGES) * 2 * KT * RS;
     const int k0 = kbeg + t * KT;
-    load_tile<T, DP>(sK, KT, kend - k0, p.d, p.vec,
-                     [&](int r) { return K + (int64_t)(k0 + r) * p.sk.n; });
-    load_tile<T, DP>(sK + KT * RS, KT, kend - k0, p.d, p.vec,
-                     [&](int r) { return V + (int64_t)(k0 + r) * p.sv.n; });
+    load_keys_tile<T, DP>(sK, KT, kend - k0, p.d, p.vec, K + (int64_t)k0 * p.sk.n, p.sk.n);
+    load_keys_tile<T, DP>(sK + KT * RS, KT, kend - k0, p.d, p.vec, V + (int64_t)k0 * p.sv.n,
+                          p.sv.n);
   };
   load_tile<T, DP>(sQ, C::ROWS, nrows, p.d, p.vec, [&](int r) {
     const int i = (r0 + r) / p.G, g = (r0 + r) - i * p.G;
@@ -306,7 +337,8 @@ __global__ void __launch_bounds__(HA_THREADS) head_fwd_kernel(HeadAttnParams p) 
         else if (p.lse)
           p.lse[srow] = lse;
       }
-      for (int c = threadIdx.x & 7; c < p.d; c += 8) {
+      // the join skips parts that saw nothing
+      for (int c = threadIdx.x & 7; c < p.d && !(p.splits > 1 && tot == 0.f); c += 8) {
         float x = 0.f;
 #pragma unroll
         for (int v = 0; v < HA_WARPS; ++v) x = fmaf(so[(v * 16 + r) * OS + c], fw[v], x);
@@ -354,11 +386,12 @@ __global__ void __launch_bounds__(HA_THREADS) head_fwd_kernel(HeadAttnParams p) 
 }
 
 // Join the parts of the key axis: out = sum_s w_s out_s, w_s = exp(lse_s -
-// lse). One warp per (episode, row, head).
+// lse). One warp per (episode, row, head): its lanes first hold the parts'
+// lse, then the columns.
 template <typename T>
-__global__ void __launch_bounds__(256) head_join_kernel(HeadAttnParams p) {
+__global__ void __launch_bounds__(128) head_join_kernel(HeadAttnParams p) {
   const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int64_t total = (int64_t)p.B * p.Nq * p.H;
   if (row >= total) return;
   const int h = (int)(row % p.H);
@@ -367,18 +400,34 @@ __global__ void __launch_bounds__(256) head_join_kernel(HeadAttnParams p) {
   const int b = (int)(bi / p.Nq);
   const int64_t srow = ((int64_t)b * p.H + h) * p.Nq + i;
   float top = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_lse[s * total + srow]);
-  float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-  if (top != -INFINITY) {
-    for (int s = 0; s < p.splits; ++s) {
-      const float ls = p.part_lse[s * total + srow];
-      if (ls == -INFINITY) continue;  // the part saw nothing
-      const float wgt = expf(ls - top);
-      sum += wgt;
-      const float* o = p.part_o + (s * total + row) * p.d;
+  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_lse[s * total + srow]);
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (lane + 32 * u < p.d) x[u] = fmaf(wgt, o[lane + 32 * u], x[u]);
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < p.splits && top != -INFINITY; s0 += 32) {
+    const float ls = s0 + lane < p.splits ? p.part_lse[(s0 + lane) * total + srow] : -INFINITY;
+    const float wgt = ls == -INFINITY ? 0.f : expf(ls - top);
+    // parts that saw nothing wrote nothing
+    uint32_t left = __ballot_sync(0xffffffffu, ls != -INFINITY);
+    while (left) {
+      float y[4][4], wv[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {  // four parts in flight
+        const int s = left ? __ffs(left) - 1 : -1;
+        if (s >= 0) left &= left - 1;
+        wv[q] = __shfl_sync(0xffffffffu, wgt, s < 0 ? 0 : s);
+        const float* o = p.part_o + ((int64_t)(s0 + (s < 0 ? 0 : s)) * total + row) * p.d;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          y[q][u] = s >= 0 && lane + 32 * u < p.d ? o[lane + 32 * u] : 0.f;
+        if (s < 0) wv[q] = 0.f;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        sum += wv[q];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = fmaf(wv[q], y[q][u], x[u]);
+      }
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -471,10 +520,9 @@ __global__ void __launch_bounds__(HA_THREADS) head_dq_kernel(HeadAttnParams p) {
   auto load_keys = [&](int t) {
     T* sK = ring + (t & 1) * 2 * KT * RS;
     const int k0 = t * KT;
-    load_tile<T, DP>(sK, KT, kend - k0, p.d, p.vec,
-                     [&](int r) { return K + (int64_t)(k0 + r) * p.sk.n; });
-    load_tile<T, DP>(sK + KT * RS, KT, kend - k0, p.d, p.vec,
-                     [&](int r) { return V + (int64_t)(k0 + r) * p.sv.n; });
+    load_keys_tile<T, DP>(sK, KT, kend - k0, p.d, p.vec, K + (int64_t)k0 * p.sk.n, p.sk.n);
+    load_keys_tile<T, DP>(sK + KT * RS, KT, kend - k0, p.d, p.vec, V + (int64_t)k0 * p.sv.n,
+                          p.sv.n);
   };
   auto row_of = [&](const T* base, const HeadStrides& s, int r) {
     const int i = (r0 + r) / p.G, g = (r0 + r) - i * p.G;
@@ -588,9 +636,15 @@ __global__ void __launch_bounds__(HA_THREADS) head_dkv_kernel(HeadAttnParams p) 
       const int i = (q0 + r) / p.G, g = (q0 + r) - i * p.G;
       return base + (int64_t)i * s.n + g * s.h;
     };
-    load_tile<T, DP>(sQ, QT, rows - q0, p.d, p.vec, [&](int r) { return row_of(Q, p.sq, r); });
-    load_tile<T, DP>(sQ + QT * RS, QT, rows - q0, p.d, p.vec,
-                     [&](int r) { return row_of(Gr, p.sg, r); });
+    if (p.G == 1) {
+      load_keys_tile<T, DP>(sQ, QT, rows - q0, p.d, p.vec, Q + (int64_t)q0 * p.sq.n, p.sq.n);
+      load_keys_tile<T, DP>(sQ + QT * RS, QT, rows - q0, p.d, p.vec, Gr + (int64_t)q0 * p.sg.n,
+                            p.sg.n);
+    } else {
+      load_tile<T, DP>(sQ, QT, rows - q0, p.d, p.vec, [&](int r) { return row_of(Q, p.sq, r); });
+      load_tile<T, DP>(sQ + QT * RS, QT, rows - q0, p.d, p.vec,
+                       [&](int r) { return row_of(Gr, p.sg, r); });
+    }
     if (threadIdx.x < QT) {
       const int r = q0 + threadIdx.x, x = threadIdx.x, st = t & 1;
       s_lse[st][x] = -INFINITY;
@@ -769,7 +823,7 @@ static cudaError_t fwd_go(const HeadAttnParams& p, cudaStream_t s) {
   e = cudaGetLastError();
   if (e != cudaSuccess || p.splits == 1) return e;
   const int64_t rows = (int64_t)p.B * p.Nq * p.H;
-  head_join_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(p);
+  head_join_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
   return cudaGetLastError();
 }
 
