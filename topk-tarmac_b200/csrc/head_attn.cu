@@ -91,6 +91,69 @@ __device__ __forceinline__ void load_keys_tile(T* dst, int n, int limit, int d, 
   load_tile<T, DP>(dst, n, limit, d, vec, [&](int r) { return first + r * stride; });
 }
 
+// fp32 rows of up to 32 columns are staged as split pairs (head_mma.cuh).
+template <typename T, int DP>
+constexpr bool ha_split() {
+  return sizeof(T) == 4 && DP <= 32;
+}
+
+// R rows of DP fp32 columns on their way from global memory to a split tile:
+// held in registers while the tile before them is used. Rows at or beyond
+// `limit` and columns at or beyond d are zero.
+template <int DP, int R>
+struct SplitRows {
+  static constexpr int C4 = DP / 4, U = R * C4 / HA_THREADS;
+  static_assert(R * C4 % HA_THREADS == 0, "whole pieces per thread");
+  float4 x[U];
+  template <typename F>
+  __device__ __forceinline__ void load(int limit, int d, int vec, F row_ptr) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = threadIdx.x + u * HA_THREADS, r = e / C4, c = (e % C4) * 4;
+      x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r >= limit || c >= d) continue;
+      const float* g = row_ptr(r) + c;
+      if (vec) {
+        x[u] = __ldg(reinterpret_cast<const float4*>(g));
+      } else {
+        x[u].x = g[0];
+        if (c + 1 < d) x[u].y = g[1];
+        if (c + 2 < d) x[u].z = g[2];
+        if (c + 3 < d) x[u].w = g[3];
+      }
+    }
+  }
+  __device__ __forceinline__ void store(float* tile) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = threadIdx.x + u * HA_THREADS;
+      hm::store_split<DP>(tile, e / C4, (e % C4) * 4, x[u]);
+    }
+  }
+};
+
+// Products on tiles of either kind.
+template <bool SPLIT, typename T, int DP, int NT>
+__device__ __forceinline__ void ha_scores(float (&c)[NT][4], const T* sA, const T* sB, int lane) {
+  if constexpr (SPLIT)
+    hm::scores_split<DP, NT>(c, sA, sB, lane);
+  else
+    hm::scores<DP, NT>(c, sA, sB, lane);
+}
+template <bool SPLIT, typename T, int DP, int NT>
+__device__ __forceinline__ void ha_aggregate(float (&o)[DP / 8][4], const float (&p)[NT][4],
+                                             const T* sB, int lane) {
+  if constexpr (SPLIT)
+    hm::aggregate_split<DP, NT>(o, p, sB, lane);
+  else
+    hm::aggregate<DP, NT>(o, p, sB, lane);
+}
+// column of score e (0 or 1) of a thread inside an 8-column tile
+template <bool SPLIT>
+__device__ __forceinline__ int ha_col(int lane, int e) {
+  return SPLIT ? (lane & 3) + 4 * e : 2 * (lane & 3) + e;
+}
+
 // visible: does the row see key j? jlim: first key beyond key_len and, for
 // past, beyond the row's position; self: the key left out, or -1.
 __device__ __forceinline__ bool sees(int j, int jlim, int self, uint32_t word) {
@@ -159,8 +222,9 @@ struct HaFwd {
   static constexpr int ROWS = NARROW ? 16 : 64;
   static constexpr int KT = NARROW ? 64 : ha_tile<T, DP>();
   static constexpr int NT = (NARROW ? 16 : KT) / 8;
-  static constexpr int RS = hm::row_stride<T, DP>();
-  static constexpr int STAGES = NARROW ? 3 : 2;
+  static constexpr bool SPLIT = !NARROW && ha_split<T, DP>();
+  static constexpr int RS = SPLIT ? hm::split_stride<DP>() : hm::row_stride<T, DP>();
+  static constexpr int STAGES = 2;
   static constexpr size_t STAGE = (size_t)2 * KT * RS * sizeof(T);
   static constexpr size_t SMEM = (size_t)ROWS * RS * sizeof(T) + STAGES * STAGE;
 };
@@ -169,6 +233,7 @@ template <typename T, int DP, bool NARROW>
 __global__ void __launch_bounds__(HA_THREADS) head_fwd_kernel(HeadAttnParams p) {
   using C = HaFwd<T, DP, NARROW>;
   constexpr int RS = C::RS, KT = C::KT, NT = C::NT;
+  constexpr bool SPLIT = C::SPLIT;
   extern __shared__ __align__(16) unsigned char ha_smem[];
   T* sQ = reinterpret_cast<T*>(ha_smem);
   T* ring = sQ + C::ROWS * RS;
@@ -198,13 +263,37 @@ __global__ void __launch_bounds__(HA_THREADS) head_fwd_kernel(HeadAttnParams p) 
     load_keys_tile<T, DP>(sK + KT * RS, KT, kend - k0, p.d, p.vec, V + (int64_t)k0 * p.sv.n,
                           p.sv.n);
   };
-  load_tile<T, DP>(sQ, C::ROWS, nrows, p.d, p.vec, [&](int r) {
+  auto q_row = [&](int r) {
     const int i = (r0 + r) / p.G, g = (r0 + r) - i * p.G;
     return Q + (int64_t)i * p.sq.n + g * p.sq.h;
-  });
-#pragma unroll
-  for (int t = 0; t < C::STAGES - 1; ++t) {
-    if (t < ntiles) load_keys(t);
+  };
+  // split rows: the next tile waits in registers
+  SplitRows<SPLIT ? DP : 16, SPLIT ? KT : 32> nk, nv;
+  auto fetch = [&](int t) {
+    if constexpr (SPLIT) {
+      const int k0 = kbeg + t * KT;
+      nk.load(kend - k0, p.d, p.vec, [&](int r) { return K + (int64_t)(k0 + r) * p.sk.n; });
+      nv.load(kend - k0, p.d, p.vec, [&](int r) { return V + (int64_t)(k0 + r) * p.sv.n; });
+    }
+  };
+  auto put = [&](int t) {
+    if constexpr (SPLIT) {
+      T* sK = ring + (t & 1) * 2 * KT * RS;
+      nk.store(sK);
+      nv.store(sK + KT * RS);
+    }
+  };
+  if constexpr (SPLIT) {
+    SplitRows<DP, C::ROWS> q;
+    q.load(nrows, p.d, p.vec, q_row);
+    q.store(sQ);
+    if (ntiles > 0) {
+      fetch(0);
+      put(0);
+    }
+  } else {
+    load_tile<T, DP>(sQ, C::ROWS, nrows, p.d, p.vec, q_row);
+    if (ntiles > 0) load_keys(0);
     cp_async_commit();
   }
 
@@ -230,16 +319,21 @@ __global__ void __launch_bounds__(HA_THREADS) head_fwd_kernel(HeadAttnParams p) 
     for (int u = 0; u < 4; ++u) o[n][u] = 0.f;
 
   for (int t = 0; t < ntiles; ++t) {
-    cp_async_wait<C::STAGES - 2>();
-    __syncthreads();
-    if (t + C::STAGES - 1 < ntiles) load_keys(t + C::STAGES - 1);
-    cp_async_commit();
+    if constexpr (SPLIT) {
+      __syncthreads();
+      if (t + 1 < ntiles) fetch(t + 1);
+    } else {
+      cp_async_wait<0>();
+      __syncthreads();
+      if (t + 1 < ntiles) load_keys(t + 1);
+      cp_async_commit();
+    }
     const T* sK = ring + (t % C::STAGES) * 2 * KT * RS + (NARROW ? warp * 16 * RS : 0);
     const T* sV = sK + KT * RS;
     const int k0 = kbeg + t * KT + (NARROW ? warp * 16 : 0);
     if (NARROW && k0 >= kend) continue;
     float s[NT][4];
-    hm::scores<DP, NT>(s, sQ + wrow * RS, sK, lane);
+    ha_scores<SPLIT, T, DP, NT>(s, sQ + wrow * RS, sK, lane);
     // masks: keys a row does not see become -inf
     const int kl = k0 + 8 * NT;
 #pragma unroll
@@ -252,7 +346,8 @@ __global__ void __launch_bounds__(HA_THREADS) head_fwd_kernel(HeadAttnParams p) 
         if (words[u] && ((n & 3) == 0)) word = (j >> 5) < p.bits_w ? __ldg(words[u] + (j >> 5)) : 0u;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          if (!sees(j + 2 * (lane & 3) + e, jlim[u], self[u], word)) s[n][2 * u + e] = -INFINITY;
+          if (!sees(j + ha_col<SPLIT>(lane, e), jlim[u], self[u], word))
+            s[n][2 * u + e] = -INFINITY;
       }
     }
     float f[2], mc[2];
@@ -284,7 +379,9 @@ __global__ void __launch_bounds__(HA_THREADS) head_fwd_kernel(HeadAttnParams p) 
       o[n][2] *= f[1];
       o[n][3] *= f[1];
     }
-    hm::aggregate<DP, NT>(o, s, sV, lane);
+    ha_aggregate<SPLIT, T, DP, NT>(o, s, sV, lane);
+    // the other buffer was last read before this step's barrier
+    if (t + 1 < ntiles) put(t + 1);
   }
   cp_async_wait<0>();
   l[0] = hm::quad_sum(l[0]);
@@ -487,7 +584,8 @@ struct HaBwd {
   static constexpr int RT = 64;                    // rows (or keys) a block owns
   static constexpr int TT = 32;                    // streamed rows per tile
   static constexpr int NT = TT / 8;
-  static constexpr int RS = hm::row_stride<T, DP>();
+  static constexpr bool SPLIT = ha_split<T, DP>();
+  static constexpr int RS = SPLIT ? hm::split_stride<DP>() : hm::row_stride<T, DP>();
   static constexpr size_t STAGE = (size_t)2 * TT * RS * sizeof(T);
   static constexpr size_t SMEM = (size_t)2 * RT * RS * sizeof(T) + 2 * STAGE;
 };
@@ -497,6 +595,7 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(HA_THREADS) head_dq_kernel(HeadAttnParams p) {
   using C = HaBwd<T, DP>;
   constexpr int RS = C::RS, KT = C::TT, NT = C::NT;
+  constexpr bool SPLIT = C::SPLIT;
   extern __shared__ __align__(16) unsigned char ha_smem[];
   T* sQ = reinterpret_cast<T*>(ha_smem);
   T* sG = sQ + C::RT * RS;
@@ -528,10 +627,39 @@ __global__ void __launch_bounds__(HA_THREADS) head_dq_kernel(HeadAttnParams p) {
     const int i = (r0 + r) / p.G, g = (r0 + r) - i * p.G;
     return base + (int64_t)i * s.n + g * s.h;
   };
-  load_tile<T, DP>(sQ, C::RT, nrows, p.d, p.vec, [&](int r) { return row_of(Q, p.sq, r); });
-  load_tile<T, DP>(sG, C::RT, nrows, p.d, p.vec, [&](int r) { return row_of(Gr, p.sg, r); });
-  if (ntiles > 0) load_keys(0);
-  cp_async_commit();
+  auto q_row = [&](int r) { return row_of(Q, p.sq, r); };
+  auto g_row = [&](int r) { return row_of(Gr, p.sg, r); };
+  SplitRows<SPLIT ? DP : 16, KT> nk, nv;  // split rows: the next tile
+  auto fetch = [&](int t) {
+    if constexpr (SPLIT) {
+      const int k0 = t * KT;
+      nk.load(kend - k0, p.d, p.vec, [&](int r) { return K + (int64_t)(k0 + r) * p.sk.n; });
+      nv.load(kend - k0, p.d, p.vec, [&](int r) { return V + (int64_t)(k0 + r) * p.sv.n; });
+    }
+  };
+  auto put = [&](int t) {
+    if constexpr (SPLIT) {
+      T* sK = ring + (t & 1) * 2 * KT * RS;
+      nk.store(sK);
+      nv.store(sK + KT * RS);
+    }
+  };
+  if constexpr (SPLIT) {
+    SplitRows<DP, C::RT> x;
+    x.load(nrows, p.d, p.vec, q_row);
+    x.store(sQ);
+    x.load(nrows, p.d, p.vec, g_row);
+    x.store(sG);
+    if (ntiles > 0) {
+      fetch(0);
+      put(0);
+    }
+  } else {
+    load_tile<T, DP>(sQ, C::RT, nrows, p.d, p.vec, q_row);
+    load_tile<T, DP>(sG, C::RT, nrows, p.d, p.vec, g_row);
+    if (ntiles > 0) load_keys(0);
+    cp_async_commit();
+  }
 
   int jlim[2], self[2];
   float nlse[2], ndelta[2];
@@ -562,16 +690,21 @@ __global__ void __launch_bounds__(HA_THREADS) head_dq_kernel(HeadAttnParams p) {
     for (int u = 0; u < 4; ++u) dq[n][u] = 0.f;
 
   for (int t = 0; t < ntiles; ++t) {
-    cp_async_wait<0>();
-    __syncthreads();
-    if (t + 1 < ntiles) load_keys(t + 1);
-    cp_async_commit();
+    if constexpr (SPLIT) {
+      __syncthreads();
+      if (t + 1 < ntiles) fetch(t + 1);
+    } else {
+      cp_async_wait<0>();
+      __syncthreads();
+      if (t + 1 < ntiles) load_keys(t + 1);
+      cp_async_commit();
+    }
     const T* sK = ring + (t & 1) * 2 * KT * RS;
     const T* sV = sK + KT * RS;
     const int k0 = t * KT, kl = k0 + KT;
     float s[NT][4], dp[NT][4];
-    hm::scores<DP, NT>(s, sQ + warp * 16 * RS, sK, lane);
-    hm::scores<DP, NT>(dp, sG + warp * 16 * RS, sV, lane);
+    ha_scores<SPLIT, T, DP, NT>(s, sQ + warp * 16 * RS, sK, lane);
+    ha_scores<SPLIT, T, DP, NT>(dp, sG + warp * 16 * RS, sV, lane);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const bool edge = kl > jlim[u] || words[u] || (self[u] >= k0 && self[u] < kl);
@@ -581,13 +714,14 @@ __global__ void __launch_bounds__(HA_THREADS) head_dq_kernel(HeadAttnParams p) {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int j = k0 + 8 * n + 2 * (lane & 3) + e;
+          const int j = k0 + 8 * n + ha_col<SPLIT>(lane, e);
           float x = hm::ex2(fmaf(s[n][2 * u + e], c2, nlse[u])) * (dp[n][2 * u + e] + ndelta[u]);
           if (edge && !sees(j, jlim[u], self[u], word)) x = 0.f;
           s[n][2 * u + e] = x;
         }
     }
-    hm::aggregate<DP, NT>(dq, s, sK, lane);
+    ha_aggregate<SPLIT, T, DP, NT>(dq, s, sK, lane);
+    if (t + 1 < ntiles) put(t + 1);
   }
   cp_async_wait<0>();
   store_frag<T, DP>(dq, p.scale, p.scale, p.d, lane, [&](int r) -> T* {
@@ -601,6 +735,7 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(HA_THREADS) head_dkv_kernel(HeadAttnParams p) {
   using C = HaBwd<T, DP>;
   constexpr int RS = C::RS, QT = C::TT, NT = C::NT;
+  constexpr bool SPLIT = C::SPLIT;
   extern __shared__ __align__(16) unsigned char ha_smem[];
   __shared__ float s_lse[2][QT], s_delta[2][QT];
   __shared__ int s_lim[2][QT], s_self[2][QT];
@@ -629,6 +764,14 @@ __global__ void __launch_bounds__(HA_THREADS) head_dkv_kernel(HeadAttnParams p) 
   const T* V = static_cast<const T*>(p.v) + w.b * p.sv.b + w.hk * p.sv.h;
   const int nqp = head_padded_rows(p.Nq);
   const int64_t total = (int64_t)p.B * nqp * p.H;
+  SplitRows<SPLIT ? DP : 16, QT> nq, ng;  // split rows: the next tile
+  auto put = [&](int t) {
+    if constexpr (SPLIT) {
+      T* sQ = ring + (t & 1) * 2 * QT * RS;
+      nq.store(sQ);
+      ng.store(sQ + QT * RS);
+    }
+  };
   auto load_rows = [&](int t) {
     const int q0 = rbeg + t * QT;
     T* sQ = ring + (t & 1) * 2 * QT * RS;
@@ -636,7 +779,10 @@ __global__ void __launch_bounds__(HA_THREADS) head_dkv_kernel(HeadAttnParams p) 
       const int i = (q0 + r) / p.G, g = (q0 + r) - i * p.G;
       return base + (int64_t)i * s.n + g * s.h;
     };
-    if (p.G == 1) {
+    if constexpr (SPLIT) {
+      nq.load(rows - q0, p.d, p.vec, [&](int r) { return row_of(Q, p.sq, r); });
+      ng.load(rows - q0, p.d, p.vec, [&](int r) { return row_of(Gr, p.sg, r); });
+    } else if (p.G == 1) {
       load_keys_tile<T, DP>(sQ, QT, rows - q0, p.d, p.vec, Q + (int64_t)q0 * p.sq.n, p.sq.n);
       load_keys_tile<T, DP>(sQ + QT * RS, QT, rows - q0, p.d, p.vec, Gr + (int64_t)q0 * p.sg.n,
                             p.sg.n);
@@ -669,11 +815,22 @@ __global__ void __launch_bounds__(HA_THREADS) head_dkv_kernel(HeadAttnParams p) 
       }
     }
   };
-  load_tile<T, DP>(sK, C::RT, nkeys, p.d, p.vec,
-                   [&](int r) { return K + (int64_t)(k0 + r) * p.sk.n; });
-  load_tile<T, DP>(sV, C::RT, nkeys, p.d, p.vec,
-                   [&](int r) { return V + (int64_t)(k0 + r) * p.sv.n; });
-  if (ntiles > 0) load_rows(0);
+  auto k_row = [&](int r) { return K + (int64_t)(k0 + r) * p.sk.n; };
+  auto v_row = [&](int r) { return V + (int64_t)(k0 + r) * p.sv.n; };
+  if constexpr (SPLIT) {
+    SplitRows<DP, C::RT> x;
+    x.load(nkeys, p.d, p.vec, k_row);
+    x.store(sK);
+    x.load(nkeys, p.d, p.vec, v_row);
+    x.store(sV);
+  } else {
+    load_tile<T, DP>(sK, C::RT, nkeys, p.d, p.vec, k_row);
+    load_tile<T, DP>(sV, C::RT, nkeys, p.d, p.vec, v_row);
+  }
+  if (ntiles > 0) {
+    load_rows(0);
+    put(0);
+  }
   cp_async_commit();
   const float c2 = p.scale * HA_LOG2E;
   float dk[DP / 8][4], dv[DP / 8][4];
@@ -691,13 +848,13 @@ __global__ void __launch_bounds__(HA_THREADS) head_dkv_kernel(HeadAttnParams p) 
     const T* sQ = ring + st * 2 * QT * RS;
     const T* sG = sQ + QT * RS;
     float s[NT][4], dp[NT][4];
-    hm::scores<DP, NT>(s, sK + warp * 16 * RS, sQ, lane);
-    hm::scores<DP, NT>(dp, sV + warp * 16 * RS, sG, lane);
+    ha_scores<SPLIT, T, DP, NT>(s, sK + warp * 16 * RS, sQ, lane);
+    ha_scores<SPLIT, T, DP, NT>(dp, sV + warp * 16 * RS, sG, lane);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int x = n * 8 + 2 * (lane & 3) + e;  // query column
+        const int x = n * 8 + ha_col<SPLIT>(lane, e);  // query column
         const float ls = s_lse[st][x], de = s_delta[st][x];
         const int lim = s_lim[st][x], self = s_self[st][x];
         const uint32_t word = s_word[st][warp >> 1][x];
@@ -710,8 +867,9 @@ __global__ void __launch_bounds__(HA_THREADS) head_dkv_kernel(HeadAttnParams p) 
           dp[n][2 * u + e] = pr == 0.f ? 0.f : pr * (dp[n][2 * u + e] + de);
         }
       }
-    hm::aggregate<DP, NT>(dv, s, sG, lane);
-    hm::aggregate<DP, NT>(dk, dp, sQ, lane);
+    ha_aggregate<SPLIT, T, DP, NT>(dv, s, sG, lane);
+    ha_aggregate<SPLIT, T, DP, NT>(dk, dp, sQ, lane);
+    if (t + 1 < ntiles) put(t + 1);
   }
   cp_async_wait<0>();
   auto place = [&](void* base, int r) -> T* {
@@ -793,9 +951,10 @@ constexpr int HA_SMS = 148;
 constexpr int HA_NARROW_ROWS = 16;
 
 // Parts of the key axis: with fewer blocks than the GPU holds at once, split
-// until there are about sixteen per SM, each of at least 256 keys: ragged
+// until there are about eight per SM, each of at least 256 keys: ragged
 // lengths leave parts without keys, and short parts even that out (32 episodes
-// of up to 16384 keys: TODO us with 16 per SM, 110 with 4).
+// of up to 16384 keys, both kernels: 69 us with 8 per SM, 71 with 16, 88 with
+// 32).
 void head_split_plan(int B, int Nq, int Nk, int H, int Hk, int* splits, int* split_keys) {
   const int64_t rows = (int64_t)Nq * (H / Hk);
   const int tile = rows <= HA_NARROW_ROWS ? 16 : 64;
@@ -803,7 +962,7 @@ void head_split_plan(int B, int Nq, int Nk, int H, int Hk, int* splits, int* spl
   *splits = 1;
   *split_keys = Nk;
   if (base >= 2 * HA_SMS || Nk < 512) return;
-  int64_t n = (16 * HA_SMS + base - 1) / base;
+  int64_t n = (8 * HA_SMS + base - 1) / base;
   if (n > Nk / 256) n = Nk / 256;
   if (n < 2) return;
   const int keys = cdiv(cdiv(Nk, (int)n), 64) * 64;

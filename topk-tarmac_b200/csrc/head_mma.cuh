@@ -192,6 +192,109 @@ __device__ __forceinline__ void aggregate(float (&o)[DP / 8][4], const float (&p
   }
 }
 
+// ---- fp32 rows of up to 32 columns, split once when they are staged --------
+// Split inside the products, every element is split by every warp that reads
+// it, and that arithmetic bounds rows this narrow. Here a shared tile holds
+// {hi, lo} pairs: element (r, k) at word r RS + ((2k) ^ (16 if r & 4)), RS =
+// 2 DP + 8. The four rows of a half-warp's 64-bit loads then fall into
+// different banks both for rows 0, 4, 1, 5 (score columns) and 0..3, 4..7.
+// Score column c of an 8-key tile is key (c >> 1) + 4 (c & 1), so that a
+// thread's two weights are the two contraction indexes of its A operand.
+template <int DP>
+constexpr int split_stride() {
+  return 2 * DP + 8;
+}
+template <int DP>
+__device__ __forceinline__ int split_word(int r, int k) {
+  return r * split_stride<DP>() + ((2 * k) ^ ((r & 4) << 2));
+}
+template <int DP>
+__device__ __forceinline__ void store_split(float* tile, int r, int c, float4 v) {
+  uint32_t h[4], l[4];
+  split_tf32(v.x, h[0], l[0]);
+  split_tf32(v.y, h[1], l[1]);
+  split_tf32(v.z, h[2], l[2]);
+  split_tf32(v.w, h[3], l[3]);
+  uint4* t = reinterpret_cast<uint4*>(tile + split_word<DP>(r, c));
+  t[0] = make_uint4(h[0], l[0], h[1], l[1]);
+  t[1] = make_uint4(h[2], l[2], h[3], l[3]);
+}
+__device__ __forceinline__ void lds_pair(uint32_t& hi, uint32_t& lo, const float* p) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  hi = v.x;
+  lo = v.y;
+}
+
+template <int DP, int NT>
+__device__ __forceinline__ void scores_split(float (&c)[NT][4], const float* sA, const float* sB,
+                                             int lane) {
+  constexpr int RS = split_stride<DP>();
+  const int r = lane >> 2, t = lane & 3;
+  const int flip_a = (r & 4) << 2;  // rows r and r + 8
+  const int rb = (r >> 1) + 4 * (r & 1), flip_b = (r & 1) << 4;
+  float small[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) c[n][u] = small[n][u] = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < DP / 8; ++ks) {
+    uint32_t ah[4], al[4];
+    const int k0 = 2 * (ks * 8 + t), k1 = k0 + 8;
+    lds_pair(ah[0], al[0], sA + r * RS + (k0 ^ flip_a));
+    lds_pair(ah[1], al[1], sA + (r + 8) * RS + (k0 ^ flip_a));
+    lds_pair(ah[2], al[2], sA + r * RS + (k1 ^ flip_a));
+    lds_pair(ah[3], al[3], sA + (r + 8) * RS + (k1 ^ flip_a));
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      uint32_t bh[2], bl[2];
+      lds_pair(bh[0], bl[0], sB + (n * 8 + rb) * RS + (k0 ^ flip_b));
+      lds_pair(bh[1], bl[1], sB + (n * 8 + rb) * RS + (k1 ^ flip_b));
+      mma_tf32(small[n], al, bh[0], bh[1]);
+      mma_tf32(c[n], ah, bh[0], bh[1]);
+      mma_tf32(small[n], ah, bl[0], bl[1]);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) c[n][u] += small[n][u];
+}
+
+template <int DP, int NT>
+__device__ __forceinline__ void aggregate_split(float (&o)[DP / 8][4], const float (&p)[NT][4],
+                                                const float* sB, int lane) {
+  constexpr int RS = split_stride<DP>();
+  const int t = lane & 3, j = lane >> 2;
+  float c[DP / 8][4], x[DP / 8][4];
+#pragma unroll
+  for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) c[n][u] = x[n][u] = 0.f;
+#pragma unroll
+  for (int k = 0; k < NT; ++k) {
+    uint32_t ah[4], al[4];
+    split_tf32(p[k][0], ah[0], al[0]);
+    split_tf32(p[k][2], ah[1], al[1]);
+    split_tf32(p[k][1], ah[2], al[2]);
+    split_tf32(p[k][3], ah[3], al[3]);
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n) {
+      uint32_t bh[2], bl[2];
+      const int w = 2 * (n * 8 + j);
+      lds_pair(bh[0], bl[0], sB + (k * 8 + t) * RS + w);
+      lds_pair(bh[1], bl[1], sB + (k * 8 + t + 4) * RS + (w ^ 16));
+      mma_tf32(x[n], al, bh[0], bh[1]);
+      mma_tf32(c[n], ah, bh[0], bh[1]);
+      mma_tf32(x[n], ah, bl[0], bl[1]);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) o[n][u] += c[n][u] + x[n][u];
+}
+
 // sum / maximum over the four lanes that share a row
 __device__ __forceinline__ float quad_sum(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 1);
