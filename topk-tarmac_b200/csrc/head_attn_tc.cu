@@ -6,13 +6,18 @@
 // 128 keys. Roles of its 20 warps (two idle):
 // * warps 4..11 and 12..19: two warpgroups per tile, two threads per row with 64
 //   of the 128 columns each. They read S from TMEM, mask, run the softmax in
-//   base 2 (row maxima meet in shared memory) and write P as bf16 over the
-//   columns of S that they own. The reference maximum moves, and O is
-//   rescaled, only when a score exceeds it by 2^8, which few tiles do.
+//   base 2 and write P as bf16 to TMEM. The reference maximum moves, and O is
+//   rescaled, only when a score of some row exceeds it by 2^8, which few tiles
+//   do: one barrier with a vote settles the others, and only those that move
+//   exchange row maxima through shared memory.
 // * warp 1: one thread issues the TMA loads (Q once, K and V in a ring).
 // * warp 0: one thread issues the products, alternating the tiles:
 //   S_g = Q_g K^T, then O_g += P_g V with P from TMEM. While one tile is in
 //   its softmax the tensor core serves the other.
+// TMEM columns: S_g at 128 g (P_g over the columns of S_g that a group owns),
+// O_g at 256 + DP g. A P_g with columns of its own, which lets S of the next
+// key tile run under the exponentials, was no faster at d = 64 (32 x 8 heads of
+// 1024 rows: 128 against 129 us) and slower with masks (204 against 184 us).
 // Bound: the special-function unit's 16 exponentials per clock per SM (1024
 // clocks for a 128 x 128 tile) against 256 d / 64 clocks for each of the two
 // products. Blocks are persistent, one per SM, and walk their items in
@@ -216,14 +221,12 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
           ok = ok && ht::wait_at(b_pfull + 8 * w, (w ? pc1 : pc0) & 1, abort_flag);
           if (w) ++pc1; else ++pc0;
           tc::fence_after_sync();
-          if (ok && leader)
+          if (ok && leader) {
             ht::issue_aggregate<HT_KEYS, 64>(tmem + 256 + w * DP, tmem + w * 128, dv, id_o, t > 0);
+            if (t + 1 == nw) ht::commit_at(b_odone + 8 * w);
+          }
           __syncwarp();
-          if (t + 1 < nw)
-            scores(w);
-          else if (ok && leader)
-            ht::commit_at(b_odone + 8 * w);
-          __syncwarp();
+          if (t + 1 < nw) scores(w);
         }
         if (ok && leader) {
           ht::commit_at(b_empty + 8 * vr.s);
@@ -248,6 +251,17 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
     const int c_lo = half * (DP / 2), c_n = max(0, min(DP / 2, p.d - c_lo));  // columns of O
     const float c2 = p.scale * HT_LOG2E;
     auto pair_sync = [&] { asm volatile("bar.sync %0, 256;" ::"r"(1 + w) : "memory"); };
+    // does any of the pair's threads say so? (a barrier)
+    auto pair_any = [&](bool x) {
+      uint32_t r;
+      asm volatile(
+          "{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, %2, 256, p;\n"
+          "selp.u32 %0, 1, 0, q;\n}\n"
+          : "=r"(r)
+          : "r"((uint32_t)x), "r"(1 + w)
+          : "memory");
+      return r != 0;
+    };
     uint32_t kc = 0, sc = 0, oc = 0;
     bool ok = true;
     // a group that gave up keeps meeting its partner: it skips the bounded
@@ -269,18 +283,24 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
           p.bits ? p.bits + it.b * p.bits_b + (int64_t)min(i, p.Nq - 1) * p.bits_w : nullptr;
       float mref = -INFINITY;  // reference maximum in exponent units
       float l = 0.f;           // this group's part of the sum
+      // the visibility words of the next key tile are on their way while this
+      // one is worked on
+      auto fetch_words = [&](int t, uint32_t (&bits)[2]) {
+        const int j = t * (HT_KEYS / 32) + half * 2;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          bits[x] = words ? (j + x < p.bits_w ? __ldg(words + j + x) : 0u) : 0xffffffffu;
+      };
+      uint32_t bits[2];
+      fetch_words(0, bits);
       for (int t = 0; t < nt; ++t) {
         const int k0 = t * HT_KEYS + half * 64;
         const bool edge = words || k0 + 64 > jlim || (self >= k0 && self < k0 + 64);
-        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-        if (edge) {
+        uint32_t seen[2];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            uint32_t bits = 0xffffffffu;
-            if (words) bits = (k0 >> 5) + x < p.bits_w ? __ldg(words + (k0 >> 5) + x) : 0u;
-            seen[x] = ht::key_word(k0 + 32 * x, jlim, self, bits);
-          }
-        }
+        for (int x = 0; x < 2; ++x)
+          seen[x] = edge ? ht::key_word(k0 + 32 * x, jlim, self, bits[x]) : 0xffffffffu;
+        if (words) fetch_words(t + 1, bits);
         if (ok) ok = ht::warp_wait(&sh.sfull[w], sc & 1, abort_flag);
         ++sc;
         tc::fence_after_sync();
@@ -298,25 +318,28 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
           for (int u = 0; u < 4; ++u)
             mx[u] = max3f(mx[u], __uint_as_float(s[x + 2 * u]), __uint_as_float(s[x + 2 * u + 1]));
         const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        sh.top[w][t & 1][half][row] = mine;
-        pair_sync();
-        const float m2 = fmaxf(mine, sh.top[w][t & 1][half ^ 1][row]) * c2;
-        float alpha = 1.f;
-        const bool move = m2 > mref + HT_MOVE || (mref == -INFINITY && m2 != -INFINITY);
-        if (move) {
-          alpha = tc::ex2_approx(mref - m2);
-          l *= alpha;
-          mref = m2;
-        }
-        // rescale O where any lane of the warp moved (PV of the last tile is
-        // complete: it was issued before the S that just arrived)
-        if (t > 0 && __any_sync(0xffffffffu, move)) {
-          for (int c = 0; c < c_n; c += 16) {
-            uint32_t o[16];
-            ht::tmem_ld(t_o + c, o);
+        if (t == 0 ||
+            pair_any(mine * c2 > mref + HT_MOVE || (mref == -INFINITY && mine != -INFINITY))) {
+          sh.top[w][t & 1][half][row] = mine;
+          pair_sync();
+          const float m2 = fmaxf(mine, sh.top[w][t & 1][half ^ 1][row]) * c2;
+          float alpha = 1.f;
+          const bool move = m2 > mref + HT_MOVE || (mref == -INFINITY && m2 != -INFINITY);
+          if (move) {
+            alpha = tc::ex2_approx(mref - m2);
+            l *= alpha;
+            mref = m2;
+          }
+          // rescale O where any lane of the warp moved (P V of the last tile is
+          // complete: it was issued before the S that just arrived)
+          if (t > 0 && __any_sync(0xffffffffu, move)) {
+            for (int c = 0; c < c_n; c += 16) {
+              uint32_t o[16];
+              ht::tmem_ld(t_o + c, o);
 #pragma unroll
-            for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * alpha);
-            ht::tmem_st(t_o + c, o);
+              for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * alpha);
+              ht::tmem_st(t_o + c, o);
+            }
           }
         }
         const float mb = mref == -INFINITY ? 0.f : -mref;
