@@ -545,37 +545,62 @@ __global__ void __launch_bounds__(128) head_join_kernel(HeadAttnParams p) {
 template <typename T>
 __global__ void __launch_bounds__(256) head_delta_kernel(HeadAttnParams p, int nqp) {
   const int64_t total = (int64_t)p.B * nqp * p.H;
-  const int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+  // a block's 128 (row, head) pairs are of one episode, four per lane group
+  // with their loads in flight together; pairs per episode are below 2^31
+  const int blocks_b = cdiv(nqp * p.H, 128);
+  const int b = (int)(blockIdx.x / (uint32_t)blocks_b);
+  const int pair0 = (int)(blockIdx.x - (uint32_t)b * blocks_b) * 128 + (threadIdx.x >> 3);
   const int sub = threadIdx.x & 7;
-  float s = 0.f;
-  const int h = (int)(row % p.H);
-  const int64_t bi = row / p.H;
-  const int i = (int)(bi % nqp);
-  const int64_t b = bi / nqp;
-  if (row < total && i < p.Nq) {
-    const T* o = static_cast<const T*>(p.o) + b * p.so.b + i * p.so.n + h * p.so.h;
-    const T* g = static_cast<const T*>(p.g) + b * p.sg.b + i * p.sg.n + h * p.sg.h;
-    if (p.vec) {
-      constexpr int E = 16 / (int)sizeof(T);
-      for (int c = sub * E; c < p.d; c += 8 * E) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(o + c));
-        const uint4 y = __ldg(reinterpret_cast<const uint4*>(g + c));
-        const T* a = reinterpret_cast<const T*>(&x);
-        const T* bq = reinterpret_cast<const T*>(&y);
+  const T *o[4], *g[4];
+  int row[4], head[4];
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < E; ++e) s = fmaf(to_f32<T>(a[e]), to_f32<T>(bq[e]), s);
+  for (int u = 0; u < 4; ++u) {
+    const int pair = pair0 + 32 * u;
+    row[u] = pair / p.H;
+    head[u] = pair - row[u] * p.H;
+    const int i = min(row[u], p.Nq - 1);
+    o[u] = static_cast<const T*>(p.o) + b * p.so.b + i * p.so.n + head[u] * p.so.h;
+    g[u] = static_cast<const T*>(p.g) + b * p.sg.b + i * p.sg.n + head[u] * p.sg.h;
+  }
+  if (p.vec) {
+    constexpr int E = 16 / (int)sizeof(T);
+    for (int c = sub * E; c < p.d; c += 8 * E) {
+      uint4 x[4], y[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        x[u] = y[u] = make_uint4(0, 0, 0, 0);
+        if (row[u] < p.Nq) {
+          x[u] = __ldg(reinterpret_cast<const uint4*>(o[u] + c));
+          y[u] = __ldg(reinterpret_cast<const uint4*>(g[u] + c));
+        }
       }
-    } else {
-      for (int c = sub; c < p.d; c += 8) s = fmaf(to_f32<T>(o[c]), to_f32<T>(g[c]), s);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const T* a = reinterpret_cast<const T*>(&x[u]);
+        const T* bq = reinterpret_cast<const T*>(&y[u]);
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[u] = fmaf(to_f32<T>(a[e]), to_f32<T>(bq[e]), s[u]);
+      }
     }
+  } else {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (row[u] < p.Nq)
+        for (int c = sub; c < p.d; c += 8)
+          s[u] = fmaf(to_f32<T>(o[u][c]), to_f32<T>(g[u][c]), s[u]);
   }
 #pragma unroll
-  for (int x = 4; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-  if (row < total && sub == 0) {
-    const float lse = i < p.Nq ? p.lse[(b * p.H + h) * p.Nq + i] : -INFINITY;
-    const int64_t srow = (b * p.H + h) * nqp + i;
-    p.delta[srow] = lse == -INFINITY ? -INFINITY : lse * -HA_LOG2E;
-    p.delta[total + srow] = -s;
+  for (int u = 0; u < 4; ++u) {
+#pragma unroll
+    for (int x = 4; x > 0; x >>= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], x);
+    if (row[u] < nqp && sub == 0) {
+      const int64_t hd = (int64_t)b * p.H + head[u];
+      const float lse = row[u] < p.Nq ? p.lse[hd * p.Nq + row[u]] : -INFINITY;
+      const int64_t srow = hd * nqp + row[u];
+      p.delta[srow] = lse == -INFINITY ? -INFINITY : lse * -HA_LOG2E;
+      p.delta[total + srow] = row[u] < p.Nq ? -s[u] : 0.f;
+    }
   }
 }
 
@@ -912,32 +937,31 @@ __global__ void __launch_bounds__(256) pack_bits_kernel(const unsigned char* v, 
     out[x] = bits;
     return;
   }
-  // any alignment: a warp reads 32 neighbouring bytes and votes
+  // any alignment: a warp walks along a row, reads 32 neighbouring bytes and
+  // votes; lane u keeps the u-th word of 32
   const int lane = threadIdx.x & 31;
-  const int64_t first = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * 32;
-  uint32_t mine = 0;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= (int64_t)B * Nq) return;
+  const unsigned char* src = v + (row / Nq) * sb + (row % Nq) * sn;
+  for (int w0 = 0; w0 < W; w0 += 32) {
+    uint32_t mine = 0;
 #pragma unroll 8
-  for (int u = 0; u < 32; ++u) {
-    const int64_t x = first + u;
-    bool on = false;
-    if (x < total) {
-      const int wd = (int)(x % W);
-      const int64_t row = x / W;
-      const int j = wd * 32 + lane;
-      if (j < Nk) on = v[(row / Nq) * sb + (row % Nq) * sn + j] != 0;
+    for (int u = 0; u < 32; ++u) {
+      const int j = (w0 + u) * 32 + lane;
+      if ((w0 + u) * 32 >= Nk) break;
+      const uint32_t word = __ballot_sync(0xffffffffu, j < Nk && src[j] != 0);
+      if (lane == u) mine = word;
     }
-    const uint32_t word = __ballot_sync(0xffffffffu, on);
-    if (lane == u) mine = word;
+    if (w0 + lane < W) out[row * W + w0 + lane] = mine;
   }
-  if (first + lane < total) out[first + lane] = mine;
 }
 
 cudaError_t launch_pack_bits(const void* v, int64_t sb, int64_t sn, int B, int Nq, int Nk,
                              uint32_t* out, cudaStream_t s) {
   const int W = cdiv(Nk, 32);
   const int vec = ((uintptr_t)v % 16 == 0) && sb % 16 == 0 && sn % 16 == 0 && Nk % 16 == 0;
-  const int64_t total = (int64_t)B * Nq * W;
-  const int64_t blocks = (total + 255) / 256;
+  const int64_t blocks =
+      vec ? ((int64_t)B * Nq * W + 255) / 256 : ((int64_t)B * Nq + 7) / 8;
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
   pack_bits_kernel<<<(unsigned)blocks, 256, 0, s>>>(static_cast<const unsigned char*>(v), sb, sn,
                                                     B, Nq, Nk, W, vec, out);
@@ -1020,9 +1044,9 @@ cudaError_t launch_head_bwd_tc(const HeadAttnParams& p, int64_t nqp, cudaStream_
 template <typename T>
 static cudaError_t bwd_any(const HeadAttnParams& p, cudaStream_t s) {
   const int nqp = head_padded_rows(p.Nq);
-  const int64_t rows = (int64_t)p.B * nqp * p.H;
-  if ((rows + 31) / 32 > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  if (rows) head_delta_kernel<T><<<(unsigned)((rows + 31) / 32), 256, 0, s>>>(p, nqp);
+  const int64_t blocks = (int64_t)p.B * cdiv((int)((int64_t)nqp * p.H), 128);
+  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  if (blocks) head_delta_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(p, nqp);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   if constexpr (sizeof(T) == 2) {

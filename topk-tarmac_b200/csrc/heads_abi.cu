@@ -49,11 +49,11 @@ int fill_attn(HeadAttnParams& p, const void* q, const void* k, const void* v,
               float scale) {
   if (dtype != TARMAC_F32 && dtype != TARMAC_BF16) return TARMAC_ERR_DTYPE;
   if (B < 0 || Nq < 0 || Nk < 0 || d < 1 || d > MAX_D) return TARMAC_ERR_SHAPE;
-  // row and key counts stay below 2^29 (position arithmetic in 32 bits), packed
-  // rows of a key head below 2^31
+  // row and key counts stay below 2^29 (position arithmetic in 32 bits), rows
+  // times heads of an episode below 2^31
   if (Nk > (1 << 29) || Nq > (1 << 29)) return TARMAC_ERR_N_TOO_LARGE;
   if (H < 1 || Hk < 1 || H % Hk) return TARMAC_ERR_HEADS;
-  if ((int64_t)Nq * (H / Hk) > 0x7fffff00) return TARMAC_ERR_N_TOO_LARGE;
+  if ((int64_t)head_padded_rows(Nq) * H > 0x7fffff00) return TARMAC_ERR_N_TOO_LARGE;
   if (peers < PEERS_ALL || peers > PEERS_PAST) return TARMAC_ERR_MODE;
   if (!(scale > 0.f) || isinf(scale)) return TARMAC_ERR_SHAPE;
   if (!aligned(key_len, 4) || !aligned(q_start, 4) || !aligned(bits, 4)) return TARMAC_ERR_ALIGN;
