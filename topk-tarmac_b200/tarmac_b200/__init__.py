@@ -8,6 +8,9 @@ Host-side package over the C ABI of ``include/tarmac_b200.h``
   Morton window selection, fused Morton selection + attention);
 * :mod:`tarmac_b200.autograd` — differentiable forms (torch.autograd.Function)
   whose backward runs the gradient kernels;
+* :mod:`tarmac_b200.heads` — a communication block of several heads built on
+  the multi-head operators (head norms with the position rotation, masked
+  attention): training over a set of agents, and one step over a history;
 * :mod:`tarmac_b200._lib` — the ctypes binding itself.
 
 The drop-in modules with the reference's import paths (``src.kernels.*``,

@@ -1,7 +1,8 @@
 """Differentiable attention-core operations (torch.autograd.Function).
 
 Forward runs the sm_100a kernels of :mod:`tarmac_b200.ops`; backward runs the
-gradient kernels (csrc/backward.cu) through the same C ABI. These give the
+gradient kernels (csrc/backward.cu; csrc/head_*.cu for the multi-head
+operators) through the same C ABI. The single-head ones give the
 gradients autograd forms through the reference's eager path
 (src/agents/mappo.py:192-231 topk_gather, 265-292 zorder_k, 361-373 dense):
 the peer selection itself carries no gradient. Gradients come back in the
@@ -99,6 +100,50 @@ class MortonPrescoreAttention(torch.autograd.Function):
         return dq.to(t), dk.to(t), dv.to(t), None, None, None, None
 
 
+class QkNormRotate(torch.autograd.Function):
+    """Head norms and position rotation (:func:`ops.qk_norm_rotate`). The
+    tables carry no gradient."""
+
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, cos, sin, eps=1e-6, interleaved=False):
+        ctx.save_for_backward(q, k, wq, wk, cos, sin)
+        ctx.how = (eps, interleaved)
+        return ops.qk_norm_rotate(q, k, wq, wk, cos, sin, eps, interleaved)
+
+    @staticmethod
+    def backward(ctx, dq_out, dk_out):
+        q, k, wq, wk, cos, sin = ctx.saved_tensors
+        dq, dk, dwq, dwk = ops.qk_norm_rotate_backward(
+            q, k, wq, wk, cos, sin, dq_out, dk_out, *ctx.how)
+        if wq is not None:
+            dwq = dwq.to(wq.dtype)
+        if wk is not None:
+            dwk = dwk.to(wk.dtype)
+        return dq, dk, dwq, dwk, None, None, None, None
+
+
+class HeadAttention(torch.autograd.Function):
+    """Masked attention with heads (:func:`ops.head_attention`); ``visible``
+    is None or the words of :func:`ops.pack_visibility`."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, peers="all", key_len=None, q_start=None,
+                visible=None, scale=None):
+        out, lse = ops.head_attention(q, k, v, peers, key_len, q_start,
+                                      visible, scale, return_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, key_len, q_start, visible)
+        ctx.how = (peers, scale)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse, key_len, q_start, visible = ctx.saved_tensors
+        peers, scale = ctx.how
+        dq, dk, dv = ops.head_attention_backward(
+            q, k, v, out, lse, dout, peers, key_len, q_start, visible, scale)
+        return dq, dk, dv, None, None, None, None, None
+
+
 def _needs_grad(*ts) -> bool:
     return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
 
@@ -129,3 +174,19 @@ def morton_prescore_attention(q, k, v, pos, topk, bits=10, scale=None):
         return MortonPrescoreAttention.apply(q, k, v, pos, topk, bits,
                                              scale)[0]
     return ops.morton_prescore_attention(q, k, v, pos, topk, bits, scale)
+
+
+def qk_norm_rotate(q, k, wq, wk, cos, sin, eps=1e-6, interleaved=False):
+    if _needs_grad(*(t for t in (q, k, wq, wk) if t is not None)):
+        return QkNormRotate.apply(q, k, wq, wk, cos, sin, eps, interleaved)
+    return ops.qk_norm_rotate(q, k, wq, wk, cos, sin, eps, interleaved)
+
+
+def head_attention(q, k, v, peers="all", key_len=None, q_start=None,
+                   visible=None, scale=None):
+    if _needs_grad(q, k, v):
+        if visible is not None and visible.dtype == torch.bool:
+            visible = ops.pack_visibility(visible)  # once for both directions
+        return HeadAttention.apply(q, k, v, peers, key_len, q_start, visible,
+                                   scale)
+    return ops.head_attention(q, k, v, peers, key_len, q_start, visible, scale)
