@@ -300,7 +300,7 @@ int tarmac_dense_attention_backward_noalloc(
  * head } int64 element strides for each input tensor in argument order, or is
  * NULL for contiguous tensors. Rows on a 16-byte grid (pointer, strides and
  * width) move as vectors, others element by element. Element offsets are 64
- * bits. Inputs that a row sees must be finite. */
+ * bits. */
 
 /* Norm of every query and key head and the position rotation, in one pass:
  *   z = x / sqrt(mean_c x_c^2 + eps) * w,
@@ -370,7 +370,9 @@ int tarmac_head_attention(const void *q, const void *k, const void *v,
 /* Its gradients, with P recomputed from lse:
  *   D_i = dout_i . out_i, dS = P (dout v^T - D),
  *   dq = scale dS k, dk = scale dS^T q, dv = P^T dout,
- * shared key heads summed over their query heads. out, lse: the forward's.
+ * shared key heads summed over their query heads. out, lse: the forward's (of
+ * all keys, where the call holds a part of them: the result is that part's
+ * share of the gradients).
  * strides: q, k, v, out, dout. dq, dk, dv: contiguous, the inputs' type; rows
  * that see nothing and keys that nothing sees get zeros. No atomics: two
  * calls give the same bits. work: 16-byte aligned scratch of

@@ -136,6 +136,25 @@ def test_rotate_zero_rows_and_values(ops):
     assert ops.qk_norm_rotate(e, e, w, w, cos, sin)[0].shape == e.shape
 
 
+def test_rotate_many_rows(ops):
+    """Rows times lanes per row past 32 bits: a row of width 1 keeps its sign
+    (x / sqrt(x^2) with eps 0), forward and in the weight's gradient."""
+    N = 2 ** 27 + 300
+    q = torch.ones(1, N, 1, 1, dtype=BF16, device="cuda")
+    q[0, -200:] = -2.0
+    q[0, 7] = -3.0
+    none = torch.empty(1, N, 0, device="cuda")
+    oq, ok = ops.qk_norm_rotate(q, q, None, None, none, none, eps=0.0)
+    assert torch.equal(oq, q.sign()) and torch.equal(ok, oq)
+    del ok, oq
+    w = torch.ones(1, device="cuda")
+    g = torch.zeros_like(q)
+    g[0, -1000:] = 1.0  # 800 rows of +1, 200 of -1, each to 2^-21
+    dq, dk, dwq, dwk = ops.qk_norm_rotate_backward(q, q, w, w, none, none, g, g, eps=0.0)
+    assert abs(dwq.item() - 600) < 1e-2 and abs(dwk.item() - 600) < 1e-2
+    assert dq.abs().max() < 2.0 ** -20 and dk.abs().max() < 2.0 ** -20  # lengths do not matter
+
+
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
@@ -260,6 +279,33 @@ def test_attention_large_scores(ops, dtype):
     (3, 512, 2, 2, 32, "others", None, 0.9)])
 def test_attention_many_tiles(ops, B, N, H, Hk, d, peers, lens, seen, dtype):
     attention_case(ops, B, N, N, H, Hk, d, dtype, peers, lens=lens, seen=seen)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_gradient_by_parts(ops, dtype):
+    """out and lse of the whole softmax with a part of its keys: that part's
+    share of the gradients."""
+    B, N, H, Hk, d, cut = 2, 200, 4, 2, 64, 72
+    g = torch.Generator().manual_seed(5)
+    q, k, v = rows(g, B, N, (H, Hk, Hk), d, dtype)
+    dout, = rows(g, B, N, (H,), d, dtype)
+    out, lse = ops.head_attention(q, k, v, "past", return_lse=True)
+    parts = []
+    for a, b in ((0, cut), (cut, N)):
+        first = torch.full((B,), -a, dtype=torch.int32, device="cuda")
+        parts.append(wide(*ops.head_attention_backward(
+            q, k[:, a:b], v[:, a:b], out, lse, dout, "past", q_start=first)))
+    qd, kd, vd, gd = wide(q, k, v, dout)
+    ref = h64.Attention(qd, kd, vd, h64.mask(B, N, N, "past", None, None, None), d ** -0.5, gd)
+    eps = 2 * (d / 8 + 8) * 2.0 ** -23 * float(ref.abs_scores.max()) \
+        + (N * (H // Hk) / 32 + 16) * 2.0 ** -22
+    rnd = 2.0 ** -8 if dtype == BF16 else 0.0
+    # a part's dq is at most dq_mag, and is rounded by itself
+    near(parts[0][0] + parts[1][0], ref.dq, eps * ref.dq_mag + rnd * (ref.dq_rnd + ref.dq_mag))
+    near(torch.cat([x[1] for x in parts], 1), ref.dk,
+         eps * ref.dk_mag + rnd * (ref.dk_rnd + ref.dk.abs()))
+    near(torch.cat([x[2] for x in parts], 1), ref.dv,
+         eps * ref.dv_mag + rnd * (ref.dv_mag + ref.dv.abs()))
 
 
 def test_attention_empty_sizes(ops):

@@ -271,7 +271,7 @@ __device__ __forceinline__ void rotate_unit(const RotateParams& p, const RotGrid
   const int h0 = w.chunk * HC;
   const int heads = is_q ? p.H : p.Hk;
   // lanes of a warp leave together only (the row sums are warp shuffles)
-  uint32_t token = (w.tblock * ROT_THREADS + threadIdx.x) >> g.lpr_log2;
+  uint32_t token = w.tblock * (ROT_THREADS >> g.lpr_log2) + (threadIdx.x >> g.lpr_log2);
   const bool live = token < (uint32_t)p.B * (uint32_t)p.N;
   if (!live) token = 0;
   const uint32_t b = g.episode(token), n = token - b * (uint32_t)p.N;
@@ -369,7 +369,8 @@ __device__ __forceinline__ void rotate_bwd_unit(const RotateParams& p, const Rot
     for (int e = 0; e < E; ++e) dwa[i][e] = dwb[i][e] = 0.f;
   }
   for (int it = 0; it < ROT_TILES; ++it) {
-    uint32_t token = ((tblock * ROT_TILES + it) * ROT_THREADS + threadIdx.x) >> g.lpr_log2;
+    uint32_t token = (tblock * ROT_TILES + it) * (ROT_THREADS >> g.lpr_log2) +
+                     (threadIdx.x >> g.lpr_log2);
     const bool live = token < tokens;
     if (__all_sync(0xffffffffu, !live)) break;
     if (!live) token = 0;
@@ -394,7 +395,7 @@ __device__ __forceinline__ void rotate_bwd_unit(const RotateParams& p, const Rot
     for (int i = 0; i < NP; ++i) sl[i].tables(p.cos + tab, p.sin + tab, p.r, g.table_vec != 0);
 #pragma unroll
     for (int h = 0; h < HC; ++h) {
-        float x[NP][E], y[NP][E], ga[NP][E], gb[NP][E];  // ga, gb: dz
+      float x[NP][E], y[NP][E], ga[NP][E], gb[NP][E];  // ga, gb: dz
       float acc[E], dot[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] = dot[e] = 0.f;
@@ -416,9 +417,10 @@ __device__ __forceinline__ void rotate_bwd_unit(const RotateParams& p, const Rot
         vmul<E>(t, gb[i], wb[i]);
         vfma<E>(dot, t, y[i], dot);
       }
-      const float rs = rsqrtf(fmaf(row_sum(vsum<E>(acc), g.lpr), g.inv_d, p.eps));
-      const float m = row_sum(vsum<E>(dot), g.lpr) * g.inv_d * rs * rs;
       const bool ok = live && h0 + h < heads;
+      float rs = rsqrtf(fmaf(row_sum(vsum<E>(acc), g.lpr), g.inv_d, p.eps));
+      if (!ok) rs = 0.f;  // no row: with eps 0 it would add 0 inf to dw
+      const float m = row_sum(vsum<E>(dot), g.lpr) * g.inv_d * rs * rs;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         float t[E], u[E];

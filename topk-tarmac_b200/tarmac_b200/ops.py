@@ -692,9 +692,10 @@ def head_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     not its own position; "past": positions up to its own) and
     ``visible[b, i, j]`` holds (bool [1 or B, Nq, Nk], or the words of
     :func:`pack_visibility`). A row that sees nothing gets 0 (lse -inf). Keys
-    and values from ``key_len`` on are not read; what a row sees must be
-    finite. One token over a long history is Nq = 1: the key axis is then
-    split over the GPU."""
+    and values from ``key_len`` on are never used, whatever they hold; those
+    before it must be finite, masked or not (a weight of zero times a NaN is a
+    NaN). One token over a long history is Nq = 1: the key axis is then split
+    over the GPU."""
     if visible is None and _attention_ready(q, k, v, peers, key_len, q_start):
         bits = None
     else:
