@@ -217,6 +217,11 @@ SHAPES = [  # B, Nq, Nk, H, Hk, d
     (2, 3, 150, 8, 2, 64),
     (2, 150, 3, 3, 3, 24),
     (2, 70, 90, 5, 1, 96),
+    (2, 33, 70, 4, 2, 64),
+    (1, 300, 3, 3, 3, 64),
+    (2, 200, 200, 4, 2, 16),
+    (1, 210, 40, 2, 1, 24),
+    (1, 40, 210, 2, 2, 8),
 ]
 
 

@@ -477,16 +477,26 @@ int head_sm_count() {
   return n;
 }
 
-// bf16 rows on the 16-byte grid with at least 128 queries; *done says whether
+// bf16 rows on the 16-byte grid, by the rules below; *done says whether
 // the call was taken.
 cudaError_t launch_head_fwd_tc(const HeadAttnParams& p, cudaStream_t s, bool* done) {
   *done = false;
-  if (!p.vec || p.splits > 1 || p.Nq < 128 || p.Nk < 1) return cudaSuccess;
+  // Short sets of rows leave these 128-row tiles half empty, and for narrow
+  // rows the products weigh little; the kernels of head_attn.cu were faster
+  // there. Measured, those against these (us): 512 x 8 heads, d = 64: N = 64
+  // 58 / 103, N = 96 140 / 113, N = 256 379 / 208; 512 x 4 heads, d = 32:
+  // N = 128 44 / 51, N = 192 82 / 91, N = 224 132 / 93; d = 16, 256 x 4 heads:
+  // N = 192 32 / 45, N = 512 152 / 130.
+  if (!p.vec || p.Nk < 1 || p.Nq <= (p.d > 32 ? 64 : 192)) return cudaSuccess;
   HtGrid gr;
   gr.nqt = cdiv(p.Nq, 128);
   const int64_t pairs = ((int64_t)gr.nqt * p.G + 1) / 2;
   const int64_t items = pairs * p.B * p.Hk;
   if (items > (1 << 30)) return cudaSuccess;
+  // With few items those kernels fill the GPU by splitting the key axis. 128
+  // rows of 8 heads, d = 64, against 2048 and 8192 keys: 40 items 28 / 27 and
+  // 67 / 92 us, 56 items 36 / 27 and 85 / 93, 128 items 63 / 28 and 161 / 96.
+  if (p.splits > 1 && items < 56) return cudaSuccess;
   CUtensorMap m[3];
   if (!head_tensor_map(&m[0], p.q, p.sq, p.B, p.Nq, p.H, p.d) ||
       !head_tensor_map(&m[1], p.k, p.sk, p.B, p.Nk, p.Hk, p.d) ||

@@ -529,11 +529,19 @@ static cudaError_t bwd_tc_go(const CUtensorMap* m, const HeadAttnParams& p, int6
   return cudaGetLastError();
 }
 
-// bf16 rows on the 16-byte grid, at least 64 queries and 64 keys; the row
+// bf16 rows on the 16-byte grid, by the rules below; the row
 // statistics are in p.delta already. *done says whether the call was taken.
 cudaError_t launch_head_bwd_tc(const HeadAttnParams& p, int64_t nqp, cudaStream_t s, bool* done) {
   *done = false;
-  if (!p.vec || p.Nq < 64 || p.Nk < 64) return cudaSuccess;
+  // Short sets leave the 128 x 128 tiles mostly empty; the kernels of
+  // head_attn.cu were faster there. Measured, those against these, dq and dk,
+  // dv together (us): 512 x 8 heads, d = 64: N = 64 138 / 220, N = 96 305 /
+  // 234, N = 256 1175 / 591; 128 x 8 heads, d = 64, rows x keys: 32 x 512 171 /
+  // 178, 40 x 512 213 / 181, 1024 x 40 406 / 334. d = 32, 512 x 4 heads:
+  // N = 192 238 / 259, N = 224 347 / 261; d = 16, 256 x 4 heads: N = 192 88 /
+  // 121, N = 256 142 / 121.
+  const int longer = p.Nq > p.Nk ? p.Nq : p.Nk;
+  if (!p.vec || p.Nk < 1 || p.Nq <= 32 || longer <= (p.d > 32 ? 64 : 192)) return cudaSuccess;
   if ((int64_t)p.B * p.H * cdiv(p.Nq, 128) > (1 << 30) ||
       (int64_t)p.B * p.Hk * cdiv(p.Nk, 128) > (1 << 30))
     return cudaSuccess;
