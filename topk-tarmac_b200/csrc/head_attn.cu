@@ -27,6 +27,7 @@ namespace tarmac {
 
 constexpr int HA_THREADS = 128;
 constexpr int HA_WARPS = 4;
+constexpr int HA_PART = 256;  // keys of a part of the key axis, at least
 constexpr float HA_LOG2E = 1.4426950408889634f;
 constexpr float HA_LN2 = 0.6931471805599453f;
 
@@ -91,7 +92,9 @@ __device__ __forceinline__ void load_keys_tile(T* dst, int n, int limit, int d, 
   load_tile<T, DP>(dst, n, limit, d, vec, [&](int r) { return first + r * stride; });
 }
 
-// fp32 rows of up to 32 columns are staged as split pairs (head_mma.cuh).
+// fp32 rows of up to 32 columns are staged as split pairs (head_mma.cuh): 64 x
+// 512 rows of 4 heads, d = 16, forward 131 us, split when read 143. Wider rows
+// would not leave room for as many blocks.
 template <typename T, int DP>
 constexpr bool ha_split() {
   return sizeof(T) == 4 && DP <= 32;
@@ -248,8 +251,12 @@ __global__ void __launch_bounds__(HA_THREADS) head_fwd_kernel(HeadAttnParams p) 
   // keys of this block: its part, cut to what any of its rows may see
   const int64_t last_pos = (int64_t)start + (r0 + nrows - 1) / p.G;
   int kend = p.peers == PEERS_PAST ? (int)max((int64_t)0, min((int64_t)len, last_pos + 1)) : len;
-  const int kbeg = p.splits > 1 ? w.split * p.split_keys : 0;
-  if (p.splits > 1) kend = min(kend, kbeg + p.split_keys);
+  int kbeg = 0;
+  if (p.splits > 1) {  // its equal share of the keys that these rows have
+    const int per = max(HA_PART, cdiv(cdiv(kend, p.splits), 64) * 64);
+    kbeg = (int)min((int64_t)kend, (int64_t)w.split * per);
+    kend = min(kend, kbeg + per);
+  }
   const int ntiles = kend > kbeg ? cdiv(kend - kbeg, KT) : 0;
 
   const T* Q = static_cast<const T*>(p.q) + w.b * p.sq.b + (int64_t)w.hk * p.G * p.sq.h;
@@ -483,26 +490,34 @@ __global__ void __launch_bounds__(HA_THREADS) head_fwd_kernel(HeadAttnParams p) 
 }
 
 // Join the parts of the key axis: out = sum_s w_s out_s, w_s = exp(lse_s -
-// lse). One warp per (episode, row, head): its lanes first hold the parts'
-// lse, then the columns.
-template <typename T>
-__global__ void __launch_bounds__(128) head_join_kernel(HeadAttnParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+// lse). One block per (episode, row, head); its warps share the parts, and
+// their sums are added in order.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) head_join_kernel(HeadAttnParams p) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ float s_x[WARPS][128], s_top[WARPS], s_sum[WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x;
   const int64_t total = (int64_t)p.B * p.Nq * p.H;
-  if (row >= total) return;
   const int h = (int)(row % p.H);
   const int64_t bi = row / p.H;
   const int i = (int)(bi % p.Nq);
   const int b = (int)(bi / p.Nq);
   const int64_t srow = ((int64_t)b * p.H + h) * p.Nq + i;
   float top = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_lse[s * total + srow]);
+  for (int s = threadIdx.x; s < p.splits; s += THREADS)
+    top = fmaxf(top, p.part_lse[s * total + srow]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) s_top[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_top[w]);
   float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < p.splits && top != -INFINITY; s0 += 32) {
-    const float ls = s0 + lane < p.splits ? p.part_lse[(s0 + lane) * total + srow] : -INFINITY;
+  // warp w takes parts w, w + WARPS, ...; its lanes hold the weights of 32
+  for (int s0 = warp; s0 < p.splits && top != -INFINITY; s0 += 32 * WARPS) {
+    const int mine = s0 + lane * WARPS;
+    const float ls = mine < p.splits ? p.part_lse[mine * total + srow] : -INFINITY;
     const float wgt = ls == -INFINITY ? 0.f : expf(ls - top);
     // parts that saw nothing wrote nothing
     uint32_t left = __ballot_sync(0xffffffffu, ls != -INFINITY);
@@ -513,7 +528,7 @@ __global__ void __launch_bounds__(128) head_join_kernel(HeadAttnParams p) {
         const int s = left ? __ffs(left) - 1 : -1;
         if (s >= 0) left &= left - 1;
         wv[q] = __shfl_sync(0xffffffffu, wgt, s < 0 ? 0 : s);
-        const float* o = p.part_o + ((int64_t)(s0 + (s < 0 ? 0 : s)) * total + row) * p.d;
+        const float* o = p.part_o + ((int64_t)(s0 + (s < 0 ? 0 : s) * WARPS) * total + row) * p.d;
 #pragma unroll
         for (int u = 0; u < 4; ++u)
           y[q][u] = s >= 0 && lane + 32 * u < p.d ? o[lane + 32 * u] : 0.f;
@@ -527,12 +542,21 @@ __global__ void __launch_bounds__(128) head_join_kernel(HeadAttnParams p) {
       }
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int u = 0; u < 4; ++u)
-    if (lane + 32 * u < p.d)
-      static_cast<T*>(p.o)[row * p.d + lane + 32 * u] = from_f32<T>(x[u] * inv);
-  if (lane == 0 && p.lse) p.lse[srow] = sum == 0.f ? -INFINITY : top + logf(sum);
+  for (int u = 0; u < 4; ++u) s_x[warp][lane + 32 * u] = x[u];
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) sum += s_sum[w];
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  for (int c = threadIdx.x; c < p.d; c += THREADS) {
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) y += s_x[w][c];
+    static_cast<T*>(p.o)[row * p.d + c] = from_f32<T>(y * inv);
+  }
+  if (threadIdx.x == 0 && p.lse) p.lse[srow] = sum == 0.f ? -INFINITY : top + logf(sum);
 }
 
 // ---------------------------------------------------------------------------
@@ -972,26 +996,25 @@ cudaError_t launch_pack_bits(const void* v, int64_t sb, int64_t sn, int B, int N
 // launches
 // ---------------------------------------------------------------------------
 constexpr int HA_SMS = 148;
+// Up to 16 packed rows a block owns one tile of 16 and its warps share the
+// keys; else 64 rows, 16 a warp. One token, 32 x 16384 keys, 16 heads on 2, d =
+// 128, bf16: 98 us with 16-row blocks, 144 with 64; 256 episodes of 16 agents,
+// 8 heads, d = 64: 20 and 27 us; of 6 agents, 4 heads, d = 16, fp32: 8 and 11.
 constexpr int HA_NARROW_ROWS = 16;
 
 // Parts of the key axis: with fewer blocks than the GPU holds at once, split
-// until there are about eight per SM, each of at least 256 keys: ragged
-// lengths leave parts without keys, and short parts even that out (32 episodes
-// of up to 16384 keys, both kernels: 69 us with 8 per SM, 71 with 16, 88 with
-// 32).
-void head_split_plan(int B, int Nq, int Nk, int H, int Hk, int* splits, int* split_keys) {
+// until there are about six per SM, each of at least 256 keys. A part is an
+// equal share of what its rows may see, so ragged lengths leave no block idle.
+// One token, 32 episodes of 16 heads on 2, d = 128, bf16: 16384 keys with four
+// parts per SM 106 us, six 95 (5.6 TB/s), eight 98; up to 16384 keys 56, 58
+// and 57 (parts of equal length, half of them empty: 63).
+int head_splits(int B, int Nq, int Nk, int H, int Hk) {
   const int64_t rows = (int64_t)Nq * (H / Hk);
   const int tile = rows <= HA_NARROW_ROWS ? 16 : 64;
   const int64_t base = (int64_t)B * Hk * ((rows + tile - 1) / tile);
-  *splits = 1;
-  *split_keys = Nk;
-  if (base >= 2 * HA_SMS || Nk < 512) return;
-  int64_t n = (8 * HA_SMS + base - 1) / base;
-  if (n > Nk / 256) n = Nk / 256;
-  if (n < 2) return;
-  const int keys = cdiv(cdiv(Nk, (int)n), 64) * 64;
-  *split_keys = keys;
-  *splits = cdiv(Nk, keys);
+  if (base >= 2 * HA_SMS || Nk < 2 * HA_PART) return 1;
+  const int64_t n = (6 * HA_SMS + base - 1) / base;
+  return (int)(n < Nk / HA_PART ? n : Nk / HA_PART);
 }
 
 template <typename T, int DP, bool NARROW>
@@ -1006,7 +1029,12 @@ static cudaError_t fwd_go(const HeadAttnParams& p, cudaStream_t s) {
   e = cudaGetLastError();
   if (e != cudaSuccess || p.splits == 1) return e;
   const int64_t rows = (int64_t)p.B * p.Nq * p.H;
-  head_join_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
+  // few rows: more warps for each. 16 rows of 256 parts: 6.3 us with 256
+  // threads, 9.4 with 128; 4096 rows of 6 parts: 6.6 us with 64, 9.7 with 128.
+  if (rows <= 4 * HA_SMS)
+    head_join_kernel<T, 256><<<(unsigned)rows, 256, 0, s>>>(p);
+  else
+    head_join_kernel<T, 64><<<(unsigned)rows, 64, 0, s>>>(p);
   return cudaGetLastError();
 }
 

@@ -20,7 +20,11 @@
 // 1024 rows: 128 against 129 us) and slower with masks (204 against 184 us).
 // Bound: the special-function unit's 16 exponentials per clock per SM (1024
 // clocks for a 128 x 128 tile) against 256 d / 64 clocks for each of the two
-// products. Blocks are persistent, one per SM, and walk their items in
+// products. Measured on B200: 2 x 8192 causal rows of 16 heads on 4, d = 128:
+// 503 us, 1.09 PFLOP/s; 32 x 1024 rows of 8 heads, d = 64: 127 us, 541 TFLOP/s
+// (its 268 M exponentials alone take 63 us at 1.8 GHz); 256 x 512 rows of 4
+// heads on 2, d = 64, with visibility words 182 us, without 143 us.
+// Blocks are persistent, one per SM, and walk their items in
 // alternating direction, so that under the past rule each gets long and short
 // tiles.
 // Every wait is bounded; one that runs out raises a flag that ends all roles,

@@ -55,7 +55,6 @@ struct HeadAttnParams {
   float scale;
   int vec;                    // 16-byte rows everywhere
   int splits;                 // forward: parts of the key axis
-  int split_keys;             // keys of a part
   float* part_o;              // [splits, B, Nq, H, d]
   float* part_lse;            // [splits, B, H, Nq]
   float* delta;               // backward: row statistics (head_attn.cu)

@@ -8,7 +8,7 @@ namespace tarmac {
 
 cudaError_t launch_head_fwd(const HeadAttnParams& p, bool bf16, cudaStream_t s);
 cudaError_t launch_head_bwd(const HeadAttnParams& p, bool bf16, cudaStream_t s);
-void head_split_plan(int B, int Nq, int Nk, int H, int Hk, int* splits, int* split_keys);
+int head_splits(int B, int Nq, int Nk, int H, int Hk);
 cudaError_t launch_pack_bits(const void* v, int64_t sb, int64_t sn, int B, int Nq, int Nk,
                              uint32_t* out, cudaStream_t s);
 
@@ -80,7 +80,6 @@ int fill_attn(HeadAttnParams& p, const void* q, const void* k, const void* v,
   p.peers = peers;
   p.scale = scale;
   p.splits = 1;
-  p.split_keys = Nk;
   return TARMAC_OK;
 }
 
@@ -200,8 +199,7 @@ int tarmac_pack_visibility(const void* visible, int64_t stride_b, int64_t stride
 
 int64_t tarmac_head_attention_workspace(int B, int Nq, int Nk, int H, int Hk, int d) {
   if (B < 1 || Nq < 1 || Nk < 1 || Hk < 1 || H < Hk || H % Hk || d < 1 || d > MAX_D) return 0;
-  int splits, keys;
-  head_split_plan(B, Nq, Nk, H, Hk, &splits, &keys);
+  const int splits = head_splits(B, Nq, Nk, H, Hk);
   if (splits == 1) return 0;
   const int64_t rows = (int64_t)B * Nq * H;
   return round16(splits * rows * d * 4) + round16(splits * rows * 4);
@@ -224,7 +222,7 @@ int tarmac_head_attention(const void* q, const void* k, const void* v, void* out
   p.sk = stride_of(strides, 1, Nk, Hk, d);
   p.sv = stride_of(strides, 2, Nk, Hk, d);
   p.vec = d * es % 16 == 0 && vec_ok(q, p.sq, es) && vec_ok(k, p.sk, es) && vec_ok(v, p.sv, es);
-  if (Nk > 0) head_split_plan(B, Nq, Nk, H, Hk, &p.splits, &p.split_keys);
+  if (Nk > 0) p.splits = head_splits(B, Nq, Nk, H, Hk);
   if (p.splits > 1) {
     if (!work) return TARMAC_ERR_NULL;
     const int64_t rows = (int64_t)B * Nq * H;
