@@ -161,7 +161,7 @@ def test_rotate_many_rows(ops):
 
 def attention_case(ops, B, Nq, Nk, H, Hk, d, dtype, peers="all", lens=None, starts=None,
                    seen=None, shift=0, seed=0, spoil=False, scale=None, shared_mask=False,
-                   size=1.0):
+                   size=1.0, broadcast=False):
     g = torch.Generator().manual_seed(seed + 31 * Nq + Nk + d)
     if Nq == Nk:
         q, k, v = rows(g, B, Nq, (H, Hk, Hk), d, dtype, shift)
@@ -171,6 +171,9 @@ def attention_case(ops, B, Nq, Nk, H, Hk, d, dtype, peers="all", lens=None, star
     if size != 1.0:
         q = q * size
     dout, = rows(g, B, Nq, (H,), d, dtype, shift)
+    if broadcast:  # one history for all episodes, one gradient for all rows
+        k, v = (t[:1].expand(B, -1, -1, -1) for t in (k, v))
+        dout = dout[:1, :1].expand(B, Nq, -1, -1)
     key_len = None if lens is None else torch.tensor(lens, dtype=torch.int32)
     q_start = None if starts is None else torch.tensor(starts, dtype=torch.int32)
     visible = None
@@ -266,6 +269,12 @@ def test_attention_long_history(ops, B, Nq, Nk, H, Hk, d, lens, dtype):
         assert ops._attention_work(B, Nq, Nk, H, Hk, d) > 0
     attention_case(ops, B, Nq, Nk, H, Hk, d, dtype, "past", lens=lens, seen=0.8,
                    starts=None if lens is None else [n - Nq for n in lens])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_broadcast_inputs(ops, dtype):
+    attention_case(ops, 3, 150, 150, 4, 2, 64, dtype, "others", broadcast=True)
+    attention_case(ops, 3, 2, 700, 4, 2, 128, dtype, "all", broadcast=True)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

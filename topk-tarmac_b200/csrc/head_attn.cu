@@ -92,9 +92,10 @@ __device__ __forceinline__ void load_keys_tile(T* dst, int n, int limit, int d, 
   load_tile<T, DP>(dst, n, limit, d, vec, [&](int r) { return first + r * stride; });
 }
 
-// fp32 rows of up to 32 columns are staged as split pairs (head_mma.cuh): 64 x
-// 512 rows of 4 heads, d = 16, forward 131 us, split when read 143. Wider rows
-// would not leave room for as many blocks.
+// Narrow fp32 rows are staged as split pairs (head_mma.cuh), up to 32 columns
+// forward and 16 backward. 64 x 512 rows of 4 heads, staged so or split when
+// read: forward d = 16 127 and 139 us, 32 215 and 227, 64 461 and 423; dk, dv
+// d = 16 255 and 267, 32 501 and 475.
 template <typename T, int DP>
 constexpr bool ha_split() {
   return sizeof(T) == 4 && DP <= 32;
@@ -633,7 +634,7 @@ struct HaBwd {
   static constexpr int RT = 64;                    // rows (or keys) a block owns
   static constexpr int TT = 32;                    // streamed rows per tile
   static constexpr int NT = TT / 8;
-  static constexpr bool SPLIT = ha_split<T, DP>();
+  static constexpr bool SPLIT = ha_split<T, DP>() && DP <= 16;
   static constexpr int RS = SPLIT ? hm::split_stride<DP>() : hm::row_stride<T, DP>();
   static constexpr size_t STAGE = (size_t)2 * TT * RS * sizeof(T);
   static constexpr size_t SMEM = (size_t)2 * RT * RS * sizeof(T) + 2 * STAGE;
@@ -1030,7 +1031,7 @@ static cudaError_t fwd_go(const HeadAttnParams& p, cudaStream_t s) {
   if (e != cudaSuccess || p.splits == 1) return e;
   const int64_t rows = (int64_t)p.B * p.Nq * p.H;
   // few rows: more warps for each. 16 rows of 256 parts: 6.3 us with 256
-  // threads, 9.4 with 128; 4096 rows of 6 parts: 6.6 us with 64, 9.7 with 128.
+  // threads, 9.4 with 128; 4096 rows of 8 parts: 6.6 us with 64, 9.7 with 128.
   if (rows <= 4 * HA_SMS)
     head_join_kernel<T, 256><<<(unsigned)rows, 256, 0, s>>>(p);
   else
