@@ -18,10 +18,13 @@
 // O_g at 256 + DP g. A P_g with columns of its own, which lets S of the next
 // key tile run under the exponentials, was no faster at d = 64 (32 x 8 heads of
 // 1024 rows: 128 against 129 us) and slower with masks (204 against 184 us).
-// Bound: the special-function unit's 16 exponentials per clock per SM (1024
-// clocks for a 128 x 128 tile) against 256 d / 64 clocks for each of the two
-// products. Measured on B200: 2 x 8192 causal rows of 16 heads on 4, d = 128:
-// 503 us, 1.09 PFLOP/s; 32 x 1024 rows of 8 heads, d = 64: 127 us, 541 TFLOP/s
+// Bound: of a tile's 1900 to 2000 clocks the special-function unit's 16
+// exponentials per clock take 1024 (128 x 128 scores), the two products 256 d /
+// 64 each; the rest is the chain from S to P and back, which two tiles in turn
+// hide in part. Forming an eighth, a quarter or half of the exponentials as a
+// polynomial on the FMA pipe gave 127, 131 and 142 us where this takes 127.
+// Measured on B200: 2 x 8192 causal rows of 16 heads on 4, d = 128:
+// 500 us, 1.10 PFLOP/s; 32 x 1024 rows of 8 heads, d = 64: 127 us, 541 TFLOP/s
 // (its 268 M exponentials alone take 63 us at 1.8 GHz); 256 x 512 rows of 4
 // heads on 2, d = 64, with visibility words 182 us, without 143 us.
 // Blocks are persistent, one per SM, and walk their items in
