@@ -22,7 +22,8 @@
 // exponentials per clock take 1024 (128 x 128 scores), the two products 256 d /
 // 64 each; the rest is the chain from S to P and back, which two tiles in turn
 // hide in part. Forming an eighth, a quarter or half of the exponentials as a
-// polynomial on the FMA pipe gave 127, 131 and 142 us where this takes 127.
+// polynomial on the FMA pipe gave 127, 131 and 142 us where this takes 127;
+// P V in two halves, the first under the exponentials of the second, 132.
 // Measured on B200: 2 x 8192 causal rows of 16 heads on 4, d = 128:
 // 500 us, 1.10 PFLOP/s; 32 x 1024 rows of 8 heads, d = 64: 127 us, 541 TFLOP/s
 // (its 268 M exponentials alone take 63 us at 1.8 GHz); 256 x 512 rows of 4
