@@ -74,6 +74,14 @@ ROTATE = [  # B, N, H, Hk, d, r, interleaved, own table, shift
     (2, 6, 4, 2, 64, 32, False, True, 3),
     (2, 6, 4, 2, 80, 80, False, True, 4),
     (700, 6, 4, 4, 16, 16, False, True, 0),
+    # rows that fill their lanes, over several row tiles of a block
+    (3, 50, 4, 2, 64, 32, False, False, 0),
+    (2, 301, 6, 2, 64, 64, True, True, 0),
+    (2, 45, 2, 6, 128, 128, False, False, 0),
+    (3, 131, 2, 4, 128, 64, False, True, 0),
+    (5, 70, 8, 4, 32, 16, True, True, 0),
+    (1, 260, 2, 2, 32, 32, False, True, 0),
+    (2, 150, 4, 6, 48, 16, False, True, 0),
 ]
 
 
