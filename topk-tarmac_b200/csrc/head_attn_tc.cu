@@ -57,7 +57,7 @@ struct HtPlan {
 
 template <int NS>
 struct HtShared {
-  uint64_t qfull, qempty, kfull[NS], vfull[NS], empty[NS], sfull[2], pfull[2], odone[2];
+  uint64_t qfull, qempty, kfull[NS], vfull[NS], empty[NS], sfull[2], pfull[2], odone[2], drain;
   uint32_t tmem;
   int abort_flag;
   float top[2][2][2][128];  // row maxima: tile, step parity, group, row
@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
       tc::mbar_init(&sh.pfull[w], 8);
       tc::mbar_init(&sh.odone[w], 1);
     }
+    tc::mbar_init(&sh.drain, 1);
     sh.abort_flag = 0;
     tc::mbar_init_fence();
   }
@@ -146,11 +147,14 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
 
   if (warp == HT_TMA_WARP) {
     if (lane == 0) {
-      uint32_t kc = 0;
-      int k = 0;
-      for (;; ++k) {
+      uint32_t kc = 0, qc = 0;  // copies issued: K and V tiles, Q tiles
+      for (int k = 0;; ++k) {
         const int item = ht_next(k);
         if (item >= gr.items) break;
+        if (ht::gives_up(ht::ROLE_LOADER, k)) {
+          *abort_flag = 1;
+          break;
+        }
         const HtItem w = ht_item(p, gr, item);
         if (!ws::wait(&sh.qempty, (k & 1) ^ 1, abort_flag)) goto tma_done;
         const int both = w.tile[1] >= 0;
@@ -158,6 +162,7 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
         for (int u = 0; u <= both; ++u)
           ht::tma_tile<DP, 128>(qa + u * TILE, &mq, &sh.qfull, w.hk * p.G + w.g[u],
                                 w.tile[u] * 128, w.b);
+        ++qc;
         for (int t = 0; t < w.n; ++t, ++kc) {
           const int s = kc % NS;
           if (!ws::wait(&sh.empty[s], ((kc / NS) & 1) ^ 1, abort_flag)) goto tma_done;
@@ -169,14 +174,10 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
         }
       }
     tma_done:
-      // the copies in flight land before the block ends
-      if (*abort_flag) {
-        if (k > 0 || kc > 0) tc::mbar_wait(&sh.qfull, 0, 1u << 16);
-        for (uint32_t c = kc > (uint32_t)NS ? kc - NS : 0; c < kc; ++c) {
-          tc::mbar_wait(&sh.kfull[c % NS], (c / NS) & 1, 1u << 16);
-          tc::mbar_wait(&sh.vfull[c % NS], (c / NS) & 1, 1u << 16);
-        }
-      }
+      // the copies in flight land before the block ends, whoever gave up
+      ht::drain_copies(&sh.qfull, 1, qc);
+      ht::drain_copies(sh.kfull, NS, kc);
+      ht::drain_copies(sh.vfull, NS, kc);
     }
     __syncwarp();
   } else if (warp == HT_MMA_WARP) {
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
         kr.next();
       }
       if (n <= 1 && ok && leader) ht::commit_at(b_qempty);
-      __syncwarp();
+      ok = ht::agree(ok);
       for (int t = 0; t < n && ok; ++t, ++kc) {
         ok = ht::wait_at(b_vfull + 8 * vr.s, vr.ph, abort_flag);
         if (t + 1 < n) wait_k();
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
           ht::commit_at(b_empty + 8 * vr.s);
           if (t + 2 == n) ht::commit_at(b_qempty);
         }
-        __syncwarp();
+        ok = ht::agree(ok);
         vr.next();
         if (t + 1 < n) kr.next();
       }
@@ -248,6 +249,7 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
     // the last commits land before the block ends
     for (uint32_t c = kc > (uint32_t)NS ? kc - NS : 0; c < kc && ok; ++c)
       ok = ht::wait_at(b_empty + 8 * (c % NS), (c / NS) & 1, abort_flag);
+    if (!ht::agree(ok)) ht::drain_products(&sh.drain, leader);
     __syncwarp();
   } else if (warp >= HT_W0) {
     // ---------------- softmax groups ----------------

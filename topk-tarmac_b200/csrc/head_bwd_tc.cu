@@ -61,7 +61,7 @@ struct HbPlan {
 template <int NX, int NY>
 struct HbShared {
   uint64_t own_full, own_empty, xfull[NX], xempty[NX], yfull[NY], yempty[NY];
-  uint64_t sfull[2], dpfull, pfull, dsfull, acc_full, acc_empty;
+  uint64_t sfull[2], dpfull, pfull, dsfull, acc_full, acc_empty, drain;
   uint32_t tmem;
   int abort_flag;
 };
@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
     tc::mbar_init(&sh.dsfull, 16);
     tc::mbar_init(&sh.acc_full, 1);
     tc::mbar_init(&sh.acc_empty, 16);
+    tc::mbar_init(&sh.drain, 1);
     sh.abort_flag = 0;
     tc::mbar_init_fence();
   }
@@ -179,10 +180,14 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
 
   if (warp == HB_TMA_WARP) {
     if (lane == 0) {
-      uint32_t c = 0, oc = 0;
+      uint32_t xc = 0, yc = 0, oc = 0;  // copies issued: X, Y and own tiles
       for (int k = 0;; ++k) {
         const int item = hb_next(k);
         if (item >= gr.items) break;
+        if (ht::gives_up(ht::ROLE_LOADER, k)) {
+          *abort_flag = 1;
+          break;
+        }
         const HbItem w = hb_item<DQ>(p, gr, item);
         if (w.n == 0) continue;
         if (!ws::wait(&sh.own_empty, (oc & 1) ^ 1, abort_flag)) goto tma_done;
@@ -191,10 +196,10 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
         ht::tma_tile<DP, 128>(own, DQ ? &mq : &mk, &sh.own_full, w.h, w.x0, w.b);
         ht::tma_tile<DP, 128>(own + TILE, DQ ? &mg : &mv, &sh.own_full, w.h, w.x0, w.b);
         int g = 0, t = w.t0;
-        for (int x = 0; x < w.n; ++x, ++c) {
-          const int sx = c % NX, sy = c % NY;
+        for (int x = 0; x < w.n; ++x) {
+          const int sx = xc % NX, sy = yc % NY;
           const int head = DQ ? w.hk : w.hk * p.G + g;
-          if (!ws::wait(&sh.xempty[sx], ((c / NX) & 1) ^ 1, abort_flag)) goto tma_done;
+          if (!ws::wait(&sh.xempty[sx], ((xc / NX) & 1) ^ 1, abort_flag)) goto tma_done;
           ht::expect_tx(&sh.xfull[sx], TILE + Plan::STATS);
           ht::tma_tile<DP, HB_T>(xr + sx * TILE, DQ ? &mk : &mq, &sh.xfull[sx], head, t * HB_T,
                                  w.b);
@@ -204,10 +209,12 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
             ht::bulk_copy(stats + sx * Plan::STATS + HB_T * 4, st + stat_plane, HB_T * 4,
                           &sh.xfull[sx]);
           }
-          if (!ws::wait(&sh.yempty[sy], ((c / NY) & 1) ^ 1, abort_flag)) goto tma_done;
+          ++xc;
+          if (!ws::wait(&sh.yempty[sy], ((yc / NY) & 1) ^ 1, abort_flag)) goto tma_done;
           ht::expect_tx(&sh.yfull[sy], TILE);
           ht::tma_tile<DP, HB_T>(yr + sy * TILE, DQ ? &mv : &mg, &sh.yfull[sy], head, t * HB_T,
                                  w.b);
+          ++yc;
           if (++t == w.t0 + w.nper) {
             t = w.t0;
             ++g;
@@ -215,13 +222,10 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
         }
       }
     tma_done:
-      if (*abort_flag) {  // the copies in flight land before the block ends
-        if (oc) tc::mbar_wait(&sh.own_full, (oc - 1) & 1, 1u << 16);
-        for (uint32_t x = c > 3u ? c - 3 : 0; x <= c; ++x) {
-          tc::mbar_wait(&sh.xfull[x % NX], (x / NX) & 1, 1u << 16);
-          tc::mbar_wait(&sh.yfull[x % NY], (x / NY) & 1, 1u << 16);
-        }
-      }
+      // the copies in flight land before the block ends, whoever gave up
+      ht::drain_copies(&sh.own_full, 1, oc);
+      ht::drain_copies(sh.xfull, NX, xc);
+      ht::drain_copies(sh.yfull, NY, yc);
     }
     __syncwarp();
   } else if (warp == HB_MMA_WARP) {
@@ -278,7 +282,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
       if (n == 1 && ok && leader) ht::commit_at(b_own_empty);
       __syncwarp();
       // the accumulators of the item before have been read
-      ok = ok && ht::wait_at(b_acc_empty, (oc & 1) ^ 1, abort_flag);
+      ok = ht::agree(ok && ht::wait_at(b_acc_empty, (oc & 1) ^ 1, abort_flag));
       ++oc;
       for (int t = 0; t < n && ok; ++t, ++c) {
         if constexpr (!DQ) {
@@ -307,6 +311,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
         if (t + 2 == n && ok && leader) ht::commit_at(b_own_empty);
         __syncwarp();
         if (DQ && t + 2 < n) issue_s();
+        ok = ht::agree(ok);
       }
       if (ok && leader) ht::commit_at(b_acc_full);
       __syncwarp();
@@ -314,7 +319,8 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
     // the last commits land before the block ends
     for (uint32_t x = c > (uint32_t)NX ? c - NX : 0; x < c && ok; ++x)
       ok = ht::wait_at(b_xempty + 8 * (x % NX), (x / NX) & 1, abort_flag);
-    if (oc && ok) ht::wait_at(b_own_empty, (oc - 1) & 1, abort_flag);
+    if (oc && ok) ok = ht::wait_at(b_own_empty, (oc - 1) & 1, abort_flag);
+    if (!ht::agree(ok)) ht::drain_products(&sh.drain, leader);
     __syncwarp();
   } else if (warp >= HB_W0) {
     // ---------------- weights ----------------

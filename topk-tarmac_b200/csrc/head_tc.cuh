@@ -21,6 +21,18 @@ namespace ht {
 
 constexpr int width(int nks) { return nks <= 4 ? 64 : 128; }  // DP
 
+// Test builds define TARMAC_GIVE_UP_AT, a number of a block's item, and
+// TARMAC_GIVE_UP_ROLE: that role gives up there as it does when one of its
+// waits runs out.
+enum Role { ROLE_LOADER = 0, ROLE_WEIGHTS = 1 };
+__device__ constexpr bool gives_up(Role role, int k) {
+#ifdef TARMAC_GIVE_UP_AT
+  return role == TARMAC_GIVE_UP_ROLE && k == TARMAC_GIVE_UP_AT;
+#else
+  return false;
+#endif
+}
+
 constexpr uint32_t BOX_ROWS = 64;
 constexpr uint32_t BOX_BYTES = 64 * 128;
 
@@ -110,6 +122,24 @@ __device__ __forceinline__ void commit_at(uint32_t a) {
   asm volatile(
       "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(a)
       : "memory");
+}
+// Wait, bounded, until the last `n` of `count` copies into a ring of n slots
+// have landed: shared memory must not be written after its block has ended.
+// Copy c completes phase c / n of its slot.
+__device__ __forceinline__ void drain_copies(uint64_t* full, uint32_t n, uint32_t count) {
+  for (uint32_t c = count > n ? count - n : 0; c < count; ++c)
+    tc::mbar_wait(&full[c % n], (c / n) & 1, WS_WAIT_LIMIT);
+}
+// The issuing warps' lanes wait each for itself. Before a loop's condition
+// they agree on whether all go on: a lane that left alone would not meet the
+// others' warp barriers.
+__device__ __forceinline__ bool agree(bool ok) { return __all_sync(0xffffffffu, ok); }
+// The same for the products that this warp's `leader` has issued, after it
+// gave up: tensor memory is freed and the operands' tiles end with the block.
+__device__ __forceinline__ void drain_products(uint64_t* drain, bool leader) {
+  if (leader) commit_at(tc::smem_addr(drain));
+  __syncwarp();
+  tc::mbar_wait(drain, 0, WS_WAIT_LIMIT);
 }
 // One lane of a converged warp. The issuing warps run their loops with all
 // lanes, so that addresses and descriptors stay in uniform registers, and
