@@ -138,3 +138,14 @@ def test_backward_loader(builds, case):
     still_right(so, case)
     for a, b in zip(by_parts(lambda *t: backward(so, *t), *args), want):
         assert torch.equal(a, b)
+
+
+def test_forward_half_of_a_row(builds, case):
+    """The warps of one half of each row's columns give up: the other half, with
+    whom they share the row's maximum and sum, is not left with finite values."""
+    so = builds(WEIGHTS)
+    want = by_parts(lambda *t: forward(so, *t), *case[:3])
+    for a, b in zip(forward(so, *case[:3]), want):
+        nan_or_right(a, b)
+        assert a.isnan().any()
+    still_right(so, case)

@@ -280,6 +280,10 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
       const int item = ht_next(k);
       if (item >= gr.items) break;
       const HtItem it = ht_item(p, gr, item);
+      if (ht::gives_up(ht::ROLE_WEIGHTS, k) && half) {
+        ok = false;
+        *abort_flag = 1;
+      }
       const uint32_t kc0 = kc;
       kc += (uint32_t)it.n;
       const int tile = w ? it.tile[1] : it.tile[0], nt = w ? it.nt[1] : it.nt[0];
@@ -388,6 +392,9 @@ __global__ void __launch_bounds__(HT_THREADS, 1)
         if (ok) ok = ht::warp_wait(&sh.odone[w], oc & 1, abort_flag);
         ++oc;
         tc::fence_after_sync();
+        // a row whose other half gave up is NaN as a whole: its reference
+        // maximum and its sum have both halves' parts
+        if (!ok) l = __int_as_float(0x7fffffff);
         sh.sum[w][half][row] = l;
         pair_sync();
         l += sh.sum[w][half ^ 1][row];
