@@ -149,3 +149,18 @@ def test_forward_half_of_a_row(builds, case):
         nan_or_right(a, b)
         assert a.isnan().any()
     still_right(so, case)
+
+
+@pytest.mark.parametrize("role", [LOADER, WEIGHTS])
+def test_backward_rows(builds, case, role):
+    """Every row of the gradients is written, also those of the items that a
+    block had not reached when it gave up."""
+    so = builds(role)
+    q, k, v, dout = case
+    out, lse = by_parts(lambda *t: forward(so, *t), q, k, v)
+    args = (q, k, v, dout, out, lse)
+    want = by_parts(lambda *t: backward(so, *t), *args)
+    for a, b in zip(backward(so, *args), want):
+        nan_or_right(a, b)
+        assert a.isnan().any()
+    still_right(so, case)

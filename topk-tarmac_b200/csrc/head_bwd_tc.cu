@@ -333,9 +333,14 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
     const uint64_t cc2 = pack2(c2, c2);
     uint32_t c = 0, ac = 0;
     bool ok = true;
-    for (int k = 0; ok; ++k) {
+    // warps that gave up walk on over the block's items and write NaN
+    for (int k = 0;; ++k) {
       const int item = hb_next(k);
       if (item >= gr.items) break;
+      if (ht::gives_up(ht::ROLE_WEIGHTS, k) && part == 1) {
+        ok = false;
+        *abort_flag = 1;
+      }
       const HbItem it = hb_item<DQ>(p, gr, item);
       const int own_row = it.x0 + row;
       float nlse = -INFINITY, ndelta = 0.f;  // -lse2 and -D of a query row
@@ -355,7 +360,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
       // keys: the query (as an index) that stands at this key's position
       const int twin = own_row - it.start;
       int tt = it.t0;  // streamed tile inside its head
-      for (int t = 0; t < it.n; ++t) {
+      for (int t = 0; t < it.n && ok; ++t) {
         const uint32_t x = c + t;
         const int x0 = tt * HB_T + part * 32;  // first column of this thread
         if (++tt == it.t0 + it.nper) tt = it.t0;
@@ -492,7 +497,12 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
       const uint32_t t_acc = tmem + lane_off + (second ? DP : 0);
       for (int cc = c0; cc < c1 && cc < p.d; cc += 16) {
         uint32_t o[16];
-        if (it.n > 0) ht::tmem_ld(t_acc + cc, o);
+        if (it.n > 0 && ok) {
+          ht::tmem_ld(t_acc + cc, o);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 16; ++u) o[u] = 0u;
+        }
         if (own_row < own_n) {
 #pragma unroll
           for (int u = 0; u < 16; u += 8) {
@@ -508,7 +518,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1)
           }
         }
       }
-      if (it.n > 0) {
+      if (it.n > 0 && ok) {
         tc::fence_before_sync();
         __syncwarp();
         if (lane == 0) ws::arrive(&sh.acc_empty);
