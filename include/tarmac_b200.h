@@ -388,6 +388,17 @@ int tarmac_head_attention_backward(const void *q, const void *k, const void *v,
                                    float scale, void *dq, void *dk, void *dv,
                                    void *work, void *stream);
 
+/* Which kernels a multi-head attention call (backward 0) or its gradients (1)
+ * with these arguments would take: host-only, as tarmac_kernel_plan below.
+ * Pointers are assumed on a 16-byte grid; strides as for those calls. Writes a
+ * NUL-terminated JSON object of at most `len` bytes: {"kernel": "head_fwd_tc",
+ * "items": n} on the tensor memory, n units of work for its persistent blocks,
+ * or {"kernel": "head_fwd", "parts": n}, the key axis in n parts; gradients
+ * {"kernel": "head_bwd_tc" or "head_bwd", "dq_items": n, "dkv_items": m}. */
+int tarmac_head_attention_plan(int backward, const int64_t *strides, int B,
+                               int Nq, int Nk, int H, int Hk, int d, int dtype,
+                               int peers, char *out, int len);
+
 /* Which kernel, and with which tiling, a call with these arguments would
  * take — host-only: no launch, no device access, callable without a GPU.
  * Replaces the tuned-configuration lookup of the reference

@@ -455,19 +455,30 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
-bool head_tensor_map(CUtensorMap* map, const void* ptr, const HeadStrides& s, int B, int N, int h,
-                     int d) {
-  const EncodeTiledFn fn = encode_fn();
-  if (!fn || (uintptr_t)ptr % 16) return false;
-  const cuuint64_t size[4] = {(cuuint64_t)d, (cuuint64_t)h, (cuuint64_t)N, (cuuint64_t)B};
+// strides of the heads, rows and episodes in bytes; false where TMA cannot
+// take them
+static bool map_strides(const HeadStrides& s, int B, int N, int h, cuuint64_t (&bytes)[3]) {
   const int64_t st[3] = {s.h, s.n, s.b};
-  cuuint64_t bytes[3];
+  const int size[3] = {h, N, B};
   for (int i = 0; i < 3; ++i) {
     // the stride of a dimension of one is never used
-    const int64_t e = size[i + 1] == 1 ? 8 : st[i];
+    const int64_t e = size[i] == 1 ? 8 : st[i];
     if (e <= 0 || e % 8 || e * 2 >= ((int64_t)1 << 40)) return false;
     bytes[i] = (cuuint64_t)(e * 2);
   }
+  return true;
+}
+bool head_map_ok(const HeadStrides& s, int B, int N, int h) {
+  cuuint64_t bytes[3];
+  return map_strides(s, B, N, h, bytes);
+}
+
+bool head_tensor_map(CUtensorMap* map, const void* ptr, const HeadStrides& s, int B, int N, int h,
+                     int d) {
+  const EncodeTiledFn fn = encode_fn();
+  cuuint64_t bytes[3];
+  if (!fn || (uintptr_t)ptr % 16 || !map_strides(s, B, N, h, bytes)) return false;
+  const cuuint64_t size[4] = {(cuuint64_t)d, (cuuint64_t)h, (cuuint64_t)N, (cuuint64_t)B};
   const cuuint32_t box[4] = {64, 1, ht::BOX_ROWS, 1}, one[4] = {1, 1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), size, bytes, box,
             one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -494,33 +505,42 @@ int head_sm_count() {
   return n;
 }
 
-// bf16 rows on the 16-byte grid, by the rules below; *done says whether
-// the call was taken.
-cudaError_t launch_head_fwd_tc(const HeadAttnParams& p, cudaStream_t s, bool* done) {
-  *done = false;
+// Items of a bf16 call that these kernels take, 0 for one that they leave:
+// rows on the 16-byte grid, by the rules below.
+int64_t head_fwd_tc_items(const HeadAttnParams& p) {
   // Short sets of rows leave these 128-row tiles half empty, and for narrow
   // rows the products weigh little; the kernels of head_attn.cu were faster
   // there. Measured, those against these (us): 512 x 8 heads, d = 64: N = 64
   // 58 / 103, N = 96 140 / 113, N = 256 379 / 208; 512 x 4 heads, d = 32:
   // N = 128 44 / 51, N = 192 82 / 91, N = 224 132 / 93; d = 16, 256 x 4 heads:
   // N = 192 32 / 45, N = 512 152 / 130.
-  if (!p.vec || p.Nk < 1 || p.Nq <= (p.d > 32 ? 64 : 192)) return cudaSuccess;
-  HtGrid gr;
-  gr.nqt = cdiv(p.Nq, 128);
-  const int64_t pairs = ((int64_t)gr.nqt * p.G + 1) / 2;
+  if (!p.vec || p.Nk < 1 || p.Nq <= (p.d > 32 ? 64 : 192)) return 0;
+  const int64_t pairs = ((int64_t)cdiv(p.Nq, 128) * p.G + 1) / 2;
   const int64_t items = pairs * p.B * p.Hk;
-  if (items > (1 << 30)) return cudaSuccess;
+  if (items > (1 << 30)) return 0;
   // With few items those kernels fill the GPU by splitting the key axis. 128
   // rows of 8 heads, d = 64, against 2048 and 8192 keys: 40 items 28 / 27 and
   // 67 / 92 us, 56 items 36 / 27 and 85 / 93, 128 items 63 / 28 and 161 / 96.
-  if (p.splits > 1 && items < 56) return cudaSuccess;
+  if (p.splits > 1 && items < 56) return 0;
+  const bool maps = head_map_ok(p.sq, p.B, p.Nq, p.H) && head_map_ok(p.sk, p.B, p.Nk, p.Hk) &&
+                    head_map_ok(p.sv, p.B, p.Nk, p.Hk);
+  return maps ? items : 0;
+}
+
+// *done says whether the call was taken.
+cudaError_t launch_head_fwd_tc(const HeadAttnParams& p, cudaStream_t s, bool* done) {
+  *done = false;
+  const int64_t items = head_fwd_tc_items(p);
+  if (!items) return cudaSuccess;
+  HtGrid gr;
+  gr.nqt = cdiv(p.Nq, 128);
   CUtensorMap m[3];
   if (!head_tensor_map(&m[0], p.q, p.sq, p.B, p.Nq, p.H, p.d) ||
       !head_tensor_map(&m[1], p.k, p.sk, p.B, p.Nk, p.Hk, p.d) ||
       !head_tensor_map(&m[2], p.v, p.sv, p.B, p.Nk, p.Hk, p.d))
     return cudaSuccess;
   const int sms = head_sm_count();
-  gr.pairs = (int)pairs;
+  gr.pairs = cdiv(gr.nqt * p.G, 2);
   gr.items = (int)items;
   gr.pair_major = p.peers == PEERS_PAST && p.B * p.Hk <= sms;
   const int grid = items < sms ? (int)items : sms;

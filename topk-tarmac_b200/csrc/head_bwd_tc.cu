@@ -548,10 +548,9 @@ static cudaError_t bwd_tc_go(const CUtensorMap* m, const HeadAttnParams& p, int6
   return cudaGetLastError();
 }
 
-// bf16 rows on the 16-byte grid, by the rules below; the row
-// statistics are in p.delta already. *done says whether the call was taken.
-cudaError_t launch_head_bwd_tc(const HeadAttnParams& p, int64_t nqp, cudaStream_t s, bool* done) {
-  *done = false;
+// Whether these kernels take a bf16 call: rows on the 16-byte grid, by the
+// rules below.
+bool head_bwd_tc_takes(const HeadAttnParams& p) {
   // Short sets leave the 128 x 128 tiles mostly empty; the kernels of
   // head_attn.cu were faster there. Measured, those against these, dq and dk,
   // dv together (us): 512 x 8 heads, d = 64: N = 64 138 / 220, N = 96 305 /
@@ -560,10 +559,19 @@ cudaError_t launch_head_bwd_tc(const HeadAttnParams& p, int64_t nqp, cudaStream_
   // N = 192 238 / 259, N = 224 347 / 261; d = 16, 256 x 4 heads: N = 192 88 /
   // 121, N = 256 142 / 121.
   const int longer = p.Nq > p.Nk ? p.Nq : p.Nk;
-  if (!p.vec || p.Nk < 1 || p.Nq <= 32 || longer <= (p.d > 32 ? 64 : 192)) return cudaSuccess;
+  if (!p.vec || p.Nk < 1 || p.Nq <= 32 || longer <= (p.d > 32 ? 64 : 192)) return false;
   if ((int64_t)p.B * p.H * cdiv(p.Nq, 128) > (1 << 30) ||
       (int64_t)p.B * p.Hk * cdiv(p.Nk, 128) > (1 << 30))
-    return cudaSuccess;
+    return false;
+  return head_map_ok(p.sq, p.B, p.Nq, p.H) && head_map_ok(p.sk, p.B, p.Nk, p.Hk) &&
+         head_map_ok(p.sv, p.B, p.Nk, p.Hk) && head_map_ok(p.sg, p.B, p.Nq, p.H);
+}
+
+// The row statistics are in p.delta already. *done says whether the call was
+// taken.
+cudaError_t launch_head_bwd_tc(const HeadAttnParams& p, int64_t nqp, cudaStream_t s, bool* done) {
+  *done = false;
+  if (!head_bwd_tc_takes(p)) return cudaSuccess;
   CUtensorMap m[4];
   if (!head_tensor_map(&m[0], p.q, p.sq, p.B, p.Nq, p.H, p.d) ||
       !head_tensor_map(&m[1], p.k, p.sk, p.B, p.Nk, p.Hk, p.d) ||

@@ -287,7 +287,8 @@ __device__ __forceinline__ uint32_t key_word(int j0, int jlim, int self, uint32_
 }  // namespace ht
 
 // Tensor map of a [B, N, h, d] bf16 tensor with 64 x 64 boxes; false where
-// TMA cannot describe it (head_attn_tc.cu).
+// TMA cannot describe it (head_attn_tc.cu). head_map_ok: do the strides allow it?
+bool head_map_ok(const HeadStrides& s, int B, int N, int h);
 bool head_tensor_map(CUtensorMap* map, const void* ptr, const HeadStrides& s, int B, int N, int h,
                      int d);
 

@@ -1,6 +1,8 @@
 // heads_abi.cu — the extern "C" entry points of the multi-head operators
 // declared in include/tarmac_b200.h: argument checks, parameters, launch.
 #include <math.h>
+#include <stdio.h>
+#include <string.h>
 
 #include "heads.cuh"
 
@@ -8,6 +10,8 @@ namespace tarmac {
 
 cudaError_t launch_head_fwd(const HeadAttnParams& p, bool bf16, cudaStream_t s);
 cudaError_t launch_head_bwd(const HeadAttnParams& p, bool bf16, cudaStream_t s);
+int64_t head_fwd_tc_items(const HeadAttnParams& p);
+bool head_bwd_tc_takes(const HeadAttnParams& p);
 int head_splits(int B, int Nq, int Nk, int H, int Hk);
 cudaError_t launch_pack_bits(const void* v, int64_t sb, int64_t sn, int B, int Nq, int Nk,
                              uint32_t* out, cudaStream_t s);
@@ -270,6 +274,48 @@ int tarmac_head_attention_backward(const void* q, const void* k, const void* v, 
   p.vec = d * es % 16 == 0 && vec_ok(q, p.sq, es) && vec_ok(k, p.sk, es) &&
           vec_ok(v, p.sv, es) && vec_ok(out, p.so, es) && vec_ok(dout, p.sg, es);
   return status(launch_head_bwd(p, dtype == TARMAC_BF16, (cudaStream_t)stream));
+}
+
+int tarmac_head_attention_plan(int backward, const int64_t* strides, int B, int Nq, int Nk, int H,
+                               int Hk, int d, int dtype, int peers, char* out, int len) {
+  if (!out || len < 1) return TARMAC_ERR_NULL;
+  out[0] = '\0';
+  // only shapes, strides and alignment count: stand-in pointers on the grid
+  const void* a = reinterpret_cast<const void*>((uintptr_t)1 << 20);
+  HeadAttnParams p;
+  const int st = fill_attn(p, a, a, a, nullptr, nullptr, nullptr, 0, B, Nq, Nk, H, Hk, d, dtype,
+                           peers, 1.f);
+  if (st != TARMAC_OK) return st;
+  const bool bf16 = dtype == TARMAC_BF16;
+  const int es = bf16 ? 2 : 4;
+  p.sq = stride_of(strides, 0, Nq, H, d);
+  p.sk = stride_of(strides, 1, Nk, Hk, d);
+  p.sv = stride_of(strides, 2, Nk, Hk, d);
+  p.vec = d * es % 16 == 0 && vec_ok(a, p.sq, es) && vec_ok(a, p.sk, es) && vec_ok(a, p.sv, es);
+  char buf[128];
+  if (backward) {
+    p.so = stride_of(strides, 3, Nq, H, d);
+    p.sg = stride_of(strides, 4, Nq, H, d);
+    p.vec = p.vec && vec_ok(a, p.so, es) && vec_ok(a, p.sg, es);
+    const bool tc = bf16 && head_bwd_tc_takes(p);
+    const int tile = tc ? 128 : 64;
+    const int64_t rows = tc ? (int64_t)p.H * cdiv(Nq, 128) : (int64_t)p.Hk * cdiv(Nq * p.G, 64);
+    snprintf(buf, sizeof buf, "{\"kernel\": \"%s\", \"dq_items\": %lld, \"dkv_items\": %lld}",
+             tc ? "head_bwd_tc" : "head_bwd", (long long)(B * rows),
+             (long long)((int64_t)B * Hk * cdiv(Nk, tile)));
+  } else {
+    if (Nk > 0) p.splits = head_splits(B, Nq, Nk, H, Hk);
+    const int64_t items = bf16 ? head_fwd_tc_items(p) : 0;
+    if (items)
+      snprintf(buf, sizeof buf, "{\"kernel\": \"head_fwd_tc\", \"items\": %lld}",
+               (long long)items);
+    else
+      snprintf(buf, sizeof buf, "{\"kernel\": \"head_fwd\", \"parts\": %d}", p.splits);
+  }
+  const int n = (int)strlen(buf);
+  if (n + 1 > len) return TARMAC_ERR_SHAPE;
+  memcpy(out, buf, (size_t)n + 1);
+  return TARMAC_OK;
 }
 
 }  // extern "C"

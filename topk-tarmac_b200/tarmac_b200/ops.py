@@ -758,6 +758,21 @@ def head_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     return dq, dk, dv
 
 
+def head_attention_plan(B: int, Nq: int, Nk: int, H: int, Hk: int, d: int,
+                        dtype: torch.dtype = torch.float32, peers: str = "all",
+                        backward: bool = False) -> dict:
+    """The kernels a contiguous :func:`head_attention` call (or its gradients)
+    with these shapes takes, e.g. {"kernel": "head_fwd_tc", "items": 240}.
+    Host-only (no GPU needed); raises :class:`TarmacError` for arguments the
+    call itself would reject."""
+    import ctypes
+    import json
+    buf = ctypes.create_string_buffer(128)
+    _lib.call("tarmac_head_attention_plan", int(backward), None, B, Nq, Nk, H,
+              Hk, d, _DTYPES[dtype], _PEERS[peers], buf, len(buf))
+    return json.loads(buf.value.decode())
+
+
 _PLAN_OPS = {"dense": 0, "topk": 1, "streaming": 2}
 _PLAN_MODES = {"argmax": _lib.SELECT_ARGMAX, "threshold": _lib.SELECT_THRESHOLD,
                "sort": _lib.SELECT_SORT}
