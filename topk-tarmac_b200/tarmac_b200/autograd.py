@@ -12,6 +12,8 @@ dtype of q.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -102,7 +104,8 @@ class MortonPrescoreAttention(torch.autograd.Function):
 
 class QkNormRotate(torch.autograd.Function):
     """Head norms and position rotation (:func:`ops.qk_norm_rotate`). The
-    tables carry no gradient."""
+    tables carry no gradient. First derivatives in reverse mode only: a second
+    derivative or a forward-mode tangent is refused."""
 
     @staticmethod
     def forward(ctx, q, k, wq, wk, cos, sin, eps=1e-6, interleaved=False):
@@ -111,6 +114,7 @@ class QkNormRotate(torch.autograd.Function):
         return ops.qk_norm_rotate(q, k, wq, wk, cos, sin, eps, interleaved)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, wq, wk, cos, sin = ctx.saved_tensors
         dq, dk, dwq, dwk = ops.qk_norm_rotate_backward(
@@ -124,7 +128,8 @@ class QkNormRotate(torch.autograd.Function):
 
 class HeadAttention(torch.autograd.Function):
     """Masked attention with heads (:func:`ops.head_attention`); ``visible``
-    is None or the words of :func:`ops.pack_visibility`."""
+    is None or the words of :func:`ops.pack_visibility`. First derivatives in
+    reverse mode only, as :class:`QkNormRotate`."""
 
     @staticmethod
     def forward(ctx, q, k, v, peers="all", key_len=None, q_start=None,
@@ -136,6 +141,7 @@ class HeadAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, key_len, q_start, visible = ctx.saved_tensors
         peers, scale = ctx.how
@@ -155,6 +161,13 @@ def dense_attention(q, k, v, scale=None):
     if _needs_grad(q, k, v):
         return DenseAttention.apply(q, k, v, scale)
     return ops.dense_attention(q, k, v, scale)
+
+
+def _has_tangent(*ts) -> bool:
+    """Does one of these carry a forward-mode tangent? The function's apply
+    then refuses it; the plain call would drop it."""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
+        forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def topk_attention(q, k, v, topk, mode="argmax", scale=None):
@@ -177,14 +190,15 @@ def morton_prescore_attention(q, k, v, pos, topk, bits=10, scale=None):
 
 
 def qk_norm_rotate(q, k, wq, wk, cos, sin, eps=1e-6, interleaved=False):
-    if _needs_grad(*(t for t in (q, k, wq, wk) if t is not None)):
+    ts = [t for t in (q, k, wq, wk) if t is not None]
+    if _needs_grad(*ts) or _has_tangent(*ts):
         return QkNormRotate.apply(q, k, wq, wk, cos, sin, eps, interleaved)
     return ops.qk_norm_rotate(q, k, wq, wk, cos, sin, eps, interleaved)
 
 
 def head_attention(q, k, v, peers="all", key_len=None, q_start=None,
                    visible=None, scale=None):
-    if _needs_grad(q, k, v):
+    if _needs_grad(q, k, v) or _has_tangent(q, k, v):
         if visible is not None and visible.dtype == torch.bool:
             visible = ops.pack_visibility(visible)  # once for both directions
         return HeadAttention.apply(q, k, v, peers, key_len, q_start, visible,
