@@ -88,5 +88,5 @@ class HeadComm(nn.Module):
         past_v[row, past_len] = v[:, 0].to(past_v.dtype)
         past_len += 1
         out = ops.head_attention(q.to(past_k.dtype), past_k, past_v, "all",
-                                 key_len=past_len)
+                                 key_len=past_len.to(torch.int32))
         return self.proj(out.flatten(2).to(x.dtype))

@@ -621,6 +621,8 @@ def _check_attention(q, k, v, peers, key_len, q_start, visible):
                 raise TypeError(f"{name} must be int32 or int64; got {t.dtype}")
             if t.device != q.device:
                 raise ValueError(f"{name} must be on the device of the queries")
+            if t.dtype is torch.int64:  # beyond 32 bits they act like the bounds
+                t = t.clamp(-2 ** 31, 2 ** 31 - 1)
             t = t.to(torch.int32).contiguous()
         ints.append(t)
     if visible is not None:
