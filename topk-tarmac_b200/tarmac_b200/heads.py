@@ -79,14 +79,33 @@ class HeadComm(nn.Module):
              past_len: torch.Tensor) -> torch.Tensor:
         """One new row per episode, x [B, 1, in_dim], over each one's past.
         ``past_k``, ``past_v`` [B, room, n_kv_heads, head_dim] hold the first
-        ``past_len`` (int64 [B]) rows; the new keys and values are written
-        behind them and ``past_len`` grows by one, in place. The caller keeps
-        ``past_len`` below the room."""
+        ``past_len`` (int32 or int64 [B]) rows; the new keys and values are
+        written behind them and ``past_len`` grows by one, in place. The caller
+        keeps ``past_len`` below the room: an episode that has none left (or a
+        negative length) gets NaN, and its last (or first) row is lost."""
+        B, shape = x.shape[0], tuple(past_k.shape)
+        if x.dim() != 3 or x.shape[1] != 1:
+            raise ValueError(f"x must be [B, 1, in_dim]; got {tuple(x.shape)}")
+        if len(shape) != 4 or shape[0] != B or shape[1] < 1 \
+                or shape[2:] != (self.heads[1], self.head_dim) or past_v.shape != shape:
+            raise ValueError(
+                f"past_k and past_v must share one [{B}, room, {self.heads[1]}, "
+                f"{self.head_dim}] shape; got {shape}, {tuple(past_v.shape)}")
+        if tuple(past_len.shape) != (B,):
+            raise ValueError(f"past_len must be [{B}]; got {tuple(past_len.shape)}")
+        if past_len.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"past_len must be int32 or int64; got {past_len.dtype}")
         q, k, v = self._qkv(x, cos, sin)
-        row = torch.arange(x.shape[0], device=x.device)
-        past_k[row, past_len] = k[:, 0].to(past_k.dtype)
-        past_v[row, past_len] = v[:, 0].to(past_v.dtype)
+        if q.dtype is not past_k.dtype:
+            q, k, v = (t.to(past_k.dtype) for t in (q, k, v))
+        n = past_len.view(B, 1, 1, 1)
+        at = n.clamp(0, shape[1] - 1)  # never written out of range
+        lost = at != n
+        row = at.long().expand(k.shape)
+        past_k.scatter_(1, row, k)
+        past_v.scatter_(1, row, v)
         past_len += 1
-        out = ops.head_attention(q.to(past_k.dtype), past_k, past_v, "all",
+        out = ops.head_attention(q, past_k, past_v, "all",
                                  key_len=past_len.to(torch.int32))
+        out.masked_fill_(lost, float("nan"))
         return self.proj(out.flatten(2).to(x.dtype))
