@@ -25,14 +25,16 @@
 // polynomial on the FMA pipe gave 127, 131 and 142 us where this takes 127;
 // P V in two halves, the first under the exponentials of the second, 132.
 // Measured on B200: 2 x 8192 causal rows of 16 heads on 4, d = 128:
-// 500 us, 1.10 PFLOP/s; 32 x 1024 rows of 8 heads, d = 64: 127 us, 541 TFLOP/s
-// (its 268 M exponentials alone take 63 us at 1.8 GHz); 256 x 512 rows of 4
-// heads on 2, d = 64, with visibility words 182 us, without 143 us.
+// 491 us, 1.12 PFLOP/s (557 us in a long run under the power limit); 32 x 1024
+// rows of 8 heads, d = 64: 129 us, 533 TFLOP/s (its 268 M exponentials alone
+// take 63 us at 1.8 GHz); 256 x 512 rows of 4 heads on 2, d = 64, with
+// visibility words 180 us, without 143 us.
 // Blocks are persistent, one per SM, and walk their items in
 // alternating direction, so that under the past rule each gets long and short
 // tiles.
-// Every wait is bounded; one that runs out raises a flag that ends all roles,
-// and the rows concerned are written as NaN.
+// Every wait is bounded; one that runs out raises a flag that ends all roles
+// once their copies and products have landed, and every row is written, NaN or
+// right.
 #include "head_tc.cuh"
 
 namespace tarmac {

@@ -25,11 +25,12 @@
 // rather than added up across blocks with atomics, so two calls give the same
 // bits) and two exponentials per pair, 1024 clocks of the special-function
 // unit per 128 x 128 tile against 256 d / 64 for a product. Measured on B200:
-// 8192 causal rows of 16 heads on 4, d = 128: dk, dv 437 us, dq 328 us (365
-// and 264 us for the products and hand-overs alone), 900 TFLOP/s of the five
-// products' flops; 32 x 1024 rows of 8 heads, d = 64: 210 and 174 us.
-// Every wait is bounded; one that runs out ends all roles and the rows
-// concerned are written as NaN.
+// 8192 causal rows of 16 heads on 4, d = 128: dk, dv 424 us, dq 308 us (365
+// and 264 us for the products and hand-overs alone, in an earlier form), 939
+// TFLOP/s of the five products' flops; 32 x 1024 rows of 8 heads, d = 64: 187
+// and 155 us.
+// Every wait is bounded; one that runs out ends all roles once their copies
+// and products have landed, and every row is written, NaN or right.
 #include <type_traits>
 
 #include "head_tc.cuh"

@@ -12,8 +12,9 @@
 // Both directions are bound by memory: each element is read once and written
 // once (backward: two reads). Measured on B200, bf16: 4 x 8192 rows of 20
 // heads, d = 128: 61 us, 5.6 TB/s; 1024 x 512 rows of 6 heads, d = 64, a table
-// per episode: 163 us, 5.4 TB/s, backward 295 us, 4.3 TB/s (it has twice the
-// arithmetic of the forward pass, and instruction issue shares the bound). A row belongs to LPR lanes, and each lane holds
+// per episode: 162 us, 5.4 TB/s, backward 291 us, 4.4 TB/s: issue is active
+// half the time there and loads are waited for, as the staging leaves three
+// blocks per SM. A row belongs to LPR lanes, and each lane holds
 // E column pairs as two vectors of E elements, so the rotation never leaves
 // the lane and the only exchange is the row's sum. Columns without a rotation
 // take cos = 1, sin = 0, which makes every lane run the same code. A lane
