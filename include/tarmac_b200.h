@@ -399,6 +399,81 @@ int tarmac_head_attention_plan(int backward, const int64_t *strides, int B,
                                int Nq, int Nk, int H, int Hk, int d, int dtype,
                                int peers, char *out, int len);
 
+/* Attention with a decay for each head: a memory of fixed size in place of a
+ * history. q, out: [B, N, H, d]; k, v: [B, N, Hk, d], H a multiple of Hk:
+ * query head h reads key head h / (H / Hk). strides: q, k, v. With
+ * l = exp(log_decay[h]) (fp32 [H], at most 0; -inf keeps nothing), for the
+ * rows t of an episode in order,
+ *   S_t = l S_(t-1) + k_t v_t^T,  out_t = scale S_t^T q_t.
+ * state: the state before the first row, fp32 [B, H, d, d] contiguous, by the
+ * columns of k and of v; NULL for zero. state_out: the state after the last
+ * row, the same layout, or NULL; it may be `state` itself. lens: int32 [B],
+ * clamped to [0, N], or NULL: rows from lens[b] on are padding, whatever they
+ * hold; they get out = 0 and leave the state alone. One new row over a kept
+ * state is N = 1. Sums and states are fp32. fp32: products as good as fp32
+ * FMAs; bf16: bf16 products with fp32 sums, the weights of the rows and the
+ * copy of the state that multiplies q rounded to bf16, what enters a returned
+ * state good to fp32. work: 16-byte aligned scratch of
+ * tarmac_decay_attention_workspace bytes (0: NULL is fine). */
+int64_t tarmac_decay_attention_workspace(int B, int N, int H, int d);
+int tarmac_decay_attention(const void *q, const void *k, const void *v,
+                           void *out, const int64_t *strides,
+                           const float *log_decay, const float *state,
+                           float *state_out, const int32_t *lens, int B, int N,
+                           int H, int Hk, int d, int dtype, float scale,
+                           void *work, void *stream);
+
+/* Its gradients. dout: the gradient of out, dstate_out (fp32, or NULL for
+ * zero) that of state_out; strides: q, k, v, dout. With
+ *   R_t = scale q_t dout_t^T + l R_(t+1),  l R_N = dstate_out,
+ * dq_t = scale S_t dout_t, dk_t = R_t v_t, dv_t = R_t^T k_t and
+ * dstate = l R_0; shared key heads are summed over their query heads. dq, dk,
+ * dv: contiguous, the inputs' type, zero on padding; dstate: fp32 [B, H, d, d]
+ * or NULL, not dstate_out. The decays get no gradient. No atomics: two calls
+ * give the same bits. work: 16-byte aligned scratch of
+ * tarmac_decay_attention_backward_workspace bytes (0: NULL is fine). */
+int64_t tarmac_decay_attention_backward_workspace(int B, int N, int H, int Hk,
+                                                  int d);
+int tarmac_decay_attention_backward(const void *q, const void *k,
+                                    const void *v, const void *dout,
+                                    const int64_t *strides,
+                                    const float *log_decay, const float *state,
+                                    const float *dstate_out,
+                                    const int32_t *lens, int B, int N, int H,
+                                    int Hk, int d, int dtype, float scale,
+                                    void *dq, void *dk, void *dv,
+                                    float *dstate, void *work, void *stream);
+
+/* The norms around a block with its gate and residual scale, in one pass. For
+ * each row of D columns (D <= 8192) of the stream x, the block's output y and
+ * the gate (or NULL: ones in place of its sigmoid),
+ *   h = x + scale sigmoid(gate) (y / sqrt(mean y^2 + eps) w_post),
+ *   z = h / sqrt(mean h^2 + eps) w_pre.
+ * Tensors are [B, N, D] of `dtype` with unit innermost stride; strides: { batch,
+ * row } int64 element strides of x, y, gate, or NULL for contiguous tensors; h
+ * and z are contiguous. w_post, w_pre, scale: fp32 [D] or NULL (ones). All
+ * arithmetic is fp32, rounded once; z follows from the unrounded h. */
+int tarmac_residual_norm(const void *x, const void *y, const void *gate,
+                         const int64_t *strides, const float *w_post,
+                         const float *w_pre, const float *scale, int B, int N,
+                         int D, int dtype, float eps, void *h, void *z,
+                         void *stream);
+
+/* Its gradients. dh, dz: gradients of h and z (NULL: zero); strides: x, y,
+ * gate, dh, dz. dx, dy, dgate (with a gate): contiguous, the inputs' type;
+ * dw_post, dw_pre, dscale: fp32 [D] or NULL, summed over the rows in a fixed
+ * order (two calls give the same bits). work: 16-byte aligned scratch of
+ * tarmac_residual_norm_workspace bytes. */
+int64_t tarmac_residual_norm_workspace(int B, int N, int D);
+int tarmac_residual_norm_backward(const void *x, const void *y,
+                                  const void *gate, const void *dh,
+                                  const void *dz, const int64_t *strides,
+                                  const float *w_post, const float *w_pre,
+                                  const float *scale, int B, int N, int D,
+                                  int dtype, float eps, void *dx, void *dy,
+                                  void *dgate, float *dw_post, float *dw_pre,
+                                  float *dscale, void *work, void *stream);
+
 /* Which kernel, and with which tiling, a call with these arguments would
  * take — host-only: no launch, no device access, callable without a GPU.
  * Replaces the tuned-configuration lookup of the reference

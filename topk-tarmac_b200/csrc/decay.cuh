@@ -1,0 +1,68 @@
+// decay.cuh — parameters of attention with a decay for each head
+// (decay_attn.cu, decay_step.cu) and how a call is divided.
+//
+// Every direction is one form over rows, with l the decay of a head:
+//   out_i = sum_{j <= i} l^(i-j) (a_i . b_j) c_j + l^(i+1) a_i . S,
+// S [columns of b, columns of c] the state before the first row, and
+//   S' = l^n S + sum_j l^(n-1-j) b_j c_j^T
+// the state after n rows. With q, k, v it is the forward pass; with dout, v, k
+// the gradient of q (the state transposed); over the rows backwards, with
+// k, q, dout and v, dout, q the gradients of v and k.
+#pragma once
+
+#include "heads.cuh"
+
+namespace tarmac {
+
+struct DecayParams {
+  const void *a, *b, *c;
+  void* out;                 // [B, N, H, d] contiguous, or NULL: states only
+  HeadStrides sa, sb, sc;
+  int ga, gb, gc;            // heads that share one head of a, b, c
+  int out_f32;               // out is fp32 (else the rows' type)
+  const float* log_decay;    // [H]
+  const int32_t* lens;       // [B] or NULL
+  const float* start;        // [B, H, d, d], the state before, or NULL (zero)
+  float* last;               // [B, H, d, d], the state after, or NULL
+  float* part;               // [segs, B, H, d, d] or NULL where segs is 1
+  int B, N, H, d;
+  int segs, seg_chunks;      // parts of the row axis and their chunks
+  int reverse;               // rows run from the last to the first
+  int transposed;            // state tensors are [columns of c, columns of b]
+  float in_scale;            // factor of every b_j c_j term
+  float out_scale;           // factor of out
+  int planes;                // bf16 parts of the weighted rows that enter S
+  int vec;                   // 16-byte rows in a, b, c
+  int vec_out;               // and in out
+};
+
+// Powers of a decay: exp(rate e). A decay of zero (rate -inf) keeps l^0 = 1.
+__device__ __forceinline__ float decay_rate(const float* log_decay, int h) {
+  const float r = __ldg(log_decay + h);
+  return r < -1e4f ? -1e4f : r;  // NaN stays
+}
+__device__ __forceinline__ int decay_len(const DecayParams& p, int b) {
+  return p.lens ? max(0, min(__ldg(p.lens + b), p.N)) : p.N;
+}
+
+constexpr int DECAY_CHUNK = 64;      // rows of a chunk, warp-level kernel
+
+struct DecayPlan {
+  int segs, seg_chunks;
+};
+DecayPlan decay_plan(int B, int N, int H);
+// parts that `part` must hold, 0 for none
+inline int64_t decay_parts(const DecayPlan& g) { return g.segs > 1 ? g.segs : 0; }
+
+// States of the segments into p.part: first what each adds, then, in place,
+// the state before each. Launches nothing where segs is 1.
+cudaError_t launch_decay_states(const DecayParams& p, bool bf16, cudaStream_t s);
+cudaError_t launch_decay_rows(const DecayParams& p, bool bf16, cudaStream_t s);
+// few rows, one after the other (forward only)
+bool decay_step_takes(int N);
+cudaError_t launch_decay_step(const DecayParams& p, bool bf16, cudaStream_t s);
+// out[., hk, .] = sum over the G heads of a key head, fp32 to the rows' type
+cudaError_t launch_decay_share(const float* x, void* out, int64_t rows, int Hk, int G, int d,
+                               bool bf16, cudaStream_t s);
+
+}  // namespace tarmac

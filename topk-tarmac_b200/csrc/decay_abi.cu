@@ -1,0 +1,308 @@
+// decay_abi.cu — the extern "C" entry points of attention with a decay for
+// each head and of the norms around a block, declared in
+// include/tarmac_b200.h: argument checks, parameters, launch.
+#include <math.h>
+#include <stdio.h>
+#include <string.h>
+
+#include "block_norm.cuh"
+#include "decay.cuh"
+
+namespace tarmac {
+
+namespace {
+
+constexpr int MAX_D = 128;
+
+bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+int status(cudaError_t e) { return e == cudaSuccess ? TARMAC_OK : TARMAC_ERR_LAUNCH; }
+int64_t round16(int64_t bytes) { return (bytes + 15) & ~(int64_t)15; }
+
+HeadStrides stride_of(const int64_t* strides, int i, int64_t N, int64_t h, int64_t d) {
+  if (strides) return HeadStrides{strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]};
+  return HeadStrides{N * h * d, h * d, d};
+}
+bool vec_ok(const void* ptr, const HeadStrides& s, int es) {
+  const int e = 16 / es;
+  return aligned(ptr, 16) && s.b % e == 0 && s.n % e == 0 && s.h % e == 0;
+}
+
+int check_sizes(int B, int N, int H, int Hk, int d, int dtype) {
+  if (dtype != TARMAC_F32 && dtype != TARMAC_BF16) return TARMAC_ERR_DTYPE;
+  if (B < 0 || N < 0 || d < 1 || d > MAX_D) return TARMAC_ERR_SHAPE;
+  if (H < 1 || Hk < 1 || H % Hk) return TARMAC_ERR_HEADS;
+  // rows in 29 bits, blocks of a launch in 31
+  if (N > (1 << 29) || (int64_t)B * H > (1 << 24)) return TARMAC_ERR_N_TOO_LARGE;
+  return TARMAC_OK;
+}
+
+// Checks shared by both directions; fills what they share.
+int fill_decay(DecayParams& p, const void* q, const void* k, const void* v,
+               const float* log_decay, const float* state, const int32_t* lens, int B, int N,
+               int H, int Hk, int d, int dtype, float scale) {
+  const int st = check_sizes(B, N, H, Hk, d, dtype);
+  if (st != TARMAC_OK) return st;
+  if (!(scale > 0.f) || isinf(scale)) return TARMAC_ERR_SHAPE;
+  if (!aligned(lens, 4) || !aligned(log_decay, 4) || !aligned(state, 4)) return TARMAC_ERR_ALIGN;
+  if (B > 0 && (!log_decay || (N > 0 && (!q || !k || !v)))) return TARMAC_ERR_NULL;
+  const int es = dtype == TARMAC_BF16 ? 2 : 4;
+  if (!aligned(q, es) || !aligned(k, es) || !aligned(v, es)) return TARMAC_ERR_ALIGN;
+  p = DecayParams{};
+  p.log_decay = log_decay;
+  p.lens = lens;
+  p.B = B;
+  p.N = N;
+  p.H = H;
+  p.d = d;
+  const DecayPlan g = decay_plan(B, N, H);
+  p.segs = g.segs;
+  p.seg_chunks = g.seg_chunks;
+  return TARMAC_OK;
+}
+
+// one operand: pointer, strides and how many heads share one of its heads
+struct Operand {
+  const void* ptr;
+  HeadStrides s;
+  int share;
+  bool vec;
+};
+void set_operands(DecayParams& p, const Operand& a, const Operand& b, const Operand& c) {
+  p.a = a.ptr;
+  p.b = b.ptr;
+  p.c = c.ptr;
+  p.sa = a.s;
+  p.sb = b.s;
+  p.sc = c.s;
+  p.ga = a.share;
+  p.gb = b.share;
+  p.gc = c.share;
+  p.vec = a.vec && b.vec && c.vec;
+}
+
+// no rows: the state stays as it was
+cudaError_t carry_state(const float* from, float* to, int64_t n, cudaStream_t s) {
+  if (!to || n == 0 || from == to) return cudaSuccess;
+  if (!from) return cudaMemsetAsync(to, 0, (size_t)n * 4, s);
+  return cudaMemcpyAsync(to, from, (size_t)n * 4, cudaMemcpyDeviceToDevice, s);
+}
+
+// episode and row stride of tensor i (two int64 each), or those of a
+// contiguous [B, N, D] tensor
+RowStrides rows_of(const int64_t* strides, int i, int64_t N, int64_t D) {
+  if (strides) return RowStrides{strides[2 * i], strides[2 * i + 1]};
+  return RowStrides{N * D, D};
+}
+
+// Checks shared by both directions; fills what they share.
+int fill_norm(NormParams& p, const void* x, const void* y, const void* gate,
+              const int64_t* strides, const float* w_post, const float* w_pre,
+              const float* scale, int B, int N, int D, int dtype, float eps) {
+  if (dtype != TARMAC_F32 && dtype != TARMAC_BF16) return TARMAC_ERR_DTYPE;
+  if (B < 0 || N < 0 || D < 1 || D > NORM_MAX_D) return TARMAC_ERR_SHAPE;
+  if (!(eps >= 0.f) || isinf(eps)) return TARMAC_ERR_SHAPE;
+  if ((int64_t)B * N > 0x7fffffff) return TARMAC_ERR_N_TOO_LARGE;  // rows in 31 bits
+  const int es = dtype == TARMAC_BF16 ? 2 : 4;
+  if (!aligned(x, es) || !aligned(y, es) || !aligned(gate, es)) return TARMAC_ERR_ALIGN;
+  if (!aligned(w_post, 4) || !aligned(w_pre, 4) || !aligned(scale, 4)) return TARMAC_ERR_ALIGN;
+  if ((int64_t)B * N > 0 && (!x || !y)) return TARMAC_ERR_NULL;
+  p = NormParams{};
+  p.x = x;
+  p.y = y;
+  p.gate = gate;
+  p.sx = rows_of(strides, 0, N, D);
+  p.sy = rows_of(strides, 1, N, D);
+  p.sg = rows_of(strides, 2, N, D);
+  p.w_post = w_post;
+  p.w_pre = w_pre;
+  p.scale = scale;
+  p.B = B;
+  p.N = N;
+  p.D = D;
+  p.eps = eps;
+  return TARMAC_OK;
+}
+
+}  // namespace
+}  // namespace tarmac
+
+using namespace tarmac;
+
+extern "C" {
+
+int64_t tarmac_decay_attention_workspace(int B, int N, int H, int d) {
+  if (check_sizes(B, N, H, 1, d, TARMAC_F32) != TARMAC_OK || B < 1 || N < 1) return 0;
+  if (decay_step_takes(N)) return 0;
+  return decay_parts(decay_plan(B, N, H)) * B * H * d * d * 4;
+}
+
+int tarmac_decay_attention(const void* q, const void* k, const void* v, void* out,
+                           const int64_t* strides, const float* log_decay, const float* state,
+                           float* state_out, const int32_t* lens, int B, int N, int H, int Hk,
+                           int d, int dtype, float scale, void* work, void* stream) {
+  DecayParams p;
+  const int st = fill_decay(p, q, k, v, log_decay, state, lens, B, N, H, Hk, d, dtype, scale);
+  if (st != TARMAC_OK || B == 0) return st;
+  if (!aligned(state_out, 4)) return TARMAC_ERR_ALIGN;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (N == 0) return status(carry_state(state, state_out, (int64_t)B * H * d * d, s));
+  if (!out) return TARMAC_ERR_NULL;
+  const bool bf16 = dtype == TARMAC_BF16;
+  const int es = bf16 ? 2 : 4, G = H / Hk;
+  if (!aligned(out, 16) || !aligned(work, 16)) return TARMAC_ERR_ALIGN;
+  const HeadStrides sq = stride_of(strides, 0, N, H, d), sk = stride_of(strides, 1, N, Hk, d),
+                    sv = stride_of(strides, 2, N, Hk, d);
+  const bool wide = d * es % 16 == 0;
+  const Operand oq = {q, sq, 1, wide && vec_ok(q, sq, es)};
+  const Operand ok = {k, sk, G, wide && vec_ok(k, sk, es)};
+  const Operand ov = {v, sv, G, wide && vec_ok(v, sv, es)};
+  p.out = out;
+  p.start = state;
+  p.last = state_out;
+  p.planes = state_out ? 3 : 2;
+  p.in_scale = 1.f;
+  p.out_scale = scale;
+  set_operands(p, oq, ok, ov);
+  if (decay_step_takes(N)) return status(launch_decay_step(p, bf16, s));
+  if (p.segs > 1 && !work) return TARMAC_ERR_NULL;
+  p.part = static_cast<float*>(work);
+  cudaError_t e = launch_decay_states(p, bf16, s);
+  if (e == cudaSuccess) e = launch_decay_rows(p, bf16, s);
+  return status(e);
+}
+
+int64_t tarmac_decay_attention_backward_workspace(int B, int N, int H, int Hk, int d) {
+  if (check_sizes(B, N, H, Hk, d, TARMAC_F32) != TARMAC_OK || B < 1 || N < 1) return 0;
+  const int64_t parts = decay_parts(decay_plan(B, N, H)) * B * H * d * d * 4;
+  // gradients of shared heads by query head, before their sum
+  const int64_t shared = H == Hk ? 0 : (int64_t)B * N * H * d * 4;
+  return round16(parts) + shared;
+}
+
+int tarmac_decay_attention_backward(const void* q, const void* k, const void* v, const void* dout,
+                                    const int64_t* strides, const float* log_decay,
+                                    const float* state, const float* dstate_out,
+                                    const int32_t* lens, int B, int N, int H, int Hk, int d,
+                                    int dtype, float scale, void* dq, void* dk, void* dv,
+                                    float* dstate, void* work, void* stream) {
+  DecayParams p;
+  const int st = fill_decay(p, q, k, v, log_decay, state, lens, B, N, H, Hk, d, dtype, scale);
+  if (st != TARMAC_OK || B == 0) return st;
+  if (!aligned(dstate, 4) || !aligned(dstate_out, 4)) return TARMAC_ERR_ALIGN;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (N == 0) return status(carry_state(dstate_out, dstate, (int64_t)B * H * d * d, s));
+  if (!dout || !dq || !dk || !dv) return TARMAC_ERR_NULL;
+  const bool bf16 = dtype == TARMAC_BF16;
+  const int es = bf16 ? 2 : 4, G = H / Hk;
+  if (!aligned(dout, es) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16) ||
+      !aligned(work, 16))
+    return TARMAC_ERR_ALIGN;
+  if (!work && tarmac_decay_attention_backward_workspace(B, N, H, Hk, d) > 0)
+    return TARMAC_ERR_NULL;
+  const HeadStrides sq = stride_of(strides, 0, N, H, d), sk = stride_of(strides, 1, N, Hk, d),
+                    sv = stride_of(strides, 2, N, Hk, d), sg = stride_of(strides, 3, N, H, d);
+  const bool wide = d * es % 16 == 0;
+  const Operand oq = {q, sq, 1, wide && vec_ok(q, sq, es)};
+  const Operand ok = {k, sk, G, wide && vec_ok(k, sk, es)};
+  const Operand ov = {v, sv, G, wide && vec_ok(v, sv, es)};
+  const Operand og = {dout, sg, 1, wide && vec_ok(dout, sg, es)};
+  const int64_t parts = decay_parts(decay_plan(B, N, H)) * B * H * d * d * 4;
+  p.part = static_cast<float*>(work);
+  float* shared = reinterpret_cast<float*>(static_cast<char*>(work) + round16(parts));
+  cudaError_t e = cudaSuccess;
+  auto run = [&](cudaError_t (*launch)(const DecayParams&, bool, cudaStream_t)) {
+    if (e == cudaSuccess) e = launch(p, bf16, s);
+  };
+  // dq_i = scale S_i dout_i, S over the rows as in the forward pass
+  p.start = state;
+  p.planes = 2;
+  p.in_scale = 1.f;
+  p.out_scale = scale;
+  set_operands(p, oq, ok, ov);
+  run(launch_decay_states);
+  set_operands(p, og, ov, ok);
+  p.transposed = 1;
+  p.out = dq;
+  run(launch_decay_rows);
+  // R_i = sum over the rows from i on of scale q dout^T:
+  // dv_i = R_i^T k_i, dk_i = R_i v_i
+  p.start = dstate_out;
+  p.planes = dstate ? 3 : 2;
+  p.reverse = 1;
+  p.transposed = 0;
+  p.in_scale = scale;
+  p.out_scale = 1.f;
+  set_operands(p, ok, oq, og);
+  run(launch_decay_states);
+  p.out_f32 = G > 1;
+  const int64_t rows = (int64_t)B * N;
+  for (int i = 0; i < 2 && e == cudaSuccess; ++i) {
+    void* to = i == 0 ? dv : dk;
+    p.out = G > 1 ? shared : to;
+    p.last = i == 0 ? dstate : nullptr;
+    if (i == 1) {
+      set_operands(p, ov, og, oq);
+      p.transposed = 1;
+    }
+    run(launch_decay_rows);
+    if (e == cudaSuccess && G > 1) e = launch_decay_share(shared, to, rows, Hk, G, d, bf16, s);
+  }
+  return status(e);
+}
+
+int tarmac_residual_norm(const void* x, const void* y, const void* gate, const int64_t* strides,
+                         const float* w_post, const float* w_pre, const float* scale, int B,
+                         int N, int D, int dtype, float eps, void* h, void* z, void* stream) {
+  NormParams p;
+  const int st = fill_norm(p, x, y, gate, strides, w_post, w_pre, scale, B, N, D, dtype, eps);
+  if (st != TARMAC_OK || (int64_t)B * N == 0) return st;
+  if (!h || !z) return TARMAC_ERR_NULL;
+  const int es = dtype == TARMAC_BF16 ? 2 : 4;
+  if (!aligned(h, es) || !aligned(z, es)) return TARMAC_ERR_ALIGN;
+  p.h = h;
+  p.z = z;
+  return status(launch_residual_norm(p, dtype == TARMAC_BF16, (cudaStream_t)stream));
+}
+
+int64_t tarmac_residual_norm_workspace(int B, int N, int D) {
+  if (B < 1 || N < 1 || D < 1 || D > NORM_MAX_D) return 0;
+  return residual_norm_bwd_work((int64_t)B * N, D) * 4;
+}
+
+int tarmac_residual_norm_backward(const void* x, const void* y, const void* gate, const void* dh,
+                                  const void* dz, const int64_t* strides, const float* w_post,
+                                  const float* w_pre, const float* scale, int B, int N, int D,
+                                  int dtype, float eps, void* dx, void* dy, void* dgate,
+                                  float* dw_post, float* dw_pre, float* dscale, void* work,
+                                  void* stream) {
+  NormParams p;
+  const int st = fill_norm(p, x, y, gate, strides, w_post, w_pre, scale, B, N, D, dtype, eps);
+  if (st != TARMAC_OK) return st;
+  if (!aligned(dw_post, 4) || !aligned(dw_pre, 4) || !aligned(dscale, 4)) return TARMAC_ERR_ALIGN;
+  cudaStream_t s = (cudaStream_t)stream;
+  if ((int64_t)B * N == 0) {  // no rows: the weights' gradients are zero
+    cudaError_t e = cudaSuccess;
+    for (float* w : {dw_post, dw_pre, dscale})
+      if (w && e == cudaSuccess) e = cudaMemsetAsync(w, 0, (size_t)D * 4, s);
+    return status(e);
+  }
+  if (!dx || !dy || (gate && !dgate) || !work) return TARMAC_ERR_NULL;
+  const int es = dtype == TARMAC_BF16 ? 2 : 4;
+  for (const void* ptr : {dh, dz, (const void*)dx, (const void*)dy, (const void*)dgate})
+    if (!aligned(ptr, es)) return TARMAC_ERR_ALIGN;
+  if (!aligned(work, 16)) return TARMAC_ERR_ALIGN;
+  p.dh = dh;
+  p.dz = dz;
+  p.sdh = rows_of(strides, 3, N, D);
+  p.sdz = rows_of(strides, 4, N, D);
+  p.dx = dx;
+  p.dy = dy;
+  p.dgate = gate ? dgate : nullptr;
+  p.dw_post = dw_post;
+  p.dw_pre = dw_pre;
+  p.dscale = dscale;
+  p.work = static_cast<float*>(work);
+  return status(launch_residual_norm_bwd(p, dtype == TARMAC_BF16, s));
+}
+
+}  // extern "C"

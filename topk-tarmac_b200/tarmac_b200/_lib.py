@@ -117,6 +117,27 @@ SIGNATURES: dict[str, tuple] = {
     "tarmac_head_attention_plan": (c_int, [
         c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
         c_int, c_char_p, c_int]),
+    "tarmac_decay_attention_workspace": (c_int64, [
+        c_int, c_int, c_int, c_int]),
+    "tarmac_decay_attention": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
+        c_void_p, c_void_p]),
+    "tarmac_decay_attention_backward_workspace": (c_int64, [
+        c_int, c_int, c_int, c_int, c_int]),
+    "tarmac_decay_attention_backward": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tarmac_residual_norm": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p]),
+    "tarmac_residual_norm_workspace": (c_int64, [
+        c_int, c_int, c_int]),
+    "tarmac_residual_norm_backward": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_void_p,
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "tarmac_kernel_plan": (c_int, [
         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p,
         c_char_p, c_int]),

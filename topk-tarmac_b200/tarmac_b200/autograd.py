@@ -150,6 +150,54 @@ class HeadAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None, None
 
 
+class DecayAttention(torch.autograd.Function):
+    """Attention with a decay for each head (:func:`ops.decay_attention`) with
+    the state after the last row. The decays carry no gradient. First
+    derivatives in reverse mode only, as :class:`QkNormRotate`."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, state=None, lens=None, scale=None):
+        ctx.save_for_backward(q, k, v, log_decay, state, lens)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)  # an unused state costs nothing
+        return ops.decay_attention(q, k, v, log_decay, state, lens, scale,
+                                   return_state=True)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dstate):
+        q, k, v, log_decay, state, lens = ctx.saved_tensors
+        if dout is None:
+            dout = torch.zeros_like(q)
+        dq, dk, dv, first = ops.decay_attention_backward(
+            q, k, v, log_decay, dout, state, dstate, lens, ctx.scale)
+        return dq, dk, dv, None, first, None, None
+
+
+class ResidualNorm(torch.autograd.Function):
+    """The norms around a block with its gate and residual scale
+    (:func:`ops.residual_norm`). First derivatives in reverse mode only, as
+    :class:`QkNormRotate`."""
+
+    @staticmethod
+    def forward(ctx, x, y, w_post=None, w_pre=None, gate=None, scale=None,
+                eps=1e-6):
+        ctx.save_for_backward(x, y, w_post, w_pre, gate, scale)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)  # an unused z costs nothing
+        return ops.residual_norm(x, y, w_post, w_pre, gate, scale, eps)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh, dz):
+        x, y, w_post, w_pre, gate, scale = ctx.saved_tensors
+        dx, dy, dwo, dwi, dgate, dsc = ops.residual_norm_backward(
+            x, y, w_post, w_pre, gate, scale, dh, dz, ctx.eps)
+        dwo, dwi, dsc = (g if g is None else g.to(w.dtype)
+                         for g, w in ((dwo, w_post), (dwi, w_pre), (dsc, scale)))
+        return dx, dy, dwo, dwi, dgate, dsc, None
+
+
 def _needs_grad(*ts) -> bool:
     return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
 
@@ -204,3 +252,23 @@ def head_attention(q, k, v, peers="all", key_len=None, q_start=None,
         return HeadAttention.apply(q, k, v, peers, key_len, q_start, visible,
                                    scale)
     return ops.head_attention(q, k, v, peers, key_len, q_start, visible, scale)
+
+
+def decay_attention(q, k, v, log_decay, state=None, lens=None, scale=None,
+                    return_state=False):
+    if torch.is_grad_enabled() and log_decay.requires_grad:
+        raise ValueError("log_decay has no gradient: pass a tensor that does "
+                         "not require one")
+    ts = [t for t in (q, k, v, log_decay, state) if t is not None]
+    if _needs_grad(*ts) or _has_tangent(*ts):
+        res = DecayAttention.apply(q, k, v, log_decay, state, lens, scale)
+        return res if return_state else res[0]
+    return ops.decay_attention(q, k, v, log_decay, state, lens, scale,
+                               return_state)
+
+
+def residual_norm(x, y, w_post=None, w_pre=None, gate=None, scale=None, eps=1e-6):
+    ts = [t for t in (x, y, w_post, w_pre, gate, scale) if t is not None]
+    if _needs_grad(*ts) or _has_tangent(*ts):
+        return ResidualNorm.apply(x, y, w_post, w_pre, gate, scale, eps)
+    return ops.residual_norm(x, y, w_post, w_pre, gate, scale, eps)

@@ -1,11 +1,13 @@
-"""A communication block of several heads: query/key/value projection, head
-norms with the position rotation, masked attention, output projection.
+"""Communication blocks of several heads: query/key/value projection, head
+norms with the position rotation, attention, output projection.
 
 The single-head module (``src.agents.mappo.AttentionComm``) lets every agent
 read every other one. This block is for agents with wider messages and a
 limited field of view (``visible``), in episodes of unequal size
 (``key_len``), or for one agent that reads its own past, step by step
-(:meth:`HeadComm.step`). It has no counterpart in the reference.
+(:meth:`HeadComm.step`). :class:`DecayComm` reads its past through a memory of
+fixed size instead, whose cost does not grow with the history, and can be
+stacked. They have no counterpart in the reference.
 """
 
 from __future__ import annotations
@@ -109,3 +111,72 @@ class HeadComm(nn.Module):
                                  key_len=past_len.to(torch.int32))
         out.masked_fill_(lost, float("nan"))
         return self.proj(out.flatten(2).to(x.dtype))
+
+
+def decay_slopes(n_heads: int) -> torch.Tensor:
+    """log of each head's decay, fp32 [n_heads]: -2 ** (-8 h / n_heads), from
+    about half a row's memory to 256 rows'."""
+    h = torch.arange(1, n_heads + 1, dtype=torch.float32)
+    return -(2.0 ** (-8.0 * h / n_heads))
+
+
+class DecayComm(nn.Module):
+    """One block of a stack over a stream of rows (B, N, dim): attention with a
+    decay for each head on the normed rows z, projected, normed, gated and
+    added to the stream x, whose norm is the next block's z."""
+
+    def __init__(self, dim: int, n_heads: int, head_dim: int,
+                 n_kv_heads: int | None = None, eps: float = 1e-6) -> None:
+        super().__init__()
+        n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
+        if n_kv_heads < 1 or n_heads % n_kv_heads:
+            raise ValueError("n_heads must be a multiple of n_kv_heads")
+        self.heads = (n_heads, n_kv_heads, n_kv_heads)
+        self.head_dim, self.eps = head_dim, eps
+        self.qkv = nn.Linear(dim, sum(self.heads) * head_dim)
+        self.gate = nn.Linear(dim, dim)
+        self.proj = nn.Linear(n_heads * head_dim, dim)
+        self.norm_q = nn.Parameter(torch.ones(head_dim))
+        self.norm_k = nn.Parameter(torch.ones(head_dim))
+        self.norm_post = nn.Parameter(torch.ones(dim))
+        self.norm_next = nn.Parameter(torch.ones(dim))
+        self.scale = nn.Parameter(torch.ones(dim))
+        self.register_buffer("log_decay", decay_slopes(n_heads))
+
+    def empty_state(self, B: int) -> torch.Tensor:
+        """The state before any row, fp32 [B, n_heads, head_dim, head_dim]."""
+        return torch.zeros(B, self.heads[0], self.head_dim, self.head_dim,
+                           device=self.log_decay.device)
+
+    def _qkv(self, z, cos, sin):
+        d = self.head_dim
+        parts = self.qkv(z).split([h * d for h in self.heads], -1)
+        q, k, v = (t.unflatten(-1, (h, d)) for t, h in zip(parts, self.heads))
+        q, k = tgrad.qk_norm_rotate(q, k, self.norm_q, self.norm_k, cos, sin, self.eps)
+        return q, k, v
+
+    def _join(self, x, z, out):
+        return tgrad.residual_norm(x, self.proj(out.flatten(2)), self.norm_post,
+                                   self.norm_next, self.gate(z), self.scale, self.eps)
+
+    def forward(self, x: torch.Tensor, z: torch.Tensor, cos: torch.Tensor,
+                sin: torch.Tensor, state: torch.Tensor | None = None,
+                lens: torch.Tensor | None = None):
+        """The rows of whole episodes at once, from ``state`` (zero when None).
+        z: the normed rows, the block's input (the first block's may be x
+        itself); ``cos``, ``sin``: the rows' table (:func:`rotation_table`);
+        rows from ``lens`` on are padding. Returns the stream, its norm and the
+        state after the last row."""
+        q, k, v = self._qkv(z, cos, sin)
+        out, state = tgrad.decay_attention(q, k, v, self.log_decay, state, lens,
+                                           return_state=True)
+        return (*self._join(x, z, out), state)
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, z: torch.Tensor, cos: torch.Tensor,
+             sin: torch.Tensor, state: torch.Tensor):
+        """One new row per episode (N = 1, or a few), ``state`` renewed in
+        place. Returns the stream and its norm."""
+        q, k, v = self._qkv(z, cos, sin)
+        out, _ = ops.decay_attention(q, k, v, self.log_decay, state, state_out=state)
+        return self._join(x, z, out)

@@ -775,6 +775,279 @@ def head_attention_plan(B: int, Nq: int, Nk: int, H: int, Hk: int, d: int,
     return json.loads(buf.value.decode())
 
 
+# ---------------------------------------------------------------------------
+# a memory of fixed size: attention with a decay for each head
+# ---------------------------------------------------------------------------
+
+def _check_state(t, name: str, q: torch.Tensor) -> torch.Tensor | None:
+    """A state tensor, fp32 [B, H, d, d], contiguous."""
+    if t is None:
+        return None
+    B, _, H, d = q.shape
+    if tuple(t.shape) != (B, H, d, d):
+        raise ValueError(f"{name} must be [{B}, {H}, {d}, {d}]; got {tuple(t.shape)}")
+    if t.dtype != torch.float32:
+        raise TypeError(f"{name} must be float32; got {t.dtype}")
+    if t.device != q.device:
+        raise ValueError(f"{name} must be on the device of the queries")
+    return t.contiguous()
+
+
+def _check_decay(q, k, v, log_decay, lens):
+    """Checked q, k, v, decays and lengths."""
+    _check_heads({"q": q, "k": k, "v": v}, q)
+    B, N, H, d = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[1] != N or k.shape[3] != d:
+        raise ValueError(f"k and v must share one [{B}, {N}, heads, {d}] shape; "
+                         f"got {tuple(k.shape)}, {tuple(v.shape)}")
+    Hk = k.shape[2]
+    if Hk < 1 or H % Hk:
+        raise ValueError(f"the query heads ({H}) must be a multiple of the key "
+                         f"heads ({Hk})")
+    if tuple(log_decay.shape) != (H,):
+        raise ValueError(f"log_decay must be [{H}]; got {tuple(log_decay.shape)}")
+    if log_decay.dtype != torch.float32:
+        raise TypeError(f"log_decay must be float32; got {log_decay.dtype}")
+    if log_decay.device != q.device:
+        raise ValueError("log_decay must be on the device of the queries")
+    if lens is not None:
+        if tuple(lens.shape) != (B,):
+            raise ValueError(f"lens must be [{B}]; got {tuple(lens.shape)}")
+        if lens.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"lens must be int32 or int64; got {lens.dtype}")
+        if lens.device != q.device:
+            raise ValueError("lens must be on the device of the queries")
+        if lens.dtype is torch.int64:  # beyond 32 bits they act like the bounds
+            lens = lens.clamp(-2 ** 31, 2 ** 31 - 1)
+        lens = lens.to(torch.int32).contiguous()
+    return (_unit_inner(q), _unit_inner(k), _unit_inner(v), log_decay.contiguous(),
+            lens)
+
+
+def _decay_ready(q, k, v, log_decay, lens) -> bool:
+    """As :func:`_rotate_ready`."""
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or v.shape != ks:
+        return False
+    t, dev = q.dtype, q.get_device()
+    return (t in _DTYPES and k.dtype is t and v.dtype is t and dev >= 0
+            and k.get_device() == dev and v.get_device() == dev
+            and ks[0] == qs[0] and ks[1] == qs[1] and ks[3] == qs[3] and ks[2] > 0
+            and qs[2] % ks[2] == 0 and q.stride(3) == 1 and k.stride(3) == 1
+            and v.stride(3) == 1 and log_decay.dtype is torch.float32
+            and log_decay.shape == (qs[2],) and log_decay.get_device() == dev
+            and log_decay.is_contiguous()
+            and (lens is None or (lens.dtype is torch.int32
+                                  and lens.shape == (qs[0],)
+                                  and lens.get_device() == dev
+                                  and lens.is_contiguous())))
+
+
+@functools.lru_cache(maxsize=1024)
+def _decay_work(B, N, H, d) -> int:
+    return _lib.lib().tarmac_decay_attention_workspace(B, N, H, d)
+
+
+@functools.lru_cache(maxsize=1024)
+def _decay_backward_work(B, N, H, Hk, d) -> int:
+    return _lib.lib().tarmac_decay_attention_backward_workspace(B, N, H, Hk, d)
+
+
+def _scratch(nbytes: int, dev: torch.device) -> torch.Tensor | None:
+    return torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+
+
+def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                    log_decay: torch.Tensor, state: torch.Tensor | None = None,
+                    lens: torch.Tensor | None = None, scale: float | None = None,
+                    return_state: bool = False,
+                    state_out: torch.Tensor | None = None):
+    """Attention with a decay for each head, a memory of fixed size: q
+    [B, N, H, d], k and v [B, N, Hk, d] with H a multiple of Hk. For the rows
+    of an episode in order, with l = exp(log_decay[h]) (fp32 [H], at most 0),
+
+        S = l S + k v^T,   out = scale S^T q   (scale: default d ** -0.5).
+
+    ``state`` (fp32 [B, H, d, d], by the columns of k, then of v) is S before
+    the first row, zero when None. Returns out [B, N, H, d], or (out, S after
+    the last row) with ``return_state`` or a ``state_out`` to write it to: a
+    contiguous tensor like ``state``, or ``state`` itself, renewed in place.
+    Rows from ``lens`` [B] on are padding, whatever they hold: they get 0 and
+    leave S alone. One new row over a kept state is N = 1."""
+    if not _decay_ready(q, k, v, log_decay, lens):
+        q, k, v, log_decay, lens = _check_decay(q, k, v, log_decay, lens)
+    start = _check_state(state, "state", q)
+    if state_out is not None:
+        if _check_state(state_out, "state_out", q) is not state_out:
+            raise ValueError("state_out must be contiguous")
+        if state is not None and state_out is not state \
+                and _overlap(state_out, start):
+            raise ValueError("state_out must be state itself or apart from it")
+    B, N, H, d = q.shape
+    out = _empty_as(q)
+    if return_state and state_out is None:
+        state_out = torch.empty((B, H, d, d), device=q.device, dtype=torch.float32)
+    work = _scratch(_decay_work(B, N, H, d), q.device)
+    _launch(q.get_device(), "tarmac_decay_attention", q.data_ptr(), k.data_ptr(),
+            v.data_ptr(), out.data_ptr(),
+            _PACK9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]),
+            log_decay.data_ptr(), _ptr(start), _ptr(state_out), _ptr(lens), B, N,
+            H, k.shape[2], d, _DTYPES[q.dtype], _scale(d, scale), _ptr(work))
+    return out if state_out is None else (out, state_out)
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Do two contiguous tensors share memory without being the same?"""
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    return a0 != b0 and a0 < b0 + 4 * b.numel() and b0 < a0 + 4 * a.numel()
+
+
+def decay_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                             log_decay: torch.Tensor, dout: torch.Tensor,
+                             state: torch.Tensor | None = None,
+                             dstate: torch.Tensor | None = None,
+                             lens: torch.Tensor | None = None,
+                             scale: float | None = None):
+    """Gradients (dq, dk, dv, dS) of :func:`decay_attention`, given those of out
+    (``dout``) and of the state that it returned (``dstate``, or None). dS, of
+    the state before the first row, is None where ``state`` is. Shared key
+    heads are summed over their query heads; padding gets zeros; the decays
+    have no gradient. Deterministic."""
+    if not _decay_ready(q, k, v, log_decay, lens):
+        q, k, v, log_decay, lens = _check_decay(q, k, v, log_decay, lens)
+    dout = _gradient(dout, q, "dout")
+    start, dstate = _check_state(state, "state", q), _check_state(dstate, "dstate", q)
+    B, N, H, d = q.shape
+    Hk = k.shape[2]
+    dq, dk, dv = _empty_as(q), _empty_as(k), _empty_as(v)
+    first = None if start is None else torch.empty_like(start)
+    work = _scratch(_decay_backward_work(B, N, H, Hk, d), q.device)
+    _launch(q.get_device(), "tarmac_decay_attention_backward", q.data_ptr(),
+            k.data_ptr(), v.data_ptr(), dout.data_ptr(),
+            _PACK12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                    *dout.stride()[:3]),
+            log_decay.data_ptr(), _ptr(start), _ptr(dstate), _ptr(lens), B, N, H,
+            Hk, d, _DTYPES[q.dtype], _scale(d, scale), dq.data_ptr(),
+            dk.data_ptr(), dv.data_ptr(), _ptr(first), _ptr(work))
+    return dq, dk, dv, first
+
+
+# ---------------------------------------------------------------------------
+# the norms around a block
+# ---------------------------------------------------------------------------
+
+_PACK10 = struct.Struct("=10q").pack
+
+
+def _norm_rows(t: torch.Tensor) -> torch.Tensor:
+    """[B, N, D] view (a copy where the strides allow none) with unit inner
+    stride. Leading dimensions that are evenly spaced become one."""
+    t = _unit_inner(t)
+    if t.dim() == 3:
+        return t
+    if t.dim() < 3:
+        return t.reshape((1,) * (3 - t.dim()) + tuple(t.shape))
+    return t.flatten(0, -3)
+
+
+def _check_norm(x, named: dict, weights: dict):
+    """The rows as [B, N, D] and the weights, checked."""
+    if not x.is_cuda:
+        raise RuntimeError("tarmac_b200 kernels need CUDA tensors (there is no "
+                           "CPU implementation)")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"tensors must be float32 or bfloat16; got {x.dtype}")
+    if x.dim() < 1:
+        raise ValueError("x must have rows of columns")
+    for name, t in named.items():
+        if t is None:
+            continue
+        if t.shape != x.shape:
+            raise ValueError(f"{name} must have the shape {tuple(x.shape)}; got "
+                             f"{tuple(t.shape)}")
+        if t.device != x.device:
+            raise ValueError(f"{name} must be on the device of x")
+        if t.dtype != x.dtype:
+            raise TypeError(f"{name} must have the dtype {x.dtype} of x; got {t.dtype}")
+    D = x.shape[-1]
+    for name, w in weights.items():
+        if w is None:
+            continue
+        if tuple(w.shape) != (D,):
+            raise ValueError(f"{name} must be [{D}]; got {tuple(w.shape)}")
+        if w.device != x.device:
+            raise ValueError(f"{name} must be on the device of x")
+    rows = [None if t is None else _norm_rows(t) for t in (x, *named.values())]
+    return rows, [None if w is None else w.float().contiguous()
+                  for w in weights.values()]
+
+
+def _row_strides(t: torch.Tensor | None) -> tuple:
+    return (0, 0) if t is None else t.stride()[:2]
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor,
+                  w_post: torch.Tensor | None = None,
+                  w_pre: torch.Tensor | None = None,
+                  gate: torch.Tensor | None = None,
+                  scale: torch.Tensor | None = None, eps: float = 1e-6):
+    """What stands between two blocks, in one pass: the norm of a block's
+    output y, its gate and residual scale, the sum with the stream x, and the
+    norm before the next block. For rows of D <= 8192 columns,
+
+        h = x + scale * sigmoid(gate) * (y / rms(y) * w_post)
+        z = h / rms(h) * w_pre,   rms(t) = sqrt(mean t^2 + eps).
+
+    x, y, gate: [..., D] fp32 or bf16 (no gate: ones in place of its sigmoid);
+    ``w_post``, ``w_pre``, ``scale``: [D] or None (ones). Returns contiguous (h, z)
+    in the inputs' dtype."""
+    (xr, yr, gr), (wo, wi, sc) = _check_norm(
+        x, {"y": y, "gate": gate},
+        {"w_post": w_post, "w_pre": w_pre, "scale": scale})
+    h, z = _empty_as(x), _empty_as(x)
+    B, N, D = xr.shape
+    _launch(x.get_device(), "tarmac_residual_norm", xr.data_ptr(), yr.data_ptr(),
+            _ptr(gr), _PACK6(*_row_strides(xr), *_row_strides(yr), *_row_strides(gr)),
+            _ptr(wo), _ptr(wi), _ptr(sc), B, N, D, _DTYPES[x.dtype], eps,
+            h.data_ptr(), z.data_ptr())
+    return h, z
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_work(B, N, D) -> int:
+    return _lib.lib().tarmac_residual_norm_workspace(B, N, D)
+
+
+def residual_norm_backward(x: torch.Tensor, y: torch.Tensor,
+                           w_post: torch.Tensor | None,
+                           w_pre: torch.Tensor | None,
+                           gate: torch.Tensor | None,
+                           scale: torch.Tensor | None,
+                           dh: torch.Tensor | None, dz: torch.Tensor | None,
+                           eps: float = 1e-6):
+    """Gradients of :func:`residual_norm` for its inputs and the gradients of
+    its outputs (None: zero): (dx, dy) and dgate in the inputs' dtype and
+    (dw_post, dw_pre, dscale) fp32 [D], as (dx, dy, dw_post, dw_pre, dgate,
+    dscale), None where the input is. Deterministic."""
+    (xr, yr, gr, hr, zr), (wo, wi, sc) = _check_norm(
+        x, {"y": y, "gate": gate, "dh": dh, "dz": dz},
+        {"w_post": w_post, "w_pre": w_pre, "scale": scale})
+    B, N, D = xr.shape
+    dx, dy = _empty_as(x), _empty_as(x)
+    dgate = None if gate is None else _empty_as(x)
+    sums = torch.empty((3, D), device=x.device, dtype=torch.float32)
+    dwo, dwi, dsc = (None if w is None else s for w, s in zip((wo, wi, sc), sums))
+    work = _scratch(_norm_work(B, N, D), x.device)
+    _launch(x.get_device(), "tarmac_residual_norm_backward", xr.data_ptr(),
+            yr.data_ptr(), _ptr(gr), _ptr(hr), _ptr(zr),
+            _PACK10(*_row_strides(xr), *_row_strides(yr), *_row_strides(gr),
+                    *_row_strides(hr), *_row_strides(zr)),
+            _ptr(wo), _ptr(wi), _ptr(sc), B, N, D, _DTYPES[x.dtype], eps,
+            dx.data_ptr(), dy.data_ptr(), _ptr(dgate), _ptr(dwo), _ptr(dwi),
+            _ptr(dsc), _ptr(work))
+    return dx, dy, dwo, dwi, dgate, dsc
+
+
 _PLAN_OPS = {"dense": 0, "topk": 1, "streaming": 2}
 _PLAN_MODES = {"argmax": _lib.SELECT_ARGMAX, "threshold": _lib.SELECT_THRESHOLD,
                "sort": _lib.SELECT_SORT}
