@@ -414,8 +414,10 @@ int tarmac_head_attention_plan(int backward, const int64_t *strides, int B,
  * FMAs; bf16: bf16 products with fp32 sums, the weights of the rows and the
  * copy of the state that multiplies q rounded to bf16, what enters a returned
  * state good to fp32. work: 16-byte aligned scratch of
- * tarmac_decay_attention_workspace bytes (0: NULL is fine). */
-int64_t tarmac_decay_attention_workspace(int B, int N, int H, int d);
+ * tarmac_decay_attention_workspace bytes (its state_out: is there one? 0
+ * bytes: NULL is fine). */
+int64_t tarmac_decay_attention_workspace(int B, int N, int H, int d, int dtype,
+                                         int state_out);
 int tarmac_decay_attention(const void *q, const void *k, const void *v,
                            void *out, const int64_t *strides,
                            const float *log_decay, const float *state,
@@ -431,9 +433,10 @@ int tarmac_decay_attention(const void *q, const void *k, const void *v,
  * dv: contiguous, the inputs' type, zero on padding; dstate: fp32 [B, H, d, d]
  * or NULL, not dstate_out. The decays get no gradient. No atomics: two calls
  * give the same bits. work: 16-byte aligned scratch of
- * tarmac_decay_attention_backward_workspace bytes (0: NULL is fine). */
+ * tarmac_decay_attention_backward_workspace bytes (its dstate: is there one? 0
+ * bytes: NULL is fine). */
 int64_t tarmac_decay_attention_backward_workspace(int B, int N, int H, int Hk,
-                                                  int d);
+                                                  int d, int dtype, int dstate);
 int tarmac_decay_attention_backward(const void *q, const void *k,
                                     const void *v, const void *dout,
                                     const int64_t *strides,

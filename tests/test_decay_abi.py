@@ -57,14 +57,16 @@ def test_decay_own_checks():
     assert _decay(True, dk=FAKE + 4) == _lib.ERR_ALIGN
     assert _decay(True, work=None) == _lib.ERR_NULL          # shared heads are summed
     assert _decay(False, B=1, N=8192, work=None) == _lib.ERR_NULL  # segments
-    so = _lib.lib()
-    assert so.tarmac_decay_attention_workspace(1, 8192, 4, 64) >= 2 * 4 * 64 * 64 * 4
-    assert so.tarmac_decay_attention_workspace(1, 1, 4, 64) == 0
-    assert so.tarmac_decay_attention_workspace(4096, 512, 4, 64) == 0
-    assert so.tarmac_decay_attention_workspace(0, 512, 4, 64) == 0
-    assert so.tarmac_decay_attention_backward_workspace(4096, 512, 4, 4, 64) == 0
-    assert so.tarmac_decay_attention_backward_workspace(4096, 512, 4, 2, 64) >= \
-        4096 * 512 * 4 * 64 * 4
+    fwd = _lib.lib().tarmac_decay_attention_workspace
+    bwd = _lib.lib().tarmac_decay_attention_backward_workspace
+    for dt in (_lib.F32, _lib.BF16):
+        assert fwd(1, 8192, 4, 64, dt, 0) >= 2 * 4 * 64 * 64 * 4
+        assert fwd(1, 1, 4, 64, dt, 1) == 0
+        assert fwd(4096, 512, 4, 64, dt, 0) == 0
+        assert fwd(0, 512, 4, 64, dt, 1) == 0
+        assert bwd(4096, 512, 4, 4, 64, dt, 0) == 0
+        assert bwd(4096, 512, 4, 2, 64, dt, 0) >= 4096 * 512 * 4 * 64 * 4
+    assert fwd(2, 8, 4, 64, 7, 0) == 0
 
 
 def _norm(backward, **kw):

@@ -24,7 +24,7 @@ struct DecayParams {
   const int32_t* lens;       // [B] or NULL
   const float* start;        // [B, H, d, d], the state before, or NULL (zero)
   float* last;               // [B, H, d, d], the state after, or NULL
-  float* part;               // [segs, B, H, d, d] or NULL where segs is 1
+  float* part;               // [segs, B, H, d, d], or NULL (decay_uses_part)
   int B, N, H, d;
   int segs, seg_chunks;      // parts of the row axis and their chunks
   int reverse;               // rows run from the last to the first
@@ -32,6 +32,7 @@ struct DecayParams {
   float in_scale;            // factor of every b_j c_j term
   float out_scale;           // factor of out
   int planes;                // bf16 parts of the weighted rows that enter S
+  int tc;                    // runs on the tensor memory (decay_tc.cu)
   int vec;                   // 16-byte rows in a, b, c
   int vec_out;               // and in out
 };
@@ -46,18 +47,28 @@ __device__ __forceinline__ int decay_len(const DecayParams& p, int b) {
 }
 
 constexpr int DECAY_CHUNK = 64;      // rows of a chunk, warp-level kernel
+constexpr int DECAY_TC_CHUNK = 128;  // and of one on the tensor memory
 
 struct DecayPlan {
   int segs, seg_chunks;
 };
-DecayPlan decay_plan(int B, int N, int H);
-// parts that `part` must hold, 0 for none
-inline int64_t decay_parts(const DecayPlan& g) { return g.segs > 1 ? g.segs : 0; }
+DecayPlan decay_plan(int B, int N, int H, int d, bool tc);
+DecayPlan decay_plan_tc(int B, int N, int H, int d);
+// may a call of these sizes run on the tensor memory?
+bool decay_tc_sizes(int B, int N, int H, int d, bool bf16);
+// Does the call keep states in p.part? (On the tensor memory the state after
+// the last row comes from the segments' states, else from the rows' kernel.)
+inline bool decay_uses_part(const DecayPlan& g, bool tc, bool last) {
+  return g.segs > 1 || (tc && last);
+}
 
 // States of the segments into p.part: first what each adds, then, in place,
-// the state before each. Launches nothing where segs is 1.
+// the state before each (and p.last, on the tensor memory). Launches nothing
+// where the call does not use p.part.
 cudaError_t launch_decay_states(const DecayParams& p, bool bf16, cudaStream_t s);
 cudaError_t launch_decay_rows(const DecayParams& p, bool bf16, cudaStream_t s);
+cudaError_t launch_decay_states_tc(const DecayParams& p, cudaStream_t s);
+cudaError_t launch_decay_rows_tc(const DecayParams& p, cudaStream_t s);
 // few rows, one after the other (forward only)
 bool decay_step_takes(int N);
 cudaError_t launch_decay_step(const DecayParams& p, bool bf16, cudaStream_t s);

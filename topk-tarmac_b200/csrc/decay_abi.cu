@@ -10,6 +10,8 @@
 
 namespace tarmac {
 
+bool head_map_ok(const HeadStrides& s, int B, int N, int h);
+
 namespace {
 
 constexpr int MAX_D = 128;
@@ -54,10 +56,23 @@ int fill_decay(DecayParams& p, const void* q, const void* k, const void* v,
   p.N = N;
   p.H = H;
   p.d = d;
-  const DecayPlan g = decay_plan(B, N, H);
+  return TARMAC_OK;
+}
+
+void set_plan(DecayParams& p, bool tc) {
+  const DecayPlan g = decay_plan(p.B, p.N, p.H, p.d, tc);
   p.segs = g.segs;
   p.seg_chunks = g.seg_chunks;
-  return TARMAC_OK;
+  p.tc = tc;
+}
+// bytes of p.part, whichever kernels the rows' layout allows
+int64_t part_bytes(int B, int N, int H, int d, bool bf16, bool last) {
+  int64_t parts = 0;
+  for (int tc = 0; tc <= (int)decay_tc_sizes(B, N, H, d, bf16); ++tc) {
+    const DecayPlan g = decay_plan(B, N, H, d, tc != 0);
+    if (decay_uses_part(g, tc != 0, last) && g.segs > parts) parts = g.segs;
+  }
+  return parts * B * H * d * d * 4;
 }
 
 // one operand: pointer, strides and how many heads share one of its heads
@@ -65,8 +80,13 @@ struct Operand {
   const void* ptr;
   HeadStrides s;
   int share;
-  bool vec;
+  bool vec, map;  // rows are vectors; TMA can describe them
 };
+Operand operand(const void* ptr, const HeadStrides& s, int B, int N, int H, int share, int d,
+                int es) {
+  const bool vec = d * es % 16 == 0 && vec_ok(ptr, s, es);
+  return Operand{ptr, s, share, vec, vec && es == 2 && head_map_ok(s, B, N, H / share)};
+}
 void set_operands(DecayParams& p, const Operand& a, const Operand& b, const Operand& c) {
   p.a = a.ptr;
   p.b = b.ptr;
@@ -130,10 +150,10 @@ using namespace tarmac;
 
 extern "C" {
 
-int64_t tarmac_decay_attention_workspace(int B, int N, int H, int d) {
-  if (check_sizes(B, N, H, 1, d, TARMAC_F32) != TARMAC_OK || B < 1 || N < 1) return 0;
+int64_t tarmac_decay_attention_workspace(int B, int N, int H, int d, int dtype, int state_out) {
+  if (check_sizes(B, N, H, 1, d, dtype) != TARMAC_OK || B < 1 || N < 1) return 0;
   if (decay_step_takes(N)) return 0;
-  return decay_parts(decay_plan(B, N, H)) * B * H * d * d * 4;
+  return part_bytes(B, N, H, d, dtype == TARMAC_BF16, state_out != 0);
 }
 
 int tarmac_decay_attention(const void* q, const void* k, const void* v, void* out,
@@ -152,28 +172,30 @@ int tarmac_decay_attention(const void* q, const void* k, const void* v, void* ou
   if (!aligned(out, 16) || !aligned(work, 16)) return TARMAC_ERR_ALIGN;
   const HeadStrides sq = stride_of(strides, 0, N, H, d), sk = stride_of(strides, 1, N, Hk, d),
                     sv = stride_of(strides, 2, N, Hk, d);
-  const bool wide = d * es % 16 == 0;
-  const Operand oq = {q, sq, 1, wide && vec_ok(q, sq, es)};
-  const Operand ok = {k, sk, G, wide && vec_ok(k, sk, es)};
-  const Operand ov = {v, sv, G, wide && vec_ok(v, sv, es)};
+  const Operand oq = operand(q, sq, B, N, H, 1, d, es), ok = operand(k, sk, B, N, H, G, d, es),
+                ov = operand(v, sv, B, N, H, G, d, es);
   p.out = out;
   p.start = state;
   p.last = state_out;
-  p.planes = state_out ? 3 : 2;
   p.in_scale = 1.f;
   p.out_scale = scale;
   set_operands(p, oq, ok, ov);
   if (decay_step_takes(N)) return status(launch_decay_step(p, bf16, s));
-  if (p.segs > 1 && !work) return TARMAC_ERR_NULL;
-  p.part = static_cast<float*>(work);
+  set_plan(p, decay_tc_sizes(B, N, H, d, bf16) && oq.map && ok.map && ov.map);
+  if (decay_uses_part(DecayPlan{p.segs, p.seg_chunks}, p.tc, state_out)) {
+    if (!work) return TARMAC_ERR_NULL;
+    p.part = static_cast<float*>(work);
+  }
+  p.planes = state_out ? 3 : 2;
   cudaError_t e = launch_decay_states(p, bf16, s);
   if (e == cudaSuccess) e = launch_decay_rows(p, bf16, s);
   return status(e);
 }
 
-int64_t tarmac_decay_attention_backward_workspace(int B, int N, int H, int Hk, int d) {
-  if (check_sizes(B, N, H, Hk, d, TARMAC_F32) != TARMAC_OK || B < 1 || N < 1) return 0;
-  const int64_t parts = decay_parts(decay_plan(B, N, H)) * B * H * d * d * 4;
+int64_t tarmac_decay_attention_backward_workspace(int B, int N, int H, int Hk, int d, int dtype,
+                                                  int dstate) {
+  if (check_sizes(B, N, H, Hk, d, dtype) != TARMAC_OK || B < 1 || N < 1) return 0;
+  const int64_t parts = part_bytes(B, N, H, d, dtype == TARMAC_BF16, dstate != 0);
   // gradients of shared heads by query head, before their sum
   const int64_t shared = H == Hk ? 0 : (int64_t)B * N * H * d * 4;
   return round16(parts) + shared;
@@ -197,17 +219,16 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
   if (!aligned(dout, es) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16) ||
       !aligned(work, 16))
     return TARMAC_ERR_ALIGN;
-  if (!work && tarmac_decay_attention_backward_workspace(B, N, H, Hk, d) > 0)
+  if (!work && tarmac_decay_attention_backward_workspace(B, N, H, Hk, d, dtype, dstate != nullptr))
     return TARMAC_ERR_NULL;
   const HeadStrides sq = stride_of(strides, 0, N, H, d), sk = stride_of(strides, 1, N, Hk, d),
                     sv = stride_of(strides, 2, N, Hk, d), sg = stride_of(strides, 3, N, H, d);
-  const bool wide = d * es % 16 == 0;
-  const Operand oq = {q, sq, 1, wide && vec_ok(q, sq, es)};
-  const Operand ok = {k, sk, G, wide && vec_ok(k, sk, es)};
-  const Operand ov = {v, sv, G, wide && vec_ok(v, sv, es)};
-  const Operand og = {dout, sg, 1, wide && vec_ok(dout, sg, es)};
-  const int64_t parts = decay_parts(decay_plan(B, N, H)) * B * H * d * d * 4;
-  p.part = static_cast<float*>(work);
+  const Operand oq = operand(q, sq, B, N, H, 1, d, es), ok = operand(k, sk, B, N, H, G, d, es),
+                ov = operand(v, sv, B, N, H, G, d, es);
+  const Operand og = operand(dout, sg, B, N, H, 1, d, es);
+  set_plan(p, decay_tc_sizes(B, N, H, d, bf16) && oq.map && ok.map && ov.map && og.map);
+  const DecayPlan plan = {p.segs, p.seg_chunks};
+  const int64_t parts = part_bytes(B, N, H, d, bf16, dstate != nullptr);
   float* shared = reinterpret_cast<float*>(static_cast<char*>(work) + round16(parts));
   cudaError_t e = cudaSuccess;
   auto run = [&](cudaError_t (*launch)(const DecayParams&, bool, cudaStream_t)) {
@@ -215,6 +236,7 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
   };
   // dq_i = scale S_i dout_i, S over the rows as in the forward pass
   p.start = state;
+  p.part = decay_uses_part(plan, p.tc, false) ? static_cast<float*>(work) : nullptr;
   p.planes = 2;
   p.in_scale = 1.f;
   p.out_scale = scale;
@@ -227,6 +249,8 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
   // R_i = sum over the rows from i on of scale q dout^T:
   // dv_i = R_i^T k_i, dk_i = R_i v_i
   p.start = dstate_out;
+  p.last = dstate;
+  p.part = decay_uses_part(plan, p.tc, dstate) ? static_cast<float*>(work) : nullptr;
   p.planes = dstate ? 3 : 2;
   p.reverse = 1;
   p.transposed = 0;

@@ -295,7 +295,8 @@ __global__ void __launch_bounds__(DA_THREADS) decay_kernel(DecayParams p) {
 }
 
 // part[s] (what segment s adds) becomes the state before segment s:
-//   X_0 = start, X_(s+1) = l^(rows of s) X_s + part[s].
+//   X_0 = start, X_(s+1) = l^(rows of s) X_s + part[s];
+// p.last, where given, the state after the last one.
 __global__ void __launch_bounds__(256) decay_join_kernel(DecayParams p, int64_t stride, int rows) {
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (e >= stride) return;
@@ -307,7 +308,7 @@ __global__ void __launch_bounds__(256) decay_join_kernel(DecayParams p, int64_t 
   float x = p.start ? p.start[e] : 0.f;
   float* at = p.part + e;
   for (int s = 0; s < p.segs; ++s, at += stride) {
-    const float add = s + 1 < p.segs ? *at : 0.f;
+    const float add = s + 1 < p.segs || p.last ? *at : 0.f;
     *at = x;
     // rows [t0, t1) of segment s
     const int t0 = p.reverse ? max(0, chunks - (s + 1) * p.seg_chunks) * rows : s * chunk_rows;
@@ -315,6 +316,7 @@ __global__ void __launch_bounds__(256) decay_join_kernel(DecayParams p, int64_t 
     const int n = max(0, min(len, t1) - t0);
     x = fmaf(expf(rate * (float)n), x, add);
   }
+  if (p.last) p.last[e] = x;
 }
 
 template <typename T>
@@ -350,8 +352,9 @@ cudaError_t decay_width(const DecayParams& p, cudaStream_t s) {
 
 }  // namespace
 
-DecayPlan decay_plan(int B, int N, int H) {
+DecayPlan decay_plan(int B, int N, int H, int d, bool tc) {
   if (B < 1 || N < 1) return DecayPlan{1, 1};
+  if (tc) return decay_plan_tc(B, N, H, d);
   const int chunks = cdiv(N, DECAY_CHUNK);
   const int64_t heads = (int64_t)B * H;
   int64_t segs = heads >= 296 ? 1 : (592 + heads - 1) / heads;
@@ -363,17 +366,26 @@ DecayPlan decay_plan(int B, int N, int H) {
   return g;
 }
 
+bool decay_tc_sizes(int B, int N, int H, int d, bool bf16) {
+  return bf16 && d > 32 && d % 8 == 0 && N > 64;
+}
+
 cudaError_t launch_decay_states(const DecayParams& p, bool bf16, cudaStream_t s) {
-  if (p.segs == 1) return cudaSuccess;
-  const cudaError_t e = bf16 ? decay_width<__nv_bfloat16, false>(p, s)
-                             : decay_width<float, false>(p, s);
+  if (!decay_uses_part(DecayPlan{p.segs, p.seg_chunks}, p.tc, p.last)) return cudaSuccess;
+  DecayParams q = p;
+  if (!p.tc) q.last = nullptr;
+  const cudaError_t e = p.tc ? launch_decay_states_tc(p, s)
+                        : bf16 ? decay_width<__nv_bfloat16, false>(p, s)
+                               : decay_width<float, false>(p, s);
   if (e != cudaSuccess) return e;
   const int64_t stride = (int64_t)p.B * p.H * p.d * p.d;
-  decay_join_kernel<<<(unsigned)((stride + 255) / 256), 256, 0, s>>>(p, stride, DECAY_CHUNK);
+  decay_join_kernel<<<(unsigned)((stride + 255) / 256), 256, 0, s>>>(
+      q, stride, p.tc ? DECAY_TC_CHUNK : DECAY_CHUNK);
   return cudaGetLastError();
 }
 
 cudaError_t launch_decay_rows(const DecayParams& p, bool bf16, cudaStream_t s) {
+  if (p.tc) return launch_decay_rows_tc(p, s);
   return bf16 ? decay_width<__nv_bfloat16, true>(p, s) : decay_width<float, true>(p, s);
 }
 

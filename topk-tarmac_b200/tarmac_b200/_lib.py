@@ -118,13 +118,13 @@ SIGNATURES: dict[str, tuple] = {
         c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
         c_int, c_char_p, c_int]),
     "tarmac_decay_attention_workspace": (c_int64, [
-        c_int, c_int, c_int, c_int]),
+        c_int, c_int, c_int, c_int, c_int, c_int]),
     "tarmac_decay_attention": (c_int, [
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
         c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
         c_void_p, c_void_p]),
     "tarmac_decay_attention_backward_workspace": (c_int64, [
-        c_int, c_int, c_int, c_int, c_int]),
+        c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "tarmac_decay_attention_backward": (c_int, [
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
         c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float,

@@ -844,13 +844,13 @@ def _decay_ready(q, k, v, log_decay, lens) -> bool:
 
 
 @functools.lru_cache(maxsize=1024)
-def _decay_work(B, N, H, d) -> int:
-    return _lib.lib().tarmac_decay_attention_workspace(B, N, H, d)
+def _decay_work(*sizes) -> int:
+    return _lib.lib().tarmac_decay_attention_workspace(*sizes)
 
 
 @functools.lru_cache(maxsize=1024)
-def _decay_backward_work(B, N, H, Hk, d) -> int:
-    return _lib.lib().tarmac_decay_attention_backward_workspace(B, N, H, Hk, d)
+def _decay_backward_work(*sizes) -> int:
+    return _lib.lib().tarmac_decay_attention_backward_workspace(*sizes)
 
 
 def _scratch(nbytes: int, dev: torch.device) -> torch.Tensor | None:
@@ -887,7 +887,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     out = _empty_as(q)
     if return_state and state_out is None:
         state_out = torch.empty((B, H, d, d), device=q.device, dtype=torch.float32)
-    work = _scratch(_decay_work(B, N, H, d), q.device)
+    work = _scratch(_decay_work(B, N, H, d, _DTYPES[q.dtype], int(state_out is not None)),
+                    q.device)
     _launch(q.get_device(), "tarmac_decay_attention", q.data_ptr(), k.data_ptr(),
             v.data_ptr(), out.data_ptr(),
             _PACK9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]),
@@ -921,7 +922,8 @@ def decay_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     Hk = k.shape[2]
     dq, dk, dv = _empty_as(q), _empty_as(k), _empty_as(v)
     first = None if start is None else torch.empty_like(start)
-    work = _scratch(_decay_backward_work(B, N, H, Hk, d), q.device)
+    work = _scratch(_decay_backward_work(B, N, H, Hk, d, _DTYPES[q.dtype],
+                                         int(first is not None)), q.device)
     _launch(q.get_device(), "tarmac_decay_attention_backward", q.data_ptr(),
             k.data_ptr(), v.data_ptr(), dout.data_ptr(),
             _PACK12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
