@@ -19,7 +19,7 @@ struct DecayParams {
   void* out;                 // [B, N, H, d] contiguous, or NULL: states only
   HeadStrides sa, sb, sc;
   int ga, gb, gc;            // heads that share one head of a, b, c
-  int out_f32;               // out is fp32 (else the rows' type)
+  int out_f32;               // out is fp32 (backwards only), else the rows' type
   const float* log_decay;    // [H]
   const int32_t* lens;       // [B] or NULL
   const float* start;        // [B, H, d, d], the state before, or NULL (zero)

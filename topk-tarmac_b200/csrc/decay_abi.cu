@@ -186,7 +186,7 @@ int tarmac_decay_attention(const void* q, const void* k, const void* v, void* ou
     if (!work) return TARMAC_ERR_NULL;
     p.part = static_cast<float*>(work);
   }
-  p.planes = state_out ? 3 : 2;
+  p.planes = state_out ? 3 : (p.tc ? 1 : 2);
   cudaError_t e = launch_decay_states(p, bf16, s);
   if (e == cudaSuccess) e = launch_decay_rows(p, bf16, s);
   return status(e);
@@ -237,7 +237,7 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
   // dq_i = scale S_i dout_i, S over the rows as in the forward pass
   p.start = state;
   p.part = decay_uses_part(plan, p.tc, false) ? static_cast<float*>(work) : nullptr;
-  p.planes = 2;
+  p.planes = p.tc ? 1 : 2;
   p.in_scale = 1.f;
   p.out_scale = scale;
   set_operands(p, oq, ok, ov);
@@ -251,7 +251,7 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
   p.start = dstate_out;
   p.last = dstate;
   p.part = decay_uses_part(plan, p.tc, dstate) ? static_cast<float*>(work) : nullptr;
-  p.planes = dstate ? 3 : 2;
+  p.planes = dstate ? 3 : (p.tc ? 1 : 2);
   p.reverse = 1;
   p.transposed = 0;
   p.in_scale = scale;

@@ -303,18 +303,25 @@ __global__ void __launch_bounds__(256) decay_join_kernel(DecayParams p, int64_t 
   const int dd = p.d * p.d;
   const int bh = (int)(e / dd), b = bh / p.H;
   const int len = decay_len(p, b), chunk_rows = p.seg_chunks * rows;
-  const int chunks = cdiv(p.N, rows);
+  const int chunks = cdiv(p.N, rows), parts = p.last ? p.segs : p.segs - 1;
   const float rate = decay_rate(p.log_decay, bh % p.H);
   float x = p.start ? p.start[e] : 0.f;
   float* at = p.part + e;
-  for (int s = 0; s < p.segs; ++s, at += stride) {
-    const float add = s + 1 < p.segs || p.last ? *at : 0.f;
-    *at = x;
-    // rows [t0, t1) of segment s
-    const int t0 = p.reverse ? max(0, chunks - (s + 1) * p.seg_chunks) * rows : s * chunk_rows;
-    const int t1 = p.reverse ? (chunks - s * p.seg_chunks) * rows : t0 + chunk_rows;
-    const int n = max(0, min(len, t1) - t0);
-    x = fmaf(expf(rate * (float)n), x, add);
+  for (int s0 = 0; s0 < p.segs; s0 += 8) {
+    float add[8];  // eight loads in flight
+#pragma unroll
+    for (int u = 0; u < 8; ++u) add[u] = s0 + u < parts ? at[(s0 + u) * stride] : 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int s = s0 + u;
+      if (s >= p.segs) break;
+      at[s * stride] = x;
+      // rows [t0, t1) of segment s
+      const int t0 = p.reverse ? max(0, chunks - (s + 1) * p.seg_chunks) * rows : s * chunk_rows;
+      const int t1 = p.reverse ? (chunks - s * p.seg_chunks) * rows : t0 + chunk_rows;
+      const int n = max(0, min(len, t1) - t0);
+      x = fmaf(expf(rate * (float)n), x, add[u]);
+    }
   }
   if (p.last) p.last[e] = x;
 }

@@ -7,25 +7,26 @@
 // decay_rows_tc_kernel gives the rows. A block walks over one unit: a head of
 // an episode, or two heads of up to 64 columns (the two 64-column halves of a
 // tile), in one segment of the row axis. Roles of its 20 warps (two idle):
-// * warp 1: one thread loads a, b, c tiles by TMA, two chunks deep.
+// * warp 1: one thread loads a, b, c tiles by TMA ahead of the products.
 // * warp 0: one thread issues the products P, a S, the state's and P c.
 // * warps 4..11 weight P (TMEM, back to TMEM as bf16, the A operand of P c) and
-//   store the rows.
+//   store the rows, through the tile of a.
 // * warps 12..19 keep the state (fp32 in TMEM: scaled by l^n before the product
-//   adds to it; a bf16 copy in shared memory multiplies a), weight b for the
-//   state's product, in two bf16 parts over b and a once those are used, and
-//   scale a S by l^(i+1) before P c adds to it.
-// TMEM columns: P of a unit's head u at 128 u, out at 256, S at 384. S has the
-// columns of c as lanes, those of b as columns; with two heads the product
-// forms all four blocks of 64 x 64 and only the two of one head each are used.
+//   adds to it; a copy in shared memory multiplies a), weight b in place for
+//   the state's product once P is formed, and scale a S by l^(i+1) before P c
+//   adds to it.
+// TMEM columns: P of a unit's head u at 128 u (one head: of two chunks in
+// turn), out at 256, S at 384. S has the columns of c as lanes, those of b as
+// columns; with two heads the product forms all four blocks of 64 x 64 and only
+// the two of one head each are used.
 // Roundings to bf16, one on the way of each term and the size of the output's
-// own: the weighted P and the copy of S. One part for the weighted b would be
-// a second for what passes through S (2.6e-3 of the rows' norm, where two give
-// 2.3e-3 and the output's rounding alone is 1.7e-3).
+// own: the weighted P and the weighted b. The copy of S is in two bf16 parts; in
+// one it would be a second rounding for what passes through S (2.6e-3 of the
+// rows' norm, where this gives 2.3e-3 and the output's rounding alone 1.7e-3).
 //
 // decay_state_tc_kernel gives what each segment adds to the state, in fp32
-// registers: the weighted b in two bf16 parts for states that only feed the
-// rows, in three (24 bits) for those that the caller gets.
+// registers: the weighted b as in the rows' kernel for states that only feed
+// the rows, in three bf16 parts (24 bits) for those that the caller gets.
 //
 // Bound by memory: four tiles a chunk (a, b, c, out), 128 KB for 2048 clocks of
 // products at d = 128 (about 5600 clocks of one SM's share of HBM).
@@ -112,9 +113,16 @@ __device__ __forceinline__ void st_piece(uint32_t a, uint4 v) {
 __device__ __forceinline__ float lo_half(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float hi_half(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
-// the pair of fp32 bits (a, b) w, as bf16
-__device__ __forceinline__ uint32_t scaled_f32(uint32_t a, uint32_t b, float w) {
-  return tc::pack_bf16x2(__uint_as_float(a) * w, __uint_as_float(b) * w);
+// eight bf16 times f
+__device__ __forceinline__ uint4 weighted(uint4 v, float f) {
+  const uint64_t ff = pack2(f, f);
+  uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 a = unpack2(ht::fmul2(pack2(lo_half(x[i]), hi_half(x[i])), ff));
+    x[i] = tc::pack_bf16x2(a.x, a.y);
+  }
+  return make_uint4(x[0], x[1], x[2], x[3]);
 }
 // the pair (a, b) as bf16; what the rounding left stays
 __device__ __forceinline__ uint32_t split_off(float& a, float& b) {
@@ -127,6 +135,116 @@ __device__ __forceinline__ uint32_t split_off(float& a, float& b) {
 __device__ __forceinline__ void tmem_ld_n(uint32_t t, uint32_t (&r)[16]) { ht::tmem_ld(t, r); }
 __device__ __forceinline__ void tmem_ld_n(uint32_t t, uint32_t (&r)[32]) { ht::tmem_ld(t, r); }
 
+// A warp's 32 rows of 128 bytes in shared memory, each lane's own, 16-byte
+// pieces swizzled by row as TMA reads them.
+__device__ __forceinline__ void stage_row(uint32_t stage, int lane, int piece,
+                                          const uint32_t (&o)[32]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      x[u] = tc::pack_bf16x2(__uint_as_float(o[8 * e + 2 * u]), __uint_as_float(o[8 * e + 2 * u + 1]));
+    st_piece(stage + lane * 128 + (((piece + e) ^ (lane & 7)) << 4),
+             make_uint4(x[0], x[1], x[2], x[3]));
+  }
+}
+__device__ __forceinline__ void stage_row32(uint32_t stage, int lane, const uint32_t (&o)[32]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    st_piece(stage + lane * 128 + ((e ^ (lane & 7)) << 4),
+             make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
+}
+// Those rows to a tensor with boxes of 32 rows, rows and columns beyond it left
+// out. One lane; the same lane waits for their having been read.
+__device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t stage, int col, int head,
+                                          int row, int b) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];\n"
+      "cp.async.bulk.commit_group;" ::"l"(map),
+      "r"(stage), "r"(col), "r"(head), "r"(row), "r"(b)
+      : "memory");
+}
+__device__ __forceinline__ void stores_read() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+// 32 rows from memory address dst on, `step` elements apart, all of one word: the
+// first n columns, where they exist; `each`: elements of 16 bytes
+template <typename T>
+__device__ __forceinline__ void fill_rows(T* dst, uint32_t word, int lane, int left, int64_t step,
+                                          int n, int each) {
+  for (int r = lane >> 3; r < min(left, 32); r += 4)
+    for (int c = (lane & 7) * each; c < n; c += 8 * each)
+      *reinterpret_cast<uint4*>(dst + r * step + c) = make_uint4(word, word, word, word);
+}
+
+// Decays below 2^-7 a row: l^-15 nears the end of fp32's range.
+constexpr float DT_STRONG = -7.f;
+
+// 32 columns j0 .. of row i of P, weighted, back to TMEM as bf16. Columns
+// 64 c .. 64 c + 63 take the 32 TMEM columns from 64 c on. w0: the warp's first
+// row. In each group of 16 columns from jb on, l^(i-j) = l^(i-jb-15) l^(15-x)
+// with the second factor from `steps` (backwards l^(jb-i) l^x); on the diagonal
+// the first is above 1, where a strong decay takes an exponential for each
+// element instead. Elements that a row does not see become zero whatever
+// they are.
+template <bool REV>
+__device__ __forceinline__ void weigh(uint32_t t_p, int j0, int i, int w0, int n, float l2,
+                                      float in_scale, const uint64_t (&steps)[8]) {
+  uint32_t pk[16];
+  const uint32_t to = t_p + (j0 & ~63) + (j0 & 32) / 2;
+  if (REV ? w0 > j0 + 31 || j0 >= n : w0 + 31 < j0) {  // no row sees any
+#pragma unroll
+    for (int e = 0; e < 16; ++e) pk[e] = 0u;
+  } else {
+    uint32_t s[32];
+    ht::tmem_ld(t_p + j0, s);
+    const bool whole = REV ? j0 >= w0 + 31 && j0 + 32 <= n : w0 >= j0 + 31;
+    if (whole || l2 >= DT_STRONG) {
+      float f = in_scale * power(l2, REV ? j0 - i : i - j0 - 15);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const uint64_t ff = pack2(f, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float2 y = unpack2(ht::fmul2(ht::fmul2(steps[e], ff),
+                                             ht::pair(s[16 * g + 2 * e], s[16 * g + 2 * e + 1])));
+          s[16 * g + 2 * e] = __float_as_uint(y.x);
+          s[16 * g + 2 * e + 1] = __float_as_uint(y.y);
+        }
+        if (g == 0) f = in_scale * power(l2, REV ? j0 + 16 - i : i - j0 - 31);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const int gap = max(0, REV ? j0 + e - i : i - j0 - e);
+        s[e] = __float_as_uint(__uint_as_float(s[e]) * in_scale * power(l2, gap));
+      }
+    }
+    if (!whole) {
+      const int lo = REV ? i - j0 : 0, hi = REV ? n - 1 - j0 : i - j0;  // columns that count
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if ((REV && e < lo) || e > hi) s[e] = 0u;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      pk[e] = tc::pack_bf16x2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+  }
+  ht::tmem_st(to, pk);
+}
+
+// 32 values times f
+__device__ __forceinline__ void times(uint32_t (&v)[32], float f) {
+  const uint64_t ff = pack2(f, f);
+#pragma unroll
+  for (int e = 0; e < 32; e += 2) {
+    const float2 y = unpack2(ht::fmul2(ht::pair(v[e], v[e + 1]), ff));
+    v[e] = __float_as_uint(y.x);
+    v[e + 1] = __float_as_uint(y.y);
+  }
+}
+
 // D[tmem] (+)= C^T B over 128 rows; both tiles by rows (MN-major operands)
 __device__ __forceinline__ void issue_state(uint32_t tmem_d, uint64_t dc, uint64_t db,
                                             uint32_t idesc, bool add) {
@@ -136,43 +254,67 @@ __device__ __forceinline__ void issue_state(uint32_t tmem_d, uint64_t dc, uint64
                  idesc, add || ks > 0);
 }
 
-struct DtShared {
-  uint64_t full_ab[2], full_c[2], empty[2];
-  uint64_t pdone, s16, o1done, oscaled, conv, udone, pready[2], pvdone, ofree, drain;
-  uint32_t tmem;
-  int abort_flag;
-  alignas(16) float steps[2][16];  // powers inside a group of 16 columns, by head of the unit
+// C[tmem_d] += A . B^T, as ht::issue_scores
+template <int NKS, int RB>
+__device__ __forceinline__ void issue_scores_add(uint32_t tmem_d, uint64_t da, uint64_t db,
+                                                 uint32_t idesc) {
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks)
+    tc::mma_bf16(tmem_d, da + ht::kstep(ks, 128), db + ht::kstep(ks, RB), idesc, true);
+}
+
+// Shared memory: a and b of two chunks, c of one (two with two heads a unit,
+// whose state is half as large), the state's copy in two parts.
+template <bool PAIR>
+struct DtPlan {
+  static constexpr int CS = PAIR ? 2 : 1;
+  static constexpr int COPY = PAIR ? DT_HALF : DT_TILE;
+  static constexpr int AT_C = 4 * DT_TILE, AT_COPY = AT_C + CS * DT_TILE;
+  static constexpr int SMEM = AT_COPY + 2 * COPY + 1024;
 };
 
-constexpr int dt_smem(bool pair) { return 6 * DT_TILE + (pair ? DT_HALF : DT_TILE) + 1024; }
+struct DtShared {
+  // by chunk, in turn of two: pdone[c & 1] is P of chunk c, and so on
+  uint64_t full_ab[2], empty_ab[2], full_c[2], empty_c[2], pdone[2], conv[2];
+  uint64_t pready[2];  // by chunk, with two heads by head
+  uint64_t s16, o1done, oscaled, udone, pvdone, ofree, drain;
+  uint32_t tmem;
+  int abort_flag;
+};
 
-template <int NKS, bool PAIR>
+template <int NKS, bool PAIR, bool REV, bool WIDE>
 __global__ void __launch_bounds__(DT_THREADS, 1)
     decay_rows_tc_kernel(const __grid_constant__ CUtensorMap ma,
                          const __grid_constant__ CUtensorMap mb,
-                         const __grid_constant__ CUtensorMap mc, DecayParams p, DtGrid g) {
-  constexpr int HEADS = PAIR ? 2 : 1;
+                         const __grid_constant__ CUtensorMap mc,
+                         const __grid_constant__ CUtensorMap mo, DecayParams p, DtGrid g) {
+  using Plan = DtPlan<PAIR>;
+  constexpr int HEADS = PAIR ? 2 : 1, CS = Plan::CS;
   extern __shared__ unsigned char dt_raw[];
   __shared__ DtShared sh;
   const uint32_t base = (tc::smem_addr(dt_raw) + 1023u) & ~1023u;
-  const uint32_t s16 = base + 6 * DT_TILE;
+  const uint32_t copy = base + Plan::AT_COPY;
+  auto tile_a = [&](uint32_t c) { return base + (c & 1) * 2 * DT_TILE; };
+  auto tile_b = [&](uint32_t c) { return base + (c & 1) * 2 * DT_TILE + DT_TILE; };
+  auto tile_c = [&](uint32_t c) { return base + Plan::AT_C + (c % CS) * DT_TILE; };
   volatile int* abort_flag = &sh.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       tc::mbar_init(&sh.full_ab[s], 1);
       tc::mbar_init(&sh.full_c[s], 1);
-      tc::mbar_init(&sh.empty[s], 1);
+      tc::mbar_init(&sh.empty_ab[s], 8);
+      tc::mbar_init(&sh.empty_c[s], 1);
+      tc::mbar_init(&sh.pdone[s], 1);
+      tc::mbar_init(&sh.conv[s], 8);
       tc::mbar_init(&sh.pready[s], 8 / HEADS);
     }
-    tc::mbar_init(&sh.pdone, 1);
     tc::mbar_init(&sh.o1done, 1);
     tc::mbar_init(&sh.udone, 1);
     tc::mbar_init(&sh.pvdone, 1);
     tc::mbar_init(&sh.drain, 1);
     tc::mbar_init(&sh.s16, 8);
     tc::mbar_init(&sh.oscaled, 8);
-    tc::mbar_init(&sh.conv, 8);
     tc::mbar_init(&sh.ofree, 8);
     sh.abort_flag = 0;
     tc::mbar_init_fence();
@@ -182,32 +324,37 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = sh.tmem, t_out = tmem + 256, t_state = tmem + 384;
+  // P of a chunk: the unit's heads side by side, or two chunks in turn
+  auto tmem_p = [&](uint32_t c, int u) { return tmem + (PAIR ? u : (int)(c & 1)) * 128; };
   // does a unit's first chunk start from a state?
   auto starts = [&](const DtUnit& w) { return p.part ? w.seg > 0 || p.start : p.start != nullptr; };
 
   if (warp == DT_TMA_WARP) {
     if (lane == 0) {
-      uint32_t c = 0;
+      uint32_t c = 0, cc = 0;  // copies of a and b, of c
       for (int k = 0, unit = blockIdx.x; unit < g.units; unit += gridDim.x, ++k) {
         if (ht::gives_up(ht::ROLE_LOADER, k)) {
           *abort_flag = 1;
           break;
         }
         const DtUnit w = dt_unit<PAIR>(p, g, unit);
-        for (int x = w.a0; x < w.a1; ++x, ++c) {
+        for (int x = w.a0; x < w.a1; ++x) {
           const int s = c & 1, row = dt_chunk(p, g, x) * DT_T;
-          if (!ws::wait(&sh.empty[s], ((c >> 1) & 1) ^ 1, abort_flag)) goto tma_done;
-          const uint32_t at = base + s * 3 * DT_TILE;
+          if (!ws::wait(&sh.empty_ab[s], ((c >> 1) & 1) ^ 1, abort_flag)) goto tma_done;
           ht::expect_tx(&sh.full_ab[s], 2 * DT_TILE);
-          dt_load<PAIR>(at, &ma, &sh.full_ab[s], p, w, p.ga, row);
-          dt_load<PAIR>(at + DT_TILE, &mb, &sh.full_ab[s], p, w, p.gb, row);
-          ht::expect_tx(&sh.full_c[s], DT_TILE);
-          dt_load<PAIR>(at + 2 * DT_TILE, &mc, &sh.full_c[s], p, w, p.gc, row);
+          dt_load<PAIR>(tile_a(c), &ma, &sh.full_ab[s], p, w, p.ga, row);
+          dt_load<PAIR>(tile_b(c), &mb, &sh.full_ab[s], p, w, p.gb, row);
+          ++c;
+          const int t = cc % CS;
+          if (!ws::wait(&sh.empty_c[t], ((cc / CS) & 1) ^ 1, abort_flag)) goto tma_done;
+          ht::expect_tx(&sh.full_c[t], DT_TILE);
+          dt_load<PAIR>(tile_c(cc), &mc, &sh.full_c[t], p, w, p.gc, row);
+          ++cc;
         }
       }
     tma_done:
       ht::drain_copies(sh.full_ab, 2, c);
-      ht::drain_copies(sh.full_c, 2, c);
+      ht::drain_copies(sh.full_c, CS, cc);
     }
     __syncwarp();
   } else if (warp == DT_MMA_WARP) {
@@ -221,47 +368,61 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
     auto wait = [&](uint64_t& bar, uint32_t parity) {
       ok = ok && ht::wait_at(tc::smem_addr(&bar), parity, abort_flag);
     };
+    // have a and b of chunk c_ landed?
+    auto landed = [&](uint32_t c_) {
+      return __all_sync(0xffffffffu, ws::test(&sh.full_ab[c_ & 1], (c_ >> 1) & 1));
+    };
+    auto form_p = [&](uint32_t c_) {  // P of chunk c_
+      wait(sh.full_ab[c_ & 1], (c_ >> 1) & 1);
+      tc::fence_after_sync();
+      if (ok && leader) {
+#pragma unroll
+        for (int u = 0; u < HEADS; ++u)
+          ht::issue_scores<NKS, 128>(tmem_p(c_, u), ht::desc128(tile_a(c_) + u * DT_HALF, 16),
+                                     ht::desc128(tile_b(c_) + u * DT_HALF, 16), id_p);
+        ht::commit_at(tc::smem_addr(&sh.pdone[c_ & 1]));
+      }
+      __syncwarp();
+    };
     for (int unit = blockIdx.x; unit < g.units && ok; unit += gridDim.x) {
       const DtUnit w = dt_unit<PAIR>(p, g, unit);
+      bool formed = false;
       for (int x = w.a0; x < w.a1 && ok; ++x, ++c) {
         const bool state = x > w.a0 || starts(w);
-        const uint32_t s = c & 1, ph = (c >> 1) & 1, odd = c & 1;
-        const uint32_t at = base + s * 3 * DT_TILE;
-        const uint64_t da = ht::desc128(at, 16), db = ht::desc128(at + DT_TILE, 16);
-        const uint64_t dc = ht::desc128(at + 2 * DT_TILE, DT_HALF);
-        wait(sh.full_ab[s], ph);
-        tc::fence_after_sync();
-        if (ok && leader) {
-#pragma unroll
-          for (int u = 0; u < HEADS; ++u)
-            ht::issue_scores<NKS, 128>(tmem + u * 128, da + u * (DT_HALF >> 4),
-                                       db + u * (DT_HALF >> 4), id_p);
-          ht::commit_at(tc::smem_addr(&sh.pdone));
-        }
-        __syncwarp();
+        const uint32_t odd = c & 1, ph = (c >> 1) & 1;
+        if (!formed) form_p(c);
+        formed = false;
         wait(sh.ofree, odd ^ 1);  // the rows of the chunk before are out
         if (state) {
           wait(sh.s16, states & 1);
           tc::fence_after_sync();
           if (ok && leader) {
 #pragma unroll
-            for (int u = 0; u < HEADS; ++u)
-              ht::issue_scores<NKS, 128>(t_out + u * 64, da + u * (DT_HALF >> 4),
-                                         ht::desc128(s16 + u * 64 * 128, 16), id_1);
+            for (int u = 0; u < HEADS; ++u) {
+              const uint64_t da = ht::desc128(tile_a(c) + u * DT_HALF, 16);
+              const uint32_t at = copy + u * 64 * 128;
+              ht::issue_scores<NKS, 128>(t_out + u * 64, da, ht::desc128(at, 16), id_1);
+              issue_scores_add<NKS, 128>(t_out + u * 64, da, ht::desc128(at + Plan::COPY, 16), id_1);
+            }
             ht::commit_at(tc::smem_addr(&sh.o1done));
           }
           __syncwarp();
         }
-        wait(sh.full_c[s], ph);
-        wait(sh.conv, odd);
+        wait(sh.full_c[c % CS], (c / CS) & 1);
+        wait(sh.conv[odd], ph);
         tc::fence_after_sync();
+        const uint64_t dc = ht::desc128(tile_c(c), DT_HALF);
         if (x + 1 < w.a1) {
           if (ok && leader) {
-            issue_state(t_state, dc, ht::desc128(at + DT_TILE, DT_HALF), id_s, state);
-            issue_state(t_state, dc, ht::desc128(at, DT_HALF), id_s, true);
+            issue_state(t_state, dc, ht::desc128(tile_b(c), DT_HALF), id_s, state);
             ht::commit_at(tc::smem_addr(&sh.udone));
           }
           __syncwarp();
+        }
+        // one head: the next chunk's P goes ahead of this one's P c
+        if (!PAIR && x + 1 < w.a1 && landed(c + 1)) {
+          form_p(c + 1);
+          formed = true;
         }
         if (state) {
           wait(sh.oscaled, states & 1);
@@ -269,23 +430,23 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
         }
 #pragma unroll
         for (int u = 0; u < HEADS; ++u) {
-          wait(sh.pready[u], odd);
+          wait(sh.pready[PAIR ? u : odd], PAIR ? odd : ph);
           tc::fence_after_sync();
           if (ok && leader)
-            ht::issue_aggregate<DT_T, 64>(t_out + u * 64, tmem + u * 128,
-                                          dc + u * (DT_HALF >> 4), id_2, state);
+            ht::issue_aggregate<DT_T, 64>(t_out + u * 64, tmem_p(c, u), dc + u * (DT_HALF >> 4),
+                                          id_2, state);
           __syncwarp();
         }
         if (ok && leader) {
           ht::commit_at(tc::smem_addr(&sh.pvdone));
-          ht::commit_at(tc::smem_addr(&sh.empty[s]));
+          ht::commit_at(tc::smem_addr(&sh.empty_c[c % CS]));
         }
         ok = ht::agree(ok);
       }
     }
-    // the last commits land before the block ends
-    for (uint32_t i = c > 2 ? c - 2 : 0; i < c && ok; ++i)
-      ok = ht::wait_at(tc::smem_addr(&sh.empty[i & 1]), (i >> 1) & 1, abort_flag);
+    // the last products are done before the block ends
+    if (c > 0 && ok)
+      ok = ht::wait_at(tc::smem_addr(&sh.empty_c[(c - 1) % CS]), ((c - 1) / CS) & 1, abort_flag);
     if (!ht::agree(ok)) ht::drain_products(&sh.drain, leader);
     __syncwarp();
   } else if (warp >= DT_W0 && warp < DT_W0 + 8) {
@@ -295,9 +456,25 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
     const int half = (warp - DT_W0) >> 2, i = threadIdx.x & 127, w0 = (warp & 3) * 32;
     const uint32_t lane_off = (uint32_t)w0 << 16;
     const int c_lo = PAIR ? 0 : half * 64, c_n = max(0, min(64, p.d - c_lo));
-    float* steps = sh.steps[half];
-    bool ok = true;
+    // The tile that holds the rows of chunk c - 1 may be loaded again once they
+    // have been read: asked for only when the next chunk is under way.
+    bool held = false;
     uint32_t c = 0;
+    auto release = [&] {
+      if (held && lane == 0) {
+        stores_read();
+        ws::arrive(&sh.empty_ab[(c - 1) & 1]);
+      }
+      held = false;
+      __syncwarp();
+    };
+    // the rows have been read from TMEM
+    auto rows_free = [&] {
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) ws::arrive(&sh.ofree);
+    };
+    bool ok = true;
     for (int k = 0, unit = blockIdx.x; unit < g.units; unit += gridDim.x, ++k) {
       const DtUnit w = dt_unit<PAIR>(p, g, unit);
       if (ht::gives_up(ht::ROLE_WEIGHTS, k)) {
@@ -307,122 +484,91 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       const int h = PAIR ? min(w.h + half, p.H - 1) : w.h;
       const bool mine = !PAIR || w.h + half < p.H;
       const float l2 = decay_rate(p.log_decay, h) * DT_LOG2E;
-      asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
-      if (i < 16) steps[i] = power(l2, p.reverse ? i : 15 - i);
-      asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+      uint64_t steps[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        steps[e] = REV ? pack2(power(l2, 2 * e), power(l2, 2 * e + 1))
+                             : pack2(power(l2, 15 - 2 * e), power(l2, 14 - 2 * e));
       for (int x = w.k0; x < w.k1; ++x) {
-        const int chunk = dt_chunk(p, g, x), row = chunk * DT_T + i;
+        const int chunk = dt_chunk(p, g, x);
         const bool live = x >= w.a0 && x < w.a1;
         const int n = live ? dt_rows(w, chunk) : 0;
         if (live) {
-          if (ok) ok = ht::warp_wait(&sh.pdone, c & 1, abort_flag);
+          if (ok) ok = ht::warp_wait(&sh.pdone[c & 1], (c >> 1) & 1, abort_flag);
           tc::fence_after_sync();
 #pragma unroll 1
-          for (int piece = 0; piece < HEADS; ++piece) {
-            const int j0 = PAIR ? piece * 64 : half * 64;
-            const uint32_t t_p = tmem + (PAIR ? half * 128 : 0) + j0 + lane_off;
-            uint32_t pk[32];
-            if (p.reverse ? w0 > j0 + 63 || j0 >= n : w0 + 31 < j0) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) pk[e] = 0u;
-            } else {
-              uint32_t s[64];
-              ht::tmem_ld(t_p, s);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const int jb = j0 + 16 * q;
-                if (p.reverse ? jb >= w0 + 31 && jb + 15 < n : w0 >= jb + 15) {
-                  const float f = p.in_scale * power(l2, p.reverse ? jb - i : i - jb - 15);
-                  const uint64_t ff = pack2(f, f);
-#pragma unroll
-                  for (int e = 0; e < 16; e += 4) {
-                    const float4 t = *reinterpret_cast<const float4*>(steps + e);
-                    const float2 y = unpack2(ht::fmul2(ht::fmul2(pack2(t.x, t.y), ff),
-                                                       ht::pair(s[16 * q + e], s[16 * q + e + 1])));
-                    const float2 z = unpack2(ht::fmul2(ht::fmul2(pack2(t.z, t.w), ff),
-                                                       ht::pair(s[16 * q + e + 2], s[16 * q + e + 3])));
-                    pk[8 * q + e / 2] = tc::pack_bf16x2(y.x, y.y);
-                    pk[8 * q + e / 2 + 1] = tc::pack_bf16x2(z.x, z.y);
-                  }
-                } else if (p.reverse ? jb + 15 < w0 || jb >= n : w0 + 31 < jb) {
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) pk[8 * q + e] = 0u;
-                } else {
-#pragma unroll
-                  for (int e = 0; e < 16; e += 2) {
-                    float y[2];
-#pragma unroll
-                    for (int v = 0; v < 2; ++v) {
-                      const int j = jb + e + v, gap = p.reverse ? j - i : i - j;
-                      const bool see = gap >= 0 && (!p.reverse || j < n);
-                      y[v] = see ? __uint_as_float(s[16 * q + e + v]) * p.in_scale *
-                                       power(l2, max(gap, 0))
-                                 : 0.f;
-                    }
-                    pk[8 * q + e / 2] = tc::pack_bf16x2(y[0], y[1]);
-                  }
-                }
-              }
-            }
-            ht::tmem_st(t_p, pk);
+          for (int j0 = PAIR ? 0 : half * 64, q = 0; q < 2 * HEADS; ++q, j0 += 32) {
+            if (q == HEADS) release();
+            weigh<REV>(tmem_p(c, half) + lane_off, j0, i, w0, n, l2, p.in_scale, steps);
           }
           ht::st_wait();
           tc::fence_before_sync();
           __syncwarp();
-          if (ok && lane == 0) ws::arrive(&sh.pready[PAIR ? half : 0]);
+          if (ok && lane == 0) ws::arrive(&sh.pready[PAIR ? half : c & 1]);
           if (ok) ok = ht::warp_wait(&sh.pvdone, c & 1, abort_flag);
           tc::fence_after_sync();
           ++c;
         }
-        const bool store = mine && row < p.N;
-        const int64_t at = (((int64_t)w.b * p.N + row) * p.H + h) * p.d + c_lo;
-        const float f = !ok ? __int_as_float(0x7fffffff) : p.out_scale;
-        const bool zero = ok && i >= n;
-#pragma unroll 1
-        for (int cc = 0; cc < c_n; cc += 32) {
+        const int64_t first = (((int64_t)w.b * p.N + chunk * DT_T + w0) * p.H + h) * p.d + c_lo;
+        const int left = mine ? p.N - chunk * DT_T - w0 : 0;  // rows of this warp to write
+        if (live && ok) {
+          // through shared memory (the chunk's a has been used), so that a
+          // store takes whole lines
+          const uint32_t stage = tile_a(c - 1) + (warp - DT_W0) * 4096;
           uint32_t o[32];
-          if (live) ht::tmem_ld(t_out + half * 64 + cc + lane_off, o);
-          if (!live || zero) {
+          auto part = [&](int col) {
+            ht::tmem_ld(t_out + half * 64 + col + lane_off, o);
+            times(o, p.out_scale);
+            if (n < DT_T && i >= n) {  // padding
 #pragma unroll
-            for (int u = 0; u < 32; ++u) o[u] = 0u;
-          }
-          if (store) {
-            if (p.out_f32) {
-              float* dst = static_cast<float*>(p.out) + at + cc;
-#pragma unroll
-              for (int u = 0; u < 32; u += 4)
-                if (cc + u < c_n)
-                  *reinterpret_cast<float4*>(dst + u) =
-                      make_float4(__uint_as_float(o[u]) * f, __uint_as_float(o[u + 1]) * f,
-                                  __uint_as_float(o[u + 2]) * f, __uint_as_float(o[u + 3]) * f);
-            } else {
-              __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + at + cc;
-#pragma unroll
-              for (int u = 0; u < 32; u += 8)
-                if (cc + u < c_n)
-                  *reinterpret_cast<uint4*>(dst + u) = make_uint4(
-                      scaled_f32(o[u], o[u + 1], f), scaled_f32(o[u + 2], o[u + 3], f),
-                      scaled_f32(o[u + 4], o[u + 5], f), scaled_f32(o[u + 6], o[u + 7], f));
+              for (int e = 0; e < 32; ++e) o[e] = 0u;
             }
+          };
+          auto store = [&](int col) {
+            tc::fence_async_smem();
+            __syncwarp();
+            if (lane == 0 && left > 0) store_box(&mo, stage, c_lo + col, h, chunk * DT_T + w0, w.b);
+            __syncwarp();
+          };
+          part(0);
+          if constexpr (!WIDE) {
+            stage_row(stage, lane, 0, o);
+            part(32);
+            stage_row(stage, lane, 4, o);
+            rows_free();
+            if (c_n > 0) store(0);
+          } else {
+            stage_row32(stage, lane, o);
+            if (c_n > 0) store(0);
+            part(32);
+            rows_free();
+            if (lane == 0) stores_read();
+            __syncwarp();
+            stage_row32(stage, lane, o);
+            if (c_n > 32) store(32);
           }
-          __syncwarp();
-        }
-        if (live) {
-          tc::fence_before_sync();
-          __syncwarp();
-          if (ok && lane == 0) ws::arrive(&sh.ofree);
+          held = true;
+        } else {
+          // padding, or rows given up
+          if constexpr (WIDE)
+            fill_rows(static_cast<float*>(p.out) + first, ok ? 0u : 0x7fffffffu, lane, left,
+                      (int64_t)p.H * p.d, c_n, 4);
+          else
+            fill_rows(static_cast<__nv_bfloat16*>(p.out) + first, ok ? 0u : 0x7fff7fffu, lane, left,
+                      (int64_t)p.H * p.d, c_n, 8);
         }
       }
     }
+    release();
   } else if (warp >= DT_W0 + 8) {
     // ---------------- the state ----------------
     const int half = (warp - DT_W0 - 8) >> 2, r = threadIdx.x & 127;
     const int tid = threadIdx.x - (DT_W0 + 8) * 32;  // 0 .. 255
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    // this thread's part of S: row r (a column of c), SN columns (of b)
-    constexpr int SP = PAIR ? 1 : 2;  // pieces of 32 columns
+    // this thread's part of S: row r (a column of c), from column s_col on
+    constexpr int SP = PAIR ? 1 : 2;  // pieces of 32 columns (of b)
     const int s_head = PAIR ? r >> 6 : 0;
-    const int s_col = half * (PAIR ? 32 : 64);  // first column inside the head
+    const int s_col = half * (PAIR ? 32 : 64);  // inside the head
     const uint32_t t_s = t_state + (PAIR ? s_head * 64 : 0) + s_col + lane_off;
     const uint32_t t_o = t_out + half * 64 + lane_off;
     bool ok = true;
@@ -438,13 +584,60 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       if (starts(w))
         start = (p.part ? p.part + (int64_t)w.seg * p.B * p.H * p.d * p.d : p.start) +
                 ((int64_t)w.b * p.H + hs) * p.d * p.d;
+      // weights of a whole chunk; a chunk of fewer rows makes its own
+      float f0[4], f1[4];
+      auto weights = [&](int n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = (tid >> 3) + 32 * e, to = max(0, REV ? row + 1 : n - 1 - row);
+          f0[e] = p.in_scale * power(l2_0, to);
+          f1[e] = PAIR ? p.in_scale * power(l2_1, to) : 0.f;
+        }
+      };
+      weights(DT_T);
+      const float whole = power(l2_s, DT_T), row_whole = power(l2_o, REV ? DT_T - 1 - r : r + 1);
+      // b of chunk c_, the unit's x_, weighted in place once P is formed
+      auto convert = [&](uint32_t c_, int x_) {
+        const int n = dt_rows(w, dt_chunk(p, g, x_));
+        if (ok) ok = ht::warp_wait(&sh.full_ab[c_ & 1], (c_ >> 1) & 1, abort_flag);
+        if (ok) ok = ht::warp_wait(&sh.pdone[c_ & 1], (c_ >> 1) & 1, abort_flag);
+        if (x_ + 1 < w.a1) {
+          if (n < DT_T) weights(n);
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const uint32_t at = tile_b(c_) + hf * DT_HALF + tid * 16;
+            uint4 v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = ld_piece(at + e * 4096);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              st_piece(at + e * 4096, weighted(v[e], PAIR && hf ? f1[e] : f0[e]));
+          }
+          if (n < DT_T) {
+            weights(DT_T);
+#pragma unroll 1
+            for (int piece = tid; piece < 2048; piece += 256)
+              if (((piece & 1023) >> 3) >= n) st_shared_zero16(tile_b(c_) + piece * 16);
+          }
+        }
+        if (n < DT_T && w.len < p.N) {
+          // rows from the length on may hold anything: those of c become zero
+          if (ok) ok = ht::warp_wait(&sh.full_c[c_ % CS], (c_ / CS) & 1, abort_flag);
+#pragma unroll 1
+          for (int piece = tid; piece < 2048; piece += 256)
+            if (((piece & 1023) >> 3) >= n) st_shared_zero16(tile_c(c_) + piece * 16);
+        }
+        tc::fence_async_smem();
+        __syncwarp();
+        if (ok && lane == 0) ws::arrive(&sh.conv[c_ & 1]);
+      };
+      if (!PAIR && w.a0 < w.a1) convert(c, w.a0);
       for (int x = w.a0; x < w.a1; ++x, ++c) {
         const int chunk = dt_chunk(p, g, x), n = dt_rows(w, chunk);
         const bool state = x > w.a0 || start;
-        const uint32_t at = base + (c & 1) * 3 * DT_TILE;
         if (state) {
           // the state before this chunk: its copy, and what the product adds to
-          const float all = power(l2_s, n);
+          const float all = n < DT_T ? power(l2_s, n) : whole;
           if (x > w.a0) {
             if (ok) ok = ht::warp_wait(&sh.udone, us & 1, abort_flag);
             ++us;
@@ -466,17 +659,22 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
                           : 0u;
               }
             }
-            const uint32_t row = s16 + (PAIR ? 0 : (b0 >> 6) * DT_HALF) + r * 128;
+            const uint32_t row = copy + (PAIR ? 0 : (b0 >> 6) * DT_HALF) + r * 128;
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
-              st_piece(row + (((((b0 & 63) + e) >> 3) ^ (r & 7)) << 4),
-                       make_uint4(scaled_f32(s[e], s[e + 1], 1.f), scaled_f32(s[e + 2], s[e + 3], 1.f),
-                                  scaled_f32(s[e + 4], s[e + 5], 1.f),
-                                  scaled_f32(s[e + 6], s[e + 7], 1.f)));
+              uint32_t hi[4], lo[4];
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                float y = __uint_as_float(s[e + 2 * v]), z = __uint_as_float(s[e + 2 * v + 1]);
+                hi[v] = split_off(y, z);
+                lo[v] = tc::pack_bf16x2(y, z);
+              }
+              const uint32_t to = row + (((((b0 & 63) + e) >> 3) ^ (r & 7)) << 4);
+              st_piece(to, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+              st_piece(to + Plan::COPY, make_uint4(lo[0], lo[1], lo[2], lo[3]));
             }
             if (x + 1 < w.a1) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * all);
+              times(s, all);
               ht::tmem_st(t_s + 32 * q, s);
             }
           }
@@ -486,52 +684,17 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           __syncwarp();
           if (ok && lane == 0) ws::arrive(&sh.s16);
         }
-        // b, weighted, in two parts: over b and over a, once P and a S are formed
-        if (ok) ok = ht::warp_wait(&sh.full_ab[c & 1], (c >> 1) & 1, abort_flag);
-        if (ok) ok = ht::warp_wait(&sh.pdone, c & 1, abort_flag);
+        if (PAIR) convert(c, x);
         if (state) {
           if (ok) ok = ht::warp_wait(&sh.o1done, states & 1, abort_flag);
           ++states;
-        }
-        if (x + 1 < w.a1) {
-#pragma unroll 4
-          for (int e = 0; e < 8; ++e) {
-            const int piece = tid + 256 * e, row = (piece & 1023) >> 3;
-            const float l2 = PAIR && e >= 4 ? l2_1 : l2_0;
-            const float f = row < n ? p.in_scale * power(l2, p.reverse ? row + 1 : n - 1 - row) : 0.f;
-            const uint4 v = ld_piece(at + DT_TILE + piece * 16);
-            const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float y = lo_half(in[i]) * f, z = hi_half(in[i]) * f;
-              if (row >= n) y = z = 0.f;
-              hi[i] = split_off(y, z);
-              lo[i] = tc::pack_bf16x2(y, z);
-            }
-            st_piece(at + DT_TILE + piece * 16, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-            st_piece(at + piece * 16, make_uint4(lo[0], lo[1], lo[2], lo[3]));
-          }
-        }
-        if (n < DT_T && w.len < p.N) {
-          // rows from the length on may hold anything: those of c become zero
-          if (ok) ok = ht::warp_wait(&sh.full_c[c & 1], (c >> 1) & 1, abort_flag);
-#pragma unroll 1
-          for (int piece = tid; piece < 2048; piece += 256)
-            if (((piece & 1023) >> 3) >= n) st_shared_zero16(at + 2 * DT_TILE + piece * 16);
-        }
-        tc::fence_async_smem();
-        __syncwarp();
-        if (ok && lane == 0) ws::arrive(&sh.conv);
-        if (state) {
           tc::fence_after_sync();
-          const float f = power(l2_o, max(0, p.reverse ? n - 1 - r : r + 1));
+          const float f = REV && n < DT_T ? power(l2_o, max(0, n - 1 - r)) : row_whole;
 #pragma unroll 1
           for (int q = 0; q < 2; ++q) {
             uint32_t o[32];
             ht::tmem_ld(t_o + 32 * q, o);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            times(o, f);
             ht::tmem_st(t_o + 32 * q, o);
           }
           ht::st_wait();
@@ -539,6 +702,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           __syncwarp();
           if (ok && lane == 0) ws::arrive(&sh.oscaled);
         }
+        if (!PAIR && x + 1 < w.a1) convert(c + 1, x + 1);
       }
     }
   }
@@ -552,11 +716,11 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
 // ---------------------------------------------------------------------------
 template <int PLANES>
 struct DsTcPlan {
-  static constexpr int NS = 2;
-  // places of the lower parts; with two, a chunk is split while the product of
-  // the one before runs
-  static constexpr int LOW = PLANES == 2 ? 2 : 1;
-  static constexpr int SMEM = (2 * NS + LOW * (PLANES - 1)) * DT_TILE + 1024;
+  static constexpr int NS = PLANES == 1 ? 3 : 2;
+  // The lower parts have one place: a chunk is split after the product of the
+  // one before. Without them it is weighted while that product runs.
+  static constexpr bool AHEAD = PLANES == 1;
+  static constexpr int SMEM = (2 * NS + PLANES - 1) * DT_TILE + 1024;
 };
 template <int NS>
 struct DsTcShared {
@@ -569,7 +733,8 @@ template <bool PAIR, int PLANES>
 __global__ void __launch_bounds__(DT_THREADS, 1)
     decay_state_tc_kernel(const __grid_constant__ CUtensorMap mb,
                           const __grid_constant__ CUtensorMap mc, DecayParams p, DtGrid g) {
-  constexpr int NS = DsTcPlan<PLANES>::NS, LOW = DsTcPlan<PLANES>::LOW;
+  constexpr int NS = DsTcPlan<PLANES>::NS;
+  constexpr bool AHEAD = DsTcPlan<PLANES>::AHEAD;
   extern __shared__ unsigned char dt_raw[];
   __shared__ DsTcShared<NS> sh;
   const uint32_t base = (tc::smem_addr(dt_raw) + 1023u) & ~1023u;
@@ -633,8 +798,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           issue_state(d, dc, ht::desc128(at, DT_HALF), id_s, false);
 #pragma unroll
           for (int q = 1; q < PLANES; ++q)
-            issue_state(d, dc, ht::desc128(extra + ((c % LOW) + q - 1) * DT_TILE, DT_HALF), id_s,
-                        true);
+            issue_state(d, dc, ht::desc128(extra + (q - 1) * DT_TILE, DT_HALF), id_s, true);
           ht::commit_at(tc::smem_addr(&sh.udone[c & 1]));
           ht::commit_at(tc::smem_addr(&sh.empty[s]));
         }
@@ -677,7 +841,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       int n_before = 0;
       for (int x = w.a0; x < w.a1; ++x, ++c) {
         const int n = dt_rows(w, dt_chunk(p, g, x)), s = c % NS;
-        if (LOW == 1 && x > w.a0) take(c - 1, n_before);
+        if (!AHEAD && x > w.a0) take(c - 1, n_before);
         if (ok) ok = ht::warp_wait(&sh.full[s], (c / NS) & 1, abort_flag);
         const uint32_t at = base + s * 2 * DT_TILE;
 #pragma unroll
@@ -698,14 +862,14 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           st_piece(at + piece * 16, make_uint4(part[0][0], part[0][1], part[0][2], part[0][3]));
 #pragma unroll
           for (int q = 1; q < PLANES; ++q)
-            st_piece(extra + ((c % LOW) + q - 1) * DT_TILE + piece * 16,
+            st_piece(extra + (q - 1) * DT_TILE + piece * 16,
                      make_uint4(part[q][0], part[q][1], part[q][2], part[q][3]));
           if (row >= n && w.len < p.N) st_shared_zero16(at + DT_TILE + piece * 16);
         }
         tc::fence_async_smem();
         __syncwarp();
         if (ok && lane == 0) ws::arrive(&sh.conv);
-        if (LOW == 2 && x > w.a0) take(c - 1, n_before);
+        if (AHEAD && x > w.a0) take(c - 1, n_before);
         n_before = n;
       }
       if (w.a1 > w.a0) take(c - 1, n_before);
@@ -740,14 +904,21 @@ int dt_blocks(const DtGrid& g) {
   return g.units < sms ? g.units : sms;
 }
 
-template <int NKS, bool PAIR>
+template <int NKS, bool PAIR, bool REV, bool WIDE>
 cudaError_t rows_go(const CUtensorMap* m, const DecayParams& p, const DtGrid& g, cudaStream_t s) {
-  constexpr int SMEM = dt_smem(PAIR);
-  const void* fn = reinterpret_cast<const void*>(&decay_rows_tc_kernel<NKS, PAIR>);
+  constexpr int SMEM = DtPlan<PAIR>::SMEM;
+  const void* fn = reinterpret_cast<const void*>(&decay_rows_tc_kernel<NKS, PAIR, REV, WIDE>);
   const cudaError_t e = raise_smem_limit(fn, SMEM);
   if (e != cudaSuccess) return e;
-  decay_rows_tc_kernel<NKS, PAIR><<<dt_blocks(g), DT_THREADS, SMEM, s>>>(m[0], m[1], m[2], p, g);
+  decay_rows_tc_kernel<NKS, PAIR, REV, WIDE>
+      <<<dt_blocks(g), DT_THREADS, SMEM, s>>>(m[0], m[1], m[2], m[3], p, g);
   return cudaGetLastError();
+}
+template <int NKS, bool PAIR>
+cudaError_t rows_way(const CUtensorMap* m, const DecayParams& p, const DtGrid& g, cudaStream_t s) {
+  if (!p.reverse) return rows_go<NKS, PAIR, false, false>(m, p, g, s);
+  return p.out_f32 ? rows_go<NKS, PAIR, true, true>(m, p, g, s)
+                   : rows_go<NKS, PAIR, true, false>(m, p, g, s);
 }
 template <bool PAIR, int PLANES>
 cudaError_t state_go(const CUtensorMap* m, const DecayParams& p, const DtGrid& g, cudaStream_t s) {
@@ -794,19 +965,21 @@ cudaError_t launch_decay_states_tc(const DecayParams& p, cudaStream_t s) {
   CUtensorMap m[2];
   if (!map_of(&m[0], p, p.b, p.sb, p.gb) || !map_of(&m[1], p, p.c, p.sc, p.gc))
     return cudaErrorInvalidValue;
-  if (p.d <= 64) return p.planes > 2 ? state_go<true, 3>(m, p, g, s) : state_go<true, 2>(m, p, g, s);
-  return p.planes > 2 ? state_go<false, 3>(m, p, g, s) : state_go<false, 2>(m, p, g, s);
+  if (p.d <= 64) return p.planes > 2 ? state_go<true, 3>(m, p, g, s) : state_go<true, 1>(m, p, g, s);
+  return p.planes > 2 ? state_go<false, 3>(m, p, g, s) : state_go<false, 1>(m, p, g, s);
 }
 
 cudaError_t launch_decay_rows_tc(const DecayParams& p, cudaStream_t s) {
-  CUtensorMap m[3];
+  CUtensorMap m[4];
+  const HeadStrides so = {(int64_t)p.N * p.H * p.d, (int64_t)p.H * p.d, p.d};
   if (!map_of(&m[0], p, p.a, p.sa, p.ga) || !map_of(&m[1], p, p.b, p.sb, p.gb) ||
-      !map_of(&m[2], p, p.c, p.sc, p.gc))
+      !map_of(&m[2], p, p.c, p.sc, p.gc) ||
+      !head_box_map(&m[3], p.out, so, p.B, p.N, p.H, p.d, p.out_f32, 32))
     return cudaErrorInvalidValue;
   const DtGrid g = dt_grid(p, p.segs);
-  if (p.d <= 64) return rows_go<4, true>(m, p, g, s);
-  if (p.d <= 96) return rows_go<6, false>(m, p, g, s);
-  return rows_go<8, false>(m, p, g, s);
+  if (p.d <= 64) return rows_way<4, true>(m, p, g, s);
+  if (p.d <= 96) return rows_way<6, false>(m, p, g, s);
+  return rows_way<8, false>(m, p, g, s);
 }
 
 }  // namespace tarmac

@@ -459,33 +459,38 @@ static EncodeTiledFn encode_fn() {
 
 // strides of the heads, rows and episodes in bytes; false where TMA cannot
 // take them
-static bool map_strides(const HeadStrides& s, int B, int N, int h, cuuint64_t (&bytes)[3]) {
+static bool map_strides(const HeadStrides& s, int B, int N, int h, int es, cuuint64_t (&bytes)[3]) {
   const int64_t st[3] = {s.h, s.n, s.b};
   const int size[3] = {h, N, B};
   for (int i = 0; i < 3; ++i) {
     // the stride of a dimension of one is never used
-    const int64_t e = size[i] == 1 ? 8 : st[i];
-    if (e <= 0 || e % 8 || e * 2 >= ((int64_t)1 << 40)) return false;
-    bytes[i] = (cuuint64_t)(e * 2);
+    const int64_t e = size[i] == 1 ? 16 / es : st[i];
+    if (e <= 0 || e * es % 16 || e * es >= ((int64_t)1 << 40)) return false;
+    bytes[i] = (cuuint64_t)(e * es);
   }
   return true;
 }
 bool head_map_ok(const HeadStrides& s, int B, int N, int h) {
   cuuint64_t bytes[3];
-  return map_strides(s, B, N, h, bytes);
+  return map_strides(s, B, N, h, 2, bytes);
+}
+
+bool head_box_map(CUtensorMap* map, const void* ptr, const HeadStrides& s, int B, int N, int h,
+                  int d, bool f32, int box_rows) {
+  const EncodeTiledFn fn = encode_fn();
+  cuuint64_t bytes[3];
+  if (!fn || (uintptr_t)ptr % 16 || !map_strides(s, B, N, h, f32 ? 4 : 2, bytes)) return false;
+  const cuuint64_t size[4] = {(cuuint64_t)d, (cuuint64_t)h, (cuuint64_t)N, (cuuint64_t)B};
+  const cuuint32_t box[4] = {f32 ? 32u : 64u, 1, (cuuint32_t)box_rows, 1}, one[4] = {1, 1, 1, 1};
+  return fn(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+            const_cast<void*>(ptr), size, bytes, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 bool head_tensor_map(CUtensorMap* map, const void* ptr, const HeadStrides& s, int B, int N, int h,
                      int d) {
-  const EncodeTiledFn fn = encode_fn();
-  cuuint64_t bytes[3];
-  if (!fn || (uintptr_t)ptr % 16 || !map_strides(s, B, N, h, bytes)) return false;
-  const cuuint64_t size[4] = {(cuuint64_t)d, (cuuint64_t)h, (cuuint64_t)N, (cuuint64_t)B};
-  const cuuint32_t box[4] = {64, 1, ht::BOX_ROWS, 1}, one[4] = {1, 1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), size, bytes, box,
-            one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return head_box_map(map, ptr, s, B, N, h, d, false, ht::BOX_ROWS);
 }
 
 template <int NKS>

@@ -291,5 +291,8 @@ __device__ __forceinline__ uint32_t key_word(int j0, int jlim, int self, uint32_
 bool head_map_ok(const HeadStrides& s, int B, int N, int h);
 bool head_tensor_map(CUtensorMap* map, const void* ptr, const HeadStrides& s, int B, int N, int h,
                      int d);
+// The same for bf16 or fp32 with boxes of 128 bytes by `box_rows` rows.
+bool head_box_map(CUtensorMap* map, const void* ptr, const HeadStrides& s, int B, int N, int h,
+                  int d, bool f32, int box_rows);
 
 }  // namespace tarmac
