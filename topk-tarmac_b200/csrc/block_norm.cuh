@@ -18,7 +18,7 @@ struct NormParams {
   RowStrides sx, sy, sg, sdh, sdz;
   const float *w_post, *w_pre, *scale;      // [D] or NULL (ones)
   float *dw_post, *dw_pre, *dscale;         // [D] or NULL
-  float* work;                    // backward: [blocks][3][D] sums
+  float* work;                    // backward: [blocks][2][D] sums
   int B, N, D;
   float eps;
 };

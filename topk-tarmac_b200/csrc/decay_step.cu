@@ -15,10 +15,15 @@ namespace tarmac {
 
 namespace {
 
-// DP columns: LPR lanes a row, RG rows a warp at once, WARPS warps a head
+constexpr int DS_ROWS = 8;  // the most that a call has here
+
+// DP columns, CB of them a block: LPR lanes a row, RG rows a warp at once, WARPS
+// warps a head. A block of all 128 columns holds 64 KB at once and was slower
+// (512 x 16 heads: 231 us).
 template <int DP>
 struct DsPlan {
-  static constexpr int LPR = DP / 4, RG = 32 / LPR;
+  static constexpr int CB = DP == 128 ? 64 : DP;
+  static constexpr int LPR = CB / 4, RG = 32 / LPR;
   static constexpr int WARPS = DP == 128 ? 8 : (DP == 64 ? 4 : 1);
   static constexpr int RPT = DP / (RG * WARPS);
   static constexpr int HEADS = WARPS == 1 ? 4 : 1;  // heads of a block
@@ -36,17 +41,48 @@ __device__ __forceinline__ float4 columns(const T* p, int c, int d, bool vec) {
   return x;
 }
 
-template <typename T, int DP>
+// four columns of a row of S, streamed past the caches' reuse
+__device__ __forceinline__ float4 load_state(const float* src, int c, int d, bool vec) {
+  if (vec) return c < d ? __ldcs(reinterpret_cast<const float4*>(src + c))
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 x;
+  x.x = c < d ? src[c] : 0.f;
+  x.y = c + 1 < d ? src[c + 1] : 0.f;
+  x.z = c + 2 < d ? src[c + 2] : 0.f;
+  x.w = c + 3 < d ? src[c + 3] : 0.f;
+  return x;
+}
+__device__ __forceinline__ void store_state(float* dst, float4 x, int c, int d, bool vec) {
+  if (vec) {
+    if (c < d) __stcs(reinterpret_cast<float4*>(dst + c), x);
+    return;
+  }
+  if (c < d) dst[c] = x.x;
+  if (c + 1 < d) dst[c + 1] = x.y;
+  if (c + 2 < d) dst[c + 2] = x.z;
+  if (c + 3 < d) dst[c + 3] = x.w;
+}
+
+// ONE: a single row. With several, the rows' values are staged first, all
+// loads in flight together, and their sums over S's rows meet at the end.
+template <typename T, int DP, bool ONE>
 __global__ void __launch_bounds__(DsPlan<DP>::THREADS) decay_step_kernel(DecayParams p,
                                                                          int vec_state) {
   using Plan = DsPlan<DP>;
   constexpr int RPT = Plan::RPT, WARPS = Plan::WARPS, RG = Plan::RG, LPR = Plan::LPR;
-  __shared__ float4 sums[WARPS > 1 ? WARPS : 1][LPR];
+  constexpr int CB = Plan::CB, ROWS = ONE ? 1 : DS_ROWS, HEADS = Plan::HEADS;
+  __shared__ float4 sums[WARPS > 1 ? ROWS : 1][WARPS > 1 ? WARPS : 1][LPR];
+  __shared__ float qk[ONE ? 1 : HEADS][ONE ? 1 : 2 * ROWS][DP];
+  __shared__ float4 vs[ONE ? 1 : HEADS][ROWS][LPR];
   const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % WARPS;
-  const int64_t bh = (int64_t)blockIdx.x * Plan::HEADS + (threadIdx.x >> 5) / WARPS;
+  const int own = (threadIdx.x >> 5) / WARPS;  // head of the block
+  const int tid = threadIdx.x % (WARPS * 32);
+  constexpr int PARTS = DP / CB;  // neighbouring blocks share a head
+  const int64_t bh = (int64_t)(blockIdx.x / PARTS) * HEADS + own;
   if (bh >= (int64_t)p.B * p.H) return;  // whole warps; such blocks have no barriers
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);
-  const int c = (lane % LPR) * 4, row0 = warp * RG + lane / LPR;  // rows row0 + i RG WARPS
+  const int c0 = (int)(blockIdx.x % PARTS) * CB, c = c0 + (lane % LPR) * 4;
+  const int row0 = warp * RG + lane / LPR;  // rows row0 + i RG WARPS
   const int len = decay_len(p, b);
   const float l = expf(decay_rate(p.log_decay, h));
   const int64_t base = bh * p.d * p.d;
@@ -54,42 +90,71 @@ __global__ void __launch_bounds__(DsPlan<DP>::THREADS) decay_step_kernel(DecayPa
 #pragma unroll
   for (int i = 0; i < RPT; ++i) {
     const int r = row0 + i * RG * WARPS;
-    S[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (p.start && r < p.d) {
-      const float* src = p.start + base + (int64_t)r * p.d;
-      if (vec_state) {
-        if (c < p.d) S[i] = *reinterpret_cast<const float4*>(src + c);
-      } else {
-        if (c < p.d) S[i].x = src[c];
-        if (c + 1 < p.d) S[i].y = src[c + 1];
-        if (c + 2 < p.d) S[i].z = src[c + 2];
-        if (c + 3 < p.d) S[i].w = src[c + 3];
-      }
-    }
+    S[i] = p.start && r < p.d ? load_state(p.start + base + (int64_t)r * p.d, c, p.d, vec_state)
+                              : make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const T* q = static_cast<const T*>(p.a) + b * p.sa.b + (h / p.ga) * p.sa.h;
   const T* k = static_cast<const T*>(p.b) + b * p.sb.b + (h / p.gb) * p.sb.h;
   const T* v = static_cast<const T*>(p.c) + b * p.sc.b + (h / p.gc) * p.sc.h;
   T* out = static_cast<T*>(p.out) + ((int64_t)b * p.N * p.H + h) * p.d;
-  for (int t = 0; t < p.N; ++t, q += p.sa.n, k += p.sb.n, v += p.sc.n,
-           out += (int64_t)p.H * p.d) {
+  auto meet = [] {
+    if constexpr (WARPS > 1)
+      __syncthreads();
+    else
+      __syncwarp();
+  };
+  if constexpr (!ONE) {
+    for (int e = tid; e < len * DP; e += WARPS * 32) {
+      const int t = e / DP, r = e % DP;
+      qk[own][2 * t][r] = r < p.d ? to_f32<T>(q[t * p.sa.n + r]) : 0.f;
+      qk[own][2 * t + 1][r] = r < p.d ? to_f32<T>(k[t * p.sb.n + r]) : 0.f;
+    }
+    for (int e = tid; e < len * LPR; e += WARPS * 32)
+      vs[own][e / LPR][e % LPR] =
+          columns<T>(v + e / LPR * p.sc.n, c0 + e % LPR * 4, p.d, p.vec);
+    meet();
+  }
+  auto write = [&](int t, int slot, float4 o) {
+    const float y[4] = {o.x * p.out_scale, o.y * p.out_scale, o.z * p.out_scale,
+                        o.w * p.out_scale};
+    T* dst = out + (int64_t)t * p.H * p.d + c0 + slot * 4;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (c0 + slot * 4 + u < p.d) dst[u] = from_f32<T>(y[u]);
+  };
+  const int rows = ONE ? 1 : p.N;
+  for (int t = 0; t < rows; ++t) {
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     if (t < len) {
-      const float4 vv = columns<T>(v, c, p.d, p.vec);
+      const float4 vv = ONE ? columns<T>(v, c, p.d, p.vec) : vs[ONE ? 0 : own][t][lane % LPR];
 #pragma unroll
       for (int i = 0; i < RPT; ++i) {
         const int r = row0 + i * RG * WARPS;
-        const float kk = r < p.d ? to_f32<T>(k[r]) : 0.f, qq = r < p.d ? to_f32<T>(q[r]) : 0.f;
+        float kk, qq;
+        if constexpr (ONE) {
+          kk = r < p.d ? to_f32<T>(k[r]) : 0.f;
+          qq = r < p.d ? to_f32<T>(q[r]) : 0.f;
+        } else {
+          qq = qk[own][2 * t][r];
+          kk = qk[own][2 * t + 1][r];
+        }
         S[i].x = fmaf(l, S[i].x, kk * vv.x);
         S[i].y = fmaf(l, S[i].y, kk * vv.y);
         S[i].z = fmaf(l, S[i].z, kk * vv.z);
         S[i].w = fmaf(l, S[i].w, kk * vv.w);
-        if (r < p.d) {
+        if (r < p.d) {  // rows beyond d are not there, even times an infinity
           o.x = fmaf(qq, S[i].x, o.x);
           o.y = fmaf(qq, S[i].y, o.y);
           o.z = fmaf(qq, S[i].z, o.z);
           o.w = fmaf(qq, S[i].w, o.w);
         }
+      }
+    }
+    if (p.last && t + 1 == rows) {
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) {
+        const int r = row0 + i * RG * WARPS;
+        if (r < p.d) store_state(p.last + base + (int64_t)r * p.d, S[i], c, p.d, vec_state);
       }
     }
 #pragma unroll
@@ -99,42 +164,27 @@ __global__ void __launch_bounds__(DsPlan<DP>::THREADS) decay_step_kernel(DecayPa
       o.z += __shfl_xor_sync(0xffffffffu, o.z, s);
       o.w += __shfl_xor_sync(0xffffffffu, o.w, s);
     }
-    if constexpr (WARPS > 1) {
-      if (t > 0) __syncthreads();  // the sums of the row before have been read
-      if (lane < LPR) sums[warp][lane] = o;
-      __syncthreads();
-      if (warp == 0 && lane < LPR) {
-#pragma unroll
-        for (int w = 1; w < WARPS; ++w) {
-          const float4 x = sums[w][lane];
-          o.x += x.x;
-          o.y += x.y;
-          o.z += x.z;
-          o.w += x.w;
-        }
-      }
-    }
-    if (warp == 0 && lane < LPR) {
-      const float y[4] = {o.x * p.out_scale, o.y * p.out_scale, o.z * p.out_scale,
-                          o.w * p.out_scale};
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (c + u < p.d) out[c + u] = from_f32<T>(y[u]);
+    if (lane < LPR) {
+      if constexpr (WARPS > 1)
+        sums[t][warp][lane] = o;
+      else
+        write(t, lane, o);
     }
   }
-  if (!p.last) return;
+  if constexpr (WARPS > 1) {
+    __syncthreads();
+    for (int e = tid; e < rows * LPR; e += WARPS * 32) {
+      const int t = e / LPR, slot = e % LPR;
+      float4 o = sums[t][0][slot];
 #pragma unroll
-  for (int i = 0; i < RPT; ++i) {
-    const int r = row0 + i * RG * WARPS;
-    if (r >= p.d) continue;
-    float* dst = p.last + base + (int64_t)r * p.d;
-    if (vec_state) {
-      if (c < p.d) *reinterpret_cast<float4*>(dst + c) = S[i];
-    } else {
-      if (c < p.d) dst[c] = S[i].x;
-      if (c + 1 < p.d) dst[c + 1] = S[i].y;
-      if (c + 2 < p.d) dst[c + 2] = S[i].z;
-      if (c + 3 < p.d) dst[c + 3] = S[i].w;
+      for (int w = 1; w < WARPS; ++w) {
+        const float4 x = sums[t][w][slot];
+        o.x += x.x;
+        o.y += x.y;
+        o.z += x.z;
+        o.w += x.w;
+      }
+      write(t, slot, o);
     }
   }
 }
@@ -143,9 +193,12 @@ template <typename T, int DP>
 cudaError_t step_go(const DecayParams& p, cudaStream_t s) {
   using Plan = DsPlan<DP>;
   const int64_t heads = (int64_t)p.B * p.H;
-  const unsigned blocks = (unsigned)((heads + Plan::HEADS - 1) / Plan::HEADS);
+  const unsigned blocks = (unsigned)((heads + Plan::HEADS - 1) / Plan::HEADS) * (DP / Plan::CB);
   const int vec_state = p.d % 4 == 0 && (uintptr_t)p.start % 16 == 0 && (uintptr_t)p.last % 16 == 0;
-  decay_step_kernel<T, DP><<<blocks, Plan::THREADS, 0, s>>>(p, vec_state);
+  if (p.N == 1)
+    decay_step_kernel<T, DP, true><<<blocks, Plan::THREADS, 0, s>>>(p, vec_state);
+  else
+    decay_step_kernel<T, DP, false><<<blocks, Plan::THREADS, 0, s>>>(p, vec_state);
   return cudaGetLastError();
 }
 template <typename T>
@@ -158,7 +211,7 @@ cudaError_t step_width(const DecayParams& p, cudaStream_t s) {
 
 }  // namespace
 
-bool decay_step_takes(int N) { return N <= 8; }
+bool decay_step_takes(int N) { return N <= DS_ROWS; }
 
 cudaError_t launch_decay_step(const DecayParams& p, bool bf16, cudaStream_t s) {
   return bf16 ? step_width<__nv_bfloat16>(p, s) : step_width<float>(p, s);
