@@ -1,5 +1,5 @@
 // decay.cuh — parameters of attention with a decay for each head
-// (decay_attn.cu, decay_step.cu) and how a call is divided.
+// (decay_tc.cu, decay_scan.cu, decay_step.cu) and how a call is divided.
 //
 // Every direction is one form over rows, with l the decay of a head:
 //   out_i = sum_{j <= i} l^(i-j) (a_i . b_j) c_j + l^(i+1) a_i . S,
@@ -16,9 +16,11 @@ namespace tarmac {
 
 struct DecayParams {
   const void *a, *b, *c;
-  void* out;                 // [B, N, H, d] contiguous, or NULL: states only
-  HeadStrides sa, sb, sc;
-  int ga, gb, gc;            // heads that share one head of a, b, c
+  const void* e;             // multiplies S from the other side (decay_one_walk)
+  void* out;                 // [B, N, H, d] contiguous: S^T a
+  void* row_out;             // the same: S e, or NULL
+  HeadStrides sa, sb, sc, se;
+  int ga, gb, gc, ge;        // heads that share one head of a, b, c, e
   int out_f32;               // out is fp32 (backwards only), else the rows' type
   const float* log_decay;    // [H]
   const int32_t* lens;       // [B] or NULL
@@ -27,14 +29,14 @@ struct DecayParams {
   float* part;               // [segs, B, H, d, d], or NULL (decay_uses_part)
   int B, N, H, d;
   int segs, seg_chunks;      // parts of the row axis and their chunks
+  int joined;                // decay_one_walk: a launch joins the segments' states
   int reverse;               // rows run from the last to the first
   int transposed;            // state tensors are [columns of c, columns of b]
   float in_scale;            // factor of every b_j c_j term
   float out_scale;           // factor of out
-  int planes;                // bf16 parts of the weighted rows that enter S
+  int planes;                // tensor memory: bf16 parts of the weighted rows that enter S
   int tc;                    // runs on the tensor memory (decay_tc.cu)
-  int vec;                   // 16-byte rows in a, b, c
-  int vec_out;               // and in out
+  int vec;                   // 16-byte rows in a, b, c, e
 };
 
 // Powers of a decay: exp(rate e). A decay of zero (rate -inf) keeps l^0 = 1.
@@ -46,8 +48,8 @@ __device__ __forceinline__ int decay_len(const DecayParams& p, int b) {
   return p.lens ? max(0, min(__ldg(p.lens + b), p.N)) : p.N;
 }
 
-constexpr int DECAY_CHUNK = 64;      // rows of a chunk, warp-level kernel
-constexpr int DECAY_TC_CHUNK = 128;  // and of one on the tensor memory
+constexpr int DECAY_CHUNK = 16;      // rows that segments are counted in
+constexpr int DECAY_TC_CHUNK = 128;  // and a chunk's on the tensor memory
 
 struct DecayPlan {
   int segs, seg_chunks;
@@ -56,6 +58,12 @@ DecayPlan decay_plan(int B, int N, int H, int d, bool tc);
 DecayPlan decay_plan_tc(int B, int N, int H, int d);
 // may a call of these sizes run on the tensor memory?
 bool decay_tc_sizes(int B, int N, int H, int d, bool bf16);
+// Do the gradients take one walk each way (dq as row_out; dv and dk as out and
+// row_out of one walk)? Else each is an out of its own, dq and dk with the state
+// transposed.
+bool decay_one_walk(int d, bool tc);
+// bytes of p.part, where the call uses it
+int64_t decay_part_bytes(const DecayPlan& g, int B, int H, int d, bool tc);
 // Does the call keep states in p.part? (On the tensor memory the state after
 // the last row comes from the segments' states, else from the rows' kernel.)
 inline bool decay_uses_part(const DecayPlan& g, bool tc, bool last) {

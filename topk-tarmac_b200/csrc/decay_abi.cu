@@ -64,15 +64,19 @@ void set_plan(DecayParams& p, bool tc) {
   p.segs = g.segs;
   p.seg_chunks = g.seg_chunks;
   p.tc = tc;
+  // the rows' kernel joins few segments itself, in less than a launch takes
+  p.joined = p.segs > 24;
 }
 // bytes of p.part, whichever kernels the rows' layout allows
 int64_t part_bytes(int B, int N, int H, int d, bool bf16, bool last) {
-  int64_t parts = 0;
+  int64_t bytes = 0;
   for (int tc = 0; tc <= (int)decay_tc_sizes(B, N, H, d, bf16); ++tc) {
     const DecayPlan g = decay_plan(B, N, H, d, tc != 0);
-    if (decay_uses_part(g, tc != 0, last) && g.segs > parts) parts = g.segs;
+    if (!decay_uses_part(g, tc != 0, last)) continue;
+    const int64_t n = decay_part_bytes(g, B, H, d, tc != 0);
+    if (n > bytes) bytes = n;
   }
-  return parts * B * H * d * d * 4;
+  return bytes;
 }
 
 // one operand: pointer, strides and how many heads share one of its heads
@@ -98,6 +102,13 @@ void set_operands(DecayParams& p, const Operand& a, const Operand& b, const Oper
   p.gb = b.share;
   p.gc = c.share;
   p.vec = a.vec && b.vec && c.vec;
+}
+
+void set_extra(DecayParams& p, const Operand& x) {
+  p.e = x.ptr;
+  p.se = x.s;
+  p.ge = x.share;
+  p.vec = p.vec && x.vec;
 }
 
 // no rows: the state stays as it was
@@ -186,7 +197,7 @@ int tarmac_decay_attention(const void* q, const void* k, const void* v, void* ou
     if (!work) return TARMAC_ERR_NULL;
     p.part = static_cast<float*>(work);
   }
-  p.planes = state_out ? 3 : (p.tc ? 1 : 2);
+  p.planes = state_out ? 3 : 1;
   cudaError_t e = launch_decay_states(p, bf16, s);
   if (e == cudaSuccess) e = launch_decay_rows(p, bf16, s);
   return status(e);
@@ -196,9 +207,9 @@ int64_t tarmac_decay_attention_backward_workspace(int B, int N, int H, int Hk, i
                                                   int dstate) {
   if (check_sizes(B, N, H, Hk, d, dtype) != TARMAC_OK || B < 1 || N < 1) return 0;
   const int64_t parts = part_bytes(B, N, H, d, dtype == TARMAC_BF16, dstate != 0);
-  // gradients of shared heads by query head, before their sum
-  const int64_t shared = H == Hk ? 0 : (int64_t)B * N * H * d * 4;
-  return round16(parts) + shared;
+  // gradients of shared heads by query head, before their sum: dk and dv
+  const int64_t shared = H == Hk ? 0 : round16((int64_t)B * N * H * d * 4);
+  return round16(parts) + 2 * shared;
 }
 
 int tarmac_decay_attention_backward(const void* q, const void* k, const void* v, const void* dout,
@@ -234,24 +245,30 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
   auto run = [&](cudaError_t (*launch)(const DecayParams&, bool, cudaStream_t)) {
     if (e == cudaSuccess) e = launch(p, bf16, s);
   };
+  const bool one_walk = decay_one_walk(d, p.tc);
   // dq_i = scale S_i dout_i, S over the rows as in the forward pass
   p.start = state;
   p.part = decay_uses_part(plan, p.tc, false) ? static_cast<float*>(work) : nullptr;
-  p.planes = p.tc ? 1 : 2;
+  p.planes = 1;
   p.in_scale = 1.f;
   p.out_scale = scale;
   set_operands(p, oq, ok, ov);
   run(launch_decay_states);
-  set_operands(p, og, ov, ok);
-  p.transposed = 1;
-  p.out = dq;
+  if (one_walk) {
+    set_extra(p, og);
+    p.row_out = dq;
+  } else {
+    set_operands(p, og, ov, ok);
+    p.transposed = 1;
+    p.out = dq;
+  }
   run(launch_decay_rows);
   // R_i = sum over the rows from i on of scale q dout^T:
   // dv_i = R_i^T k_i, dk_i = R_i v_i
   p.start = dstate_out;
   p.last = dstate;
   p.part = decay_uses_part(plan, p.tc, dstate) ? static_cast<float*>(work) : nullptr;
-  p.planes = dstate ? 3 : (p.tc ? 1 : 2);
+  p.planes = dstate ? 3 : 1;
   p.reverse = 1;
   p.transposed = 0;
   p.in_scale = scale;
@@ -259,17 +276,24 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
   set_operands(p, ok, oq, og);
   run(launch_decay_states);
   p.out_f32 = G > 1;
-  const int64_t rows = (int64_t)B * N;
-  for (int i = 0; i < 2 && e == cudaSuccess; ++i) {
-    void* to = i == 0 ? dv : dk;
-    p.out = G > 1 ? shared : to;
-    p.last = i == 0 ? dstate : nullptr;
-    if (i == 1) {
-      set_operands(p, ov, og, oq);
-      p.transposed = 1;
-    }
+  float* shared_k = shared + round16((int64_t)B * N * H * d * 4) / 4;
+  p.out = G > 1 ? shared : dv;
+  if (one_walk) {
+    set_extra(p, ov);
+    p.row_out = G > 1 ? shared_k : dk;
     run(launch_decay_rows);
-    if (e == cudaSuccess && G > 1) e = launch_decay_share(shared, to, rows, Hk, G, d, bf16, s);
+  } else {
+    run(launch_decay_rows);
+    set_operands(p, ov, og, oq);
+    p.transposed = 1;
+    p.last = nullptr;
+    p.out = G > 1 ? shared_k : dk;
+    run(launch_decay_rows);
+  }
+  if (G > 1) {
+    const int64_t rows = (int64_t)B * N;
+    if (e == cudaSuccess) e = launch_decay_share(shared, dv, rows, Hk, G, d, bf16, s);
+    if (e == cudaSuccess) e = launch_decay_share(shared_k, dk, rows, Hk, G, d, bf16, s);
   }
   return status(e);
 }

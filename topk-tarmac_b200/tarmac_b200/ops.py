@@ -784,6 +784,9 @@ def _check_state(t, name: str, q: torch.Tensor) -> torch.Tensor | None:
     if t is None:
         return None
     B, _, H, d = q.shape
+    if t.dtype is torch.float32 and t.shape == (B, H, d, d) \
+            and t.get_device() == q.get_device() and t.is_contiguous():
+        return t
     if tuple(t.shape) != (B, H, d, d):
         raise ValueError(f"{name} must be [{B}, {H}, {d}, {d}]; got {tuple(t.shape)}")
     if t.dtype != torch.float32:
@@ -984,6 +987,23 @@ def _check_norm(x, named: dict, weights: dict):
                   for w in weights.values()]
 
 
+def _norm_ready(x, rows, weights) -> bool:
+    """As :func:`_rotate_ready`: may x and the other rows [B, N, D] and the
+    weights be passed on as they are?"""
+    shape, t, dev = x.shape, x.dtype, x.get_device()
+    if len(shape) != 3 or t not in _DTYPES or dev < 0 or x.stride(2) != 1:
+        return False
+    for r in rows:
+        if r is not None and not (r.shape == shape and r.dtype is t
+                                  and r.get_device() == dev and r.stride(2) == 1):
+            return False
+    for w in weights:
+        if w is not None and not (w.dtype is torch.float32 and w.shape == shape[2:]
+                                  and w.get_device() == dev and w.stride(0) == 1):
+            return False
+    return True
+
+
 def _row_strides(t: torch.Tensor | None) -> tuple:
     return (0, 0) if t is None else t.stride()[:2]
 
@@ -1003,9 +1023,12 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor,
     x, y, gate: [..., D] fp32 or bf16 (no gate: ones in place of its sigmoid);
     ``w_post``, ``w_pre``, ``scale``: [D] or None (ones). Returns contiguous (h, z)
     in the inputs' dtype."""
-    (xr, yr, gr), (wo, wi, sc) = _check_norm(
-        x, {"y": y, "gate": gate},
-        {"w_post": w_post, "w_pre": w_pre, "scale": scale})
+    if _norm_ready(x, (y, gate), (w_post, w_pre, scale)):
+        xr, yr, gr, wo, wi, sc = x, y, gate, w_post, w_pre, scale
+    else:
+        (xr, yr, gr), (wo, wi, sc) = _check_norm(
+            x, {"y": y, "gate": gate},
+            {"w_post": w_post, "w_pre": w_pre, "scale": scale})
     h, z = _empty_as(x), _empty_as(x)
     B, N, D = xr.shape
     _launch(x.get_device(), "tarmac_residual_norm", xr.data_ptr(), yr.data_ptr(),
@@ -1031,14 +1054,19 @@ def residual_norm_backward(x: torch.Tensor, y: torch.Tensor,
     its outputs (None: zero): (dx, dy) and dgate in the inputs' dtype and
     (dw_post, dw_pre, dscale) fp32 [D], as (dx, dy, dw_post, dw_pre, dgate,
     dscale), None where the input is. Deterministic."""
-    (xr, yr, gr, hr, zr), (wo, wi, sc) = _check_norm(
-        x, {"y": y, "gate": gate, "dh": dh, "dz": dz},
-        {"w_post": w_post, "w_pre": w_pre, "scale": scale})
+    if _norm_ready(x, (y, gate, dh, dz), (w_post, w_pre, scale)):
+        xr, yr, gr, hr, zr, wo, wi, sc = x, y, gate, dh, dz, w_post, w_pre, scale
+    else:
+        (xr, yr, gr, hr, zr), (wo, wi, sc) = _check_norm(
+            x, {"y": y, "gate": gate, "dh": dh, "dz": dz},
+            {"w_post": w_post, "w_pre": w_pre, "scale": scale})
     B, N, D = xr.shape
     dx, dy = _empty_as(x), _empty_as(x)
     dgate = None if gate is None else _empty_as(x)
-    sums = torch.empty((3, D), device=x.device, dtype=torch.float32)
-    dwo, dwi, dsc = (None if w is None else s for w, s in zip((wo, wi, sc), sums))
+    dwo, dwi, dsc = torch.empty((3, D), device=x.device, dtype=torch.float32)
+    dwo = None if wo is None else dwo
+    dwi = None if wi is None else dwi
+    dsc = None if sc is None else dsc
     work = _scratch(_norm_work(B, N, D), x.device)
     _launch(x.get_device(), "tarmac_residual_norm_backward", xr.data_ptr(),
             yr.data_ptr(), _ptr(gr), _ptr(hr), _ptr(zr),
