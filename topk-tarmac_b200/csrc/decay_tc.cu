@@ -631,7 +631,6 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
         __syncwarp();
         if (ok && lane == 0) ws::arrive(&sh.conv[c_ & 1]);
       };
-      if (!PAIR && w.a0 < w.a1) convert(c, w.a0);
       for (int x = w.a0; x < w.a1; ++x, ++c) {
         const int chunk = dt_chunk(p, g, x), n = dt_rows(w, chunk);
         const bool state = x > w.a0 || start;
@@ -684,7 +683,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           __syncwarp();
           if (ok && lane == 0) ws::arrive(&sh.s16);
         }
-        if (PAIR) convert(c, x);
+        convert(c, x);
         if (state) {
           if (ok) ok = ht::warp_wait(&sh.o1done, states & 1, abort_flag);
           ++states;
@@ -702,7 +701,6 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           __syncwarp();
           if (ok && lane == 0) ws::arrive(&sh.oscaled);
         }
-        if (!PAIR && x + 1 < w.a1) convert(c + 1, x + 1);
       }
     }
   }
