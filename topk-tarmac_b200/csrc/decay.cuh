@@ -29,7 +29,7 @@ struct DecayParams {
   float* part;               // [segs, B, H, d, d], or NULL (decay_uses_part)
   int B, N, H, d;
   int segs, seg_chunks;      // parts of the row axis and their chunks
-  int joined;                // decay_one_walk: a launch joins the segments' states
+  int joined;                // a launch of its own joins the segments' states
   int reverse;               // rows run from the last to the first
   int transposed;            // state tensors are [columns of c, columns of b]
   float in_scale;            // factor of every b_j c_j term

@@ -64,8 +64,13 @@ void set_plan(DecayParams& p, bool tc) {
   p.segs = g.segs;
   p.seg_chunks = g.seg_chunks;
   p.tc = tc;
-  // the rows' kernel joins few segments itself, in less than a launch takes
-  p.joined = p.segs > 24;
+}
+// Does a launch of its own join the segments' states? Up to 32 columns off the
+// tensor memory the rows' kernel joins few of them as it starts, in less than a
+// launch takes (16 states of 16 x 16 a head: 4.8 us). On the tensor memory that
+// was slower (4 of 128 x 128: 26 us more against 9).
+void set_joined(DecayParams& p) {
+  p.joined = !decay_one_walk(p.d, p.tc) || p.segs > 24;
 }
 // bytes of p.part, whichever kernels the rows' layout allows
 int64_t part_bytes(int B, int N, int H, int d, bool bf16, bool last) {
@@ -198,6 +203,7 @@ int tarmac_decay_attention(const void* q, const void* k, const void* v, void* ou
     p.part = static_cast<float*>(work);
   }
   p.planes = state_out ? 3 : 1;
+  set_joined(p);
   cudaError_t e = launch_decay_states(p, bf16, s);
   if (e == cudaSuccess) e = launch_decay_rows(p, bf16, s);
   return status(e);
@@ -253,6 +259,7 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
   p.in_scale = 1.f;
   p.out_scale = scale;
   set_operands(p, oq, ok, ov);
+  set_joined(p);
   run(launch_decay_states);
   if (one_walk) {
     set_extra(p, og);
@@ -274,6 +281,7 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
   p.in_scale = scale;
   p.out_scale = 1.f;
   set_operands(p, ok, oq, og);
+  set_joined(p);
   run(launch_decay_states);
   p.out_f32 = G > 1;
   float* shared_k = shared + round16((int64_t)B * N * H * d * 4) / 4;

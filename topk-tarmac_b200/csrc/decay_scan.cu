@@ -385,33 +385,42 @@ __global__ void __launch_bounds__(SC_WARPS * 32, ScPlan<T, DP>::BLOCKS)
 // part[s] (what segment s adds) becomes the state before segment s:
 //   X_0 = start, X_(s+1) = l^(rows of s) X_s + part[s];
 // p.last, where given, the state after the last one.
-__global__ void __launch_bounds__(256) decay_join_kernel(DecayParams p, int64_t stride, int rows) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// V elements a thread.
+template <int V>
+__global__ void __launch_bounds__(128) decay_join_kernel(DecayParams p, int64_t stride, int rows) {
+  const int64_t e = ((int64_t)blockIdx.x * 128 + threadIdx.x) * V;
   if (e >= stride) return;
-  const int dd = p.d * p.d;
-  const int bh = (int)(e / dd), b = bh / p.H;
+  struct alignas(4 * V) Vec {
+    float x[V];
+  };
+  const unsigned dd = p.d * p.d;
+  const int bh = V == 1 || stride >> 32 ? (int)(e / dd) : (int)((unsigned)e / dd), b = bh / p.H;
   const int len = decay_len(p, b), chunk_rows = p.seg_chunks * rows;
   const int chunks = cdiv(p.N, rows), parts = p.last ? p.segs : p.segs - 1;
   const float rate = decay_rate(p.log_decay, bh % p.H);
-  float x = p.start ? p.start[e] : 0.f;
+  Vec x = {};
+  if (p.start) x = *reinterpret_cast<const Vec*>(p.start + e);
   float* at = p.part + e;
   for (int s0 = 0; s0 < p.segs; s0 += 8) {
-    float add[8];  // eight loads in flight
+    Vec add[8] = {};  // eight loads in flight
 #pragma unroll
-    for (int u = 0; u < 8; ++u) add[u] = s0 + u < parts ? at[(s0 + u) * stride] : 0.f;
+    for (int u = 0; u < 8; ++u)
+      if (s0 + u < parts) add[u] = *reinterpret_cast<const Vec*>(at + (s0 + u) * stride);
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int s = s0 + u;
       if (s >= p.segs) break;
-      at[s * stride] = x;
+      *reinterpret_cast<Vec*>(at + s * stride) = x;
       // rows [t0, t1) of segment s
       const int t0 = p.reverse ? max(0, chunks - (s + 1) * p.seg_chunks) * rows : s * chunk_rows;
       const int t1 = p.reverse ? (chunks - s * p.seg_chunks) * rows : t0 + chunk_rows;
       const int n = max(0, min(len, t1) - t0);
-      x = fmaf(expf(rate * (float)n), x, add[u]);
+      const float all = expf(rate * (float)n);
+#pragma unroll
+      for (int v = 0; v < V; ++v) x.x[v] = fmaf(all, x.x[v], add[u].x[v]);
     }
   }
-  if (p.last) p.last[e] = x;
+  if (p.last) *reinterpret_cast<Vec*>(p.last + e) = x;
 }
 
 // The same for parts as the lanes hold them (pairs; a warp has 512 of each of
@@ -537,8 +546,8 @@ cudaError_t launch_decay_states(const DecayParams& p, bool bf16, cudaStream_t s)
   if (!p.tc) q.last = nullptr;
   const cudaError_t e = p.tc ? launch_decay_states_tc(p, s) : launch_scan(p, SC_STATES, bf16, s);
   if (e != cudaSuccess) return e;
+  if (!p.joined) return e;
   if (decay_one_walk(p.d, p.tc)) {
-    if (!p.joined) return e;
     const int64_t heads = (int64_t)p.B * p.H;
     const int64_t pairs = p.d <= 16 ? (heads + 1) / 2 * 256 : heads * 512;
     decay_join_lanes_kernel<<<(unsigned)((pairs + 255) / 256), 256, 0, s>>>(p, pairs,
@@ -546,8 +555,11 @@ cudaError_t launch_decay_states(const DecayParams& p, bool bf16, cudaStream_t s)
     return cudaGetLastError();
   }
   const int64_t stride = (int64_t)p.B * p.H * p.d * p.d;
-  decay_join_kernel<<<(unsigned)((stride + 255) / 256), 256, 0, s>>>(
-      q, stride, p.tc ? DECAY_TC_CHUNK : DECAY_CHUNK);
+  const int chunk = p.tc ? DECAY_TC_CHUNK : DECAY_CHUNK;
+  if (p.d % 4 == 0 && (uintptr_t)p.start % 16 == 0 && (uintptr_t)q.last % 16 == 0)
+    decay_join_kernel<4><<<(unsigned)((stride / 4 + 127) / 128), 128, 0, s>>>(q, stride, chunk);
+  else
+    decay_join_kernel<1><<<(unsigned)((stride + 127) / 128), 128, 0, s>>>(q, stride, chunk);
   return cudaGetLastError();
 }
 

@@ -837,32 +837,58 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
         tc::fence_before_sync();
       };
       int n_before = 0;
+      // weights of a whole chunk; a chunk of fewer rows makes its own
+      float f[4];
+      auto weights = [&](int n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = ((tid + 512 * e) & 1023) >> 3;
+          f[e] = p.in_scale * power(PAIR && e >= 2 ? l2_1 : l2_0,
+                                    max(0, p.reverse ? row + 1 : n - 1 - row));
+        }
+      };
+      weights(DT_T);
       for (int x = w.a0; x < w.a1; ++x, ++c) {
         const int n = dt_rows(w, dt_chunk(p, g, x)), s = c % NS;
+        if (n < DT_T) weights(n);
         if (!AHEAD && x > w.a0) take(c - 1, n_before);
         if (ok) ok = ht::warp_wait(&sh.full[s], (c / NS) & 1, abort_flag);
         const uint32_t at = base + s * 2 * DT_TILE;
+        uint4 v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = ld_piece(at + (tid + 512 * e) * 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int piece = tid + 512 * e, row = (piece & 1023) >> 3;
-          const float l2 = PAIR && e >= 2 ? l2_1 : l2_0;
-          const float f = row < n ? p.in_scale * power(l2, p.reverse ? row + 1 : n - 1 - row) : 0.f;
-          const uint4 v = ld_piece(at + piece * 16);
-          const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-          uint32_t part[PLANES][4];
+          const int piece = tid + 512 * e;
+          if constexpr (PLANES == 1) {
+            st_piece(at + piece * 16, weighted(v[e], f[e]));
+          } else {
+            const uint32_t in[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
+            uint32_t part[PLANES][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float a = lo_half(in[i]) * f, b = hi_half(in[i]) * f;
-            if (row >= n) a = b = 0.f;
+            for (int i = 0; i < 4; ++i) {
+              float a = lo_half(in[i]) * f[e], b = hi_half(in[i]) * f[e];
 #pragma unroll
-            for (int q = 0; q < PLANES; ++q) part[q][i] = split_off(a, b);
+              for (int q = 0; q < PLANES; ++q) part[q][i] = split_off(a, b);
+            }
+            st_piece(at + piece * 16, make_uint4(part[0][0], part[0][1], part[0][2], part[0][3]));
+#pragma unroll
+            for (int q = 1; q < PLANES; ++q)
+              st_piece(extra + (q - 1) * DT_TILE + piece * 16,
+                       make_uint4(part[q][0], part[q][1], part[q][2], part[q][3]));
           }
-          st_piece(at + piece * 16, make_uint4(part[0][0], part[0][1], part[0][2], part[0][3]));
-#pragma unroll
-          for (int q = 1; q < PLANES; ++q)
-            st_piece(extra + (q - 1) * DT_TILE + piece * 16,
-                     make_uint4(part[q][0], part[q][1], part[q][2], part[q][3]));
-          if (row >= n && w.len < p.N) st_shared_zero16(at + DT_TILE + piece * 16);
+        }
+        if (n < DT_T) {  // rows that are not there, whatever the tiles hold
+          weights(DT_T);
+#pragma unroll 1
+          for (int e = 0; e < 4; ++e) {
+            const int piece = tid + 512 * e;
+            if (((piece & 1023) >> 3) < n) continue;
+            st_shared_zero16(at + piece * 16);
+            for (int q = 1; q < PLANES; ++q)
+              st_shared_zero16(extra + (q - 1) * DT_TILE + piece * 16);
+            if (w.len < p.N) st_shared_zero16(at + DT_TILE + piece * 16);
+          }
         }
         tc::fence_async_smem();
         __syncwarp();
