@@ -188,12 +188,11 @@ def test_layouts(N, d, wrap, dtype):
 @pytest.mark.parametrize("N", [3, 130])
 def test_broadcast_keys(N, dtype):
     """Keys and values of one episode read by all (stride 0)."""
-    from tarmac_b200 import ops
     c = Case(3, N, 2, 2, 32, dtype)
-    k, v = c.k[:1].cuda().expand(3, -1, -1, -1), c.v[:1].cuda().expand(3, -1, -1, -1)
-    q, rate = c.q.cuda(), c.rate.cuda()
-    got = ops.decay_attention(q, k, v, rate)
-    assert torch.equal(got, ops.decay_attention(q, k.contiguous(), v.contiguous(), rate))
+    for i in (1, 2):  # k, v
+        c.clean[i] = c.clean[i][:1].expand(3, -1, -1, -1)
+    c.k, c.v = c.clean[1], c.clean[2]
+    c.check(c.run(lambda t: t[:1].expand(3, -1, -1, -1) if (t[0] == t[1]).all() else t))
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -180,7 +180,8 @@ __global__ void __launch_bounds__(SC_WARPS * 32, ScPlan<T, DP>::BLOCKS)
       }
   }
   if (!STATES && parts) {
-    // joined: the segments before as one; else one after the other
+    // joined: the segments before as one; else one after the other (the loads of
+    // several in flight together spill)
     for (int s = p.joined ? seg : 0; s < (p.joined ? seg + 1 : seg); ++s) {
       const int n = !p.joined ? rows_in(s)
                     : REV     ? max(0, s0 - max(0, end - len))
@@ -529,7 +530,12 @@ DecayPlan decay_plan(int B, int N, int H, int d, bool tc) {
 }
 
 bool decay_tc_sizes(int B, int N, int H, int d, bool bf16) {
-  return bf16 && d > 32 && d % 8 == 0 && N > 64;
+  // Measured, the tensor memory against the recurrent form (us, the forward pass
+  // with the gradients): 2048 heads, d = 64: 16 rows 104 / 102, 32 rows 108 /
+  // 184; d = 128: 16 rows 156 / 342; 4 heads, d = 64: 16 rows 33 / 31, 32 rows
+  // 33 / 49, 64 rows 33 / 104. Narrow: 32 x 4096 rows of 8 heads, d = 32: 435 /
+  // 992; 64 x 4096, d = 16: 808 / 823.
+  return bf16 && d >= 16 && d % 8 == 0 && N >= (d > 64 ? 12 : 24);
 }
 bool decay_one_walk(int d, bool tc) { return !tc && d <= 32; }
 
