@@ -447,6 +447,17 @@ int tarmac_decay_attention_backward(const void *q, const void *k,
                                     void *dq, void *dk, void *dv,
                                     float *dstate, void *work, void *stream);
 
+/* Which kernels such a call (backward 0; state: with a state_out) or its
+ * gradients (1; state: with a dstate) would take: host-only, as
+ * tarmac_kernel_plan below. Pointers are assumed on a 16-byte grid; strides as
+ * for those calls. Writes a NUL-terminated JSON object of at most `len` bytes:
+ * {"kernel": "decay_step", "segments": 1}, the rows one after the other, or
+ * {"kernel": "decay_tc" (tensor memory) or "decay_scan", "segments": n,
+ * "states": true where a launch forms states of segments first}. */
+int tarmac_decay_attention_plan(int backward, const int64_t *strides, int B,
+                                int N, int H, int Hk, int d, int dtype,
+                                int state, char *out, int len);
+
 /* The norms around a block with its gate and residual scale, in one pass. For
  * each row of D columns (D <= 8192) of the stream x, the block's output y and
  * the gate (or NULL: ones in place of its sigmoid),

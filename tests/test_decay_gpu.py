@@ -308,3 +308,39 @@ def test_long_offsets():
     rate = c.rate.cuda()
     want = ops.decay_attention(*(t.cuda() for t in (c.q, c.k, c.v)), rate)
     assert torch.equal(ops.decay_attention(*views, rate), want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,N,H,Hk,d", [(160, 70, 3, 3, 40), (90, 130, 5, 1, 24), (320, 40, 1, 1, 72)])
+def test_many_units(B, N, H, Hk, d, dtype):
+    """More heads than SMs, odd numbers of heads, lengths of every kind: blocks
+    walk over several units."""
+    lens = [(37 * b) % (N + 3) for b in range(B)]
+    c = Case(B, N, H, Hk, d, dtype, state=False, lens=lens)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("N,H,Hk,d", [(260, 4, 2, 64), (260, 3, 1, 16), (390, 2, 2, 128)])
+def test_several_chunks_and_strong_decays(N, H, Hk, d):
+    for decay in ("strong", "ends"):
+        for lens in (None, [N - 130, 1]):
+            c = Case(2, N, H, Hk, d, BF16, lens=lens, decay=decay)
+            c.check(c.run())
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on two streams do not share anything."""
+    from tarmac_b200 import ops
+    cases = [Case(1, 1500, 4, 2, 64, BF16), Case(1, 1500, 4, 2, 32, F32)]
+    for c in cases:
+        args = [t.cuda() for t in (c.q, c.k, c.v, c.rate, c.state)]
+        want = ops.decay_attention(*args, return_state=True)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got += [ops.decay_attention(*args, return_state=True) for _ in range(5)]
+        torch.cuda.synchronize()
+        for out, S in got:
+            assert torch.equal(out, want[0]) and torch.equal(S, want[1])

@@ -306,6 +306,36 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
   return status(e);
 }
 
+int tarmac_decay_attention_plan(int backward, const int64_t* strides, int B, int N, int H, int Hk,
+                                int d, int dtype, int state, char* out, int len) {
+  if (!out || len < 1) return TARMAC_ERR_NULL;
+  out[0] = '\0';
+  const int st = check_sizes(B, N, H, Hk, d, dtype);
+  if (st != TARMAC_OK) return st;
+  const bool bf16 = dtype == TARMAC_BF16;
+  const int es = bf16 ? 2 : 4, G = H / Hk;
+  // only sizes, strides and alignment count: stand-in pointers on the grid
+  const void* a = reinterpret_cast<const void*>((uintptr_t)1 << 20);
+  char buf[128];
+  if (!backward && decay_step_takes(N)) {
+    snprintf(buf, sizeof buf, "{\"kernel\": \"decay_step\", \"segments\": 1}");
+  } else {
+    bool tc = decay_tc_sizes(B, N, H, d, bf16);
+    for (int i = 0; i < 3 + (backward != 0); ++i) {
+      const int share = i == 1 || i == 2 ? G : 1;
+      tc = tc && operand(a, stride_of(strides, i, N, H / share, d), B, N, H, share, d, es).map;
+    }
+    const DecayPlan g = decay_plan(B, N, H, d, tc);
+    snprintf(buf, sizeof buf, "{\"kernel\": \"%s\", \"segments\": %d, \"states\": %s}",
+             tc ? "decay_tc" : "decay_scan", g.segs,
+             decay_uses_part(g, tc, state != 0) ? "true" : "false");
+  }
+  const int n = (int)strlen(buf);
+  if (n + 1 > len) return TARMAC_ERR_SHAPE;
+  memcpy(out, buf, (size_t)n + 1);
+  return TARMAC_OK;
+}
+
 int tarmac_residual_norm(const void* x, const void* y, const void* gate, const int64_t* strides,
                          const float* w_post, const float* w_pre, const float* scale, int B,
                          int N, int D, int dtype, float eps, void* h, void* z, void* stream) {

@@ -495,14 +495,16 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
         const int n = live ? dt_rows(w, chunk) : 0;
         if (live) {
           if (ok) ok = ht::warp_wait(&sh.pdone[c & 1], (c >> 1) & 1, abort_flag);
-          tc::fence_after_sync();
+          if (ok) {
+            tc::fence_after_sync();
 #pragma unroll 1
-          for (int j0 = PAIR ? 0 : half * 64, q = 0; q < 2 * HEADS; ++q, j0 += 32) {
-            if (q == HEADS) release();
-            weigh<REV>(tmem_p(c, half) + lane_off, j0, i, w0, n, l2, p.in_scale, steps);
+            for (int j0 = PAIR ? 0 : half * 64, q = 0; q < 2 * HEADS; ++q, j0 += 32) {
+              if (q == HEADS) release();
+              weigh<REV>(tmem_p(c, half) + lane_off, j0, i, w0, n, l2, p.in_scale, steps);
+            }
+            ht::st_wait();
+            tc::fence_before_sync();
           }
-          ht::st_wait();
-          tc::fence_before_sync();
           __syncwarp();
           if (ok && lane == 0) ws::arrive(&sh.pready[PAIR ? half : c & 1]);
           if (ok) ok = ht::warp_wait(&sh.pvdone, c & 1, abort_flag);
@@ -571,9 +573,10 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
     const int s_col = half * (PAIR ? 32 : 64);  // inside the head
     const uint32_t t_s = t_state + (PAIR ? s_head * 64 : 0) + s_col + lane_off;
     const uint32_t t_o = t_out + half * 64 + lane_off;
+    // a warp that gave up leaves: it must not touch what the others still use
     bool ok = true;
     uint32_t c = 0, states = 0, us = 0;
-    for (int unit = blockIdx.x; unit < g.units; unit += gridDim.x) {
+    for (int unit = blockIdx.x; unit < g.units && ok; unit += gridDim.x) {
       const DtUnit w = dt_unit<PAIR>(p, g, unit);
       const int h0 = w.h, h1 = PAIR ? min(w.h + 1, p.H - 1) : w.h;
       const float l2_0 = decay_rate(p.log_decay, h0) * DT_LOG2E;
@@ -599,8 +602,9 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       // b of chunk c_, the unit's x_, weighted in place once P is formed
       auto convert = [&](uint32_t c_, int x_) {
         const int n = dt_rows(w, dt_chunk(p, g, x_));
-        if (ok) ok = ht::warp_wait(&sh.full_ab[c_ & 1], (c_ >> 1) & 1, abort_flag);
-        if (ok) ok = ht::warp_wait(&sh.pdone[c_ & 1], (c_ >> 1) & 1, abort_flag);
+        ok = ht::warp_wait(&sh.full_ab[c_ & 1], (c_ >> 1) & 1, abort_flag) &&
+             ht::warp_wait(&sh.pdone[c_ & 1], (c_ >> 1) & 1, abort_flag);
+        if (!ok) return;
         if (x_ + 1 < w.a1) {
           if (n < DT_T) weights(n);
 #pragma unroll
@@ -622,14 +626,15 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
         }
         if (n < DT_T && w.len < p.N) {
           // rows from the length on may hold anything: those of c become zero
-          if (ok) ok = ht::warp_wait(&sh.full_c[c_ % CS], (c_ / CS) & 1, abort_flag);
+          ok = ht::warp_wait(&sh.full_c[c_ % CS], (c_ / CS) & 1, abort_flag);
+          if (!ok) return;
 #pragma unroll 1
           for (int piece = tid; piece < 2048; piece += 256)
             if (((piece & 1023) >> 3) >= n) st_shared_zero16(tile_c(c_) + piece * 16);
         }
         tc::fence_async_smem();
         __syncwarp();
-        if (ok && lane == 0) ws::arrive(&sh.conv[c_ & 1]);
+        if (lane == 0) ws::arrive(&sh.conv[c_ & 1]);
       };
       for (int x = w.a0; x < w.a1; ++x, ++c) {
         const int chunk = dt_chunk(p, g, x), n = dt_rows(w, chunk);
@@ -638,7 +643,8 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           // the state before this chunk: its copy, and what the product adds to
           const float all = n < DT_T ? power(l2_s, n) : whole;
           if (x > w.a0) {
-            if (ok) ok = ht::warp_wait(&sh.udone, us & 1, abort_flag);
+            ok = ht::warp_wait(&sh.udone, us & 1, abort_flag);
+            if (!ok) break;
             ++us;
             tc::fence_after_sync();
           }
@@ -681,11 +687,13 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           tc::fence_before_sync();
           tc::fence_async_smem();
           __syncwarp();
-          if (ok && lane == 0) ws::arrive(&sh.s16);
+          if (lane == 0) ws::arrive(&sh.s16);
         }
         convert(c, x);
+        if (!ok) break;
         if (state) {
-          if (ok) ok = ht::warp_wait(&sh.o1done, states & 1, abort_flag);
+          ok = ht::warp_wait(&sh.o1done, states & 1, abort_flag);
+          if (!ok) break;
           ++states;
           tc::fence_after_sync();
           const float f = REV && n < DT_T ? power(l2_o, max(0, n - 1 - r)) : row_whole;
@@ -699,7 +707,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           ht::st_wait();
           tc::fence_before_sync();
           __syncwarp();
-          if (ok && lane == 0) ws::arrive(&sh.oscaled);
+          if (lane == 0) ws::arrive(&sh.oscaled);
         }
       }
     }
@@ -828,6 +836,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       // S = l^n S + the product of chunk c_
       auto take = [&](uint32_t c_, int n) {
         if (ok) ok = ht::warp_wait(&sh.udone[c_ & 1], (c_ >> 1) & 1, abort_flag);
+        if (!ok) return;
         tc::fence_after_sync();
         uint32_t u[SC];
         tmem_ld_n(t_s + (c_ & 1) * 128, u);
@@ -853,6 +862,8 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
         if (n < DT_T) weights(n);
         if (!AHEAD && x > w.a0) take(c - 1, n_before);
         if (ok) ok = ht::warp_wait(&sh.full[s], (c / NS) & 1, abort_flag);
+        // a warp that gave up does not touch what the others still use
+        if (!ok) continue;
         const uint32_t at = base + s * 2 * DT_TILE;
         uint4 v[4];
 #pragma unroll
@@ -892,7 +903,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
         }
         tc::fence_async_smem();
         __syncwarp();
-        if (ok && lane == 0) ws::arrive(&sh.conv);
+        if (lane == 0) ws::arrive(&sh.conv);
         if (AHEAD && x > w.a0) take(c - 1, n_before);
         n_before = n;
       }

@@ -129,6 +129,9 @@ SIGNATURES: dict[str, tuple] = {
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
         c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tarmac_decay_attention_plan": (c_int, [
+        c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+        c_char_p, c_int]),
     "tarmac_residual_norm": (c_int, [
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
         c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p]),

@@ -876,7 +876,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     the last row) with ``return_state`` or a ``state_out`` to write it to: a
     contiguous tensor like ``state``, or ``state`` itself, renewed in place.
     Rows from ``lens`` [B] on are padding, whatever they hold: they get 0 and
-    leave S alone. One new row over a kept state is N = 1."""
+    leave S alone; those before must be finite (a head's infinity may reach its
+    rows as a NaN). One new row over a kept state is N = 1."""
     if not _decay_ready(q, k, v, log_decay, lens):
         q, k, v, log_decay, lens = _check_decay(q, k, v, log_decay, lens)
     start = _check_state(state, "state", q)
@@ -935,6 +936,22 @@ def decay_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             Hk, d, _DTYPES[q.dtype], _scale(d, scale), dq.data_ptr(),
             dk.data_ptr(), dv.data_ptr(), _ptr(first), _ptr(work))
     return dq, dk, dv, first
+
+
+def decay_attention_plan(B: int, N: int, H: int, Hk: int, d: int,
+                         dtype: torch.dtype = torch.float32, state: bool = False,
+                         backward: bool = False) -> dict:
+    """The kernels a contiguous :func:`decay_attention` call (or its gradients)
+    with these shapes takes, e.g. {"kernel": "decay_tc", "segments": 4, "states":
+    True}; ``state``: with a state returned (a gradient of the one given).
+    Host-only (no GPU needed); raises :class:`TarmacError` for arguments the
+    call itself would reject."""
+    import ctypes
+    import json
+    buf = ctypes.create_string_buffer(128)
+    _lib.call("tarmac_decay_attention_plan", int(backward), None, B, N, H, Hk, d,
+              _DTYPES[dtype], int(state), buf, len(buf))
+    return json.loads(buf.value.decode())
 
 
 # ---------------------------------------------------------------------------
