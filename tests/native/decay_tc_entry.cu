@@ -39,7 +39,7 @@ ENTRY rows(const void* a, const void* b, const void* c, const float* log_decay, 
            int N, int H, int d, void* stream) {
   DecayParams p = params(a, b, c, log_decay, B, N, H, d);
   p.out = out;
-  return (int)launch_decay_rows_tc(p, (cudaStream_t)stream);
+  return (int)launch_decay_rows_tc(&p, 1, (cudaStream_t)stream);
 }
 
 // what the rows add to the state

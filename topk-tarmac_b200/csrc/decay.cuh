@@ -54,8 +54,9 @@ constexpr int DECAY_TC_CHUNK = 128;  // and a chunk's on the tensor memory
 struct DecayPlan {
   int segs, seg_chunks;
 };
-DecayPlan decay_plan(int B, int N, int H, int d, bool tc);
-DecayPlan decay_plan_tc(int B, int N, int H, int d);
+// jobs: sums over the same rows that a launch on the tensor memory takes
+DecayPlan decay_plan(int B, int N, int H, int d, bool tc, int jobs);
+DecayPlan decay_plan_tc(int B, int N, int H, int d, int jobs);
 // may a call of these sizes run on the tensor memory?
 bool decay_tc_sizes(int B, int N, int H, int d, bool bf16);
 // Do the gradients take one walk each way (dq as row_out; dv and dk as out and
@@ -76,7 +77,7 @@ inline bool decay_uses_part(const DecayPlan& g, bool tc, bool last) {
 cudaError_t launch_decay_states(const DecayParams& p, bool bf16, cudaStream_t s);
 cudaError_t launch_decay_rows(const DecayParams& p, bool bf16, cudaStream_t s);
 cudaError_t launch_decay_states_tc(const DecayParams& p, cudaStream_t s);
-cudaError_t launch_decay_rows_tc(const DecayParams& p, cudaStream_t s);
+cudaError_t launch_decay_rows_tc(const DecayParams* p, int jobs, cudaStream_t s);
 // few rows, one after the other (forward only)
 bool decay_step_takes(int N);
 cudaError_t launch_decay_step(const DecayParams& p, bool bf16, cudaStream_t s);

@@ -15,6 +15,7 @@ bool head_map_ok(const HeadStrides& s, int B, int N, int h);
 namespace {
 
 constexpr int MAX_D = 128;
+constexpr int GRADIENTS = 3;  // sums of a backward call: dq, dv, dk
 
 bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 int status(cudaError_t e) { return e == cudaSuccess ? TARMAC_OK : TARMAC_ERR_LAUNCH; }
@@ -59,8 +60,8 @@ int fill_decay(DecayParams& p, const void* q, const void* k, const void* v,
   return TARMAC_OK;
 }
 
-void set_plan(DecayParams& p, bool tc) {
-  const DecayPlan g = decay_plan(p.B, p.N, p.H, p.d, tc);
+void set_plan(DecayParams& p, bool tc, int jobs) {
+  const DecayPlan g = decay_plan(p.B, p.N, p.H, p.d, tc, jobs);
   p.segs = g.segs;
   p.seg_chunks = g.seg_chunks;
   p.tc = tc;
@@ -72,16 +73,27 @@ void set_plan(DecayParams& p, bool tc) {
 void set_joined(DecayParams& p) {
   p.joined = !decay_one_walk(p.d, p.tc) || p.segs > 24;
 }
-// bytes of p.part, whichever kernels the rows' layout allows
-int64_t part_bytes(int B, int N, int H, int d, bool bf16, bool last) {
-  int64_t bytes = 0;
-  for (int tc = 0; tc <= (int)decay_tc_sizes(B, N, H, d, bf16); ++tc) {
-    const DecayPlan g = decay_plan(B, N, H, d, tc != 0);
-    if (!decay_uses_part(g, tc != 0, last)) continue;
-    const int64_t n = decay_part_bytes(g, B, H, d, tc != 0);
-    if (n > bytes) bytes = n;
-  }
-  return bytes;
+// bytes of p.part, 0 where the call does not use it
+int64_t part_bytes(int B, int N, int H, int d, bool tc, int jobs, bool last) {
+  const DecayPlan g = decay_plan(B, N, H, d, tc, jobs);
+  return decay_uses_part(g, tc, last) ? round16(decay_part_bytes(g, B, H, d, tc)) : 0;
+}
+// The gradients' scratch: states forwards at 0, backwards at `back` (on the tensor
+// memory both are needed at once), the gradients of shared heads by query head,
+// dv and dk, before their sum.
+struct BackwardWork {
+  int64_t back, dv, dk, bytes;
+};
+BackwardWork backward_work(int B, int N, int H, int Hk, int d, bool tc, bool dstate) {
+  const int64_t ahead = part_bytes(B, N, H, d, tc, GRADIENTS, false);
+  const int64_t behind = part_bytes(B, N, H, d, tc, GRADIENTS, dstate);
+  const int64_t shared = H == Hk ? 0 : round16((int64_t)B * N * H * d * 4);
+  BackwardWork w;
+  w.back = tc ? ahead : 0;
+  w.dv = w.back + behind;
+  w.dk = w.dv + shared;
+  w.bytes = w.dk + shared;
+  return w;
 }
 
 // one operand: pointer, strides and how many heads share one of its heads
@@ -169,7 +181,12 @@ extern "C" {
 int64_t tarmac_decay_attention_workspace(int B, int N, int H, int d, int dtype, int state_out) {
   if (check_sizes(B, N, H, 1, d, dtype) != TARMAC_OK || B < 1 || N < 1) return 0;
   if (decay_step_takes(N)) return 0;
-  return part_bytes(B, N, H, d, dtype == TARMAC_BF16, state_out != 0);
+  int64_t bytes = 0;  // whichever kernels the rows' layout allows
+  for (int tc = 0; tc <= (int)decay_tc_sizes(B, N, H, d, dtype == TARMAC_BF16); ++tc) {
+    const int64_t n = part_bytes(B, N, H, d, tc != 0, 1, state_out != 0);
+    if (n > bytes) bytes = n;
+  }
+  return bytes;
 }
 
 int tarmac_decay_attention(const void* q, const void* k, const void* v, void* out,
@@ -197,7 +214,7 @@ int tarmac_decay_attention(const void* q, const void* k, const void* v, void* ou
   p.out_scale = scale;
   set_operands(p, oq, ok, ov);
   if (decay_step_takes(N)) return status(launch_decay_step(p, bf16, s));
-  set_plan(p, decay_tc_sizes(B, N, H, d, bf16) && oq.map && ok.map && ov.map);
+  set_plan(p, decay_tc_sizes(B, N, H, d, bf16) && oq.map && ok.map && ov.map, 1);
   if (decay_uses_part(DecayPlan{p.segs, p.seg_chunks}, p.tc, state_out)) {
     if (!work) return TARMAC_ERR_NULL;
     p.part = static_cast<float*>(work);
@@ -212,10 +229,12 @@ int tarmac_decay_attention(const void* q, const void* k, const void* v, void* ou
 int64_t tarmac_decay_attention_backward_workspace(int B, int N, int H, int Hk, int d, int dtype,
                                                   int dstate) {
   if (check_sizes(B, N, H, Hk, d, dtype) != TARMAC_OK || B < 1 || N < 1) return 0;
-  const int64_t parts = part_bytes(B, N, H, d, dtype == TARMAC_BF16, dstate != 0);
-  // gradients of shared heads by query head, before their sum: dk and dv
-  const int64_t shared = H == Hk ? 0 : round16((int64_t)B * N * H * d * 4);
-  return round16(parts) + 2 * shared;
+  int64_t bytes = 0;
+  for (int tc = 0; tc <= (int)decay_tc_sizes(B, N, H, d, dtype == TARMAC_BF16); ++tc) {
+    const int64_t n = backward_work(B, N, H, Hk, d, tc != 0, dstate != 0).bytes;
+    if (n > bytes) bytes = n;
+  }
+  return bytes;
 }
 
 int tarmac_decay_attention_backward(const void* q, const void* k, const void* v, const void* dout,
@@ -243,18 +262,29 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
   const Operand oq = operand(q, sq, B, N, H, 1, d, es), ok = operand(k, sk, B, N, H, G, d, es),
                 ov = operand(v, sv, B, N, H, G, d, es);
   const Operand og = operand(dout, sg, B, N, H, 1, d, es);
-  set_plan(p, decay_tc_sizes(B, N, H, d, bf16) && oq.map && ok.map && ov.map && og.map);
+  set_plan(p, decay_tc_sizes(B, N, H, d, bf16) && oq.map && ok.map && ov.map && og.map,
+           GRADIENTS);
   const DecayPlan plan = {p.segs, p.seg_chunks};
-  const int64_t parts = part_bytes(B, N, H, d, bf16, dstate != nullptr);
-  float* shared = reinterpret_cast<float*>(static_cast<char*>(work) + round16(parts));
+  const BackwardWork at = backward_work(B, N, H, Hk, d, p.tc, dstate != nullptr);
+  char* scratch = static_cast<char*>(work);
   cudaError_t e = cudaSuccess;
   auto run = [&](cudaError_t (*launch)(const DecayParams&, bool, cudaStream_t)) {
     if (e == cudaSuccess) e = launch(p, bf16, s);
   };
+  // On the tensor memory the three gradients are one launch; otherwise they
+  // follow their states.
+  DecayParams jobs[GRADIENTS];
+  int n = 0;
+  auto rows = [&] {
+    if (p.tc)
+      jobs[n++] = p;
+    else
+      run(launch_decay_rows);
+  };
   const bool one_walk = decay_one_walk(d, p.tc);
   // dq_i = scale S_i dout_i, S over the rows as in the forward pass
   p.start = state;
-  p.part = decay_uses_part(plan, p.tc, false) ? static_cast<float*>(work) : nullptr;
+  p.part = decay_uses_part(plan, p.tc, false) ? reinterpret_cast<float*>(scratch) : nullptr;
   p.planes = 1;
   p.in_scale = 1.f;
   p.out_scale = scale;
@@ -269,12 +299,13 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
     p.transposed = 1;
     p.out = dq;
   }
-  run(launch_decay_rows);
+  rows();
   // R_i = sum over the rows from i on of scale q dout^T:
   // dv_i = R_i^T k_i, dk_i = R_i v_i
   p.start = dstate_out;
   p.last = dstate;
-  p.part = decay_uses_part(plan, p.tc, dstate) ? static_cast<float*>(work) : nullptr;
+  p.part = decay_uses_part(plan, p.tc, dstate) ? reinterpret_cast<float*>(scratch + at.back)
+                                               : nullptr;
   p.planes = dstate ? 3 : 1;
   p.reverse = 1;
   p.transposed = 0;
@@ -284,24 +315,26 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
   set_joined(p);
   run(launch_decay_states);
   p.out_f32 = G > 1;
-  float* shared_k = shared + round16((int64_t)B * N * H * d * 4) / 4;
-  p.out = G > 1 ? shared : dv;
+  float* shared_v = reinterpret_cast<float*>(scratch + at.dv);
+  float* shared_k = reinterpret_cast<float*>(scratch + at.dk);
+  p.out = G > 1 ? shared_v : dv;
   if (one_walk) {
     set_extra(p, ov);
     p.row_out = G > 1 ? shared_k : dk;
-    run(launch_decay_rows);
+    rows();
   } else {
-    run(launch_decay_rows);
+    rows();
     set_operands(p, ov, og, oq);
     p.transposed = 1;
     p.last = nullptr;
     p.out = G > 1 ? shared_k : dk;
-    run(launch_decay_rows);
+    rows();
   }
+  if (n > 0 && e == cudaSuccess) e = launch_decay_rows_tc(jobs, n, s);
   if (G > 1) {
-    const int64_t rows = (int64_t)B * N;
-    if (e == cudaSuccess) e = launch_decay_share(shared, dv, rows, Hk, G, d, bf16, s);
-    if (e == cudaSuccess) e = launch_decay_share(shared_k, dk, rows, Hk, G, d, bf16, s);
+    const int64_t tokens = (int64_t)B * N;
+    if (e == cudaSuccess) e = launch_decay_share(shared_v, dv, tokens, Hk, G, d, bf16, s);
+    if (e == cudaSuccess) e = launch_decay_share(shared_k, dk, tokens, Hk, G, d, bf16, s);
   }
   return status(e);
 }
@@ -325,7 +358,7 @@ int tarmac_decay_attention_plan(int backward, const int64_t* strides, int B, int
       const int share = i == 1 || i == 2 ? G : 1;
       tc = tc && operand(a, stride_of(strides, i, N, H / share, d), B, N, H, share, d, es).map;
     }
-    const DecayPlan g = decay_plan(B, N, H, d, tc);
+    const DecayPlan g = decay_plan(B, N, H, d, tc, backward ? GRADIENTS : 1);
     snprintf(buf, sizeof buf, "{\"kernel\": \"%s\", \"segments\": %d, \"states\": %s}",
              tc ? "decay_tc" : "decay_scan", g.segs,
              decay_uses_part(g, tc, state != 0) ? "true" : "false");

@@ -512,9 +512,9 @@ cudaError_t launch_scan(const DecayParams& p, int mode, bool bf16, cudaStream_t 
 
 }  // namespace
 
-DecayPlan decay_plan(int B, int N, int H, int d, bool tc) {
+DecayPlan decay_plan(int B, int N, int H, int d, bool tc, int jobs) {
   if (B < 1 || N < 1) return DecayPlan{1, 1};
-  if (tc) return decay_plan_tc(B, N, H, d);
+  if (tc) return decay_plan_tc(B, N, H, d, jobs);
   const int64_t heads = (int64_t)B * H;
   const int64_t warps = d <= 16 ? (heads + 1) / 2 : heads * (d <= 32 ? 1 : (d <= 64 ? 2 : 4));
   const int chunks = cdiv(N, DECAY_CHUNK);
@@ -570,7 +570,7 @@ cudaError_t launch_decay_states(const DecayParams& p, bool bf16, cudaStream_t s)
 }
 
 cudaError_t launch_decay_rows(const DecayParams& p, bool bf16, cudaStream_t s) {
-  if (p.tc) return launch_decay_rows_tc(p, s);
+  if (p.tc) return launch_decay_rows_tc(&p, 1, s);
   return launch_scan(p, p.row_out && !p.out ? SC_ROWS : SC_COLS, bf16, s);
 }
 

@@ -4,9 +4,10 @@
 //   P = a b^T, out = (l^(i-j) P, j <= i) c + l^(i+1) a S,
 //   S = l^n S + (l^(n-1-j) b)^T c.
 //
-// decay_rows_tc_kernel gives the rows. A block walks over one unit: a head of
-// an episode, or two heads of up to 64 columns (the two 64-column halves of a
-// tile), in one segment of the row axis. Roles of its 20 warps (two idle):
+// decay_rows_tc_kernel gives the rows, of one sum or of the gradients' three. A
+// block walks over one unit: a head of an episode, or two heads of up to 64
+// columns (the two 64-column halves of a tile), in one segment of the row axis.
+// Roles of its 20 warps (two idle):
 // * warp 1: one thread loads a, b, c tiles by TMA ahead of the products.
 // * warp 0: one thread issues the products P, a S, the state's and P c.
 // * warps 4..11 weight P (TMEM, back to TMEM as bf16, the A operand of P c) and
@@ -49,10 +50,16 @@ constexpr int DT_HALF = DT_TILE / 2;
 constexpr float DT_LOG2E = 1.4426950408889634f;
 
 struct DtGrid {
-  int units, head_units, chunks;
+  int units, head_units, chunks, jobs;
+};
+// Up to three sums over the same heads and rows in one launch: the gradients.
+// Their units lie side by side, as they read the same tensors.
+struct DtJobs {
+  CUtensorMap map[3][4];  // a, b, c, out
+  DecayParams p[3];
 };
 
-// One unit: episode, first head, rows, and the chunks k in [k0, k1) in the
+// One unit (of a job): episode, first head, rows, and the chunks k in [k0, k1) in the
 // order they are walked; those in [a0, a1) have rows.
 struct DtUnit {
   int b, h, seg, len, k0, k1, a0, a1;
@@ -60,6 +67,7 @@ struct DtUnit {
 template <bool PAIR>
 __device__ __forceinline__ DtUnit dt_unit(const DecayParams& p, const DtGrid& g, int unit) {
   DtUnit w;
+  unit /= g.jobs;
   const int x = unit % g.head_units, y = unit / g.head_units;
   w.h = PAIR ? 2 * x : x;
   w.b = y % p.B;
@@ -282,12 +290,9 @@ struct DtShared {
   int abort_flag;
 };
 
-template <int NKS, bool PAIR, bool REV, bool WIDE>
+template <int NKS, bool PAIR>
 __global__ void __launch_bounds__(DT_THREADS, 1)
-    decay_rows_tc_kernel(const __grid_constant__ CUtensorMap ma,
-                         const __grid_constant__ CUtensorMap mb,
-                         const __grid_constant__ CUtensorMap mc,
-                         const __grid_constant__ CUtensorMap mo, DecayParams p, DtGrid g) {
+    decay_rows_tc_kernel(const __grid_constant__ DtJobs jobs, DtGrid g) {
   using Plan = DtPlan<PAIR>;
   constexpr int HEADS = PAIR ? 2 : 1, CS = Plan::CS;
   extern __shared__ unsigned char dt_raw[];
@@ -327,7 +332,9 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
   // P of a chunk: the unit's heads side by side, or two chunks in turn
   auto tmem_p = [&](uint32_t c, int u) { return tmem + (PAIR ? u : (int)(c & 1)) * 128; };
   // does a unit's first chunk start from a state?
-  auto starts = [&](const DtUnit& w) { return p.part ? w.seg > 0 || p.start : p.start != nullptr; };
+  auto starts = [](const DecayParams& p, const DtUnit& w) {
+    return p.part ? w.seg > 0 || p.start : p.start != nullptr;
+  };
 
   if (warp == DT_TMA_WARP) {
     if (lane == 0) {
@@ -337,18 +344,20 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           *abort_flag = 1;
           break;
         }
+        const DecayParams& p = jobs.p[unit % g.jobs];
+        const CUtensorMap* map = jobs.map[unit % g.jobs];
         const DtUnit w = dt_unit<PAIR>(p, g, unit);
         for (int x = w.a0; x < w.a1; ++x) {
           const int s = c & 1, row = dt_chunk(p, g, x) * DT_T;
           if (!ws::wait(&sh.empty_ab[s], ((c >> 1) & 1) ^ 1, abort_flag)) goto tma_done;
           ht::expect_tx(&sh.full_ab[s], 2 * DT_TILE);
-          dt_load<PAIR>(tile_a(c), &ma, &sh.full_ab[s], p, w, p.ga, row);
-          dt_load<PAIR>(tile_b(c), &mb, &sh.full_ab[s], p, w, p.gb, row);
+          dt_load<PAIR>(tile_a(c), map, &sh.full_ab[s], p, w, p.ga, row);
+          dt_load<PAIR>(tile_b(c), map + 1, &sh.full_ab[s], p, w, p.gb, row);
           ++c;
           const int t = cc % CS;
           if (!ws::wait(&sh.empty_c[t], ((cc / CS) & 1) ^ 1, abort_flag)) goto tma_done;
           ht::expect_tx(&sh.full_c[t], DT_TILE);
-          dt_load<PAIR>(tile_c(cc), &mc, &sh.full_c[t], p, w, p.gc, row);
+          dt_load<PAIR>(tile_c(cc), map + 2, &sh.full_c[t], p, w, p.gc, row);
           ++cc;
         }
       }
@@ -385,10 +394,11 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       __syncwarp();
     };
     for (int unit = blockIdx.x; unit < g.units && ok; unit += gridDim.x) {
+      const DecayParams& p = jobs.p[unit % g.jobs];
       const DtUnit w = dt_unit<PAIR>(p, g, unit);
       bool formed = false;
       for (int x = w.a0; x < w.a1 && ok; ++x, ++c) {
-        const bool state = x > w.a0 || starts(w);
+        const bool state = x > w.a0 || starts(p, w);
         const uint32_t odd = c & 1, ph = (c >> 1) & 1;
         if (!formed) form_p(c);
         formed = false;
@@ -455,7 +465,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
     // all of head `half`
     const int half = (warp - DT_W0) >> 2, i = threadIdx.x & 127, w0 = (warp & 3) * 32;
     const uint32_t lane_off = (uint32_t)w0 << 16;
-    const int c_lo = PAIR ? 0 : half * 64, c_n = max(0, min(64, p.d - c_lo));
+    const int c_lo = PAIR ? 0 : half * 64, c_n = max(0, min(64, jobs.p[0].d - c_lo));
     // The tile that holds the rows of chunk c - 1 may be loaded again once they
     // have been read: asked for only when the next chunk is under way.
     bool held = false;
@@ -476,6 +486,9 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
     };
     bool ok = true;
     for (int k = 0, unit = blockIdx.x; unit < g.units; unit += gridDim.x, ++k) {
+      const DecayParams& p = jobs.p[unit % g.jobs];
+      const CUtensorMap* map_out = &jobs.map[unit % g.jobs][3];
+      const bool rev = p.reverse;
       const DtUnit w = dt_unit<PAIR>(p, g, unit);
       if (ht::gives_up(ht::ROLE_WEIGHTS, k)) {
         ok = false;
@@ -487,8 +500,8 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       uint64_t steps[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        steps[e] = REV ? pack2(power(l2, 2 * e), power(l2, 2 * e + 1))
-                             : pack2(power(l2, 15 - 2 * e), power(l2, 14 - 2 * e));
+        steps[e] = rev ? pack2(power(l2, 2 * e), power(l2, 2 * e + 1))
+                       : pack2(power(l2, 15 - 2 * e), power(l2, 14 - 2 * e));
       for (int x = w.k0; x < w.k1; ++x) {
         const int chunk = dt_chunk(p, g, x);
         const bool live = x >= w.a0 && x < w.a1;
@@ -500,7 +513,11 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
 #pragma unroll 1
             for (int j0 = PAIR ? 0 : half * 64, q = 0; q < 2 * HEADS; ++q, j0 += 32) {
               if (q == HEADS) release();
-              weigh<REV>(tmem_p(c, half) + lane_off, j0, i, w0, n, l2, p.in_scale, steps);
+              const uint32_t t_p = tmem_p(c, half) + lane_off;
+              if (rev)
+                weigh<true>(t_p, j0, i, w0, n, l2, p.in_scale, steps);
+              else
+                weigh<false>(t_p, j0, i, w0, n, l2, p.in_scale, steps);
             }
             ht::st_wait();
             tc::fence_before_sync();
@@ -529,11 +546,11 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           auto store = [&](int col) {
             tc::fence_async_smem();
             __syncwarp();
-            if (lane == 0 && left > 0) store_box(&mo, stage, c_lo + col, h, chunk * DT_T + w0, w.b);
+            if (lane == 0 && left > 0) store_box(map_out, stage, c_lo + col, h, chunk * DT_T + w0, w.b);
             __syncwarp();
           };
           part(0);
-          if constexpr (!WIDE) {
+          if (!p.out_f32) {
             stage_row(stage, lane, 0, o);
             part(32);
             stage_row(stage, lane, 4, o);
@@ -552,7 +569,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           held = true;
         } else {
           // padding, or rows given up
-          if constexpr (WIDE)
+          if (p.out_f32)
             fill_rows(static_cast<float*>(p.out) + first, ok ? 0u : 0x7fffffffu, lane, left,
                       (int64_t)p.H * p.d, c_n, 4);
           else
@@ -577,6 +594,8 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
     bool ok = true;
     uint32_t c = 0, states = 0, us = 0;
     for (int unit = blockIdx.x; unit < g.units && ok; unit += gridDim.x) {
+      const DecayParams& p = jobs.p[unit % g.jobs];
+      const bool rev = p.reverse;
       const DtUnit w = dt_unit<PAIR>(p, g, unit);
       const int h0 = w.h, h1 = PAIR ? min(w.h + 1, p.H - 1) : w.h;
       const float l2_0 = decay_rate(p.log_decay, h0) * DT_LOG2E;
@@ -584,7 +603,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       const float l2_s = s_head ? l2_1 : l2_0, l2_o = PAIR && half ? l2_1 : l2_0;
       const int hs = s_head ? h1 : h0, rc = PAIR ? r & 63 : r;
       const float* start = nullptr;
-      if (starts(w))
+      if (starts(p, w))
         start = (p.part ? p.part + (int64_t)w.seg * p.B * p.H * p.d * p.d : p.start) +
                 ((int64_t)w.b * p.H + hs) * p.d * p.d;
       // weights of a whole chunk; a chunk of fewer rows makes its own
@@ -592,13 +611,13 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       auto weights = [&](int n) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int row = (tid >> 3) + 32 * e, to = max(0, REV ? row + 1 : n - 1 - row);
+          const int row = (tid >> 3) + 32 * e, to = max(0, rev ? row + 1 : n - 1 - row);
           f0[e] = p.in_scale * power(l2_0, to);
           f1[e] = PAIR ? p.in_scale * power(l2_1, to) : 0.f;
         }
       };
       weights(DT_T);
-      const float whole = power(l2_s, DT_T), row_whole = power(l2_o, REV ? DT_T - 1 - r : r + 1);
+      const float whole = power(l2_s, DT_T), row_whole = power(l2_o, rev ? DT_T - 1 - r : r + 1);
       // b of chunk c_, the unit's x_, weighted in place once P is formed
       auto convert = [&](uint32_t c_, int x_) {
         const int n = dt_rows(w, dt_chunk(p, g, x_));
@@ -696,7 +715,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           if (!ok) break;
           ++states;
           tc::fence_after_sync();
-          const float f = REV && n < DT_T ? power(l2_o, max(0, n - 1 - r)) : row_whole;
+          const float f = rev && n < DT_T ? power(l2_o, max(0, n - 1 - r)) : row_whole;
 #pragma unroll 1
           for (int q = 0; q < 2; ++q) {
             uint32_t o[32];
@@ -927,11 +946,12 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
 // ---------------------------------------------------------------------------
 // launch
 // ---------------------------------------------------------------------------
-DtGrid dt_grid(const DecayParams& p, int segs) {
+DtGrid dt_grid(const DecayParams& p, int segs, int jobs) {
   DtGrid g;
   g.head_units = p.d <= 64 ? cdiv(p.H, 2) : p.H;
   g.chunks = cdiv(p.N, DT_T);
-  g.units = g.head_units * p.B * segs;
+  g.jobs = jobs;
+  g.units = g.head_units * p.B * segs * jobs;
   return g;
 }
 int dt_blocks(const DtGrid& g) {
@@ -939,21 +959,14 @@ int dt_blocks(const DtGrid& g) {
   return g.units < sms ? g.units : sms;
 }
 
-template <int NKS, bool PAIR, bool REV, bool WIDE>
-cudaError_t rows_go(const CUtensorMap* m, const DecayParams& p, const DtGrid& g, cudaStream_t s) {
+template <int NKS, bool PAIR>
+cudaError_t rows_go(const DtJobs& jobs, const DtGrid& g, cudaStream_t s) {
   constexpr int SMEM = DtPlan<PAIR>::SMEM;
-  const void* fn = reinterpret_cast<const void*>(&decay_rows_tc_kernel<NKS, PAIR, REV, WIDE>);
+  const void* fn = reinterpret_cast<const void*>(&decay_rows_tc_kernel<NKS, PAIR>);
   const cudaError_t e = raise_smem_limit(fn, SMEM);
   if (e != cudaSuccess) return e;
-  decay_rows_tc_kernel<NKS, PAIR, REV, WIDE>
-      <<<dt_blocks(g), DT_THREADS, SMEM, s>>>(m[0], m[1], m[2], m[3], p, g);
+  decay_rows_tc_kernel<NKS, PAIR><<<dt_blocks(g), DT_THREADS, SMEM, s>>>(jobs, g);
   return cudaGetLastError();
-}
-template <int NKS, bool PAIR>
-cudaError_t rows_way(const CUtensorMap* m, const DecayParams& p, const DtGrid& g, cudaStream_t s) {
-  if (!p.reverse) return rows_go<NKS, PAIR, false, false>(m, p, g, s);
-  return p.out_f32 ? rows_go<NKS, PAIR, true, true>(m, p, g, s)
-                   : rows_go<NKS, PAIR, true, false>(m, p, g, s);
 }
 template <bool PAIR, int PLANES>
 cudaError_t state_go(const CUtensorMap* m, const DecayParams& p, const DtGrid& g, cudaStream_t s) {
@@ -972,19 +985,23 @@ bool map_of(CUtensorMap* m, const DecayParams& p, const void* ptr, const HeadStr
 
 }  // namespace
 
-// Segments of a call: the walk over the longest block, with the states' pass
-// where there are segments (about half the rows' time) and what a unit costs
-// beside its chunks (about one chunk). Host arithmetic for 148 SMs, so that a
-// caller can ask for the scratch without a GPU.
-DecayPlan decay_plan_tc(int B, int N, int H, int d) {
+// Segments of a call of `jobs` sums, by the longest walk of a block in chunks: a
+// unit costs one and a half beside its own, a chunk of the states' pass two
+// thirds of one, its launch and the joining four. The gradients' three sums need
+// two such passes. Host arithmetic for 148 SMs, so that a caller can ask for the
+// scratch without a GPU. 2 x 8192 rows of 16 heads, d = 128, gradients: 96 units
+// of 64 chunks 184 us, three segments with their states 219.
+DecayPlan decay_plan_tc(int B, int N, int H, int d, int jobs) {
   const int64_t heads = (int64_t)B * (d <= 64 ? cdiv(H, 2) : H);
   const int chunks = cdiv(N, DT_T);
   DecayPlan best = {1, chunks};
   double least = 0;
   for (int want = 1; want <= chunks && want <= 256; ++want) {
     const int per = cdiv(chunks, want), segs = cdiv(chunks, per);
-    const double turns = (double)((heads * segs + 147) / 148);
-    const double cost = turns * (per + 1) * (segs > 1 ? 1.5 : 1.0) + (segs > 1 ? 2.0 : 0.0);
+    double cost = (double)((heads * segs * jobs + 147) / 148) * (per + 1.5);
+    if (segs > 1)
+      cost += (jobs > 1 ? 2 : 1) *
+              ((double)((heads * (segs - 1) + 147) / 148) * (per + 1.5) * 0.65 + 4.0);
     if (want == 1 || cost < least) {
       least = cost;
       best = DecayPlan{segs, per};
@@ -995,7 +1012,7 @@ DecayPlan decay_plan_tc(int B, int N, int H, int d) {
 
 cudaError_t launch_decay_states_tc(const DecayParams& p, cudaStream_t s) {
   // the last segment's share counts only where the state after it is wanted
-  const DtGrid g = dt_grid(p, p.last ? p.segs : p.segs - 1);
+  const DtGrid g = dt_grid(p, p.last ? p.segs : p.segs - 1, 1);
   if (g.units == 0) return cudaSuccess;
   CUtensorMap m[2];
   if (!map_of(&m[0], p, p.b, p.sb, p.gb) || !map_of(&m[1], p, p.c, p.sc, p.gc))
@@ -1004,17 +1021,22 @@ cudaError_t launch_decay_states_tc(const DecayParams& p, cudaStream_t s) {
   return p.planes > 2 ? state_go<false, 3>(m, p, g, s) : state_go<false, 1>(m, p, g, s);
 }
 
-cudaError_t launch_decay_rows_tc(const DecayParams& p, cudaStream_t s) {
-  CUtensorMap m[4];
-  const HeadStrides so = {(int64_t)p.N * p.H * p.d, (int64_t)p.H * p.d, p.d};
-  if (!map_of(&m[0], p, p.a, p.sa, p.ga) || !map_of(&m[1], p, p.b, p.sb, p.gb) ||
-      !map_of(&m[2], p, p.c, p.sc, p.gc) ||
-      !head_box_map(&m[3], p.out, so, p.B, p.N, p.H, p.d, p.out_f32, 32))
-    return cudaErrorInvalidValue;
-  const DtGrid g = dt_grid(p, p.segs);
-  if (p.d <= 64) return rows_way<4, true>(m, p, g, s);
-  if (p.d <= 96) return rows_way<6, false>(m, p, g, s);
-  return rows_way<8, false>(m, p, g, s);
+cudaError_t launch_decay_rows_tc(const DecayParams* p, int jobs, cudaStream_t s) {
+  DtJobs all;
+  for (int j = 0; j < jobs; ++j) {
+    const DecayParams& q = p[j];
+    const HeadStrides so = {(int64_t)q.N * q.H * q.d, (int64_t)q.H * q.d, q.d};
+    CUtensorMap* m = all.map[j];
+    if (!map_of(&m[0], q, q.a, q.sa, q.ga) || !map_of(&m[1], q, q.b, q.sb, q.gb) ||
+        !map_of(&m[2], q, q.c, q.sc, q.gc) ||
+        !head_box_map(&m[3], q.out, so, q.B, q.N, q.H, q.d, q.out_f32, 32))
+      return cudaErrorInvalidValue;
+    all.p[j] = q;
+  }
+  const DtGrid g = dt_grid(p[0], p[0].segs, jobs);
+  if (p[0].d <= 64) return rows_go<4, true>(all, g, s);
+  if (p[0].d <= 96) return rows_go<6, false>(all, g, s);
+  return rows_go<8, false>(all, g, s);
 }
 
 }  // namespace tarmac
