@@ -128,3 +128,22 @@ def test_block_arguments():
     assert m.empty_state(3).shape == (3, 4, 8, 8)
     assert "log_decay" in m.state_dict()
     assert (decay_slopes(8) < 0).all() and decay_slopes(8)[-1] == -1 / 256
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_cast_block_keeps_its_decays(dtype):
+    m = DecayComm(24, 6, 16)
+    want = decay_slopes(6)
+    for step in (lambda: m.to(dtype), lambda: m.double(), lambda: m.to(dtype), lambda: m.float()):
+        step()
+        assert torch.equal(m.log_decay.float(), want)
+    assert m.log_decay.dtype is torch.float32 and "log_decay" in m.state_dict()
+    assert m.to(dtype).log_decay.dtype is torch.float32 and m.proj.weight.dtype is dtype
+
+
+def test_room_for_a_state_renewed_in_place():
+    """fp32 rows of 16 columns over several segments: each reads the state."""
+    sizes = 3, 500, 2, 16, _lib.F32
+    assert ops.decay_attention_plan(*sizes[:3], 1, 16, torch.float32)["segments"] > 1
+    room = _lib.lib().tarmac_decay_attention_workspace
+    assert room(*sizes, 1) >= room(*sizes, 0) + 3 * 2 * 16 * 16 * 4 > 0

@@ -207,6 +207,24 @@ def test_state_in_place(B, N, d, dtype):
     assert got is S and torch.equal(S, want) and torch.equal(out, out2)
 
 
+@pytest.mark.parametrize("B,N,d,segments", [(2, 100, 16, 3), (3, 1300, 32, 41), (1, 9000, 16, 188)])
+def test_state_in_place_by_segments(B, N, d, segments):
+    """Up to 32 columns every segment reads the state before the first row; what
+    the last one writes must not reach the others."""
+    from tarmac_b200 import ops
+    plan = ops.decay_attention_plan(B, N, 2, 1, d, F32, state=True)
+    assert plan["kernel"] == "decay_scan" and plan["segments"] == segments
+    c = Case(B, N, 2, 1, d, F32)
+    q, k, v, S, rate = (t.cuda() for t in (c.q, c.k, c.v, c.state, c.rate))
+    lens = torch.full((B,), N, dtype=torch.int32, device="cuda")
+    lens[0] = 1
+    out, want = ops.decay_attention(q, k, v, rate, S, lens, return_state=True)
+    for _ in range(5):
+        s = S.clone()
+        out2, got = ops.decay_attention(q, k, v, rate, s, lens, state_out=s)
+        assert got is s and torch.equal(s, want) and torch.equal(out, out2)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_parts_in_turn(dtype):
     """A history in calls of unequal size, the state handed on, against one

@@ -126,6 +126,19 @@ def test_steps_equal_one_pass(dtype):
     assert (S - want[2]).abs().max() <= tol * want[2].abs().max()
 
 
+def test_a_renewed_state_is_noticed():
+    """A state that autograd saved and a later call renewed in place."""
+    from tarmac_b200 import autograd, ops
+    q, k, v = (torch.randn(2, 4, 2, 16, device="cuda", requires_grad=True) for _ in range(3))
+    rate = torch.tensor([-0.1, -0.5], device="cuda")
+    S = torch.randn(2, 2, 16, 16, device="cuda")
+    out = autograd.decay_attention(q, k, v, rate, S)
+    with torch.no_grad():
+        ops.decay_attention(q, k, v, rate, S, state_out=S)
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+
+
 def test_unused_outputs():
     """Only one of the outputs takes part in the loss."""
     from tarmac_b200 import autograd

@@ -78,6 +78,13 @@ int64_t part_bytes(int B, int N, int H, int d, bool tc, int jobs, bool last) {
   const DecayPlan g = decay_plan(B, N, H, d, tc, jobs);
   return decay_uses_part(g, tc, last) ? round16(decay_part_bytes(g, B, H, d, tc)) : 0;
 }
+// Up to 32 columns off the tensor memory the blocks of every segment read p.start
+// and those of the last write p.last. Where the two are one, all read a copy,
+// behind p.part. Its bytes, for a call that returns a state:
+int64_t copy_bytes(int B, int N, int H, int d, bool tc) {
+  if (!decay_one_walk(d, tc) || decay_plan(B, N, H, d, tc, 1).segs == 1) return 0;
+  return round16((int64_t)B * H * d * d * 4);
+}
 // The gradients' scratch: states forwards at 0, backwards at `back` (on the tensor
 // memory both are needed at once), the gradients of shared heads by query head,
 // dv and dk, before their sum.
@@ -128,7 +135,7 @@ void set_extra(DecayParams& p, const Operand& x) {
   p.vec = p.vec && x.vec;
 }
 
-// no rows: the state stays as it was
+// a state as it is, or zero
 cudaError_t carry_state(const float* from, float* to, int64_t n, cudaStream_t s) {
   if (!to || n == 0 || from == to) return cudaSuccess;
   if (!from) return cudaMemsetAsync(to, 0, (size_t)n * 4, s);
@@ -183,7 +190,8 @@ int64_t tarmac_decay_attention_workspace(int B, int N, int H, int d, int dtype, 
   if (decay_step_takes(N)) return 0;
   int64_t bytes = 0;  // whichever kernels the rows' layout allows
   for (int tc = 0; tc <= (int)decay_tc_sizes(B, N, H, d, dtype == TARMAC_BF16); ++tc) {
-    const int64_t n = part_bytes(B, N, H, d, tc != 0, 1, state_out != 0);
+    const int64_t n = part_bytes(B, N, H, d, tc != 0, 1, state_out != 0) +
+                      (state_out ? copy_bytes(B, N, H, d, tc != 0) : 0);
     if (n > bytes) bytes = n;
   }
   return bytes;
@@ -221,7 +229,13 @@ int tarmac_decay_attention(const void* q, const void* k, const void* v, void* ou
   }
   p.planes = state_out ? 3 : 1;
   set_joined(p);
-  cudaError_t e = launch_decay_states(p, bf16, s);
+  cudaError_t e = cudaSuccess;
+  if (state && state == state_out && copy_bytes(B, N, H, d, p.tc)) {
+    char* copy = static_cast<char*>(work) + part_bytes(B, N, H, d, p.tc, 1, true);
+    p.start = reinterpret_cast<const float*>(copy);
+    e = carry_state(state, reinterpret_cast<float*>(copy), (int64_t)B * H * d * d, s);
+  }
+  if (e == cudaSuccess) e = launch_decay_states(p, bf16, s);
   if (e == cudaSuccess) e = launch_decay_rows(p, bf16, s);
   return status(e);
 }

@@ -143,6 +143,14 @@ class DecayComm(nn.Module):
         self.scale = nn.Parameter(torch.ones(dim))
         self.register_buffer("log_decay", decay_slopes(n_heads))
 
+    def _apply(self, fn, recurse=True):
+        """A cast to a shorter type leaves the decays in fp32."""
+        kept = self.log_decay
+        super()._apply(fn, recurse)
+        if self.log_decay.element_size() < kept.element_size():
+            self.log_decay = kept.to(self.log_decay.device, torch.float32)
+        return self
+
     def empty_state(self, B: int) -> torch.Tensor:
         """The state before any row, fp32 [B, n_heads, head_dim, head_dim]."""
         return torch.zeros(B, self.heads[0], self.head_dim, self.head_dim,

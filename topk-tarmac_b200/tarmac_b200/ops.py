@@ -889,6 +889,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             raise ValueError("state_out must be state itself or apart from it")
     B, N, H, d = q.shape
     out = _empty_as(q)
+    if state_out is not None:  # a graph that saved what it holds now has to know
+        torch.autograd.graph.increment_version(state_out)
     if return_state and state_out is None:
         state_out = torch.empty((B, H, d, d), device=q.device, dtype=torch.float32)
     work = _scratch(_decay_work(B, N, H, d, _DTYPES[q.dtype], int(state_out is not None)),
