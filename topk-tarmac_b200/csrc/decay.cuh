@@ -81,8 +81,9 @@ cudaError_t launch_decay_rows_tc(const DecayParams* p, int jobs, cudaStream_t s)
 // few rows, one after the other (forward only)
 bool decay_step_takes(int N);
 cudaError_t launch_decay_step(const DecayParams& p, bool bf16, cudaStream_t s);
-// out[., hk, .] = sum over the G heads of a key head, fp32 to the rows' type
-cudaError_t launch_decay_share(const float* x, void* out, int64_t rows, int Hk, int G, int d,
-                               bool bf16, cudaStream_t s);
+// out0, out1 [rows, Hk, d] = sums over the G heads of a key head of x and of what
+// stands x_step elements on, fp32 to the rows' type
+cudaError_t launch_decay_share(const float* x, int64_t x_step, void* out0, void* out1,
+                               int64_t rows, int Hk, int G, int d, bool bf16, cudaStream_t s);
 
 }  // namespace tarmac

@@ -345,11 +345,8 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
     rows();
   }
   if (n > 0 && e == cudaSuccess) e = launch_decay_rows_tc(jobs, n, s);
-  if (G > 1) {
-    const int64_t tokens = (int64_t)B * N;
-    if (e == cudaSuccess) e = launch_decay_share(shared_v, dv, tokens, Hk, G, d, bf16, s);
-    if (e == cudaSuccess) e = launch_decay_share(shared_k, dk, tokens, Hk, G, d, bf16, s);
-  }
+  if (G > 1 && e == cudaSuccess)
+    e = launch_decay_share(shared_v, (at.dk - at.dv) / 4, dv, dk, (int64_t)B * N, Hk, G, d, bf16, s);
   return status(e);
 }
 

@@ -455,19 +455,46 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-template <typename T>
+// out[., hk, .] = sum over the G heads of a key head; blockIdx.y: of the two
+// tensors. V elements a thread, all G loads in flight; bound by memory.
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
-    decay_share_kernel(const float* x, T* out, int64_t n, int G, int d) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    decay_share_kernel(const float* x, int64_t x_step, T* out0, T* out1, int64_t n, int G, int d) {
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
   if (e >= n) return;
-  const int64_t row = e / d;  // [B, N, Hk]
-  const float* src = x + row * G * d + e % d;
-  float s = 0.f;
-  for (int g = 0; g < G; ++g) s += src[(int64_t)g * d];
-  out[e] = from_f32<T>(s);
+  struct alignas(4 * V) In {
+    float x[V];
+  };
+  struct alignas(sizeof(T) * V) Out {
+    T x[V];
+  };
+  const int64_t row = n >> 32 ? e / d : (int64_t)((unsigned)e / (unsigned)d);  // [B, N, Hk]
+  const float* src = x + blockIdx.y * x_step + row * G * d + (e - row * d);
+  In s = {};
+#pragma unroll 4
+  for (int g = 0; g < G; ++g) {
+    const In y = *reinterpret_cast<const In*>(src + (int64_t)g * d);
+#pragma unroll
+    for (int v = 0; v < V; ++v) s.x[v] += y.x[v];
+  }
+  Out o;
+#pragma unroll
+  for (int v = 0; v < V; ++v) o.x[v] = from_f32<T>(s.x[v]);
+  *reinterpret_cast<Out*>((blockIdx.y ? out1 : out0) + e) = o;
 }
 
-
+template <typename T>
+cudaError_t share_go(const float* x, int64_t x_step, void* out0, void* out1, int64_t n, int G,
+                     int d, cudaStream_t s) {
+  const int V = d % 4 == 0 ? 4 : 1;
+  const dim3 grid((unsigned)((n / V + 255) / 256), 2);
+  T *o0 = static_cast<T*>(out0), *o1 = static_cast<T*>(out1);
+  if (V == 4)
+    decay_share_kernel<T, 4><<<grid, 256, 0, s>>>(x, x_step, o0, o1, n, G, d);
+  else
+    decay_share_kernel<T, 1><<<grid, 256, 0, s>>>(x, x_step, o0, o1, n, G, d);
+  return cudaGetLastError();
+}
 
 template <typename T, int DP, bool REV, int MODE>
 cudaError_t scan_go(const DecayParams& p, cudaStream_t s) {
@@ -574,15 +601,11 @@ cudaError_t launch_decay_rows(const DecayParams& p, bool bf16, cudaStream_t s) {
   return launch_scan(p, p.row_out && !p.out ? SC_ROWS : SC_COLS, bf16, s);
 }
 
-cudaError_t launch_decay_share(const float* x, void* out, int64_t rows, int Hk, int G, int d,
-                               bool bf16, cudaStream_t s) {
+cudaError_t launch_decay_share(const float* x, int64_t x_step, void* out0, void* out1,
+                               int64_t rows, int Hk, int G, int d, bool bf16, cudaStream_t s) {
   const int64_t n = rows * Hk * d;
-  const unsigned blocks = (unsigned)((n + 255) / 256);
-  if (bf16)
-    decay_share_kernel<<<blocks, 256, 0, s>>>(x, static_cast<__nv_bfloat16*>(out), n, G, d);
-  else
-    decay_share_kernel<<<blocks, 256, 0, s>>>(x, static_cast<float*>(out), n, G, d);
-  return cudaGetLastError();
+  return bf16 ? share_go<__nv_bfloat16>(x, x_step, out0, out1, n, G, d, s)
+              : share_go<float>(x, x_step, out0, out1, n, G, d, s);
 }
 
 }  // namespace tarmac

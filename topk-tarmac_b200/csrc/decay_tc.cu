@@ -1,5 +1,5 @@
 // decay_tc.cu — attention with a decay for each head on the tensor memory
-// (tcgen05), bf16 rows of 40 to 128 columns. The form is that of decay.cuh, in
+// (tcgen05), bf16 rows of 16 to 128 columns. The form is that of decay.cuh, in
 // chunks of 128 rows:
 //   P = a b^T, out = (l^(i-j) P, j <= i) c + l^(i+1) a S,
 //   S = l^n S + (l^(n-1-j) b)^T c.
@@ -253,11 +253,12 @@ __device__ __forceinline__ void times(uint32_t (&v)[32], float f) {
   }
 }
 
-// D[tmem] (+)= C^T B over 128 rows; both tiles by rows (MN-major operands)
+// D[tmem] (+)= C^T B over ROWS rows; both tiles by rows (MN-major operands)
+template <int ROWS = DT_T>
 __device__ __forceinline__ void issue_state(uint32_t tmem_d, uint64_t dc, uint64_t db,
                                             uint32_t idesc, bool add) {
 #pragma unroll
-  for (int ks = 0; ks < DT_T / 16; ++ks)
+  for (int ks = 0; ks < ROWS / 16; ++ks)
     tc::mma_bf16(tmem_d, dc + (uint64_t)((ks * 2048) >> 4), db + (uint64_t)((ks * 2048) >> 4),
                  idesc, add || ks > 0);
 }
@@ -739,17 +740,18 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
 // ---------------------------------------------------------------------------
 // what each segment adds to the state
 // ---------------------------------------------------------------------------
+// A chunk is split and multiplied by halves of 64 rows: one half's product runs
+// while the other is split, and the lower parts need one place only.
 template <int PLANES>
 struct DsTcPlan {
   static constexpr int NS = PLANES == 1 ? 3 : 2;
-  // The lower parts have one place: a chunk is split after the product of the
-  // one before. Without them it is weighted while that product runs.
-  static constexpr bool AHEAD = PLANES == 1;
   static constexpr int SMEM = (2 * NS + PLANES - 1) * DT_TILE + 1024;
 };
 template <int NS>
 struct DsTcShared {
-  uint64_t full[NS], empty[NS], conv, udone[2], drain;
+  uint64_t full[NS], empty[NS];
+  uint64_t conv[2], done[2];  // by half: split, multiplied
+  uint64_t drain;
   uint32_t tmem;
   int abort_flag;
 };
@@ -759,7 +761,6 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
     decay_state_tc_kernel(const __grid_constant__ CUtensorMap mb,
                           const __grid_constant__ CUtensorMap mc, DecayParams p, DtGrid g) {
   constexpr int NS = DsTcPlan<PLANES>::NS;
-  constexpr bool AHEAD = DsTcPlan<PLANES>::AHEAD;
   extern __shared__ unsigned char dt_raw[];
   __shared__ DsTcShared<NS> sh;
   const uint32_t base = (tc::smem_addr(dt_raw) + 1023u) & ~1023u;
@@ -771,9 +772,10 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       tc::mbar_init(&sh.full[s], 1);
       tc::mbar_init(&sh.empty[s], 1);
     }
-    tc::mbar_init(&sh.conv, 16);
-    tc::mbar_init(&sh.udone[0], 1);
-    tc::mbar_init(&sh.udone[1], 1);
+    for (int q = 0; q < 2; ++q) {
+      tc::mbar_init(&sh.conv[q], 16);
+      tc::mbar_init(&sh.done[q], 1);
+    }
     tc::mbar_init(&sh.drain, 1);
     sh.abort_flag = 0;
     tc::mbar_init_fence();
@@ -815,19 +817,24 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       const DtUnit w = dt_unit<PAIR>(p, g, unit);
       for (int x = w.a0; x < w.a1 && ok; ++x, ++c) {
         const uint32_t s = c % NS, at = base + s * 2 * DT_TILE;
-        const uint64_t dc = ht::desc128(at + DT_TILE, DT_HALF);
-        ok = ht::wait_at(tc::smem_addr(&sh.conv), c & 1, abort_flag);
-        tc::fence_after_sync();
-        if (ok && leader) {
-          const uint32_t d = tmem + (c & 1) * 128;
-          issue_state(d, dc, ht::desc128(at, DT_HALF), id_s, false);
+        const uint32_t d = tmem + (c & 1) * 128;
 #pragma unroll
-          for (int q = 1; q < PLANES; ++q)
-            issue_state(d, dc, ht::desc128(extra + (q - 1) * DT_TILE, DT_HALF), id_s, true);
-          ht::commit_at(tc::smem_addr(&sh.udone[c & 1]));
-          ht::commit_at(tc::smem_addr(&sh.empty[s]));
+        for (int hf = 0; hf < 2; ++hf) {
+          ok = ok && ht::wait_at(tc::smem_addr(&sh.conv[hf]), c & 1, abort_flag);
+          tc::fence_after_sync();
+          if (ok && leader) {
+            const uint32_t rows = hf * DT_HALF / 2;  // bytes of half a tile's rows
+            const uint64_t dc = ht::desc128(at + DT_TILE + rows, DT_HALF);
+#pragma unroll
+            for (int q = 0; q < PLANES; ++q)
+              issue_state<DT_T / 2>(
+                  d, dc, ht::desc128((q ? extra + (q - 1) * DT_TILE : at) + rows, DT_HALF), id_s,
+                  hf || q);
+            ht::commit_at(tc::smem_addr(&sh.done[hf]));
+            if (hf) ht::commit_at(tc::smem_addr(&sh.empty[s]));
+          }
+          __syncwarp();
         }
-        __syncwarp();
         ok = ht::agree(ok);
       }
     }
@@ -854,7 +861,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       for (int e = 0; e < SC; ++e) S[e] = 0.f;
       // S = l^n S + the product of chunk c_
       auto take = [&](uint32_t c_, int n) {
-        if (ok) ok = ht::warp_wait(&sh.udone[c_ & 1], (c_ >> 1) & 1, abort_flag);
+        if (ok) ok = ht::warp_wait(&sh.done[1], c_ & 1, abort_flag);
         if (!ok) return;
         tc::fence_after_sync();
         uint32_t u[SC];
@@ -879,51 +886,62 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       for (int x = w.a0; x < w.a1; ++x, ++c) {
         const int n = dt_rows(w, dt_chunk(p, g, x)), s = c % NS;
         if (n < DT_T) weights(n);
-        if (!AHEAD && x > w.a0) take(c - 1, n_before);
         if (ok) ok = ht::warp_wait(&sh.full[s], (c / NS) & 1, abort_flag);
         // a warp that gave up does not touch what the others still use
         if (!ok) continue;
         const uint32_t at = base + s * 2 * DT_TILE;
+        // pieces tid + 512 e: those with e = hf and hf + 2 are rows of half hf
         uint4 v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = ld_piece(at + (tid + 512 * e) * 16);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int piece = tid + 512 * e;
-          if constexpr (PLANES == 1) {
-            st_piece(at + piece * 16, weighted(v[e], f[e]));
-          } else {
-            const uint32_t in[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
-            uint32_t part[PLANES][4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float a = lo_half(in[i]) * f[e], b = hi_half(in[i]) * f[e];
-#pragma unroll
-              for (int q = 0; q < PLANES; ++q) part[q][i] = split_off(a, b);
-            }
-            st_piece(at + piece * 16, make_uint4(part[0][0], part[0][1], part[0][2], part[0][3]));
-#pragma unroll
-            for (int q = 1; q < PLANES; ++q)
-              st_piece(extra + (q - 1) * DT_TILE + piece * 16,
-                       make_uint4(part[q][0], part[q][1], part[q][2], part[q][3]));
+        for (int hf = 0; hf < 2; ++hf) {
+          // This half of the chunk before is multiplied: its lower parts may go, and
+          // the issuing warp has seen its conv. (A unit ends with a take.)
+          if (x > w.a0) {
+            if (hf)
+              take(c - 1, n_before);
+            else
+              ok = ht::warp_wait(&sh.done[0], (c - 1) & 1, abort_flag);
           }
-        }
-        if (n < DT_T) {  // rows that are not there, whatever the tiles hold
-          weights(DT_T);
-#pragma unroll 1
-          for (int e = 0; e < 4; ++e) {
+          if (!ok) break;
+#pragma unroll
+          for (int e = hf; e < 4; e += 2) {
             const int piece = tid + 512 * e;
-            if (((piece & 1023) >> 3) < n) continue;
-            st_shared_zero16(at + piece * 16);
-            for (int q = 1; q < PLANES; ++q)
-              st_shared_zero16(extra + (q - 1) * DT_TILE + piece * 16);
-            if (w.len < p.N) st_shared_zero16(at + DT_TILE + piece * 16);
+            if constexpr (PLANES == 1) {
+              st_piece(at + piece * 16, weighted(v[e], f[e]));
+            } else {
+              const uint32_t in[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
+              uint32_t part[PLANES][4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float a = lo_half(in[i]) * f[e], b = hi_half(in[i]) * f[e];
+#pragma unroll
+                for (int q = 0; q < PLANES; ++q) part[q][i] = split_off(a, b);
+              }
+              st_piece(at + piece * 16, make_uint4(part[0][0], part[0][1], part[0][2], part[0][3]));
+#pragma unroll
+              for (int q = 1; q < PLANES; ++q)
+                st_piece(extra + (q - 1) * DT_TILE + piece * 16,
+                         make_uint4(part[q][0], part[q][1], part[q][2], part[q][3]));
+            }
           }
+          if (n < (hf + 1) * DT_T / 2) {  // rows that are not there, whatever the tiles hold
+#pragma unroll 1
+            for (int e = hf; e < 4; e += 2) {
+              const int piece = tid + 512 * e;
+              if (((piece & 1023) >> 3) < n) continue;
+              st_shared_zero16(at + piece * 16);
+              for (int q = 1; q < PLANES; ++q)
+                st_shared_zero16(extra + (q - 1) * DT_TILE + piece * 16);
+              if (w.len < p.N) st_shared_zero16(at + DT_TILE + piece * 16);
+            }
+          }
+          tc::fence_async_smem();
+          __syncwarp();
+          if (lane == 0) ws::arrive(&sh.conv[hf]);
         }
-        tc::fence_async_smem();
-        __syncwarp();
-        if (lane == 0) ws::arrive(&sh.conv);
-        if (AHEAD && x > w.a0) take(c - 1, n_before);
+        if (n < DT_T) weights(DT_T);
         n_before = n;
       }
       if (w.a1 > w.a0) take(c - 1, n_before);
