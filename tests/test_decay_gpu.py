@@ -362,3 +362,29 @@ def test_two_streams_at_once():
         torch.cuda.synchronize()
         for out, S in got:
             assert torch.equal(out, want[0]) and torch.equal(S, want[1])
+
+
+@pytest.mark.parametrize("B,d", [(1480, 16), (600, 32), (222, 48), (74, 128)])
+def test_slow_decays_in_one_walk(B, d):
+    """fp32 rows, one walk over all of them, heads that keep about 128 rows. A term
+    m rows old is off by 8 2^-25 inside 16 rows and by 2^-25 for each 16 (on
+    average 16 2^-25 = 4.8e-7, random signs over heads and rows put aside), its
+    sums by the roundings of the 64 rows or so after it (rms 2^-25 each, 8 of them
+    as one: 2.4e-7) and of the output: 1e-6 of the norm. A decay off by 2^-25 in
+    every row would be off by 128 2^-25 = 3.8e-6."""
+    from tarmac_b200 import ops
+    N, H, Hk, some = 512, 2, 1, 3
+    for backward in (False, True):
+        plan = ops.decay_attention_plan(B, N, H, Hk, d, F32, state=True, backward=backward)
+        assert plan["kernel"] == "decay_scan" and plan["segments"] == 1
+    g = torch.Generator().manual_seed(d)
+    q, k, v, dout = (torch.randn(B, N, h, d, generator=g) for h in (H, Hk, Hk, H))
+    S, dS = (torch.randn(B, H, d, d, generator=g) for _ in range(2))
+    rate = -1.0 / torch.tensor([111.0, 143.0])
+    gpu = [t.cuda() for t in (q, k, v, rate, dout, S, dS)]
+    got = ops.decay_attention(*gpu[:4], gpu[5], return_state=True)
+    got = (*got, *ops.decay_attention_backward(*gpu[:6], gpu[6]))
+    q, k, v, dout, S, dS = (t[:some].double() for t in (q, k, v, dout, S, dS))
+    want = d64.decay_grads(q, k, v, rate, d ** -0.5, dout, S, None, dS)
+    for i, (a, b) in enumerate(zip(got, want)):
+        assert (a[:some].double().cpu() - b).norm() <= 1e-6 * b.norm(), i

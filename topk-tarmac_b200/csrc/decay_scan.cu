@@ -134,7 +134,11 @@ __global__ void __launch_bounds__(SC_WARPS * 32, ScPlan<T, DP>::BLOCKS)
     }
   }
   const bool there = bh0 + own < heads;
-  const float rate = decay_rate(p.log_decay, h), l = expf(rate);
+  // A rounded decay would be off by the same 2^-25 in every row: one row in 16 takes
+  // one that makes up for it (N rows of a slow decay: 2e-7 off, not N 2^-25).
+  const float rate = decay_rate(p.log_decay, h);
+  const double exact = exp((double)rate);
+  const float l = (float)exact, mend = l > 0.5f ? (float)(exact + 15. * (exact - l)) : l;
   // those that some head of the warp has, and how they are walked: y in [0, n)
   const int x0 = REV ? max(s0, end - most) : s0, x1 = REV ? s1 : min(s1, most);
   const int rows = x1 - x0, row0 = REV ? (STATES ? end - x1 : end - 1 - x0) : (STATES ? x1 - 1 : x0);
@@ -234,7 +238,7 @@ __global__ void __launch_bounds__(SC_WARPS * 32, ScPlan<T, DP>::BLOCKS)
     }
     cp_async_commit();
   };
-  const uint64_t ll = pack2(l, l);
+  const uint64_t ll = pack2(l, l), ll_mend = pack2(mend, mend);
   // Rows: the decay of S before each; backwards it follows the sum, so the first
   // has none. States: the weight of b.
   uint64_t w = REV != STATES ? pack2(1.f, 1.f) : ll;
@@ -292,13 +296,15 @@ __global__ void __launch_bounds__(SC_WARPS * 32, ScPlan<T, DP>::BLOCKS)
       if constexpr (OUT_C) read_pairs<R, NG>(av, row + AT_A + a_at);
       // a row that this lane's head does not have leaves S alone
       const bool live = HEADS == 1 || row_at(y + t) < len;
+      const uint64_t lt = ((y + t) & 15) == 8 ? ll_mend : ll;
+      if (!STATES && !REV) w = lt;
       const uint64_t wt = STATES || live ? w : pack2(1.f, 1.f);
       if constexpr (STATES) {
 #pragma unroll
         for (int i = 0; i < R / 2; ++i) bv[i] = mul2(bv[i], wt);
-        if (live) w = mul2(w, ll);
+        if (live) w = mul2(w, lt);
       } else if (REV && live) {
-        w = ll;
+        w = lt;
       }
       float o[C], cv[C], ev[OUT_R ? C : 1];
       read_cols(cv, row + AT_C);
