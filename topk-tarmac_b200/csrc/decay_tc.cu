@@ -29,8 +29,15 @@
 // registers: the weighted b as in the rows' kernel for states that only feed
 // the rows, in three bf16 parts (24 bits) for those that the caller gets.
 //
-// Bound by memory: four tiles a chunk (a, b, c, out), 128 KB for 2048 clocks of
-// products at d = 128 (about 5600 clocks of one SM's share of HBM).
+// Measured: 2 x 8192 rows of 16 heads, d = 128, the gradients 184 us (64 chunks of
+// 5500 clocks in each of 96 blocks), the forward pass 27 us of states, 5 of
+// joining and 66 of rows; 32 x 1024 rows of 8 heads, d = 64, gradients 95 us. A
+// chunk at d = 128 has 1280 clocks of products and four tiles to move, 128 KB or
+// 5700 clocks of an SM's share of HBM where no other block reads them too. The
+// chain bounds the rest: state, a S, out, rows follow one another, and what runs
+// beside them is the next P and the weights (tensor pipe 25-37 %, issue 35-43 %).
+// Bound of the states' pass: issue of the split (54 %; two halves a chunk in turn
+// 34 us, a whole chunk at once 43: 2 x 8192 rows of 16 heads on 4, d = 128).
 // Every wait is bounded; one that runs out ends all roles once their copies
 // and products have landed, and every row is written, NaN or right.
 #include "decay.cuh"
@@ -375,6 +382,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
     const bool leader = ht::elect_one();
     bool ok = true;
     uint32_t c = 0, states = 0;  // chunks, and those with a state
+    bool formed = false;         // is P of chunk c?
     auto wait = [&](uint64_t& bar, uint32_t parity) {
       ok = ok && ht::wait_at(tc::smem_addr(&bar), parity, abort_flag);
     };
@@ -397,7 +405,6 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
     for (int unit = blockIdx.x; unit < g.units && ok; unit += gridDim.x) {
       const DecayParams& p = jobs.p[unit % g.jobs];
       const DtUnit w = dt_unit<PAIR>(p, g, unit);
-      bool formed = false;
       for (int x = w.a0; x < w.a1 && ok; ++x, ++c) {
         const bool state = x > w.a0 || starts(p, w);
         const uint32_t odd = c & 1, ph = (c >> 1) & 1;
@@ -430,8 +437,9 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           }
           __syncwarp();
         }
-        // one head: the next chunk's P goes ahead of this one's P c
-        if (!PAIR && x + 1 < w.a1 && landed(c + 1)) {
+        // one head: the next chunk's P, this unit's or the next one's, goes ahead of
+        // this one's P c
+        if (!PAIR && landed(c + 1)) {
           form_p(c + 1);
           formed = true;
         }

@@ -874,10 +874,11 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     ``state`` (fp32 [B, H, d, d], by the columns of k, then of v) is S before
     the first row, zero when None. Returns out [B, N, H, d], or (out, S after
     the last row) with ``return_state`` or a ``state_out`` to write it to: a
-    contiguous tensor like ``state``, or ``state`` itself, renewed in place.
-    Rows from ``lens`` [B] on are padding, whatever they hold: they get 0 and
-    leave S alone; those before must be finite (a head's infinity may reach its
-    rows as a NaN). One new row over a kept state is N = 1."""
+    contiguous tensor like ``state`` and apart from all inputs, or ``state``
+    itself, renewed in place. Rows from ``lens`` [B] on are padding, whatever
+    they hold: they get 0 and leave S alone; those before must be finite (a
+    head's infinity may reach its rows as a NaN). One new row over a kept state
+    is N = 1."""
     if not _decay_ready(q, k, v, log_decay, lens):
         q, k, v, log_decay, lens = _check_decay(q, k, v, log_decay, lens)
     start = _check_state(state, "state", q)
