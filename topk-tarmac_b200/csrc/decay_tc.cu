@@ -57,16 +57,18 @@ constexpr int DT_HALF = DT_TILE / 2;
 constexpr float DT_LOG2E = 1.4426950408889634f;
 
 struct DtGrid {
-  int units, head_units, chunks, jobs;
+  int units, head_units, chunks;  // units of a job
 };
-// Up to three sums over the same heads and rows in one launch: the gradients.
-// Their units lie side by side, as they read the same tensors.
+// One sum, the forward pass, or the gradients' three over the same heads and rows
+// in one launch. A block stays with one job; those of the three lie side by side,
+// as they read the same tensors.
+template <int JOBS>
 struct DtJobs {
-  CUtensorMap map[3][4];  // a, b, c, out
-  DecayParams p[3];
+  CUtensorMap map[JOBS][4];  // a, b, c, out
+  DecayParams p[JOBS];
 };
 
-// One unit (of a job): episode, first head, rows, and the chunks k in [k0, k1) in the
+// One unit: episode, first head, rows, and the chunks k in [k0, k1) in the
 // order they are walked; those in [a0, a1) have rows.
 struct DtUnit {
   int b, h, seg, len, k0, k1, a0, a1;
@@ -74,11 +76,10 @@ struct DtUnit {
 template <bool PAIR>
 __device__ __forceinline__ DtUnit dt_unit(const DecayParams& p, const DtGrid& g, int unit) {
   DtUnit w;
-  unit /= g.jobs;
-  const int x = unit % g.head_units, y = unit / g.head_units;
+  const unsigned y = (unsigned)unit / (unsigned)g.head_units, x = unit - y * g.head_units;
   w.h = PAIR ? 2 * x : x;
-  w.b = y % p.B;
-  w.seg = y / p.B;
+  w.seg = y / (unsigned)p.B;
+  w.b = y - w.seg * p.B;
   w.len = decay_len(p, w.b);
   const int full = cdiv(w.len, DT_T);
   w.k0 = w.seg * p.seg_chunks;
@@ -298,9 +299,9 @@ struct DtShared {
   int abort_flag;
 };
 
-template <int NKS, bool PAIR>
+template <int NKS, bool PAIR, int JOBS>
 __global__ void __launch_bounds__(DT_THREADS, 1)
-    decay_rows_tc_kernel(const __grid_constant__ DtJobs jobs, DtGrid g) {
+    decay_rows_tc_kernel(const __grid_constant__ DtJobs<JOBS> jobs, DtGrid g) {
   using Plan = DtPlan<PAIR>;
   constexpr int HEADS = PAIR ? 2 : 1, CS = Plan::CS;
   extern __shared__ unsigned char dt_raw[];
@@ -312,6 +313,12 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
   auto tile_c = [&](uint32_t c) { return base + Plan::AT_C + (c % CS) * DT_TILE; };
   volatile int* abort_flag = &sh.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int job = JOBS == 1 ? 0 : blockIdx.x % JOBS;
+  const int first_unit = blockIdx.x / JOBS, unit_step = gridDim.x / JOBS;
+  const DecayParams& p = jobs.p[job];
+  const CUtensorMap* map = jobs.map[job];
+  const bool rev = JOBS > 1 && p.reverse, f32 = JOBS > 1 && p.out_f32;
+  const bool transposed = JOBS > 1 && p.transposed;
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       tc::mbar_init(&sh.full_ab[s], 1);
@@ -340,20 +347,18 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
   // P of a chunk: the unit's heads side by side, or two chunks in turn
   auto tmem_p = [&](uint32_t c, int u) { return tmem + (PAIR ? u : (int)(c & 1)) * 128; };
   // does a unit's first chunk start from a state?
-  auto starts = [](const DecayParams& p, const DtUnit& w) {
+  auto starts = [&](const DtUnit& w) {
     return p.part ? w.seg > 0 || p.start : p.start != nullptr;
   };
 
   if (warp == DT_TMA_WARP) {
     if (lane == 0) {
       uint32_t c = 0, cc = 0;  // copies of a and b, of c
-      for (int k = 0, unit = blockIdx.x; unit < g.units; unit += gridDim.x, ++k) {
+      for (int k = 0, unit = first_unit; unit < g.units; unit += unit_step, ++k) {
         if (ht::gives_up(ht::ROLE_LOADER, k)) {
           *abort_flag = 1;
           break;
         }
-        const DecayParams& p = jobs.p[unit % g.jobs];
-        const CUtensorMap* map = jobs.map[unit % g.jobs];
         const DtUnit w = dt_unit<PAIR>(p, g, unit);
         for (int x = w.a0; x < w.a1; ++x) {
           const int s = c & 1, row = dt_chunk(p, g, x) * DT_T;
@@ -402,11 +407,10 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       }
       __syncwarp();
     };
-    for (int unit = blockIdx.x; unit < g.units && ok; unit += gridDim.x) {
-      const DecayParams& p = jobs.p[unit % g.jobs];
+    for (int unit = first_unit; unit < g.units && ok; unit += unit_step) {
       const DtUnit w = dt_unit<PAIR>(p, g, unit);
       for (int x = w.a0; x < w.a1 && ok; ++x, ++c) {
-        const bool state = x > w.a0 || starts(p, w);
+        const bool state = x > w.a0 || starts(w);
         const uint32_t odd = c & 1, ph = (c >> 1) & 1;
         if (!formed) form_p(c);
         formed = false;
@@ -474,7 +478,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
     // all of head `half`
     const int half = (warp - DT_W0) >> 2, i = threadIdx.x & 127, w0 = (warp & 3) * 32;
     const uint32_t lane_off = (uint32_t)w0 << 16;
-    const int c_lo = PAIR ? 0 : half * 64, c_n = max(0, min(64, jobs.p[0].d - c_lo));
+    const int c_lo = PAIR ? 0 : half * 64, c_n = max(0, min(64, p.d - c_lo));
     // The tile that holds the rows of chunk c - 1 may be loaded again once they
     // have been read: asked for only when the next chunk is under way.
     bool held = false;
@@ -494,10 +498,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       if (lane == 0) ws::arrive(&sh.ofree);
     };
     bool ok = true;
-    for (int k = 0, unit = blockIdx.x; unit < g.units; unit += gridDim.x, ++k) {
-      const DecayParams& p = jobs.p[unit % g.jobs];
-      const CUtensorMap* map_out = &jobs.map[unit % g.jobs][3];
-      const bool rev = p.reverse;
+    for (int k = 0, unit = first_unit; unit < g.units; unit += unit_step, ++k) {
       const DtUnit w = dt_unit<PAIR>(p, g, unit);
       if (ht::gives_up(ht::ROLE_WEIGHTS, k)) {
         ok = false;
@@ -555,11 +556,11 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           auto store = [&](int col) {
             tc::fence_async_smem();
             __syncwarp();
-            if (lane == 0 && left > 0) store_box(map_out, stage, c_lo + col, h, chunk * DT_T + w0, w.b);
+            if (lane == 0 && left > 0) store_box(map + 3, stage, c_lo + col, h, chunk * DT_T + w0, w.b);
             __syncwarp();
           };
           part(0);
-          if (!p.out_f32) {
+          if (!f32) {
             stage_row(stage, lane, 0, o);
             part(32);
             stage_row(stage, lane, 4, o);
@@ -578,7 +579,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           held = true;
         } else {
           // padding, or rows given up
-          if (p.out_f32)
+          if (f32)
             fill_rows(static_cast<float*>(p.out) + first, ok ? 0u : 0x7fffffffu, lane, left,
                       (int64_t)p.H * p.d, c_n, 4);
           else
@@ -602,9 +603,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
     // a warp that gave up leaves: it must not touch what the others still use
     bool ok = true;
     uint32_t c = 0, states = 0, us = 0;
-    for (int unit = blockIdx.x; unit < g.units && ok; unit += gridDim.x) {
-      const DecayParams& p = jobs.p[unit % g.jobs];
-      const bool rev = p.reverse;
+    for (int unit = first_unit; unit < g.units && ok; unit += unit_step) {
       const DtUnit w = dt_unit<PAIR>(p, g, unit);
       const int h0 = w.h, h1 = PAIR ? min(w.h + 1, p.H - 1) : w.h;
       const float l2_0 = decay_rate(p.log_decay, h0) * DT_LOG2E;
@@ -612,7 +611,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       const float l2_s = s_head ? l2_1 : l2_0, l2_o = PAIR && half ? l2_1 : l2_0;
       const int hs = s_head ? h1 : h0, rc = PAIR ? r & 63 : r;
       const float* start = nullptr;
-      if (starts(p, w))
+      if (starts(w))
         start = (p.part ? p.part + (int64_t)w.seg * p.B * p.H * p.d * p.d : p.start) +
                 ((int64_t)w.b * p.H + hs) * p.d * p.d;
       // weights of a whole chunk; a chunk of fewer rows makes its own
@@ -687,7 +686,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
               for (int e = 0; e < 32; ++e) {
                 const int bc = b0 + e;
                 const bool in = rc < p.d && bc < p.d;
-                s[e] = in ? __float_as_uint(__ldg(start + (p.transposed ? rc * p.d + bc
+                s[e] = in ? __float_as_uint(__ldg(start + (transposed ? rc * p.d + bc
                                                                         : bc * p.d + rc)))
                           : 0u;
               }
@@ -972,26 +971,25 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
 // ---------------------------------------------------------------------------
 // launch
 // ---------------------------------------------------------------------------
-DtGrid dt_grid(const DecayParams& p, int segs, int jobs) {
+DtGrid dt_grid(const DecayParams& p, int segs) {
   DtGrid g;
   g.head_units = p.d <= 64 ? cdiv(p.H, 2) : p.H;
   g.chunks = cdiv(p.N, DT_T);
-  g.jobs = jobs;
-  g.units = g.head_units * p.B * segs * jobs;
+  g.units = g.head_units * p.B * segs;
   return g;
 }
-int dt_blocks(const DtGrid& g) {
-  const int sms = head_sm_count();
-  return g.units < sms ? g.units : sms;
+int dt_blocks(const DtGrid& g, int jobs) {
+  const int most = head_sm_count() / jobs;
+  return jobs * (g.units < most ? g.units : most);
 }
 
-template <int NKS, bool PAIR>
-cudaError_t rows_go(const DtJobs& jobs, const DtGrid& g, cudaStream_t s) {
+template <int NKS, bool PAIR, int JOBS>
+cudaError_t rows_go(const DtJobs<JOBS>& jobs, const DtGrid& g, cudaStream_t s) {
   constexpr int SMEM = DtPlan<PAIR>::SMEM;
-  const void* fn = reinterpret_cast<const void*>(&decay_rows_tc_kernel<NKS, PAIR>);
+  const void* fn = reinterpret_cast<const void*>(&decay_rows_tc_kernel<NKS, PAIR, JOBS>);
   const cudaError_t e = raise_smem_limit(fn, SMEM);
   if (e != cudaSuccess) return e;
-  decay_rows_tc_kernel<NKS, PAIR><<<dt_blocks(g), DT_THREADS, SMEM, s>>>(jobs, g);
+  decay_rows_tc_kernel<NKS, PAIR, JOBS><<<dt_blocks(g, JOBS), DT_THREADS, SMEM, s>>>(jobs, g);
   return cudaGetLastError();
 }
 template <bool PAIR, int PLANES>
@@ -1000,7 +998,7 @@ cudaError_t state_go(const CUtensorMap* m, const DecayParams& p, const DtGrid& g
   const void* fn = reinterpret_cast<const void*>(&decay_state_tc_kernel<PAIR, PLANES>);
   const cudaError_t e = raise_smem_limit(fn, SMEM);
   if (e != cudaSuccess) return e;
-  decay_state_tc_kernel<PAIR, PLANES><<<dt_blocks(g), DT_THREADS, SMEM, s>>>(m[0], m[1], p, g);
+  decay_state_tc_kernel<PAIR, PLANES><<<dt_blocks(g, 1), DT_THREADS, SMEM, s>>>(m[0], m[1], p, g);
   return cudaGetLastError();
 }
 
@@ -1024,7 +1022,8 @@ DecayPlan decay_plan_tc(int B, int N, int H, int d, int jobs) {
   double least = 0;
   for (int want = 1; want <= chunks && want <= 256; ++want) {
     const int per = cdiv(chunks, want), segs = cdiv(chunks, per);
-    double cost = (double)((heads * segs * jobs + 147) / 148) * (per + 1.5);
+    const int blocks = 148 / jobs;
+    double cost = (double)((heads * segs + blocks - 1) / blocks) * (per + 1.5);
     if (segs > 1)
       cost += (jobs > 1 ? 2 : 1) *
               ((double)((heads * (segs - 1) + 147) / 148) * (per + 1.5) * 0.65 + 4.0);
@@ -1038,7 +1037,7 @@ DecayPlan decay_plan_tc(int B, int N, int H, int d, int jobs) {
 
 cudaError_t launch_decay_states_tc(const DecayParams& p, cudaStream_t s) {
   // the last segment's share counts only where the state after it is wanted
-  const DtGrid g = dt_grid(p, p.last ? p.segs : p.segs - 1, 1);
+  const DtGrid g = dt_grid(p, p.last ? p.segs : p.segs - 1);
   if (g.units == 0) return cudaSuccess;
   CUtensorMap m[2];
   if (!map_of(&m[0], p, p.b, p.sb, p.gb) || !map_of(&m[1], p, p.c, p.sc, p.gc))
@@ -1047,9 +1046,10 @@ cudaError_t launch_decay_states_tc(const DecayParams& p, cudaStream_t s) {
   return p.planes > 2 ? state_go<false, 3>(m, p, g, s) : state_go<false, 1>(m, p, g, s);
 }
 
-cudaError_t launch_decay_rows_tc(const DecayParams* p, int jobs, cudaStream_t s) {
-  DtJobs all;
-  for (int j = 0; j < jobs; ++j) {
+template <int JOBS>
+cudaError_t launch_jobs(const DecayParams* p, cudaStream_t s) {
+  DtJobs<JOBS> all;
+  for (int j = 0; j < JOBS; ++j) {
     const DecayParams& q = p[j];
     const HeadStrides so = {(int64_t)q.N * q.H * q.d, (int64_t)q.H * q.d, q.d};
     CUtensorMap* m = all.map[j];
@@ -1059,10 +1059,16 @@ cudaError_t launch_decay_rows_tc(const DecayParams* p, int jobs, cudaStream_t s)
       return cudaErrorInvalidValue;
     all.p[j] = q;
   }
-  const DtGrid g = dt_grid(p[0], p[0].segs, jobs);
-  if (p[0].d <= 64) return rows_go<4, true>(all, g, s);
-  if (p[0].d <= 96) return rows_go<6, false>(all, g, s);
-  return rows_go<8, false>(all, g, s);
+  const DtGrid g = dt_grid(p[0], p[0].segs);
+  if (p[0].d <= 64) return rows_go<4, true, JOBS>(all, g, s);
+  if (p[0].d <= 96) return rows_go<6, false, JOBS>(all, g, s);
+  return rows_go<8, false, JOBS>(all, g, s);
+}
+cudaError_t launch_decay_rows_tc(const DecayParams* p, int jobs, cudaStream_t s) {
+  if (jobs == 3) return launch_jobs<3>(p, s);
+  // a single one is the forward pass's
+  if (jobs != 1 || p->reverse || p->transposed || p->out_f32) return cudaErrorInvalidValue;
+  return launch_jobs<1>(p, s);
 }
 
 }  // namespace tarmac
