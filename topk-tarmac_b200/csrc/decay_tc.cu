@@ -29,9 +29,9 @@
 // registers: the weighted b as in the rows' kernel for states that only feed
 // the rows, in three bf16 parts (24 bits) for those that the caller gets.
 //
-// Measured: 2 x 8192 rows of 16 heads, d = 128, the gradients 184 us (64 chunks of
-// 5500 clocks in each of 96 blocks), the forward pass 27 us of states, 5 of
-// joining and 66 of rows; 32 x 1024 rows of 8 heads, d = 64, gradients 95 us. A
+// Measured: 2 x 8192 rows of 16 heads, d = 128, the gradients 190-196 us (64 chunks
+// of 5800 clocks in each of 96 blocks), the forward pass 28 us of states, 5 of
+// joining and 56 of rows; 32 x 1024 rows of 8 heads, d = 64, 37 and 93 us. A
 // chunk at d = 128 has 1280 clocks of products and four tiles to move, 128 KB or
 // 5700 clocks of an SM's share of HBM where no other block reads them too. The
 // chain bounds the rest: state, a S, out, rows follow one another, and what runs
@@ -1014,7 +1014,8 @@ bool map_of(CUtensorMap* m, const DecayParams& p, const void* ptr, const HeadStr
 // thirds of one, its launch and the joining four. The gradients' three sums need
 // two such passes. Host arithmetic for 148 SMs, so that a caller can ask for the
 // scratch without a GPU. 2 x 8192 rows of 16 heads, d = 128, gradients: 96 units
-// of 64 chunks 184 us, three segments with their states 219.
+// of 64 chunks 184 us, three segments with their states 219 (an earlier form of
+// the rows' kernel).
 DecayPlan decay_plan_tc(int B, int N, int H, int d, int jobs) {
   const int64_t heads = (int64_t)B * (d <= 64 ? cdiv(H, 2) : H);
   const int chunks = cdiv(N, DT_T);
