@@ -70,11 +70,11 @@ class Case:
         return out, last, dq, dk, dv, first
 
     def check(self, got):
-        """fp32 1e-5 of the sum of absolute terms: two products of 3 2^-22
-        each, exponents up to 88 before a power is zero (88 2^-24), 2^-24 for
-        each addition that a term passes (a few dozen).
-        bf16: a weight or the state's copy is off by 2^-8 and then the output,
-        by each term; as independent errors they leave at most 2^-8 of the
+        """fp32 1e-5 of the sum of absolute terms: exponents up to 88 before a
+        power is zero (88 2^-24), 2^-24 for each product and addition that a
+        term passes (a few dozen).
+        bf16: a weight of P or of b is off by 2^-8 and then the output, by each
+        term; as independent errors they leave at most 2^-8 of the
         tensor's norm (three roundings of rms 2^-8 / sqrt 3 each). States
         are fp32's for both types."""
         want, mags = self.want(), self.mags()
@@ -223,6 +223,25 @@ def test_state_in_place_by_segments(B, N, d, segments):
         s = S.clone()
         out2, got = ops.decay_attention(q, k, v, rate, s, lens, state_out=s)
         assert got is s and torch.equal(s, want) and torch.equal(out, out2)
+
+
+def test_state_in_place_captured():
+    """A captured call that renews its state, replayed: call after call."""
+    from tarmac_b200 import ops
+    c = Case(2, 100, 2, 1, 16, F32)
+    q, k, v, S, rate = (t.cuda() for t in (c.q, c.k, c.v, c.state, c.rate))
+    want, s = S.clone(), S.clone()
+    for _ in range(3):
+        o, want = ops.decay_attention(q, k, v, rate, want, return_state=True)
+    ops.decay_attention(q, k, v, rate, S.clone(), return_state=True)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, _ = ops.decay_attention(q, k, v, rate, s, state_out=s)
+    s.copy_(S)
+    for _ in range(3):
+        g.replay()
+    assert torch.equal(s, want) and torch.equal(out, o)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

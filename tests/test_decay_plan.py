@@ -15,8 +15,10 @@ F32, BF16 = torch.float32, torch.bfloat16
     ((256, 1, 4, 4, 16), F32, "decay_step"),
     ((256, 8, 4, 4, 128), BF16, "decay_step"),
     ((256, 9, 4, 4, 16), F32, "decay_scan"),
-    ((256, 23, 4, 4, 64), BF16, "decay_scan"),
-    ((256, 24, 4, 4, 64), BF16, "decay_tc"),
+    ((256, 23, 4, 4, 32), BF16, "decay_scan"),
+    ((256, 24, 4, 4, 32), BF16, "decay_tc"),
+    ((256, 15, 4, 4, 64), BF16, "decay_scan"),
+    ((256, 16, 4, 4, 64), BF16, "decay_tc"),
     ((256, 24, 4, 4, 64), F32, "decay_scan"),
     ((256, 11, 4, 4, 72), BF16, "decay_scan"),
     ((256, 12, 4, 4, 72), BF16, "decay_tc"),

@@ -567,11 +567,11 @@ DecayPlan decay_plan(int B, int N, int H, int d, bool tc, int jobs) {
 
 bool decay_tc_sizes(int B, int N, int H, int d, bool bf16) {
   // Measured, the tensor memory against the recurrent form (us, the forward pass
-  // with the gradients): 2048 heads, d = 64: 16 rows 104 / 102, 32 rows 108 /
-  // 184; d = 128: 16 rows 156 / 342; 4 heads, d = 64: 16 rows 33 / 31, 32 rows
-  // 33 / 49, 64 rows 33 / 104. Narrow: 32 x 4096 rows of 8 heads, d = 32: 435 /
-  // 992; 64 x 4096, d = 16: 808 / 823.
-  return bf16 && d >= 16 && d % 8 == 0 && N >= (d > 64 ? 12 : 24);
+  // with the gradients): d = 64: 2048 heads, 12 rows 103 / 88, 16 rows 104 / 108,
+  // 32 rows 104 / 184; 4 heads, 12 to 32 rows 18 / 29 to 49; d = 128, 2048 heads:
+  // 16 rows 161 / 342; d = 32: 2048 heads, 16 rows 104 / 43, 4 heads 18 / 27, 32 x
+  // 4096 rows of 8 heads 446 / 992; d = 16, 64 x 4096 rows 808 / 823.
+  return bf16 && d >= 16 && d % 8 == 0 && N >= (d > 64 ? 12 : (d > 32 ? 16 : 24));
 }
 bool decay_one_walk(int d, bool tc) { return !tc && d <= 32; }
 
