@@ -1,0 +1,59 @@
+"""Attention with a decay whose heads keep thousands of rows: a decay rounded to
+fp32 and applied again and again must not add its rounding up.
+
+Heads keep about T rows and read T rows. A factor off by e in each of T / n
+places is off by e m at an age of m places, and the state by 0.43 T / n e of its
+norm (the root mean square of an age under weights exp(-a / T) over [0, T]). The
+rates are those around -1 / T whose l^n is farthest from an fp32 number,
+e close to 2^-25. What remains is the rounding of the sums: one of the state a
+place leaves sqrt(0.34 T / n) of at most 2^-24 / sqrt(3) (a uniform rounding's root
+mean square, at the mantissa where it is largest) of the norm."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def closed(k, v, rate, start=None, scale=1.0):
+    """l^N start + scale sum_t l^(N - 1 - t) k_t v_t^T in float64, [B, H, d, d]."""
+    N, H, d = k.shape[1], rate.shape[0], k.shape[3]
+    age = torch.arange(N - 1, -1, -1, device=k.device, dtype=torch.float64)[:, None]
+    w = torch.exp(rate.double() * age)[None, :, :, None] * scale  # [1, N, H, 1]
+    heads = []
+    for h in range(H):
+        a, b = (t[:, :, h * t.shape[2] // H].double() for t in (k, v))
+        heads.append((a * w[:, :, h]).transpose(1, 2) @ b)
+    S = torch.stack(heads, 1)
+    if start is not None:
+        S = S + torch.exp(rate.double() * N)[:, None, None] * start.double()
+    return S
+
+
+def off(got, want):
+    """The largest distance of a head, of its norm."""
+    return ((got.double() - want).flatten(2).norm(dim=2) / want.flatten(2).norm(dim=2)).max()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 8])
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+def test_steps_in_place(d, rows, dtype):
+    """600 rows in calls of one or eight over a state renewed in place. A row
+    rounds the state twice: sqrt(2 0.34 600) 2^-24 / sqrt(3) = 7e-7, bound 1e-6; a
+    decay off in every row would leave 0.43 600 2^-25 = 7.7e-6."""
+    from tarmac_b200 import ops
+    B, T = 3, 600
+    keep = torch.tensor([532.0, 516.0, 585.0, 483.0, 522.0, 716.0])
+    rate, H = (-1.0 / keep).cuda(), 6
+    g = torch.Generator(device="cuda").manual_seed(d + rows)
+    q, k, v = (torch.randn(B, T, H, d, generator=g, device="cuda").to(dtype) for _ in range(3))
+    S = torch.randn(B, H, d, d, generator=g, device="cuda")
+    want = closed(k, v, rate, S)
+    for t in range(0, T, rows):
+        ops.decay_attention(*(x[:, t:t + rows] for x in (q, k, v)), rate, S, state_out=S)
+    assert off(S, want) <= 1e-6

@@ -44,6 +44,21 @@ __device__ __forceinline__ float decay_rate(const float* log_decay, int h) {
   const float r = __ldg(log_decay + h);
   return r < -1e4f ? -1e4f : r;  // NaN stays
 }
+// The decay of n rows, l^n = exp(rate n), that is applied to a state again and
+// again: by one fp32 number every application would be off by the same rounding.
+struct DecayPower {
+  float base, add;  // l^n = base + add
+  __device__ __forceinline__ DecayPower(float rate, float n) {
+    const float m = expm1f(rate * n), e = expf(rate * n);
+    // slow: 1 + m, m good to 24 bits of its own. Fast, or NaN: what is rounded is
+    // gone after a few applications.
+    const bool slow = m > -0.5f;
+    base = slow ? 1.f : 0.f;
+    add = slow ? m : e;
+  }
+  // l^n s, rounded once
+  __device__ __forceinline__ float times(float s) const { return fmaf(add, s, base * s); }
+};
 __device__ __forceinline__ int decay_len(const DecayParams& p, int b) {
   return p.lens ? max(0, min(__ldg(p.lens + b), p.N)) : p.N;
 }
