@@ -7,10 +7,13 @@
 // A thread holds four neighbouring columns of RPT of S's rows; the lanes of a
 // row are neighbours, so a warp moves whole 16-byte vectors of consecutive
 // rows. Only the sum over S's rows crosses threads: by shuffles in the warp,
-// then through shared memory. The state may be renewed in place: a block reads
-// its head's state before it writes it. 512 x 16 heads of 128 columns: 173 us a
-// call, 6.3 TB/s (96 % of the copy rate); 1024 x 8 heads of 64: 49 us; 256 x 4
-// heads of 16: 3.3 us, latency.
+// then through shared memory. A state that is renewed row by row, call after call,
+// must not gather the rounding of l: 600 rows of slow decays were 8e-6 of the norm
+// off 64 bits with l in one fp32 number, 6e-7 with l as 1 + m (DecayPower). The
+// state may be renewed in place: a block reads its head's state before it writes
+// it. 512 x 16 heads of 128 columns: 173 us a call that is repeated, 6.3 TB/s (96 %
+// of the copy rate), 201 us when L2 holds none of it; 1024 x 8 heads of 64: 49 us;
+// 256 x 4 heads of 16: 3.4 us, latency.
 #include "decay.cuh"
 
 namespace tarmac {
