@@ -34,6 +34,12 @@ def closed(k, v, rate, start=None, scale=1.0):
     return S
 
 
+def first_state(q, dout, rate, dstate, scale):
+    """The gradient of the state before the first row: l R_0."""
+    lam = torch.exp(rate.double())[:, None, None]
+    return lam * closed(q.flip(1), dout.flip(1), rate, dstate / lam, scale)
+
+
 def off(got, want):
     """The largest distance of a head, of its norm."""
     return ((got.double() - want).flatten(2).norm(dim=2) / want.flatten(2).norm(dim=2)).max()
@@ -57,3 +63,33 @@ def test_steps_in_place(d, rows, dtype):
     for t in range(0, T, rows):
         ops.decay_attention(*(x[:, t:t + rows] for x in (q, k, v)), rate, S, state_out=S)
     assert off(S, want) <= 1e-6
+
+
+def both_states(B, N, H, Hk, d, dtype, keep, kernel, segments, tol, expand):
+    """The state after the last row and the gradient of the first."""
+    from tarmac_b200 import ops
+    for backward in (False, True):
+        plan = ops.decay_attention_plan(B, N, H, Hk, d, dtype, state=True, backward=backward)
+        assert plan["kernel"] == kernel
+        assert segments[0] <= plan["segments"] <= segments[1]
+    rate = (-1.0 / torch.tensor(keep)).cuda()
+    g = torch.Generator(device="cuda").manual_seed(N + d)
+    b = 1 if expand else B
+    q, k, v, dout = (torch.randn(b, N, h, d, generator=g, device="cuda").to(dtype)
+                     .expand(B, -1, -1, -1) for h in (H, Hk, Hk, H))
+    S, dS = (torch.randn(b, H, d, d, generator=g, device="cuda").expand(B, -1, -1, -1)
+             for _ in range(2))
+    last = ops.decay_attention(q, k, v, rate, S, return_state=True)[1]
+    first = ops.decay_attention_backward(q, k, v, rate, dout, S, dS)[3]
+    some = [0, B - 1] if B > 1 else [0]
+    q, k, v, dout, S, dS = (t[some] for t in (q, k, v, dout, S, dS))
+    assert off(last[some], closed(k, v, rate, S)) <= tol
+    assert off(first[some], first_state(q, dout, rate, dS, d ** -0.5)) <= tol
+
+
+@pytest.mark.parametrize("B,d", [(1480, 8), (592, 24), (222, 40), (74, 72)])
+def test_one_walk(B, d):
+    """fp32 rows one after the other, 16384 of them. One rounding of the state a
+    row: sqrt(0.34 16384) 2^-24 / sqrt(3) = 2.6e-6, 16 rows by themselves 2.4e-7:
+    bound 3e-6. Off once in 16 rows: 0.43 1024 2^-25 = 1.3e-5."""
+    both_states(B, 16384, 2, 2, d, F32, [16384.0, 15794.0], "decay_scan", (1, 1), 3e-6, True)

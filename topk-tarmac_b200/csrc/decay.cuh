@@ -59,6 +59,24 @@ struct DecayPower {
   // l^n s, rounded once
   __device__ __forceinline__ float times(float s) const { return fmaf(add, s, base * s); }
 };
+// The same as one factor at a time, where a product takes no second number: next()
+// gives an fp32 number near l^n whose roundings are made up for by those after it,
+// so that no run of them is off by more than 2^-24. `of`: what l^n itself is off
+// from `hi` counts that many times.
+struct DecayFactor {
+  float hi, lo, left;
+  __device__ __forceinline__ static DecayFactor make(float rate, float n, float of = 1.f) {
+    const DecayPower l(rate, n);
+    const float hi = l.base + l.add;
+    // base is 1 and add in (-0.5, 0], or base is 0: the difference is exact
+    return DecayFactor{hi, of * (l.add - (hi - l.base)), 0.f};
+  }
+  __device__ __forceinline__ float next() {
+    const float want = left + lo, x = hi + want;
+    left = want - (x - hi);
+    return x;
+  }
+};
 __device__ __forceinline__ int decay_len(const DecayParams& p, int b) {
   return p.lens ? max(0, min(__ldg(p.lens + b), p.N)) : p.N;
 }
