@@ -93,3 +93,14 @@ def test_one_walk(B, d):
     row: sqrt(0.34 16384) 2^-24 / sqrt(3) = 2.6e-6, 16 rows by themselves 2.4e-7:
     bound 3e-6. Off once in 16 rows: 0.43 1024 2^-25 = 1.3e-5."""
     both_states(B, 16384, 2, 2, d, F32, [16384.0, 15794.0], "decay_scan", (1, 1), 3e-6, True)
+
+
+@pytest.mark.parametrize("H,d,keep", [
+    (8, 16, [57737.0, 66781.0, 63963.0, 71565.0, 72941.0, 58589.0, 65536.0, 60000.0]),
+    (1, 40, [66781.0])])
+def test_many_segments(H, d, keep):
+    """fp32 rows in 683 segments of 96 or 820 of 80. A segment's rows: weights off
+    by up to 96 2^-25 / 2, as a random walk sqrt(96) 2^-24 / sqrt(3) = 3.4e-7; a rounding
+    where segments are joined: sqrt(0.34 820) 2^-24 / sqrt(3) = 5.7e-7; bound 1.5e-6. Off
+    in every segment: 0.43 683 2^-25 = 8.7e-6."""
+    both_states(1, 65536, H, H, d, F32, keep, "decay_scan", (600, 900), 1.5e-6, False)
