@@ -104,3 +104,15 @@ def test_many_segments(H, d, keep):
     where segments are joined: sqrt(0.34 820) 2^-24 / sqrt(3) = 5.7e-7; bound 1.5e-6. Off
     in every segment: 0.43 683 2^-25 = 8.7e-6."""
     both_states(1, 65536, H, H, d, F32, keep, "decay_scan", (600, 900), 1.5e-6, False)
+
+
+@pytest.mark.parametrize("B,N,H,Hk,d,keep", [
+    (37, 65536, 8, 8, 16, [66780.0, 76152.0, 57800.0, 77396.0, 55900.0, 71496.0, 65536.0, 60000.0]),
+    (18, 32768, 8, 1, 72, [33390.0, 38076.0, 28900.0, 38698.0, 27950.0, 35748.0, 32768.0, 30000.0])])
+def test_many_chunks(B, N, H, Hk, d, keep):
+    """bf16 rows, chunks of 128 on the tensor memory. A weight is off by 2^-22 (the
+    exponential) and no more for what follows; a chunk's product sums 24 steps,
+    truncated: 24 2^-23 2/3 of it, 1.9e-6, all toward zero; a rounding of the state a
+    chunk: sqrt(0.34 512) 2^-24 / sqrt(3) = 4.6e-7: bound 2.6e-6. Off in every chunk by
+    2^-25: 0.43 512 2^-25 = 6.6e-6, by the exponential's 2^-22 eight times that."""
+    both_states(B, N, H, Hk, d, BF16, keep, "decay_tc", (1, 1), 2.6e-6, False)

@@ -614,7 +614,9 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       if (starts(w))
         start = (p.part ? p.part + (int64_t)w.seg * p.B * p.H * p.d * p.d : p.start) +
                 ((int64_t)w.b * p.H + hs) * p.d * p.d;
-      // weights of a whole chunk; a chunk of fewer rows makes its own
+      // weights of a whole chunk; a chunk of fewer rows makes its own. `whole` is off
+      // by up to 2^-22 in every chunk, 5e-5 of the norm after 512 of slow decays: below
+      // the rows' bf16, where what the states' kernel does about it took 3 to 20 %.
       float f0[4], f1[4];
       auto weights = [&](int n) {
 #pragma unroll
@@ -763,6 +765,20 @@ struct DsTcShared {
   int abort_flag;
 };
 
+// The decay l^128 = hi + lo of whole chunks; out of line, as most of the kernel never
+// needs its registers (2 x 8192 rows of 16 heads on 4: 33.9 us, 34.6 in line).
+__device__ __noinline__ DecayFactor whole_chunk(const float* log_decay, int h) {
+  return DecayFactor::make(decay_rate(log_decay, h), (float)DT_T);
+}
+// That of the k-th whole chunk of a walk: fp32 numbers around l^128, in [1/2, 1] where
+// lo is not zero, whose sum is that of as many l^128 to 2^-24. One number for all
+// would be off by the same rounding, the exponential's 2^-22, in every chunk (512
+// chunks of slow decays: 1.8e-5 of the state's norm off 64 bits, 7e-7).
+__device__ __forceinline__ float chunk_decay(const DecayFactor& l, int k) {
+  auto steps = [](float x) { return (x + 0.75f) - 0.75f; };  // to a multiple of 2^-24
+  return l.hi + (steps((float)(k + 1) * l.lo) - steps((float)k * l.lo));
+}
+
 template <bool PAIR, int PLANES>
 __global__ void __launch_bounds__(DT_THREADS, 1)
     decay_state_tc_kernel(const __grid_constant__ CUtensorMap mb,
@@ -863,17 +879,18 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       const float l2_0 = decay_rate(p.log_decay, h0) * DT_LOG2E;
       const float l2_1 = decay_rate(p.log_decay, h1) * DT_LOG2E;
       const float l2_s = s_head ? l2_1 : l2_0;
+      DecayFactor whole = {};  // once the first chunk is under way
       float S[SC];
 #pragma unroll
       for (int e = 0; e < SC; ++e) S[e] = 0.f;
-      // S = l^n S + the product of chunk c_
-      auto take = [&](uint32_t c_, int n) {
+      // S = l^n S + the product of chunk c_, the unit's k-th
+      auto take = [&](uint32_t c_, int n, int k) {
         if (ok) ok = ht::warp_wait(&sh.done[1], c_ & 1, abort_flag);
         if (!ok) return;
         tc::fence_after_sync();
         uint32_t u[SC];
         tmem_ld_n(t_s + (c_ & 1) * 128, u);
-        const float all = power(l2_s, n);
+        const float all = n < DT_T || k == 0 ? power(l2_s, n) : chunk_decay(whole, k);
 #pragma unroll
         for (int e = 0; e < SC; ++e) S[e] = fmaf(all, S[e], __uint_as_float(u[e]));
         tc::fence_before_sync();
@@ -907,7 +924,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           // the issuing warp has seen its conv. (A unit ends with a take.)
           if (x > w.a0) {
             if (hf)
-              take(c - 1, n_before);
+              take(c - 1, n_before, x - 1 - w.a0);
             else
               ok = ht::warp_wait(&sh.done[0], (c - 1) & 1, abort_flag);
           }
@@ -949,9 +966,11 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
           if (lane == 0) ws::arrive(&sh.conv[hf]);
         }
         if (n < DT_T) weights(DT_T);
+        if (x == w.a0 && x + 1 < w.a1)
+          whole = whole_chunk(p.log_decay, s_head ? h1 : h0);
         n_before = n;
       }
-      if (w.a1 > w.a0) take(c - 1, n_before);
+      if (w.a1 > w.a0) take(c - 1, n_before, w.a1 - 1 - w.a0);
       const bool mine = !PAIR || w.h + s_head < p.H;
       if (mine && rc < p.d) {
         float* dst = p.part + (((int64_t)w.seg * p.B + w.b) * p.H + (s_head ? h1 : h0)) * p.d * p.d;
