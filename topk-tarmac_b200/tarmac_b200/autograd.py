@@ -151,27 +151,30 @@ class HeadAttention(torch.autograd.Function):
 
 
 class DecayAttention(torch.autograd.Function):
-    """Attention with a decay for each head (:func:`ops.decay_attention`) with
-    the state after the last row. The decays carry no gradient. First
-    derivatives in reverse mode only, as :class:`QkNormRotate`."""
+    """Attention with a decay for each head (:func:`ops.decay_attention`), with
+    the state after the last row where ``return_state`` asks for it. The decays
+    carry no gradient. First derivatives in reverse mode only, as
+    :class:`QkNormRotate`."""
 
     @staticmethod
-    def forward(ctx, q, k, v, log_decay, state=None, lens=None, scale=None):
+    def forward(ctx, q, k, v, log_decay, state=None, lens=None, scale=None,
+                return_state=True):
         ctx.save_for_backward(q, k, v, log_decay, state, lens)
         ctx.scale = scale
         ctx.set_materialize_grads(False)  # an unused state costs nothing
         return ops.decay_attention(q, k, v, log_decay, state, lens, scale,
-                                   return_state=True)
+                                   return_state=return_state)
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dout, dstate):
+    def backward(ctx, dout, dstate=None):
         q, k, v, log_decay, state, lens = ctx.saved_tensors
         if dout is None:
             dout = torch.zeros_like(q)
         dq, dk, dv, first = ops.decay_attention_backward(
-            q, k, v, log_decay, dout, state, dstate, lens, ctx.scale)
-        return dq, dk, dv, None, first, None, None
+            q, k, v, log_decay, dout, state, dstate, lens, ctx.scale,
+            need_dstate=ctx.needs_input_grad[4])
+        return dq, dk, dv, None, first, None, None, None
 
 
 class ResidualNorm(torch.autograd.Function):
@@ -261,8 +264,8 @@ def decay_attention(q, k, v, log_decay, state=None, lens=None, scale=None,
                          "not require one")
     ts = [t for t in (q, k, v, log_decay, state) if t is not None]
     if _needs_grad(*ts) or _has_tangent(*ts):
-        res = DecayAttention.apply(q, k, v, log_decay, state, lens, scale)
-        return res if return_state else res[0]
+        return DecayAttention.apply(q, k, v, log_decay, state, lens, scale,
+                                    return_state)
     return ops.decay_attention(q, k, v, log_decay, state, lens, scale,
                                return_state)
 

@@ -915,12 +915,13 @@ def decay_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                              state: torch.Tensor | None = None,
                              dstate: torch.Tensor | None = None,
                              lens: torch.Tensor | None = None,
-                             scale: float | None = None):
+                             scale: float | None = None,
+                             need_dstate: bool = True):
     """Gradients (dq, dk, dv, dS) of :func:`decay_attention`, given those of out
     (``dout``) and of the state that it returned (``dstate``, or None). dS, of
-    the state before the first row, is None where ``state`` is. Shared key
-    heads are summed over their query heads; padding gets zeros; the decays
-    have no gradient. Deterministic."""
+    the state before the first row, is None where ``state`` is, or without
+    ``need_dstate``. Shared key heads are summed over their query heads; padding
+    gets zeros; the decays have no gradient. Deterministic."""
     if not _decay_ready(q, k, v, log_decay, lens):
         q, k, v, log_decay, lens = _check_decay(q, k, v, log_decay, lens)
     dout = _gradient(dout, q, "dout")
@@ -928,7 +929,7 @@ def decay_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     B, N, H, d = q.shape
     Hk = k.shape[2]
     dq, dk, dv = _empty_as(q), _empty_as(k), _empty_as(v)
-    first = None if start is None else torch.empty_like(start)
+    first = torch.empty_like(start) if need_dstate and start is not None else None
     work = _scratch(_decay_backward_work(B, N, H, Hk, d, _DTYPES[q.dtype],
                                          int(first is not None)), q.device)
     _launch(q.get_device(), "tarmac_decay_attention_backward", q.data_ptr(),
