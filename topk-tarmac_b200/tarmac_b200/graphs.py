@@ -28,12 +28,32 @@ Rules:
   clone it to keep it.
 * The example call runs a few times on a side stream before the capture, so
   that one-time set-up inside the library (kernel attribute changes) happens
-  outside the graph.
+  outside the graph. Tensor arguments that the call changes (a state renewed in
+  place, a history that grows) are given their contents back afterwards, so
+  that nothing has happened to them until the first replay. A replay changes
+  the tensors that it is passed: the example's own in place, others by a copy
+  back; autograd learns of it. What ``fn`` changes without being passed it (a
+  state that a closure holds) is out of reach: pass it as an argument.
 """
 
 from __future__ import annotations
 
 import torch
+
+
+def _version(t) -> int:
+    """How often t was written in place, as far as autograd knows."""
+    return t._version if torch.is_tensor(t) and not t.is_inference() else 0
+
+
+def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Do both hold the same bits? (A NaN equals itself.)"""
+    def words(t):
+        if t.is_complex():
+            t = torch.view_as_real(t)
+        size = {1: torch.uint8, 2: torch.int16, 4: torch.int32, 8: torch.int64}
+        return t.detach().contiguous().view(size[t.element_size()])
+    return torch.equal(words(a), words(b))
 
 
 class GraphedCall:
@@ -48,12 +68,22 @@ class GraphedCall:
         self._static = list(example_args)
         self._consts = [None if torch.is_tensor(a) else a for a in example_args]
         cur = torch.cuda.current_stream(dev)
+        before = [a.detach().clone() if torch.is_tensor(a) else None for a in example_args]
+        versions = [_version(a) for a in example_args]
         side = torch.cuda.Stream(dev)
         side.wait_stream(cur)
         with torch.cuda.stream(side):
             for _ in range(max(1, warmup)):
                 fn(*self._static)
         cur.wait_stream(side)
+        # the arguments that the call changes (by an example of zeros, perhaps not)
+        self._renewed = [b is not None and (_version(a) != v or not _same(a, b))
+                         for a, b, v in zip(example_args, before, versions)]
+        with torch.no_grad():
+            for a, b, renewed in zip(example_args, before, self._renewed):
+                if renewed:
+                    a.copy_(b)
+        del before
         torch.cuda.synchronize(dev)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
@@ -74,4 +104,10 @@ class GraphedCall:
                 raise ValueError("GraphedCall: a non-tensor argument differs from the "
                                  "example call")
         self.graph.replay()
+        for dst, src, renewed in zip(self._static, args, self._renewed):
+            if renewed:
+                torch.autograd.graph.increment_version(dst)
+                if src is not dst:
+                    with torch.no_grad():
+                        src.copy_(dst, non_blocking=True)
         return self.output
