@@ -141,6 +141,30 @@ def test_a_cast_block_keeps_its_decays(dtype):
     assert m.to(dtype).log_decay.dtype is torch.float32 and m.proj.weight.dtype is dtype
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_cast_block_keeps_its_norms_weights(dtype):
+    """What the kernels read in fp32 is neither rounded nor cast call after call."""
+    m = DecayComm(24, 6, 16)
+    own = ("norm_q", "norm_k", "norm_post", "norm_next", "scale")
+    torch.manual_seed(0)
+    with torch.no_grad():
+        for n in own:
+            getattr(m, n).add_(0.1 * torch.randn_like(getattr(m, n)))
+    want = {n: getattr(m, n).detach().clone() for n in own}
+    params = dict(m.named_parameters())
+    for p in m.parameters():
+        p.grad = torch.ones_like(p)
+    for step in (lambda: m.to(dtype), lambda: m.double(), lambda: m.to(dtype)):
+        step()
+        for n in own:
+            w = getattr(m, n)
+            assert w is params[n] and w.requires_grad
+            assert w.dtype == w.grad.dtype == m.log_decay.dtype
+            assert torch.equal(w.detach().float(), want[n])
+        assert m.qkv.weight.dtype == m.qkv.weight.grad.dtype == m.gate.bias.dtype
+    assert m.scale.dtype is torch.float32 and m.gate.weight.dtype is dtype
+
+
 def test_room_for_a_state_renewed_in_place():
     """fp32 rows of 16 columns over several segments: each reads the state."""
     sizes = 3, 500, 2, 16, _lib.F32

@@ -173,3 +173,33 @@ def test_other_derivatives_are_refused():
                      lambda: autograd.residual_norm(dual, x)):
             with pytest.raises((RuntimeError, NotImplementedError)):
                 call()
+
+
+def test_a_cast_block_reads_its_norms_weights_as_they_are():
+    """bf16 rows, fp32 norms: the block's outputs are the operators' on the weights
+    before the cast, to the bit, and their gradients come in fp32."""
+    from tarmac_b200 import ops
+    from tarmac_b200.heads import DecayComm, rotation_table
+    torch.manual_seed(5)
+    B, N, dim, d = 2, 40, 32, 16
+    m = DecayComm(dim, 2, d).cuda()
+    own = ("norm_q", "norm_k", "norm_post", "norm_next", "scale")
+    with torch.no_grad():
+        for n in own:
+            getattr(m, n).add_(0.1 * torch.randn_like(getattr(m, n)))
+    wq, wk, wo, wi, sc = (getattr(m, n).detach().clone() for n in own)
+    m.bfloat16()
+    x = torch.randn(B, N, dim, device="cuda", dtype=torch.bfloat16)
+    cos, sin = rotation_table(torch.arange(N, device="cuda")[None], d)
+    with torch.no_grad():
+        q, k, v = (t.unflatten(-1, (2, d)) for t in m.qkv(x).split(2 * d, -1))
+        q, k = ops.qk_norm_rotate(q, k, wq, wk, cos, sin, m.eps)
+        out = ops.decay_attention(q, k, v, m.log_decay)
+        want = ops.residual_norm(x, m.proj(out.flatten(2)), wo, wi, m.gate(x), sc, m.eps)
+    h, z, _ = m(x, x, cos, sin)
+    assert torch.equal(h, want[0]) and torch.equal(z, want[1])
+    (h.float().sum() + z.float().square().sum()).backward()
+    for n in own:
+        g = getattr(m, n).grad
+        assert g.dtype is torch.float32 and g.isfinite().all() and g.abs().max() > 0
+    assert m.qkv.weight.grad.dtype is torch.bfloat16

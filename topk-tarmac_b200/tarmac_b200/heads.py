@@ -144,12 +144,19 @@ class DecayComm(nn.Module):
         self.register_buffer("log_decay", decay_slopes(n_heads))
 
     def _apply(self, fn, recurse=True):
-        """A cast to a shorter type leaves the decays in fp32."""
-        kept = self.log_decay
-        super()._apply(fn, recurse)
-        if self.log_decay.element_size() < kept.element_size():
-            self.log_decay = kept.to(self.log_decay.device, torch.float32)
-        return self
+        """A cast to a shorter type is for the products: the decays, the norms'
+        weights and the scale, which the kernels read in fp32, stay in it."""
+        own = [t for p in self._parameters.values() for t in (p, p.grad)]
+        own += self._buffers.values()
+
+        def keep(t):
+            new = fn(t)
+            if new.dtype != t.dtype and new.element_size() < 4 \
+                    and any(t is o for o in own):
+                new = t.to(new.device, torch.float32)
+            return new
+
+        return super()._apply(keep, recurse)
 
     def empty_state(self, B: int) -> torch.Tensor:
         """The state before any row, fp32 [B, n_heads, head_dim, head_dim]."""
