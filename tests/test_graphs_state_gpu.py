@@ -116,3 +116,41 @@ def test_blocks():
         got = step(a, c, s, kept[2], kept[3], n)
         assert torch.equal(got, y) and torch.equal(n, want_n)
     assert torch.equal(kept[0], kept[2]) and torch.equal(kept[1], kept[3])
+
+
+def test_no_room_for_copies(monkeypatch):
+    """Arguments that the device cannot hold twice are kept in host memory."""
+    from tarmac_b200 import graphs
+    q, k, v, rate, S = stream(4)
+
+    class Full(torch.Tensor):
+        def clone(self, *a, **kw):
+            raise torch.OutOfMemoryError("no room")
+
+    monkeypatch.setattr(torch.Tensor, "clone", Full.clone)
+    mine, want_S = S + 0, S + 0
+    step = graphs.GraphedCall(renew, *rows(0, q, k, v), rate, mine)
+    monkeypatch.undo()
+    assert torch.equal(mine, want_S)
+    assert torch.equal(step(*rows(1, q, k, v), rate, mine), renew(*rows(1, q, k, v), rate, want_S))
+    assert torch.equal(mine, want_S)
+
+
+def test_arguments_of_other_types():
+    """Whatever a function takes: masks, complex numbers, scalars, views, NaN."""
+    from tarmac_b200.graphs import GraphedCall
+    x = torch.full((4, 6), float("nan"), device="cuda")
+    mask = torch.tensor([True, False, True, True], device="cuda")
+    z = torch.randn(3, dtype=torch.complex64, device="cuda").conj()
+    one = torch.ones((), device="cuda", dtype=torch.float64)
+    wide = torch.randn(1, 6, device="cuda").expand(4, 6)
+    args = (x.t(), mask, z, one, wide)
+    versions = [t._version for t in args]
+
+    def fn(x, mask, z, one, wide):
+        return mask[:, None] * wide * one, z * 2, x.isnan().sum()
+
+    step = GraphedCall(fn, *args)
+    for a, b in zip(step(*args), fn(*args)):
+        assert torch.equal(a, b)
+    assert versions == [t._version for t in args]

@@ -46,14 +46,31 @@ def _version(t) -> int:
     return t._version if torch.is_tensor(t) and not t.is_inference() else 0
 
 
-def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Do both hold the same bits? (A NaN equals itself.)"""
-    def words(t):
-        if t.is_complex():
-            t = torch.view_as_real(t)
+def _keep(t):
+    """A copy of a tensor, in host memory where the device has no room."""
+    if not torch.is_tensor(t):
+        return None
+    try:
+        return t.detach().clone()
+    except torch.OutOfMemoryError:
+        return t.detach().cpu()
+
+
+def _changed(t: torch.Tensor, before: torch.Tensor, version: int) -> bool:
+    """Was t written since? By autograd's count, or by its bits (a NaN equals
+    itself), in case something wrote it without telling."""
+    if _version(t) != version:
+        return True
+    if before.device != t.device:
+        return t.is_inference()  # has no count
+
+    def words(x):
+        x = x.detach().resolve_conj().resolve_neg()
+        x = torch.view_as_real(x) if x.is_complex() else x
         size = {1: torch.uint8, 2: torch.int16, 4: torch.int32, 8: torch.int64}
-        return t.detach().contiguous().view(size[t.element_size()])
-    return torch.equal(words(a), words(b))
+        return x.contiguous().view(size[x.element_size()])
+
+    return not torch.equal(words(t), words(before))
 
 
 class GraphedCall:
@@ -68,7 +85,7 @@ class GraphedCall:
         self._static = list(example_args)
         self._consts = [None if torch.is_tensor(a) else a for a in example_args]
         cur = torch.cuda.current_stream(dev)
-        before = [a.detach().clone() if torch.is_tensor(a) else None for a in example_args]
+        before = [_keep(a) for a in example_args]
         versions = [_version(a) for a in example_args]
         side = torch.cuda.Stream(dev)
         side.wait_stream(cur)
@@ -76,13 +93,12 @@ class GraphedCall:
             for _ in range(max(1, warmup)):
                 fn(*self._static)
         cur.wait_stream(side)
-        # the arguments that the call changes (by an example of zeros, perhaps not)
-        self._renewed = [b is not None and (_version(a) != v or not _same(a, b))
-                         for a, b, v in zip(example_args, before, versions)]
+        # the arguments that the call changes
+        self._renewed = [i for i, (a, b, v) in enumerate(zip(example_args, before, versions))
+                         if b is not None and _changed(a, b, v)]
         with torch.no_grad():
-            for a, b, renewed in zip(example_args, before, self._renewed):
-                if renewed:
-                    a.copy_(b)
+            for i in self._renewed:
+                example_args[i].copy_(before[i])
         del before
         torch.cuda.synchronize(dev)
         self.graph = torch.cuda.CUDAGraph()
@@ -104,10 +120,9 @@ class GraphedCall:
                 raise ValueError("GraphedCall: a non-tensor argument differs from the "
                                  "example call")
         self.graph.replay()
-        for dst, src, renewed in zip(self._static, args, self._renewed):
-            if renewed:
-                torch.autograd.graph.increment_version(dst)
-                if src is not dst:
-                    with torch.no_grad():
-                        src.copy_(dst, non_blocking=True)
+        for i in self._renewed:
+            torch.autograd.graph.increment_version(self._static[i])
+            if args[i] is not self._static[i]:
+                with torch.no_grad():
+                    args[i].copy_(self._static[i], non_blocking=True)
         return self.output
