@@ -19,9 +19,9 @@
 // asynchronous copies, one tile ahead.
 // Bound by issue: at d = 32 a row takes 96 clocks of a scheduler's FMA pipe and
 // about as many slots for reads, copies into pairs and sums. Measured, gradients
-// with the forward pass: 64 x 512 rows of 4 heads, d = 16, 83 us; 300 x 723 rows
-// of 8 heads, d = 32, 1203 us (FMA pipe 58-62 %, issue 51-59 % of the peak); 32 x
-// 512 rows of 4 heads, d = 64, 349 us.
+// with the forward pass: 64 x 512 rows of 4 heads, d = 16, 84 us; 300 x 723 rows
+// of 8 heads, d = 32, 1211 us (FMA pipe 56-62 %, issue 51-60 % of the peak); 32 x
+// 512 rows of 4 heads, d = 64, 351 us.
 //
 // Where episodes and heads are too few to fill the GPU the row axis is cut in
 // segments: a first launch forms what each segment adds to the state; up to 32

@@ -11,9 +11,9 @@
 // must not gather the rounding of l: 600 rows of slow decays were 8e-6 of the norm
 // off 64 bits with l in one fp32 number, 6e-7 with l as 1 + m (DecayPower). The
 // state may be renewed in place: a block reads its head's state before it writes
-// it. 512 x 16 heads of 128 columns: 173 us a call that is repeated, 6.3 TB/s (96 %
-// of the copy rate), 201 us when L2 holds none of it; 1024 x 8 heads of 64: 49 us;
-// 256 x 4 heads of 16: 3.4 us, latency.
+// it. 512 x 16 heads of 128 columns: 201 us with L2 flushed, 5.4 TB/s (82 % of the
+// copy rate), 173-180 us a call when calls follow one another; 1024 x 8 heads of 64:
+// 49 us; 256 x 4 heads of 16: 3.4 us, latency.
 #include "decay.cuh"
 
 namespace tarmac {

@@ -36,7 +36,7 @@
 // 5700 clocks of an SM's share of HBM where no other block reads them too. The
 // chain bounds the rest: state, a S, out, rows follow one another, and what runs
 // beside them is the next P and the weights (tensor pipe 25-37 %, issue 35-43 %).
-// Bound of the states' pass: issue of the split (54 %; two halves a chunk in turn
+// Bound of the states' pass: issue of the split (58 %; two halves a chunk in turn
 // 34 us, a whole chunk at once 43: 2 x 8192 rows of 16 heads on 4, d = 128).
 // Every wait is bounded; one that runs out ends all roles once their copies
 // and products have landed, and every row is written, NaN or right.

@@ -877,8 +877,9 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     contiguous tensor like ``state`` and apart from all inputs, or ``state``
     itself, renewed in place. Rows from ``lens`` [B] on are padding, whatever
     they hold: they get 0 and leave S alone; those before must be finite (a
-    head's infinity may reach its rows as a NaN). One new row over a kept state
-    is N = 1."""
+    head's infinity may reach any of its rows as a NaN). One new row over a
+    kept state is N = 1; a state renewed call after call does not gather the
+    rounding of its decay."""
     if not _decay_ready(q, k, v, log_decay, lens):
         q, k, v, log_decay, lens = _check_decay(q, k, v, log_decay, lens)
     start = _check_state(state, "state", q)
