@@ -154,3 +154,28 @@ def test_arguments_of_other_types():
     for a, b in zip(step(*args), fn(*args)):
         assert torch.equal(a, b)
     assert versions == [t._version for t in args]
+
+
+def test_garbage_graphs_do_not_end_a_capture():
+    """A graph in a reference cycle that nobody holds is released before the capture,
+    not by a collection in it."""
+    import gc
+    from tarmac_b200 import ops
+    from tarmac_b200.graphs import GraphedCall
+    x = torch.randn(4, 8, 16, device="cuda")
+    gc.collect()
+    gc.disable()
+    try:
+        old = [GraphedCall(ops.dense_attention, x, x, x)]
+        old.append(old)
+        del old
+
+        def fn(x):
+            if torch.cuda.is_current_stream_capturing():
+                gc.collect()
+            return ops.dense_attention(x, x, x)
+
+        step = GraphedCall(fn, x)
+    finally:
+        gc.enable()
+    assert torch.equal(step(x), ops.dense_attention(x, x, x))

@@ -38,6 +38,8 @@ Rules:
 
 from __future__ import annotations
 
+import gc
+
 import torch
 
 
@@ -101,6 +103,7 @@ class GraphedCall:
                 example_args[i].copy_(before[i])
         del before
         torch.cuda.synchronize(dev)
+        gc.collect()  # graphs in garbage cycles: their release would end the capture
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.output = fn(*self._static)
