@@ -429,7 +429,8 @@ int tarmac_decay_attention(const void *q, const void *k, const void *v,
  * zero) that of state_out; strides: q, k, v, dout. With
  *   R_t = scale q_t dout_t^T + l R_(t+1),  l R_N = dstate_out,
  * dq_t = scale S_t dout_t, dk_t = R_t v_t, dv_t = R_t^T k_t and
- * dstate = l R_0; shared key heads are summed over their query heads. dq, dk,
+ * dstate = l R_0; shared key heads are summed over their query heads. scale is
+ * from 2^-60 to 2^20 here (TARMAC_ERR_SHAPE). dq, dk,
  * dv: contiguous, the inputs' type, zero on padding; dstate: fp32 [B, H, d, d]
  * or NULL, not dstate_out. The decays get no gradient. No atomics: two calls
  * give the same bits. work: 16-byte aligned scratch of

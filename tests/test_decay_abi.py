@@ -69,6 +69,16 @@ def test_decay_own_checks():
     assert fwd(2, 8, 4, 64, 7, 0) == 0
 
 
+@pytest.mark.parametrize("scale,status", [
+    (2.0 ** -60, _lib.OK), (2.0 ** 20, _lib.OK), (2.0 ** -61, _lib.ERR_SHAPE),
+    (2.0 ** 21, _lib.ERR_SHAPE), (1e-40, _lib.ERR_SHAPE)])
+def test_scales_of_the_gradients(scale, status):
+    """Beyond these bounds powers of a decay or the state over the scale could leave
+    fp32's range."""
+    assert _decay(True, B=0, scale=scale) == status
+    assert _decay(False, B=0, scale=scale) == _lib.OK
+
+
 def _norm(backward, **kw):
     a = dict(x=FAKE, y=FAKE, gate=FAKE, dh=FAKE, dz=FAKE, w=None, B=2, N=3, D=64, dtype=_lib.F32,
              eps=1e-6, o=FAKE, o2=FAKE, dgate=FAKE, work=FAKE)

@@ -169,3 +169,26 @@ def test_streams_hand_on_their_results():
         torch.cuda.synchronize()
         for x, y in zip(got, want):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -60, 2.0 ** 20])
+@pytest.mark.parametrize("N,d,dtype", [(150, 64, BF16), (150, 72, BF16), (150, 32, F32), (60, 48, F32)])
+def test_the_ends_of_the_scales(N, d, dtype, scale):
+    """The largest and smallest scale of the gradients, with decays on both sides of
+    2^-7 a row: the first state's gradient is the scale's alone, so that neither term
+    hides the other (bounds as in test_many_heads)."""
+    from tarmac_b200 import ops
+    t = rows(2, N, 4, d, dtype, 4)
+    rate = torch.tensor([-0.02, -4.84, -4.86, -7.0], device="cuda")
+    S = torch.randn(2, 4, d, d, device="cuda")
+    got = ops.decay_attention_backward(*t[:3], rate, t[3], S, S * scale, scale=scale)
+    args = [x.double().cpu() for x in t]
+    s = S.double().cpu()
+    want = d64.decay_grads(*args[:3], rate.cpu(), scale, args[3], s, None, s * scale)[2:]
+    mags = [x.abs() for x in args]
+    mags = d64.decay_grads(*mags[:3], rate.cpu(), scale, mags[3], s.abs(), None, s.abs() * scale)[2:]
+    for i, (a, b, m) in enumerate(zip(got, want, mags)):
+        tol = 1e-5 * m
+        if dtype is BF16 and i < 3:
+            tol = tol + 2 ** -8 * (m + b.abs())
+        assert ((a.double().cpu() - b).abs() <= tol).all(), i

@@ -259,7 +259,11 @@ int tarmac_decay_attention_backward(const void* q, const void* k, const void* v,
                                     float* dstate, void* work, void* stream) {
   DecayParams p;
   const int st = fill_decay(p, q, k, v, log_decay, state, lens, B, N, H, Hk, d, dtype, scale);
-  if (st != TARMAC_OK || B == 0) return st;
+  if (st != TARMAC_OK) return st;
+  // it stands in every term of R here, next to powers of up to l^-15 (2^105) on the
+  // tensor memory, and the recurrence divides the state by it
+  if (scale < 0x1p-60f || scale > 0x1p20f) return TARMAC_ERR_SHAPE;
+  if (B == 0) return TARMAC_OK;
   if (!aligned(dstate, 4) || !aligned(dstate_out, 4)) return TARMAC_ERR_ALIGN;
   cudaStream_t s = (cudaStream_t)stream;
   if (N == 0) return status(carry_state(dstate_out, dstate, (int64_t)B * H * d * d, s));

@@ -922,7 +922,8 @@ def decay_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     (``dout``) and of the state that it returned (``dstate``, or None). dS, of
     the state before the first row, is None where ``state`` is, or without
     ``need_dstate``. Shared key heads are summed over their query heads; padding
-    gets zeros; the decays have no gradient. Deterministic."""
+    gets zeros; the decays have no gradient; ``scale`` is from 2 ** -60 to 2 ** 20.
+    Deterministic."""
     if not _decay_ready(q, k, v, log_decay, lens):
         q, k, v, log_decay, lens = _check_decay(q, k, v, log_decay, lens)
     dout = _gradient(dout, q, "dout")
